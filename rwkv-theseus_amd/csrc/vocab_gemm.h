@@ -1,0 +1,273 @@
+// Matrix product of the vocabulary losses (gfx950): C[m][n] = sum_k X(m, k) Y(n, k), bfloat16
+// operands, float32 sums, for the three products of a vocabulary head:
+//
+//   logits   Z = H W^T      X = H [m][k], Y = W [n][k]      both rows run along the contraction
+//   dhidden  G W            X = G [m][k], Y = W [k][n]      Y's rows run along the output
+//   dweight  G^T H          X = G [k][m], Y = H [k][n]      both rows run along the outputs
+//
+// so no operand is ever transposed in memory: an operand whose rows run along the output is
+// staged as it lies and read with the LDS transpose read.
+//
+// One workgroup of 8 waves makes a BM x BN tile in steps of 64 along the contraction.  A step's
+// operands go from memory to LDS by LDS DMA (1 KB an instruction, no registers) into one of NST
+// stages; a wave reads the fragments of one half step (32) while its matrix instructions work on
+// the other half, so a step has one barrier, and a stage is refilled as soon as the second
+// half's fragments have left it, a whole step before it is read again.
+//
+// The matrix instruction is given Y as its row operand and X as its column operand: the
+// accumulator then holds four consecutive n of one m in each lane, which is what row-major
+// outputs store at once and what a softmax over n reduces inside a lane.
+//
+// LDS layouts (16-byte chunks, swizzled by row so that fragment reads spread over the banks):
+//   rows along k  ("RowK"): [BM][64], 128-byte rows, chunk c of row r at c ^ (r & 7), read 16
+//                 bytes at a time; where the other operand needs transpose reads, chunk c at
+//                 c ^ (2 ((r >> 1) & 3)) and read 8 + 8 bytes in the transpose read's order of k
+//                 (slots 0-3 = k0 + 4q + e, 4-7 = k0 + 16 + 4q + e).
+//   rows along the output ("RowN"): [64][BN], chunk c of row r at c ^ (2 (r & 7)), read by
+//                 ds_read_b64_tr_b16.
+#pragma once
+
+#include <type_traits>
+
+#include "wkv7_io.h"
+
+namespace vocab {
+
+using wkv7::f32x4_t;
+
+constexpr int BK = 64;  // contraction per step
+
+enum Lay { RowK, RowN };
+
+// One operand: rows of `ld` elements.  RowK: outer index -> row, `outer` valid rows, the
+// contraction's `K` elements in every row.  RowN: contraction index -> row, `inner` valid rows,
+// `outer` elements valid in a row (a multiple of 8).  Rows and columns beyond are read from the
+// last valid place; the other operand is zero there, or the output is not stored.
+struct Operand {
+    const uint16_t* p;
+    long ld;
+    int outer, inner;
+};
+
+struct Tiles {
+    int m, n;     // tiles of the output
+    int splits;   // parts of the contraction
+    int steps;    // steps of one part (the last may have fewer)
+    int all;      // steps in all
+    int group;    // m tiles that run together
+};
+
+struct Where {
+    int m, n, part;
+};
+// Workgroup b runs on XCD b % 8: each XCD takes a run of consecutive tiles, ordered in groups of
+// `group` m tiles that share the n tiles they walk over, so that an XCD's L2 serves both operands.
+__device__ __forceinline__ Where tile_of(const Tiles& t, int b, int total) {
+    const int each = total >> 3;
+    int id = b < each * 8 ? (b & 7) * each + (b >> 3) : b;
+    const int mn = t.m * t.n;
+    Where w;
+    w.part = id / mn;
+    id -= w.part * mn;
+    const int per = t.group * t.n, g = id / per, first = g * t.group;
+    const int size = min(t.m - first, t.group);
+    id -= g * per;
+    w.n = id / size;
+    w.m = first + (id - w.n * size);
+    return w;
+}
+
+// LDS DMA of 1 KB into `lds` (byte address), from base + voff.
+__device__ __forceinline__ void dma(uint32_t lds, const uint8_t* base, uint32_t voff) {
+    wkv7::dma_kb(lds, wkv7::dma_rsrc(base, 0xffffffffu), voff, 0);
+}
+
+// The stage loader of one operand for a wave: its 1 KB pieces w, w + 8, ... of a [B][64] or
+// [64][B] tile.
+template <Lay L, int B, bool PERM> struct Loader {
+    static constexpr int PIECES = B * BK * 2 / 1024 / 8;   // per wave
+    static constexpr int PER = L == RowK ? 8 : 512 / B;    // rows in a piece
+    static_assert(B * BK * 2 % 8192 == 0 && (L == RowK || B == 256 || B == 128 || B == 64), "tile");
+    const uint8_t* base;
+    uint32_t row, col, ld2;
+    int rows_left;  // RowK: valid rows from the tile's first; RowN: valid rows from the part's first
+
+    __device__ __forceinline__ Loader(const Operand& o, int x0, int k0, int wave, int lane) {
+        ld2 = (uint32_t)(o.ld * 2);
+        if constexpr (L == RowK) {
+            const int r = 8 * wave + (lane >> 3);
+            const int c = PERM ? (lane & 7) ^ (2 * ((r >> 1) & 3)) : (lane & 7) ^ (r & 7);
+            base = reinterpret_cast<const uint8_t*>(o.p + (long)x0 * o.ld + k0);
+            row = r * ld2;
+            col = 16 * c;
+            rows_left = o.outer - x0;
+        } else {
+            constexpr int CH = B / 8;  // chunks in a row
+            const int r = PER * wave + lane / CH;
+            const int c = (lane & (CH - 1)) ^ ((2 * (r & 7)) & (CH - 1));
+            base = reinterpret_cast<const uint8_t*>(o.p + (long)k0 * o.ld + x0);
+            row = r * ld2;
+            col = 2 * min(8 * c, o.outer - x0 - 8);
+            rows_left = o.inner - k0;
+        }
+    }
+    // piece j of the next step into the tile at `lds`; advance() after the last one
+    __device__ __forceinline__ void issue(uint32_t lds, int j, int wave) const {
+        const int last = L == RowK ? rows_left - 1 : min(rows_left - 1, BK - 1);
+        const uint32_t r = min(row + (uint32_t)(8 * PER * j) * ld2, (uint32_t)max(last, 0) * ld2);
+        dma(lds + (uint32_t)(wave + 8 * j) * 1024, base, r + col);
+    }
+    // to the next step; past the last one the loader stays there (its pieces are then not used)
+    __device__ __forceinline__ void advance(bool more) {
+        if constexpr (L == RowK) base += more ? BK * 2 : 0;
+        else {
+            base += more ? (long)BK * ld2 : 0;
+            rows_left -= more ? BK : 0;
+        }
+    }
+};
+
+// The fragment reader of one operand for a wave: fragment i = outer 16 i .. + 15 from the wave's
+// first, half step h, from the tile at LDS byte address `at`.
+template <Lay L, int B, bool PERM> struct Reader {
+    uint32_t a;
+    __device__ __forceinline__ Reader(int x0, int lane) {
+        const int r16 = lane & 15, q = lane >> 4;
+        if constexpr (L == RowK) {
+            const int r = x0 + r16;
+            if constexpr (PERM) a = r * 128 + 8 * (q & 1) + 16 * ((q >> 1) ^ (2 * ((r >> 1) & 3)));
+            else a = r * 128 + 16 * (q ^ (r & 7));
+        } else {
+            constexpr int CH = B / 8;
+            const int r = 4 * q + (r16 >> 2);
+            const int c = (x0 / 8 + ((r16 & 3) >> 1)) ^ ((2 * (r & 7)) & (CH - 1));
+            a = r * (B * 2) + 16 * c + 8 * (r16 & 1);
+        }
+    }
+    __device__ __forceinline__ uint4 get(const uint8_t* lds, uint32_t at, int i, int h) const {
+        if constexpr (L == RowK) {
+            if constexpr (PERM) {
+                const uint8_t* p = lds + at + 2048 * i;
+                const uint2 lo = *reinterpret_cast<const uint2*>(p + (a ^ (64 * h)));
+                const uint2 hi = *reinterpret_cast<const uint2*>(p + (a ^ (64 * h + 32)));
+                return make_uint4(lo.x, lo.y, hi.x, hi.y);
+            } else {
+                return *reinterpret_cast<const uint4*>(lds + at + 2048 * i + (a ^ (64 * h)));
+            }
+        } else {
+            // (outer 16 i is chunk 2 i: an exclusive or inside the wave's first chunks, which are a multiple of its fragments)
+            const uint8_t* p = lds + at + (a ^ (32 * i)) + 32 * h * (B * 2);
+            const uint2 lo = wkv7::tr_at(reinterpret_cast<const uint16_t*>(p));
+            const uint2 hi = wkv7::tr_at(reinterpret_cast<const uint16_t*>(p + 16 * (B * 2)));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+    }
+};
+
+template <int N> __device__ __forceinline__ void wait_barrier() {
+    wkv7::vm_wait_n<N>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// A BM x BN tile: WM x WN waves of TM x TN fragments, NST stages.  Leaves acc[tn][tm] (lane:
+// n = 16 tn + 4 (lane / 16) + e, m = 16 tm + lane % 16 from the wave's first) and every DMA
+// landed; the caller puts a barrier before it writes to LDS.
+template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct Product {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NST = NST_;
+    static constexpr Lay LX = LX_, LY = LY_;
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+    static constexpr bool PERM = LX == RowN || LY == RowN;
+    static constexpr int STAGE = (BM + BN) * BK * 2;
+    static constexpr int LDS = NST * STAGE;
+    static constexpr int THREADS = 512;
+    static_assert(WM * WN == 8, "eight waves");
+    using LoadX = Loader<LX, BM, PERM>;
+    using LoadY = Loader<LY, BN, PERM>;
+    static constexpr int PIECES = LoadX::PIECES + LoadY::PIECES;
+
+    f32x4_t acc[TN][TM];
+
+    __device__ __forceinline__ void run(uint8_t* lds, const Operand& X, const Operand& Y, int m0, int n0, int step0, int steps) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+        LoadX lx(X, m0, step0 * BK, wave, lane);
+        LoadY ly(Y, n0, step0 * BK, wave, lane);
+        const Reader<LX, BM, PERM> rx((wave / WN) * TM * 16, lane);
+        const Reader<LY, BN, PERM> ry((wave % WN) * TN * 16, lane);
+        auto piece = [&](int stage, int j) {
+            if (j < LoadX::PIECES) lx.issue(lds0 + stage * STAGE, j, wave);
+            else ly.issue(lds0 + stage * STAGE + BM * BK * 2, j - LoadX::PIECES, wave);
+        };
+#pragma unroll
+        for (int tn = 0; tn < TN; tn++)
+#pragma unroll
+            for (int tm = 0; tm < TM; tm++) acc[tn][tm] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NST; s++) {
+#pragma unroll
+            for (int j = 0; j < PIECES; j++) piece(s, j);
+            lx.advance(s + 1 < steps);
+            ly.advance(s + 1 < steps);
+        }
+        wait_barrier<(NST - 1) * PIECES>();
+
+        // One half step is TN groups of TM matrix instructions.  A y fragment's registers take the
+        // next half's fragment as soon as its group is done; x, used by every group, has two sets.
+        uint4 x0[TM], x1[TM], y[TN];
+        auto read_x = [&](uint4 (&x)[TM], int stage, int i, int h) { x[i] = rx.get(lds, stage * STAGE, i, h); };
+        auto read_y = [&](int stage, int i, int h) { y[i] = ry.get(lds, stage * STAGE + BM * BK * 2, i, h); };
+        auto group = [&](const uint4 (&x)[TM], int tn) {
+#pragma unroll
+            for (int tm = 0; tm < TM; tm++) acc[tn][tm] = wkv7::mma32(acc[tn][tm], y[tn], x[tm]);
+        };
+        // groups G0 .. TN - 1 with the next half's reads: x in the first groups, y behind its group
+        auto groups = [&](const uint4 (&x)[TM], uint4 (&xn)[TM], int stage, int h, auto first, auto fill, int fstage) {
+            constexpr int G0 = decltype(first)::value, NG = TN - G0;
+            constexpr int XG = NG >= 4 ? 2 : 1, XPER = (TM + XG - 1) / XG, YPER = (TN + NG - 1) / NG, FPER = (PIECES + NG - 1) / NG;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                if constexpr (decltype(fill)::value) {
+#pragma unroll
+                    for (int j = g * FPER; j < (g + 1) * FPER && j < PIECES; j++) piece(fstage, j);
+                }
+#pragma unroll
+                for (int i = g * XPER; i < (g + 1) * XPER && i < TM; i++) read_x(xn, stage, i, h);
+                group(x, G0 + g);
+#pragma unroll
+                for (int i = 0; i < TN; i++)
+                    if (i / YPER == g && i <= G0 + g) read_y(stage, i, h);
+                if (g == NG - 1) {
+#pragma unroll
+                    for (int i = 0; i < TN; i++)
+                        if (i / YPER > g || i > G0 + i / YPER) read_y(stage, i, h);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        constexpr int BG = TN >= 8 ? 2 : 0;  // groups of the second half ahead of the barrier
+        using None = std::integral_constant<int, 0>;
+        using Late = std::integral_constant<int, BG>;
+#pragma unroll
+        for (int i = 0; i < TM; i++) read_x(x0, 0, i, 0);
+#pragma unroll
+        for (int i = 0; i < TN; i++) read_y(0, i, 0);
+        int cur = 0;
+        for (int s = 0; s < steps; s++) {
+            groups(x0, x1, cur, 1, None{}, std::false_type{}, 0);
+            // (the stage's last reads complete under these)
+#pragma unroll
+            for (int g = 0; g < BG; g++) group(x1, g);
+            __builtin_amdgcn_sched_barrier(0);
+            // the next stage has landed, and every wave has read all of this one
+            wait_barrier<(NST - 2) * PIECES>();
+            const int next = cur + 1 == NST ? 0 : cur + 1;
+            groups(x1, x0, next, 0, Late{}, std::true_type{}, cur);
+            lx.advance(s + 1 + NST < steps);
+            ly.advance(s + 1 + NST < steps);
+            cur = next;
+        }
+        wkv7::vm_wait_n<0>();
+    }
+};
+
+}  // namespace vocab

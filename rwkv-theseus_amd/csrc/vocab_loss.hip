@@ -1,0 +1,672 @@
+// Losses over a large vocabulary and their gradients without keeping the logits (C ABI:
+// include/theseus_vocab.h, where the formulas are).
+//
+// Launches of one call, on the caller's stream:
+//   targets        every token's q, Q, sum q log q and weight from the labels or the teacher's logits
+//   target_logits  z at the target indices, one wave a (token, target): a dot product of width D
+//   weight_sum     MEAN: the sum of the weights (one workgroup, fixed order)
+//   then for each piece of rows
+//     logits       z's tiles on the matrix cores; of each 256-column tile a row's maximum and sum
+//                  of exponentials are kept and, for gradients, the exponentials (float16,
+//                  2^15 e^{z - tile maximum}: 11 significant bits down to e^-20 of the maximum)
+//     rows         log-sum-exp of a row from its tiles, the row's loss
+//     probs        exponentials -> G in place (bfloat16: the one rounding of the gradients' left factor)
+//     target_probs G at the target indices, from the float32 z of target_logits: p - 1 of a
+//                  confident token would be lost in a rounded p
+//     dhidden, dweight   G W and G^T H (vocab_gemm.h; float32 sums, rounded once)
+//   loss_sum       SUM, MEAN: one workgroup, fixed order
+//
+// The gradients take three products of 2 M V D operations, not the four of a backward that
+// forms the logits again: with SUM and MEAN the upstream gradient is one number, applied to the
+// results (theseus_vocab_scale).
+#include "../../include/theseus_vocab.h"
+#include "../../include/theseus_wkv7.h"
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "vocab_gemm.h"
+
+namespace vocab {
+
+using wkv7::bf16_to_f32;
+using wkv7::f32_to_bf16;
+using wkv7::f32x2_to_bf16x2;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float E_SHIFT = 15.f;  // kept exponentials are 2^15 e^{z - max}
+constexpr int BN_LOGITS = 256;   // columns of a logits tile
+constexpr int SKIP = -1, BAD = -2;
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+
+__device__ __forceinline__ float wave_sum(float x) {
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+
+// ---------------------------------------------------------------------------------- targets
+struct Targets {
+    long rows, vocab;
+    int K, top_bf16;
+    const int64_t* index;
+    const void* top;          // null: labels
+    const float* teacher_lse;
+    const float* row_weight;
+    long long ignore;
+    float inv_T;
+    int* j;        // [M][K] index, SKIP or BAD
+    float* q;      // [M][K] (teacher only)
+    float4* row;   // [M] {Q, sum q log q, weight, 0}
+};
+
+// One wave a token.
+__global__ __launch_bounds__(256) void targets_kernel(Targets t) {
+    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (i >= t.rows) return;
+    float weight = t.row_weight ? t.row_weight[i] : 1.f;
+    auto place = [&](int64_t v) { return v < 0 || v >= t.vocab ? BAD : (int)v; };
+    if (!t.top) {
+        if (lane == 0) {
+            const int64_t v = t.index[i];
+            const bool left_out = v == t.ignore;
+            t.j[i] = left_out ? SKIP : place(v);
+            t.row[i] = make_float4(1.f, 0.f, left_out ? 0.f : weight, 0.f);
+        }
+        return;
+    }
+    float x[THESEUS_VOCAB_MAX_TOP / 64], top = -INFINITY;
+    for (int s = 0; s < THESEUS_VOCAB_MAX_TOP / 64; s++) {
+        const int k = 64 * s + lane;
+        x[s] = -INFINITY;
+        if (k < t.K) {
+            const long at = i * t.K + k;
+            x[s] = (t.top_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(t.top)[at]) : static_cast<const float*>(t.top)[at]) * t.inv_T;
+        }
+        top = fmaxf(top, x[s]);
+    }
+    top = wave_max(top);
+    float sum = 0.f, base;
+    if (t.teacher_lse) {
+        base = t.teacher_lse[i];
+    } else {
+        // (a token of whom the teacher kept nothing has q = 0 throughout)
+        for (int s = 0; s < THESEUS_VOCAB_MAX_TOP / 64; s++) sum += x[s] == -INFINITY ? 0.f : expf(x[s] - top);
+        sum = wave_sum(sum);
+        base = top + logf(sum);
+    }
+    float Q = 0.f, H = 0.f;
+    for (int s = 0; s < THESEUS_VOCAB_MAX_TOP / 64; s++) {
+        const int k = 64 * s + lane;
+        if (k < t.K) {
+            const float lq = x[s] - base, q = x[s] == -INFINITY ? 0.f : expf(lq);
+            const long at = i * t.K + k;
+            t.q[at] = q;
+            t.j[at] = q == 0.f ? SKIP : place(t.index[at]);
+            Q += q;
+            H += q == 0.f ? 0.f : q * lq;
+        }
+    }
+    Q = wave_sum(Q);
+    H = wave_sum(H);
+    if (lane == 0) t.row[i] = make_float4(Q, H, weight, 0.f);
+}
+
+// z log2(e) / T at the target indices, one wave a (token, target); D a multiple of 64, rows 16-byte aligned.
+__global__ __launch_bounds__(256) void target_logits(long pairs, int K, int D, const uint16_t* x, long ldx, const uint16_t* w,
+                                                     long ldw, const int* j, float scale, float* z) {
+    const int lane = threadIdx.x & 63;
+    for (long p = (long)blockIdx.x * 4 + (threadIdx.x >> 6); p < pairs; p += (long)gridDim.x * 4) {
+        const int v = j[p];
+        if (v < 0) {
+            if (lane == 0) z[p] = v == BAD ? NAN : 0.f;
+            continue;
+        }
+        const uint4* a = reinterpret_cast<const uint4*>(x + (p / K) * ldx);
+        const uint4* b = reinterpret_cast<const uint4*>(w + (long)v * ldw);
+        float s = 0.f;
+        for (int c = lane; c < D / 8; c += 64) {
+            const uint4 u = a[c], y = b[c];
+            auto two = [&](uint32_t m, uint32_t n) {
+                s += __uint_as_float(m << 16) * __uint_as_float(n << 16);
+                s += __uint_as_float(m & 0xffff0000u) * __uint_as_float(n & 0xffff0000u);
+            };
+            two(u.x, y.x);
+            two(u.y, y.y);
+            two(u.z, y.z);
+            two(u.w, y.w);
+        }
+        s = wave_sum(s);
+        if (lane == 0) z[p] = s * scale;
+    }
+}
+
+// sum over 1024 threads in a fixed order, valid in thread 0
+__device__ __forceinline__ double block_sum(double x, double* red) {
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    double s = 0.0;
+    if (threadIdx.x == 0)
+        for (int k = 0; k < 16; k++) s += red[k];
+    return s;
+}
+__global__ __launch_bounds__(1024) void weight_sum(long rows, const float4* row, float* out) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (long i = threadIdx.x; i < rows; i += 1024) s += row[i].z;
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) *out = s == 0.0 ? 0.f : (float)(1.0 / s);
+}
+__global__ __launch_bounds__(1024) void loss_sum(long rows, const float* losses, const float* inv_weight, float* out) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (long i = threadIdx.x; i < rows; i += 1024) s += losses[i];
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) *out = (float)(inv_weight ? s * *inv_weight : s);
+}
+
+// ---------------------------------------------------------------------------------- logits
+struct LogitsOut {
+    int M, N, Ne;     // rows, vocabulary, columns kept (Ne >= N, zero beyond N)
+    float scale;      // log2(e) / T
+    float2* part;     // [M][tiles] {maximum, sum of 2^15 exp} of a tile, base 2
+    uint16_t* e;      // [..][lde]
+    long lde;
+};
+
+template <class P, bool KEEP>
+__global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y, Tiles t, LogitsOut o) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
+    const Where at = tile_of(t, blockIdx.x, gridDim.x);
+    const int m0 = at.m * P::BM, n0 = at.n * P::BN;
+    P g;
+    g.run(lds, X, Y, m0, n0, 0, t.all);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    const int wm = wave / P::WN, wn = wave % P::WN;
+    const int mw = wm * P::TM * 16 + r16, nw = n0 + wn * P::TN * 16 + 4 * q;
+    float* red = reinterpret_cast<float*>(lds);  // [2][WN][BM]
+    float top[P::TM];
+    const bool edge = n0 + P::BN > o.N;
+#pragma unroll
+    for (int tm = 0; tm < P::TM; tm++) {
+        top[tm] = -INFINITY;
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float z = g.acc[tn][tm][e] * o.scale;
+                if (edge && nw + 16 * tn + e >= o.N) z = -INFINITY;
+                g.acc[tn][tm][e] = z;
+                top[tm] = fmaxf(top[tm], z);
+            }
+        top[tm] = fmaxf(top[tm], __shfl_xor(top[tm], 16, 64));
+        top[tm] = fmaxf(top[tm], __shfl_xor(top[tm], 32, 64));
+    }
+    __syncthreads();
+    if (q == 0)
+#pragma unroll
+        for (int tm = 0; tm < P::TM; tm++) red[wn * P::BM + mw + 16 * tm] = top[tm];
+    __syncthreads();
+#pragma unroll
+    for (int tm = 0; tm < P::TM; tm++) {
+        const int m = mw + 16 * tm;
+        float all = red[m];
+#pragma unroll
+        for (int w = 1; w < P::WN; w++) all = fmaxf(all, red[w * P::BM + m]);
+        const float shift = E_SHIFT - all;
+        float sum = 0.f;
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float x = exp2_(g.acc[tn][tm][e] + shift);
+                g.acc[tn][tm][e] = x;
+                sum += x;
+            }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        top[tm] = all;
+        if (q == 0) red[(P::WN + wn) * P::BM + m] = sum;
+    }
+    __syncthreads();
+    if (wn == 0 && q == 0)
+#pragma unroll
+        for (int tm = 0; tm < P::TM; tm++) {
+            const int m = mw + 16 * tm;
+            if (m0 + m < o.M) {
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < P::WN; w++) sum += red[(P::WN + w) * P::BM + m];
+                o.part[(long)(m0 + m) * t.n + at.n] = make_float2(top[tm], sum);
+            }
+        }
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int tm = 0; tm < P::TM; tm++) {
+            const int m = m0 + mw + 16 * tm;
+            if (m < o.M) {
+                uint16_t* row = o.e + (long)m * o.lde;
+#pragma unroll
+                for (int tn = 0; tn < P::TN; tn++) {
+                    const int n = nw + 16 * tn;
+                    if (n < o.Ne) {
+                        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+                        const f32x4_t a = g.acc[tn][tm];
+                        const h4 h = {(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]};
+                        *reinterpret_cast<uint2*>(row + n) = __builtin_bit_cast(uint2, h);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------- rows
+// One wave a token of the piece: maximum and sum over its tiles, the token's loss.  Nothing is
+// taken from a rounded log-sum-exp: for a confident token, lse - z and p - 1 are small
+// differences of (z - maximum) and of the sum.
+struct Rows {
+    long rows;
+    int tiles, K;
+    const float2* part;
+    const float4* row;
+    const float *q, *z;
+    float TT;
+    float2* norm;  // {maximum (base 2), 1 / sum of 2^15 exp}
+    float* loss;
+};
+__global__ __launch_bounds__(256) void rows_kernel(Rows p) {
+    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (i >= p.rows) return;
+    const float2* part = p.part + i * p.tiles;
+    float top = -INFINITY;
+    for (int t = lane; t < p.tiles; t += 64) top = fmaxf(top, part[t].x);
+    top = wave_max(top);
+    float sum = 0.f;
+    for (int t = lane; t < p.tiles; t += 64) sum += part[t].y * exp2_(part[t].x - top);
+    sum = wave_sum(sum);
+    const float lse = logf(sum * exp2_(-E_SHIFT));  // above the maximum
+    const float4 row = p.row[i];
+    float s = 0.f;
+    for (int k = lane; k < p.K; k += 64) {
+        const float q = p.q ? p.q[i * p.K + k] : 1.f;
+        if (q != 0.f) s += q * (LN2 * (top - p.z[i * p.K + k]) + lse);
+    }
+    s = wave_sum(s);
+    if (lane == 0) {
+        p.norm[i] = make_float2(top, 1.f / sum);
+        if (p.loss) p.loss[i] = row.z == 0.f ? 0.f : p.TT * row.z * (s + row.y);
+    }
+}
+
+// ---------------------------------------------------------------------------------- G
+struct Probs {
+    int rows, M;            // rows of the piece (padded to 64: zeros), its tokens
+    int tiles, K;
+    long lde;
+    uint16_t* e;
+    const float2* part;
+    const float4* row;
+    const float2* norm;
+    const float *inv_weight, *row_grad;
+    const int* j;
+    const float *q, *z;
+    float T;
+};
+__device__ __forceinline__ float row_factor(const Probs& p, long i) {  // T c_i
+    float c = p.row[i].z;
+    if (p.inv_weight) c *= *p.inv_weight;
+    if (p.row_grad) c *= p.row_grad[i];
+    return p.T * c;
+}
+// blockIdx.x: 2048 columns of row blockIdx.y; 8 columns a thread
+__global__ __launch_bounds__(256) void probs_kernel(Probs p) {
+    const long i = blockIdx.y;
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 8;
+    if (n >= p.lde) return;
+    uint4* at = reinterpret_cast<uint4*>(p.e + i * p.lde + n);
+    float f = 0.f;
+    if (i < p.M) {
+        f = row_factor(p, i);
+        if (f != 0.f) f *= p.row[i].x * p.norm[i].y * exp2_(p.part[i * p.tiles + n / BN_LOGITS].x - p.norm[i].x);
+    }
+    if (f == 0.f) {
+        *at = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    uint4 u = *at;
+    auto two = [&](uint32_t& x) {
+        const h2 h = __builtin_bit_cast(h2, x);
+        x = f32x2_to_bf16x2((float)h[0] * f, (float)h[1] * f);
+    };
+    two(u.x);
+    two(u.y);
+    two(u.z);
+    two(u.w);
+    *at = u;
+}
+// one thread a (token, target); equal indices of one token write the same value
+__global__ __launch_bounds__(256) void target_probs(Probs p) {
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (long)p.M * p.K) return;
+    const long i = at / p.K;
+    const int v = p.j[at];
+    if (v < 0) return;
+    const float f = row_factor(p, i);
+    float g = 0.f;
+    if (f != 0.f) {
+        float q = 0.f;
+        if (!p.q) q = 1.f;
+        else
+            for (int k = 0; k < p.K; k++)
+                if (p.j[i * p.K + k] == v) q += p.q[i * p.K + k];
+        g = f * (p.row[i].x * (exp2_(p.z[at] - p.norm[i].x + E_SHIFT) * p.norm[i].y) - q);
+    }
+    p.e[i * p.lde + v] = f32_to_bf16(g);
+}
+
+// ---------------------------------------------------------------------------------- gradients
+// bfloat16 C; float32 parts of the contraction; float32 sum over row pieces (bfloat16 from the last)
+enum OutMode { OutBf16, OutPart, OutAdd };
+struct GradOut {
+    int M, N;
+    uint16_t* c;   // [M][ldc]
+    long ldc;
+    float* f;      // OutPart: [splits][M][ldf]; OutAdd: [M][ldf]
+    long ldf;
+    int first, last;  // OutAdd: of the row pieces
+};
+
+template <class P, OutMode MODE>
+__global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, Tiles t, GradOut o) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
+    const Where at = tile_of(t, blockIdx.x, gridDim.x);
+    const int m0 = at.m * P::BM, n0 = at.n * P::BN, s0 = at.part * t.steps;
+    P g;
+    g.run(lds, X, Y, m0, n0, s0, min(t.steps, t.all - s0));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    const int mw = m0 + (wave / P::WN) * P::TM * 16 + r16, nw = n0 + (wave % P::WN) * P::TN * 16 + 4 * q;
+    const bool four = (o.ldc & 3) == 0;  // (a row of C starts on 8 bytes)
+#pragma unroll
+    for (int tm = 0; tm < P::TM; tm++) {
+        const long m = mw + 16 * tm;
+        if (m >= o.M) continue;
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++) {
+            const int n = nw + 16 * tn;
+            if (n >= o.N) continue;
+            f32x4_t a = g.acc[tn][tm];
+            if constexpr (MODE == OutPart) {
+                *reinterpret_cast<f32x4_t*>(o.f + ((long)at.part * o.M + m) * o.ldf + n) = a;
+                continue;
+            }
+            if constexpr (MODE == OutAdd) {
+                f32x4_t* f = reinterpret_cast<f32x4_t*>(o.f + m * o.ldf + n);
+                if (!o.first) a += *f;
+                if (!o.last) {
+                    *f = a;
+                    continue;
+                }
+            }
+            uint16_t* c = o.c + m * o.ldc + n;
+            const uint2 u = make_uint2(f32x2_to_bf16x2(a[0], a[1]), f32x2_to_bf16x2(a[2], a[3]));
+            if (four) {  // (N is a multiple of 4 then too)
+                *reinterpret_cast<uint2*>(c) = u;
+            } else {
+                const uint32_t w[2] = {u.x, u.y};
+                for (int e = 0; e < 4 && n + e < o.N; e++) c[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            }
+        }
+    }
+}
+// the parts of a contraction added in order, 4 columns a thread
+__global__ __launch_bounds__(256) void add_parts(int M, int N, int splits, const float* f, long ldf, uint16_t* c, long ldc) {
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const long m = blockIdx.y;
+    if (n >= N) return;
+    f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; s++) a += *reinterpret_cast<const f32x4_t*>(f + ((long)s * M + m) * ldf + n);
+    for (int e = 0; e < 4 && n + e < N; e++) c[m * ldc + n + e] = f32_to_bf16(a[e]);
+}
+
+// copies rows of D elements (any alignment) to rows of Dp, zeros beyond D
+__global__ __launch_bounds__(256) void pad_rows(long rows, int D, int Dp, const uint16_t* x, long ld, uint16_t* out) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= Dp) return;
+    for (long i = blockIdx.y; i < rows; i += gridDim.y) out[i * Dp + c] = c < D ? x[i * ld + c] : 0;
+}
+
+__global__ __launch_bounds__(256) void scale_kernel(uint16_t* x, long n, const float* factor) {
+    const float f = *factor;
+    if (f == 1.f) return;
+    const bool wide = ((uintptr_t)x & 15) == 0;
+    const long n8 = wide ? n / 8 : 0, step = (long)gridDim.x * 256, first = (long)blockIdx.x * 256 + threadIdx.x;
+    auto two = [&](uint32_t u) { return f32x2_to_bf16x2(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f); };
+    for (long i = first; i < n8; i += step) {
+        uint4 u = reinterpret_cast<uint4*>(x)[i];
+        u = make_uint4(two(u.x), two(u.y), two(u.z), two(u.w));
+        reinterpret_cast<uint4*>(x)[i] = u;
+    }
+    for (long i = 8 * n8 + first; i < n; i += step) x[i] = f32_to_bf16(bf16_to_f32(x[i]) * f);
+}
+
+__global__ __launch_bounds__(256) void zero_kernel(uint16_t* x, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) x[i] = 0;
+}
+
+// ---------------------------------------------------------------------------------- host
+using Logits256 = Product<256, 256, 4, 2, 2, RowK, RowK>;
+using Logits64 = Product<64, 256, 1, 8, 4, RowK, RowK>;
+using Dhidden = Product<256, 256, 4, 2, 2, RowK, RowN>;
+using Dweight = Product<256, 256, 4, 2, 2, RowN, RowN>;
+
+static long up(long x, long to) { return (x + to - 1) / to * to; }
+static long ceil_div(long x, long y) { return (x + y - 1) / y; }
+
+struct Plan {
+    long M, V, D, K, Dp, lde, piece;  // Dp: width in the products; lde: kept columns; piece: rows
+    int pieces, tiles;                // row pieces; logits tiles of a row
+    bool grads, pad;
+    int splits;                       // of dhidden's contraction
+    size_t j, q, row, z, part, norm, loss, inv, e, acc, parts, hidden, weight, bytes;
+};
+
+constexpr long MAX_PIECE = 32768;  // rows: a grid's y dimension
+
+static int device_cus() {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
+    return n > 0 ? n : 256;
+}
+
+static int check(const theseus_vocab_loss_args* a) {
+    if (!a) return THESEUS_WKV7_ERR_NULL;
+    if (a->rows < 0 || a->rows > (1ll << 30) || a->vocab < 1 || a->vocab > (1ll << 22) || a->width < 1 || a->width > (1 << 17) ||
+        a->targets < 1 || a->targets > THESEUS_VOCAB_MAX_TOP || (!a->top_values && a->targets != 1) || a->hidden_stride < a->width ||
+        a->weight_stride < a->width || a->piece_rows < 0 || !(a->temperature > 0.f) || !isfinite(a->temperature))
+        return THESEUS_WKV7_ERR_SHAPE;
+    // (a tile's rows are addressed by 32-bit byte offsets)
+    if (a->hidden_stride > (1ll << 21) || a->weight_stride > (1ll << 21)) return THESEUS_WKV7_ERR_SHAPE;
+    if (a->top_dtype != THESEUS_VOCAB_BF16 && a->top_dtype != THESEUS_VOCAB_FP32) return THESEUS_WKV7_ERR_DTYPE;
+    if (a->reduction < THESEUS_VOCAB_NONE || a->reduction > THESEUS_VOCAB_MEAN) return THESEUS_WKV7_ERR_FLAGS;
+    return THESEUS_WKV7_OK;
+}
+
+static Plan plan(const theseus_vocab_loss_args* a) {
+    Plan p{};
+    p.M = a->rows, p.V = a->vocab, p.D = a->width, p.K = a->targets;
+    p.Dp = up(p.D, BK);
+    p.pad = p.D != p.Dp || a->hidden_stride % 8 || a->weight_stride % 8 || ((uintptr_t)a->hidden | (uintptr_t)a->weight) % 16;
+    p.grads = a->dhidden || a->dweight;
+    p.lde = up(p.V, BK);
+    p.tiles = (int)ceil_div(p.V, BN_LOGITS);
+    long cap = a->piece_rows ? up(a->piece_rows, 256) : p.grads ? (2l << 30) / (2 * p.lde) / 256 * 256 : MAX_PIECE;
+    cap = cap < 256 ? 256 : cap > MAX_PIECE ? MAX_PIECE : cap;
+    p.pieces = (int)ceil_div(p.M, cap);
+    p.piece = up(ceil_div(p.M, p.pieces ? p.pieces : 1), 256);
+    p.pieces = (int)ceil_div(p.M, p.piece ? p.piece : 256);
+    const long rows = p.M < p.piece ? p.M : p.piece;  // of the largest piece
+    if (a->dhidden) {
+        // fill the CUs: dhidden has few tiles (rows x D) and a long contraction (V)
+        const long t = ceil_div(rows, Dhidden::BM) * ceil_div(p.D, Dhidden::BN), steps = p.lde / BK;
+        long s = t >= device_cus() * 4 ? 1 : ceil_div(device_cus() * 4, t);
+        if (s > 16) s = 16;
+        while (s > 1 && steps / s < 16) s--;
+        p.splits = (int)s;
+    }
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += (n + 255) / 256 * 256;
+        return here;
+    };
+    p.j = take(p.M * p.K * 4);
+    p.q = take(a->top_values ? p.M * p.K * 4 : 0);
+    p.row = take(p.M * 16);
+    p.z = take(p.M * p.K * 4);
+    p.loss = take(a->loss && a->reduction != THESEUS_VOCAB_NONE ? p.M * 4 : 0);
+    p.inv = take(4);
+    p.norm = take(rows * 8);
+    p.part = take((size_t)rows * p.tiles * 8);
+    p.e = take(p.grads ? (size_t)up(rows, BK) * p.lde * 2 : 0);
+    p.acc = take(a->dweight && p.pieces > 1 ? (size_t)p.V * up(p.D, 4) * 4 : 0);
+    p.parts = take(p.splits > 1 ? (size_t)p.splits * rows * up(p.D, 4) * 4 : 0);
+    p.hidden = take(p.pad ? (size_t)p.M * p.Dp * 2 : 0);
+    p.weight = take(p.pad ? (size_t)p.V * p.Dp * 2 : 0);
+    p.bytes = at;
+    return p;
+}
+
+static Tiles tiles(long M, long N, int BM, int BN, long K, int splits) {
+    Tiles t;
+    t.m = (int)ceil_div(M, BM), t.n = (int)ceil_div(N, BN);
+    t.all = (int)(K / BK);
+    t.steps = (int)ceil_div(t.all, splits);
+    t.splits = (int)ceil_div(t.all, t.steps);
+    t.group = t.m < 8 ? t.m : 8;
+    return t;
+}
+
+static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hipStream_t st) {
+    auto at = [&](size_t off) { return ws + off; };
+    int* j = reinterpret_cast<int*>(at(p.j));
+    float* q = a->top_values ? reinterpret_cast<float*>(at(p.q)) : nullptr;
+    float4* row = reinterpret_cast<float4*>(at(p.row));
+    float* z = reinterpret_cast<float*>(at(p.z));
+    float* inv = a->reduction == THESEUS_VOCAB_MEAN ? reinterpret_cast<float*>(at(p.inv)) : nullptr;
+    float2* norm = reinterpret_cast<float2*>(at(p.norm));
+    float2* part = reinterpret_cast<float2*>(at(p.part));
+    uint16_t* e = reinterpret_cast<uint16_t*>(at(p.e));
+    const bool reduce = a->loss && a->reduction != THESEUS_VOCAB_NONE;
+    float* losses = reduce ? reinterpret_cast<float*>(at(p.loss)) : a->loss;
+    const uint16_t* H = static_cast<const uint16_t*>(a->hidden);
+    const uint16_t* W = static_cast<const uint16_t*>(a->weight);
+    long ldh = a->hidden_stride, ldw = a->weight_stride;
+    const float inv_T = 1.f / a->temperature;
+    if (p.M == 0) {
+        if (reduce) loss_sum<<<1, 1024, 0, st>>>(0, nullptr, nullptr, a->loss);
+        if (a->dweight) zero_kernel<<<1024, 256, 0, st>>>(static_cast<uint16_t*>(a->dweight), p.V * p.D);
+        return 0;
+    }
+    if (p.pad) {
+        uint16_t *h = reinterpret_cast<uint16_t*>(at(p.hidden)), *w = reinterpret_cast<uint16_t*>(at(p.weight));
+        const unsigned gx = (unsigned)ceil_div(p.Dp, 256);
+        pad_rows<<<dim3(gx, (unsigned)(p.M < 32768 ? p.M : 32768)), 256, 0, st>>>(p.M, (int)p.D, (int)p.Dp, H, ldh, h);
+        pad_rows<<<dim3(gx, (unsigned)(p.V < 32768 ? p.V : 32768)), 256, 0, st>>>(p.V, (int)p.D, (int)p.Dp, W, ldw, w);
+        H = h, W = w, ldh = ldw = p.Dp;
+    }
+    Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight,
+              a->ignore_index, inv_T, j, q, row};
+    targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
+    const long pairs = p.M * p.K;
+    target_logits<<<(unsigned)(ceil_div(pairs, 4) < 65536 ? ceil_div(pairs, 4) : 65536), 256, 0, st>>>(
+        pairs, (int)p.K, (int)p.Dp, H, ldh, W, ldw, j, LOG2E * inv_T, z);
+    if (inv) weight_sum<<<1, 1024, 0, st>>>(p.M, row, inv);
+
+    for (int piece = 0; piece < p.pieces; piece++) {
+        const long i0 = piece * p.piece, m = p.M - i0 < p.piece ? p.M - i0 : p.piece;
+        const uint16_t* Hp = H + i0 * ldh;
+        const Operand X{Hp, ldh, (int)m, (int)p.Dp}, Y{W, ldw, (int)p.V, (int)p.Dp};
+        const LogitsOut lo{(int)m, (int)p.V, (int)p.lde, LOG2E * inv_T, part, e, p.lde};
+        auto logits = [&](auto tag) {
+            using P = decltype(tag);
+            const Tiles tl = tiles(m, p.V, P::BM, P::BN, p.Dp, 1);
+            if (p.grads) logits_kernel<P, true><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
+            else logits_kernel<P, false><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
+        };
+        if (m <= 64) logits(Logits64{});
+        else logits(Logits256{});
+        const Rows rw{m, p.tiles, (int)p.K, part, row + i0, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
+                      a->temperature * a->temperature, norm, losses ? losses + i0 : nullptr};
+        rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
+        if (!p.grads) continue;
+
+        const long mp = up(m, BK);
+        const Probs pr{(int)mp, (int)m, p.tiles, (int)p.K, p.lde, e, part, row + i0, norm, inv,
+                       a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, a->temperature};
+        probs_kernel<<<dim3((unsigned)ceil_div(p.lde, 2048), (unsigned)mp), 256, 0, st>>>(pr);
+        target_probs<<<(unsigned)ceil_div(m * p.K, 256), 256, 0, st>>>(pr);
+        if (a->dhidden) {
+            uint16_t* dh = static_cast<uint16_t*>(a->dhidden) + i0 * p.D;
+            const Operand GX{e, p.lde, (int)m, (int)p.lde}, WY{W, ldw, (int)p.Dp, (int)p.V};
+            const Tiles tl = tiles(m, p.D, Dhidden::BM, Dhidden::BN, p.lde, p.splits);
+            float* parts = reinterpret_cast<float*>(at(p.parts));
+            const GradOut go{(int)m, (int)p.D, dh, p.D, parts, up(p.D, 4), 0, 0};
+            if (tl.splits > 1) {
+                grad_kernel<Dhidden, OutPart><<<tl.m * tl.n * tl.splits, 512, 0, st>>>(GX, WY, tl, go);
+                add_parts<<<dim3((unsigned)ceil_div(p.D, 1024), (unsigned)m), 256, 0, st>>>((int)m, (int)p.D, tl.splits, parts, up(p.D, 4), dh, p.D);
+            } else {
+                grad_kernel<Dhidden, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, WY, tl, go);
+            }
+        }
+        if (a->dweight) {
+            const Operand GX{e, p.lde, (int)p.lde, (int)mp}, HY{Hp, ldh, (int)p.Dp, (int)m};
+            const Tiles tl = tiles(p.V, p.D, Dweight::BM, Dweight::BN, mp, 1);
+            const GradOut go{(int)p.V, (int)p.D, static_cast<uint16_t*>(a->dweight), p.D, reinterpret_cast<float*>(at(p.acc)),
+                             up(p.D, 4), piece == 0, piece == p.pieces - 1};
+            if (p.pieces > 1) grad_kernel<Dweight, OutAdd><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
+            else grad_kernel<Dweight, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
+        }
+    }
+    if (reduce) loss_sum<<<1, 1024, 0, st>>>(p.M, losses, inv, a->loss);
+    return 0;
+}
+
+}  // namespace vocab
+
+extern "C" {
+
+size_t theseus_vocab_loss_workspace_size(const theseus_vocab_loss_args* args) {
+    return vocab::check(args) ? 0 : vocab::plan(args).bytes;
+}
+
+int theseus_vocab_loss(const theseus_vocab_loss_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (int e = vocab::check(a)) return e;
+    if (a->rows && (!a->hidden || !a->weight || !a->index)) return THESEUS_WKV7_ERR_NULL;
+    const vocab::Plan p = vocab::plan(a);
+    if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return THESEUS_WKV7_ERR_WORKSPACE;
+    vocab::run(a, p, static_cast<uint8_t*>(workspace), stream);
+    return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
+}
+
+int theseus_vocab_scale(void* x, long long n, const float* factor, hipStream_t stream) {
+    if (n < 0) return THESEUS_WKV7_ERR_SHAPE;
+    if (!x || !factor) return THESEUS_WKV7_ERR_NULL;
+    if (!n) return THESEUS_WKV7_OK;
+    const long blocks = vocab::ceil_div(n, 8 * 256);
+    vocab::scale_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(static_cast<uint16_t*>(x), n, factor);
+    return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -1,0 +1,257 @@
+"""What a language model's head is trained on and answers with, over a large vocabulary
+(C ABI: include/theseus_vocab.h).
+
+The reference distils its student layers against hidden states and checks the converted model by
+a divergence over full logits (theseus/losses.py:5-30, validate.py).  These operators are what
+training the whole student takes next: losses on the head's output that never hold the
+[tokens, vocabulary] logits, and the few logits of a teacher that are worth keeping.
+
+* ``linear_cross_entropy(hidden, weight, labels)``: softmax cross entropy of hidden @ weight.T;
+* ``linear_top_distillation(hidden, weight, top_values, top_indices)``: the divergence of the
+  student's softmax from a teacher of whom each token's top logits are known;
+* ``top_logits(logits, k)``: those top logits and indices, and the row's log-sum-exp.
+
+The losses are differentiable in ``hidden`` and ``weight`` (bfloat16; under autocast other types
+are cast as ``torch.nn.functional.linear`` casts them).  With ``reduction="mean"`` or ``"sum"``
+the gradients are made together with the loss, in three products, and the backward multiplies
+them by the upstream gradient; with ``"none"`` the backward forms the probabilities again.
+A second backward through the same loss (retain_graph) makes the gradients anew.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .wkv7 import extension
+
+MAX_TOP = 256  # THESEUS_VOCAB_MAX_TOP
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+
+class LossArgs(ctypes.Structure):
+    """theseus_vocab_loss_args."""
+    _fields_ = ([(n, ctypes.c_longlong) for n in ("rows", "vocab")] + [(n, ctypes.c_int) for n in ("width", "targets")]
+                + [(n, ctypes.c_void_p) for n in ("hidden", "weight")]
+                + [(n, ctypes.c_longlong) for n in ("hidden_stride", "weight_stride")]
+                + [(n, ctypes.c_void_p) for n in ("index", "top_values")]
+                + [(n, ctypes.c_int) for n in ("top_dtype", "reduction")]
+                + [(n, ctypes.c_void_p) for n in ("teacher_lse", "row_weight")]
+                + [("ignore_index", ctypes.c_longlong), ("temperature", ctypes.c_float)]
+                + [(n, ctypes.c_void_p) for n in ("loss", "row_grad", "dhidden", "dweight")]
+                + [("piece_rows", ctypes.c_longlong)])
+
+
+_bound = None
+
+
+def _lib():
+    global _bound
+    lib = extension().lib
+    if _bound is None:
+        vp, i32, i64, sz, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t, ctypes.c_float
+        lib.theseus_vocab_loss_workspace_size.argtypes = [ctypes.POINTER(LossArgs)]
+        lib.theseus_vocab_loss_workspace_size.restype = sz
+        lib.theseus_vocab_loss.argtypes = [ctypes.POINTER(LossArgs), vp, sz, vp]
+        lib.theseus_vocab_loss.restype = i32
+        lib.theseus_vocab_scale.argtypes = [vp, i64, vp, vp]
+        lib.theseus_vocab_scale.restype = i32
+        lib.theseus_vocab_top_workspace_size.argtypes = [i64, i64, i32, i32]
+        lib.theseus_vocab_top_workspace_size.restype = sz
+        lib.theseus_vocab_top.argtypes = [i64, i64, i32, i32, f32, vp, i64, vp, vp, vp, vp, sz, vp]
+        lib.theseus_vocab_top.restype = i32
+        _bound = True
+    return lib
+
+
+def _check(status):
+    if status:
+        raise RuntimeError("theseus_vocab: " + extension().lib.theseus_wkv7_error_string(status).decode())
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Call:
+    """One loss's inputs, checked and laid out for theseus_vocab_loss."""
+
+    def __init__(self, hidden, weight, index, top_values, teacher_lse, row_weight, ignore_index, temperature, reduction,
+                 piece_rows):
+        self.index, self.top_values, self.teacher_lse, self.row_weight = index, top_values, teacher_lse, row_weight
+        self.ignore_index, self.temperature, self.reduction = ignore_index, temperature, reduction
+        self.piece_rows, self.targets = piece_rows, 1 if top_values is None else top_values.shape[1]
+        self.rows, self.vocab, self.width = hidden.shape[0], weight.shape[0], hidden.shape[1]
+        self.device = hidden.device
+
+    def run(self, hidden, weight, loss, row_grad, dhidden, dweight):
+        lib = _lib()
+        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        a = LossArgs(self.rows, self.vocab, self.width, self.targets, p(hidden), p(weight),
+                     max(hidden.stride(0), self.width), max(weight.stride(0), self.width),
+                     p(self.index), p(self.top_values),
+                     0 if self.top_values is None else _DTYPES[self.top_values.dtype], _REDUCTIONS[self.reduction],
+                     p(self.teacher_lse), p(self.row_weight), self.ignore_index, self.temperature, p(loss), p(row_grad),
+                     p(dhidden), p(dweight), self.piece_rows)
+        with torch.cuda.device(self.device):
+            nbytes = int(lib.theseus_vocab_loss_workspace_size(ctypes.byref(a)))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            _check(lib.theseus_vocab_loss(ctypes.byref(a), ws.data_ptr(), nbytes, _stream(self.device)))
+
+    def new_loss(self):
+        return torch.empty(self.rows if self.reduction == "none" else (), dtype=torch.float32, device=self.device)
+
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, call):
+        loss = call.new_loss()
+        need_h, need_w = ctx.needs_input_grad[:2]
+        ctx.call, ctx.made = call, None
+        dh = dw = None
+        if call.reduction != "none":
+            dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need_h else None
+            dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None
+            ctx.made = (dh, dw)
+        call.run(hidden, weight, loss, None, dh, dw)
+        ctx.save_for_backward(hidden, weight)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        call, made, ctx.made = ctx.call, ctx.made, None
+        grad = grad.float().contiguous()
+        if made is None:
+            hidden, weight = ctx.saved_tensors
+            need_h, need_w = ctx.needs_input_grad[:2]
+            made = (torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need_h else None,
+                    torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None)
+            if call.reduction == "none":
+                call.run(hidden, weight, None, grad, *made)
+                return (*made, None)
+            call.run(hidden, weight, None, None, *made)
+        lib = _lib()
+        with torch.cuda.device(call.device):
+            for x in made:
+                if x is not None and x.numel():
+                    _check(lib.theseus_vocab_scale(x.data_ptr(), x.numel(), grad.data_ptr(), _stream(call.device)))
+        return (*made, None)
+
+
+def _rows(x, name, rows, device, dtypes, tail=()):
+    """x [..., *tail] as contiguous [rows, *tail] on the device."""
+    if x.dtype not in dtypes:
+        raise TypeError(f"theseus_vocab: {name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {x.dtype}")
+    if x.device != device:
+        raise ValueError(f"theseus_vocab: {name} must be on {device}, got {x.device}")
+    if tuple(x.shape) != rows + tail:
+        raise ValueError(f"theseus_vocab: {name} must have shape {list(rows + tail)}, got {list(x.shape)}")
+    return x.detach().reshape(-1, *tail).contiguous()
+
+
+def _matrix(x, name):
+    """[n][d] with unit stride along d and rows apart (a strided view's rows are read in place)."""
+    if x.stride(1) == 1 and x.stride(0) >= x.shape[1] or x.shape[0] == 1 and x.stride(1) == 1:
+        return x
+    return x.contiguous()
+
+
+def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_index, temperature, reduction, piece_rows):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"theseus_vocab: unknown reduction {reduction!r} (none, sum or mean)")
+    if not (hidden.is_cuda and weight.is_cuda):
+        raise ValueError("theseus_vocab: hidden and weight must be CUDA tensors")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"theseus_vocab: expected hidden [..., D] and weight [V, D], got {list(hidden.shape)} and {list(weight.shape)}")
+    if weight.device != hidden.device:
+        raise ValueError(f"theseus_vocab: weight must be on {hidden.device}, got {weight.device}")
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(dt), weight.to(dt)
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError(f"theseus_vocab: hidden and weight must be bfloat16 (or cast by autocast), got {hidden.dtype} and {weight.dtype}")
+    if not temperature > 0 or temperature == float("inf"):
+        raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
+    if piece_rows < 0:
+        raise ValueError(f"theseus_vocab: piece_rows must not be negative, got {piece_rows}")
+    tokens, device = tuple(hidden.shape[:-1]), hidden.device
+    index = _rows(index, "labels" if top_values is None else "top_indices", tokens, device, (torch.int64,),
+                  () if top_values is None else (index.shape[-1] if index.dim() else 0,))
+    if top_values is not None:
+        k = index.shape[-1]
+        if not 1 <= k <= MAX_TOP:
+            raise ValueError(f"theseus_vocab: 1 to {MAX_TOP} top logits per token, got {k}")
+        top_values = _rows(top_values, "top_values", tokens, device, tuple(_DTYPES), (k,))
+    if teacher_lse is not None:
+        teacher_lse = _rows(teacher_lse, "teacher_lse", tokens, device, (torch.float32,))
+    if row_weight is not None:
+        row_weight = _rows(row_weight, "token_weight", tokens, device, (torch.float32,))
+    h, w = _matrix(hidden.reshape(-1, hidden.shape[-1]), "hidden"), _matrix(weight, "weight")
+    call = _Call(h, w, index, top_values, teacher_lse, row_weight, ignore_index, float(temperature), reduction, piece_rows)
+    if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
+        loss = _Loss.apply(h, w, call)
+    else:
+        loss = call.new_loss()
+        call.run(h, w, loss, None, None, None)
+    return loss.reshape(tokens) if reduction == "none" else loss
+
+
+def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, reduction="mean", piece_rows=0):
+    """Softmax cross entropy of ``hidden @ weight.T`` without the logits.
+
+    hidden [..., D], weight [V, D] bfloat16, labels [...] int64.  Returns float32: each token's
+    -log p(label) (reduction "none", shape [...]), their sum, or their mean over the tokens whose
+    label is not ``ignore_index`` (0 where there is none).  A label outside the vocabulary makes
+    its loss NaN.  ``piece_rows``: tokens whose probabilities the gradients hold at a time
+    (0: as many as 2 GiB take)."""
+    return _loss(hidden, weight, labels, None, None, None, int(ignore_index), 1.0, reduction, int(piece_rows))
+
+
+def linear_top_distillation(hidden, weight, top_values, top_indices, *, temperature=1.0, teacher_lse=None,
+                            token_weight=None, reduction="mean", piece_rows=0):
+    """T^2 sum_k q_k (log q_k - log p_k): the divergence of p = softmax(hidden @ weight.T / T)
+    from a teacher's top logits, without the student's logits.
+
+    top_values [..., K] (bfloat16 or float32 logits) and top_indices [..., K] int64, K <= 256, as
+    ``top_logits`` gives them; -inf entries are left out, equal indices add up.  q is the
+    teacher's softmax over the K, or with ``teacher_lse`` [...] (``top_logits``' third result at
+    the same temperature) the teacher's own probabilities, what lies outside the K left out.
+    token_weight [...] float32 multiplies the tokens' losses (0: the token adds nothing).
+    Returns float32: the tokens' losses (reduction "none"), their sum, or the sum over the sum of
+    the weights ("mean"; 0 where that is 0)."""
+    return _loss(hidden, weight, top_indices, top_values, teacher_lse, token_weight, -100, temperature, reduction,
+                 int(piece_rows))
+
+
+@torch.no_grad()
+def top_logits(logits, k, *, temperature=1.0):
+    """The k largest logits of each row: (values [..., k] in the logits' type, indices [..., k]
+    int64, lse [...] float32), largest first, equal ones by the lowest index, NaN above every
+    number; lse = logsumexp(logits / temperature).
+
+    logits [..., V] bfloat16 or float32 (rows may lie apart: a slice of a wider tensor is read in
+    place), 1 <= k <= min(V, 256).  Not differentiable."""
+    if not logits.is_cuda:
+        raise ValueError("theseus_vocab: logits must be a CUDA tensor")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"theseus_vocab: logits must be bfloat16 or float32, got {logits.dtype}")
+    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], MAX_TOP):
+        raise ValueError(f"theseus_vocab: k must be in 1..min(V, {MAX_TOP}), got {k} for logits {list(logits.shape)}")
+    if not temperature > 0 or temperature == float("inf"):
+        raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
+    V, rows = logits.shape[-1], logits.shape[:-1]
+    x = _matrix(logits.detach().reshape(-1, V), "logits")
+    n, dt, dev = x.shape[0], _DTYPES[x.dtype], x.device
+    values = torch.empty((*rows, k), dtype=x.dtype, device=dev)
+    indices = torch.empty((*rows, k), dtype=torch.int64, device=dev)
+    lse = torch.empty(rows, dtype=torch.float32, device=dev)
+    lib = _lib()
+    with torch.cuda.device(dev):
+        nbytes = int(lib.theseus_vocab_top_workspace_size(n, V, k, dt))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _check(lib.theseus_vocab_top(n, V, k, dt, float(temperature), x.data_ptr(), max(x.stride(0), V), values.data_ptr(),
+                                     indices.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                                     _stream(dev)))
+    return values, indices, lse
