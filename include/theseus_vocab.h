@@ -77,8 +77,9 @@ size_t theseus_vocab_loss_workspace_size(const theseus_vocab_loss_args* args);
 int theseus_vocab_loss(const theseus_vocab_loss_args* args, void* workspace, size_t workspace_bytes,
                        hipStream_t stream);
 
-/* x *= *factor for n bfloat16 values, nothing moved where the factor (device memory) is 1. */
-int theseus_vocab_scale(void* x, long long n, const float* factor, hipStream_t stream);
+/* x and y *= *factor for nx and ny bfloat16 values (a NULL of 0 values is left out), nothing moved
+ * where the factor (device memory) is 1. */
+int theseus_vocab_scale(void* x, long long nx, void* y, long long ny, const float* factor, hipStream_t stream);
 
 /* logits [M][V] bfloat16 or float32, row_stride elements from row to row, M >= 0, V in
  * 1 .. 2^30, k in 1 .. min(V, THESEUS_VOCAB_MAX_TOP).  values [M][k] in the logits' type and

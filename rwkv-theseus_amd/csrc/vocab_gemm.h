@@ -21,7 +21,7 @@
 // LDS layouts (16-byte chunks, swizzled by row so that fragment reads spread over the banks):
 //   rows along k  ("RowK"): [BM][64], 128-byte rows, chunk c of row r at c ^ (r & 7), read 16
 //                 bytes at a time; where the other operand needs transpose reads, chunk c at
-//                 c ^ (2 ((r >> 1) & 3)) and read 8 + 8 bytes in the transpose read's order of k
+//                 c ^ ((r >> 1) & 7) and read 8 + 8 bytes in the transpose read's order of k
 //                 (slots 0-3 = k0 + 4q + e, 4-7 = k0 + 16 + 4q + e).
 //   rows along the output ("RowN"): [64][BN], chunk c of row r at c ^ (2 (r & 7)), read by
 //                 ds_read_b64_tr_b16.
@@ -96,7 +96,7 @@ template <Lay L, int B, bool PERM> struct Loader {
         ld2 = (uint32_t)(o.ld * 2);
         if constexpr (L == RowK) {
             const int r = 8 * wave + (lane >> 3);
-            const int c = PERM ? (lane & 7) ^ (2 * ((r >> 1) & 3)) : (lane & 7) ^ (r & 7);
+            const int c = (lane & 7) ^ (PERM ? (r >> 1) & 7 : r & 7);
             base = reinterpret_cast<const uint8_t*>(o.p + (long)x0 * o.ld + k0);
             row = r * ld2;
             col = 16 * c;
@@ -135,7 +135,7 @@ template <Lay L, int B, bool PERM> struct Reader {
         const int r16 = lane & 15, q = lane >> 4;
         if constexpr (L == RowK) {
             const int r = x0 + r16;
-            if constexpr (PERM) a = r * 128 + 8 * (q & 1) + 16 * ((q >> 1) ^ (2 * ((r >> 1) & 3)));
+            if constexpr (PERM) a = r * 128 + 8 * (q & 1) + 16 * ((q >> 1) ^ ((r >> 1) & 7));
             else a = r * 128 + 16 * (q ^ (r & 7));
         } else {
             constexpr int CH = B / 8;
@@ -244,7 +244,7 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        constexpr int BG = TN >= 8 ? 2 : 0;  // groups of the second half ahead of the barrier
+        constexpr int BG = TN >= 8 ? 1 : 0;  // groups of the second half ahead of the barrier
         using None = std::integral_constant<int, 0>;
         using Late = std::integral_constant<int, BG>;
 #pragma unroll
@@ -269,5 +269,29 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
         wkv7::vm_wait_n<0>();
     }
 };
+
+// The workgroup's tile of 16-bit values to memory, whole rows at a time: an accumulator lane holds
+// 8 bytes of a row, which stored as they are reach memory as 32-byte pieces of 16 rows (8192 x
+// 65536 exponentials at D = 640: 1080 us, and 920 by whole rows; a weight gradient of 65536 x
+// 5120 from 64 tokens 233 and 158).  Each wave turns its own tile in its own part of LDS (16-byte chunk c of row r at
+// c ^ (r mod chunks)).  pack(tn, tm): the lane's four values; put(m, n, v): eight values of row m
+// from column n, both from the workgroup's first.  The caller puts a barrier before.
+template <class P, class Pack, class Put> __device__ __forceinline__ void store_rows(uint8_t* lds, Pack pack, Put put) {
+    constexpr int CH = P::TN * 2, ROW = CH * 16;  // chunks and bytes of a row of the wave's tile
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    uint8_t* mine = lds + wave * (P::TM * 16 * ROW);
+#pragma unroll
+    for (int tm = 0; tm < P::TM; tm++)
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++)
+            *reinterpret_cast<uint2*>(mine + (16 * tm + r16) * ROW + (((2 * tn + (q >> 1)) ^ (r16 & (CH - 1))) << 4) + 8 * (q & 1)) = pack(tn, tm);
+    wkv7::wave_lds_fence();
+    const int c = lane & (CH - 1), m0 = (wave / P::WN) * P::TM * 16, n = (wave % P::WN) * P::TN * 16 + 8 * c;
+#pragma unroll
+    for (int i = 0; i < P::TM * 16 * CH / 64; i++) {
+        const int r = i * (64 / CH) + lane / CH;
+        put(m0 + r, n, *reinterpret_cast<const uint4*>(mine + r * ROW + ((c ^ (r & (CH - 1))) << 4)));
+    }
+}
 
 }  // namespace vocab

@@ -2,19 +2,20 @@
 // include/theseus_vocab.h, where the formulas are).
 //
 // Launches of one call, on the caller's stream:
-//   targets        every token's q, Q, sum q log q and weight from the labels or the teacher's logits
-//   target_logits  z at the target indices, one wave a (token, target): a dot product of width D
-//   weight_sum     MEAN: the sum of the weights (one workgroup, fixed order)
+//   targets        every token's q, Q, sum q log q and weight from the labels or the teacher's
+//                  logits; z at the target indices, one wave a (token, target)
+//   sums           MEAN with several pieces: the sum of the weights (one workgroup, fixed order)
 //   then for each piece of rows
 //     logits       z's tiles on the matrix cores; of each 256-column tile a row's maximum and sum
 //                  of exponentials are kept and, for gradients, the exponentials (float16,
 //                  2^15 e^{z - tile maximum}: 11 significant bits down to e^-20 of the maximum)
 //     rows         log-sum-exp of a row from its tiles, the row's loss
-//     probs        exponentials -> G in place (bfloat16: the one rounding of the gradients' left factor)
-//     target_probs G at the target indices, from the float32 z of target_logits: p - 1 of a
+//     sums         one piece: the reduced loss and, for MEAN, the sum of the weights
+//     probs        exponentials -> G in place (bfloat16: the one rounding of the gradients' left
+//                  factor); at the target indices from the float32 z of `targets`: p - 1 of a
 //                  confident token would be lost in a rounded p
 //     dhidden, dweight   G W and G^T H (vocab_gemm.h; float32 sums, rounded once)
-//   loss_sum       SUM, MEAN: one workgroup, fixed order
+//   sums           several pieces: the reduced loss
 //
 // The gradients take three products of 2 M V D operations, not the four of a backward that
 // forms the logits again: with SUM and MEAN the upstream gradient is one number, applied to the
@@ -53,8 +54,10 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // ---------------------------------------------------------------------------------- targets
 struct Targets {
-    long rows, vocab;
-    int K, top_bf16;
+    long pairs, vocab;
+    int K, D, top_bf16;
+    const uint16_t *x, *w;    // rows of D elements, a multiple of 64, 16-byte aligned
+    long ldx, ldw;
     const int64_t* index;
     const void* top;          // null: labels
     const float* teacher_lse;
@@ -63,89 +66,98 @@ struct Targets {
     float inv_T;
     int* j;        // [M][K] index, SKIP or BAD
     float* q;      // [M][K] (teacher only)
+    float* z;      // [M][K] z log2(e) / T at the target
     float4* row;   // [M] {Q, sum q log q, weight, 0}
 };
 
-// One wave a token.
+// One wave a (token, target): the token's q (again for each of its targets: K values against the
+// D of the dot product), then z at its own target.  The first target's wave writes the token's.
 __global__ __launch_bounds__(256) void targets_kernel(Targets t) {
-    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long p = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    if (i >= t.rows) return;
-    float weight = t.row_weight ? t.row_weight[i] : 1.f;
+    if (p >= t.pairs) return;
+    const long i = t.top ? p / t.K : p;
+    const int k0 = (int)(p - i * t.K);
     auto place = [&](int64_t v) { return v < 0 || v >= t.vocab ? BAD : (int)v; };
+    const float weight = t.row_weight ? t.row_weight[i] : 1.f;
+    int v;
     if (!t.top) {
+        const int64_t y = t.index[i];
+        v = y == t.ignore ? SKIP : place(y);
         if (lane == 0) {
-            const int64_t v = t.index[i];
-            const bool left_out = v == t.ignore;
-            t.j[i] = left_out ? SKIP : place(v);
-            t.row[i] = make_float4(1.f, 0.f, left_out ? 0.f : weight, 0.f);
+            t.j[i] = v;
+            t.row[i] = make_float4(1.f, 0.f, y == t.ignore ? 0.f : weight, 0.f);
         }
+    } else {
+        constexpr int S = THESEUS_VOCAB_MAX_TOP / 64;
+        float x[S], top = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const int k = 64 * s + lane;
+            x[s] = -INFINITY;
+            if (64 * s < t.K && k < t.K) {
+                const long at = i * t.K + k;
+                x[s] = (t.top_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(t.top)[at]) : static_cast<const float*>(t.top)[at]) * t.inv_T;
+            }
+            top = fmaxf(top, x[s]);
+        }
+        float base;
+        if (t.teacher_lse) {
+            base = t.teacher_lse[i];
+        } else {
+            // (a token of whom the teacher kept nothing has q = 0 throughout)
+            top = wave_max(top);
+            float sum = 0.f;
+#pragma unroll
+            for (int s = 0; s < S; s++)
+                if (64 * s < t.K) sum += x[s] == -INFINITY ? 0.f : expf(x[s] - top);
+            base = top + logf(wave_sum(sum));
+        }
+        if (k0 == 0) {
+            float Q = 0.f, H = 0.f;
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                const int k = 64 * s + lane;
+                if (k < t.K) {
+                    const float lq = x[s] - base, q = x[s] == -INFINITY ? 0.f : expf(lq);
+                    const long at = i * t.K + k;
+                    t.q[at] = q;
+                    t.j[at] = q == 0.f ? SKIP : place(t.index[at]);
+                    Q += q;
+                    H += q == 0.f ? 0.f : q * lq;
+                }
+            }
+            Q = wave_sum(Q);
+            H = wave_sum(H);
+            if (lane == 0) t.row[i] = make_float4(Q, H, weight, 0.f);
+        }
+        float own = x[0];
+#pragma unroll
+        for (int s = 1; s < S; s++) own = s == k0 >> 6 ? x[s] : own;
+        own = __shfl(own, k0 & 63, 64);
+        v = own == -INFINITY || expf(own - base) == 0.f ? SKIP : place(t.index[p]);
+    }
+    if (v < 0) {
+        if (lane == 0) t.z[p] = v == BAD ? NAN : 0.f;
         return;
     }
-    float x[THESEUS_VOCAB_MAX_TOP / 64], top = -INFINITY;
-    for (int s = 0; s < THESEUS_VOCAB_MAX_TOP / 64; s++) {
-        const int k = 64 * s + lane;
-        x[s] = -INFINITY;
-        if (k < t.K) {
-            const long at = i * t.K + k;
-            x[s] = (t.top_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(t.top)[at]) : static_cast<const float*>(t.top)[at]) * t.inv_T;
-        }
-        top = fmaxf(top, x[s]);
+    const uint4* a = reinterpret_cast<const uint4*>(t.x + i * t.ldx);
+    const uint4* b = reinterpret_cast<const uint4*>(t.w + (long)v * t.ldw);
+    float s = 0.f;
+#pragma unroll 4
+    for (int c = lane; c < t.D / 8; c += 64) {
+        const uint4 u = a[c], y = b[c];
+        auto two = [&](uint32_t m, uint32_t n) {
+            s += __uint_as_float(m << 16) * __uint_as_float(n << 16);
+            s += __uint_as_float(m & 0xffff0000u) * __uint_as_float(n & 0xffff0000u);
+        };
+        two(u.x, y.x);
+        two(u.y, y.y);
+        two(u.z, y.z);
+        two(u.w, y.w);
     }
-    top = wave_max(top);
-    float sum = 0.f, base;
-    if (t.teacher_lse) {
-        base = t.teacher_lse[i];
-    } else {
-        // (a token of whom the teacher kept nothing has q = 0 throughout)
-        for (int s = 0; s < THESEUS_VOCAB_MAX_TOP / 64; s++) sum += x[s] == -INFINITY ? 0.f : expf(x[s] - top);
-        sum = wave_sum(sum);
-        base = top + logf(sum);
-    }
-    float Q = 0.f, H = 0.f;
-    for (int s = 0; s < THESEUS_VOCAB_MAX_TOP / 64; s++) {
-        const int k = 64 * s + lane;
-        if (k < t.K) {
-            const float lq = x[s] - base, q = x[s] == -INFINITY ? 0.f : expf(lq);
-            const long at = i * t.K + k;
-            t.q[at] = q;
-            t.j[at] = q == 0.f ? SKIP : place(t.index[at]);
-            Q += q;
-            H += q == 0.f ? 0.f : q * lq;
-        }
-    }
-    Q = wave_sum(Q);
-    H = wave_sum(H);
-    if (lane == 0) t.row[i] = make_float4(Q, H, weight, 0.f);
-}
-
-// z log2(e) / T at the target indices, one wave a (token, target); D a multiple of 64, rows 16-byte aligned.
-__global__ __launch_bounds__(256) void target_logits(long pairs, int K, int D, const uint16_t* x, long ldx, const uint16_t* w,
-                                                     long ldw, const int* j, float scale, float* z) {
-    const int lane = threadIdx.x & 63;
-    for (long p = (long)blockIdx.x * 4 + (threadIdx.x >> 6); p < pairs; p += (long)gridDim.x * 4) {
-        const int v = j[p];
-        if (v < 0) {
-            if (lane == 0) z[p] = v == BAD ? NAN : 0.f;
-            continue;
-        }
-        const uint4* a = reinterpret_cast<const uint4*>(x + (p / K) * ldx);
-        const uint4* b = reinterpret_cast<const uint4*>(w + (long)v * ldw);
-        float s = 0.f;
-        for (int c = lane; c < D / 8; c += 64) {
-            const uint4 u = a[c], y = b[c];
-            auto two = [&](uint32_t m, uint32_t n) {
-                s += __uint_as_float(m << 16) * __uint_as_float(n << 16);
-                s += __uint_as_float(m & 0xffff0000u) * __uint_as_float(n & 0xffff0000u);
-            };
-            two(u.x, y.x);
-            two(u.y, y.y);
-            two(u.z, y.z);
-            two(u.w, y.w);
-        }
-        s = wave_sum(s);
-        if (lane == 0) z[p] = s * scale;
-    }
+    s = wave_sum(s);
+    if (lane == 0) t.z[p] = s * (LOG2E * t.inv_T);
 }
 
 // sum over 1024 threads in a fixed order, valid in thread 0
@@ -158,19 +170,23 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
         for (int k = 0; k < 16; k++) s += red[k];
     return s;
 }
-__global__ __launch_bounds__(1024) void weight_sum(long rows, const float4* row, float* out) {
-    __shared__ double red[16];
-    double s = 0.0;
-    for (long i = threadIdx.x; i < rows; i += 1024) s += row[i].z;
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) *out = s == 0.0 ? 0.f : (float)(1.0 / s);
-}
-__global__ __launch_bounds__(1024) void loss_sum(long rows, const float* losses, const float* inv_weight, float* out) {
-    __shared__ double red[16];
-    double s = 0.0;
-    for (long i = threadIdx.x; i < rows; i += 1024) s += losses[i];
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) *out = (float)(inv_weight ? s * *inv_weight : s);
+// MEAN: *inv = 1 / sum of the weights (0 where that is 0); with losses, *out = their sum, times
+// *inv for MEAN.
+__global__ __launch_bounds__(1024) void sums_kernel(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
+    __shared__ double red[2][16];
+    double w = 0.0, s = 0.0;
+#pragma unroll 4
+    for (long i = threadIdx.x; i < rows; i += 1024) {
+        if (mean) w += row[i].z;
+        if (losses) s += losses[i];
+    }
+    if (mean) w = block_sum(w, red[0]);
+    s = block_sum(s, red[1]);
+    if (threadIdx.x == 0) {
+        const double f = !mean ? 1.0 : w == 0.0 ? 0.0 : 1.0 / w;
+        if (inv) *inv = (float)f;
+        if (out) *out = (float)(s * f);
+    }
 }
 
 // ---------------------------------------------------------------------------------- logits
@@ -194,20 +210,23 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
     const int wm = wave / P::WN, wn = wave % P::WN;
     const int mw = wm * P::TM * 16 + r16, nw = n0 + wn * P::TN * 16 + 4 * q;
     float* red = reinterpret_cast<float*>(lds);  // [2][WN][BM]
-    float top[P::TM];
-    const bool edge = n0 + P::BN > o.N;
-#pragma unroll
-    for (int tm = 0; tm < P::TM; tm++) {
-        top[tm] = -INFINITY;
+    if (n0 + P::BN > o.N) {
 #pragma unroll
         for (int tn = 0; tn < P::TN; tn++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float z = g.acc[tn][tm][e] * o.scale;
-                if (edge && nw + 16 * tn + e >= o.N) z = -INFINITY;
-                g.acc[tn][tm][e] = z;
-                top[tm] = fmaxf(top[tm], z);
-            }
+            for (int e = 0; e < 4; e++)
+                if (nw + 16 * tn + e >= o.N)
+#pragma unroll
+                    for (int tm = 0; tm < P::TM; tm++) g.acc[tn][tm][e] = -INFINITY;
+    }
+    float top[P::TM];
+#pragma unroll
+    for (int tm = 0; tm < P::TM; tm++) {
+        top[tm] = g.acc[0][tm][0];
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top[tm] = fmaxf(top[tm], g.acc[tn][tm][e]);
         top[tm] = fmaxf(top[tm], __shfl_xor(top[tm], 16, 64));
         top[tm] = fmaxf(top[tm], __shfl_xor(top[tm], 32, 64));
     }
@@ -222,13 +241,14 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
         float all = red[m];
 #pragma unroll
         for (int w = 1; w < P::WN; w++) all = fmaxf(all, red[w * P::BM + m]);
+        all *= o.scale;
         const float shift = E_SHIFT - all;
         float sum = 0.f;
 #pragma unroll
         for (int tn = 0; tn < P::TN; tn++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float x = exp2_(g.acc[tn][tm][e] + shift);
+                const float x = exp2_(fmaf(g.acc[tn][tm][e], o.scale, shift));
                 g.acc[tn][tm][e] = x;
                 sum += x;
             }
@@ -250,23 +270,14 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
             }
         }
     if constexpr (KEEP) {
-#pragma unroll
-        for (int tm = 0; tm < P::TM; tm++) {
-            const int m = m0 + mw + 16 * tm;
-            if (m < o.M) {
-                uint16_t* row = o.e + (long)m * o.lde;
-#pragma unroll
-                for (int tn = 0; tn < P::TN; tn++) {
-                    const int n = nw + 16 * tn;
-                    if (n < o.Ne) {
-                        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-                        const f32x4_t a = g.acc[tn][tm];
-                        const h4 h = {(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]};
-                        *reinterpret_cast<uint2*>(row + n) = __builtin_bit_cast(uint2, h);
-                    }
-                }
-            }
-        }
+        __syncthreads();
+        store_rows<P>(lds, [&](int tn, int tm) {
+            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+            const f32x4_t a = g.acc[tn][tm];
+            return __builtin_bit_cast(uint2, h4{(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]});
+        }, [&](int m, int n, uint4 v) {
+            if (m0 + m < o.M && n0 + n < o.Ne) *reinterpret_cast<uint4*>(o.e + (long)(m0 + m) * o.lde + n0 + n) = v;
+        });
     }
 }
 
@@ -311,8 +322,8 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows p) {
 
 // ---------------------------------------------------------------------------------- G
 struct Probs {
-    int rows, M;            // rows of the piece (padded to 64: zeros), its tokens
-    int tiles, K;
+    int M, K;               // the piece's tokens (its rows up to a multiple of 64 become zeros)
+    int tiles, cols;        // logits tiles of a row, columns of one (a power of two)
     long lde;
     uint16_t* e;
     const float2* part;
@@ -329,51 +340,46 @@ __device__ __forceinline__ float row_factor(const Probs& p, long i) {  // T c_i
     if (p.row_grad) c *= p.row_grad[i];
     return p.T * c;
 }
-// blockIdx.x: 2048 columns of row blockIdx.y; 8 columns a thread
+// blockIdx.x: 2048 columns of row blockIdx.y; 8 columns a thread, then the targets among them
 __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
     const long i = blockIdx.y;
-    const int n = (blockIdx.x * 256 + threadIdx.x) * 8;
-    if (n >= p.lde) return;
-    uint4* at = reinterpret_cast<uint4*>(p.e + i * p.lde + n);
-    float f = 0.f;
-    if (i < p.M) {
-        f = row_factor(p, i);
-        if (f != 0.f) f *= p.row[i].x * p.norm[i].y * exp2_(p.part[i * p.tiles + n / BN_LOGITS].x - p.norm[i].x);
-    }
+    const int n0 = blockIdx.x * 2048, n = n0 + threadIdx.x * 8;
+    uint16_t* row = p.e + i * p.lde;
+    const float f = i < p.M ? row_factor(p, i) : 0.f;
+    uint4* at = reinterpret_cast<uint4*>(row + n);
     if (f == 0.f) {
-        *at = make_uint4(0, 0, 0, 0);
+        if (n < p.lde) *at = make_uint4(0, 0, 0, 0);
         return;
     }
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    uint4 u = *at;
-    auto two = [&](uint32_t& x) {
-        const h2 h = __builtin_bit_cast(h2, x);
-        x = f32x2_to_bf16x2((float)h[0] * f, (float)h[1] * f);
-    };
-    two(u.x);
-    two(u.y);
-    two(u.z);
-    two(u.w);
-    *at = u;
-}
-// one thread a (token, target); equal indices of one token write the same value
-__global__ __launch_bounds__(256) void target_probs(Probs p) {
-    const long at = (long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (long)p.M * p.K) return;
-    const long i = at / p.K;
-    const int v = p.j[at];
-    if (v < 0) return;
-    const float f = row_factor(p, i);
-    float g = 0.f;
-    if (f != 0.f) {
-        float q = 0.f;
-        if (!p.q) q = 1.f;
-        else
-            for (int k = 0; k < p.K; k++)
-                if (p.j[i * p.K + k] == v) q += p.q[i * p.K + k];
-        g = f * (p.row[i].x * (exp2_(p.z[at] - p.norm[i].x + E_SHIFT) * p.norm[i].y) - q);
+    const float Q = p.row[i].x;
+    const float2 norm = p.norm[i];
+    if (n < p.lde) {
+        const float g = f * Q * norm.y * exp2_(p.part[i * p.tiles + n / p.cols].x - norm.x);
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        uint4 u = *at;
+        auto two = [&](uint32_t& x) {
+            const h2 h = __builtin_bit_cast(h2, x);
+            x = f32x2_to_bf16x2((float)h[0] * g, (float)h[1] * g);
+        };
+        two(u.x);
+        two(u.y);
+        two(u.z);
+        two(u.w);
+        *at = u;
     }
-    p.e[i * p.lde + v] = f32_to_bf16(g);
+    __syncthreads();
+    if (threadIdx.x < p.K) {  // (equal indices of one token write the same value)
+        const long t = i * p.K + threadIdx.x;
+        const int v = p.j[t];
+        if (v >= n0 && v < n0 + 2048) {
+            float q = 0.f;
+            if (!p.q) q = 1.f;
+            else
+                for (int k = 0; k < p.K; k++)
+                    if (p.j[i * p.K + k] == v) q += p.q[i * p.K + k];
+            row[v] = f32_to_bf16(f * (Q * (exp2_(p.z[t] - norm.x + E_SHIFT) * norm.y) - q));
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------- gradients
@@ -397,38 +403,40 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
     g.run(lds, X, Y, m0, n0, s0, min(t.steps, t.all - s0));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
     const int mw = m0 + (wave / P::WN) * P::TM * 16 + r16, nw = n0 + (wave % P::WN) * P::TN * 16 + 4 * q;
-    const bool four = (o.ldc & 3) == 0;  // (a row of C starts on 8 bytes)
+    if constexpr (MODE != OutBf16) {
 #pragma unroll
-    for (int tm = 0; tm < P::TM; tm++) {
-        const long m = mw + 16 * tm;
-        if (m >= o.M) continue;
+        for (int tm = 0; tm < P::TM; tm++) {
+            const long m = mw + 16 * tm;
 #pragma unroll
-        for (int tn = 0; tn < P::TN; tn++) {
-            const int n = nw + 16 * tn;
-            if (n >= o.N) continue;
-            f32x4_t a = g.acc[tn][tm];
-            if constexpr (MODE == OutPart) {
-                *reinterpret_cast<f32x4_t*>(o.f + ((long)at.part * o.M + m) * o.ldf + n) = a;
-                continue;
-            }
-            if constexpr (MODE == OutAdd) {
-                f32x4_t* f = reinterpret_cast<f32x4_t*>(o.f + m * o.ldf + n);
-                if (!o.first) a += *f;
-                if (!o.last) {
-                    *f = a;
-                    continue;
+            for (int tn = 0; tn < P::TN; tn++) {
+                const int n = nw + 16 * tn;
+                if (m >= o.M || n >= o.N) continue;
+                if constexpr (MODE == OutPart) {
+                    *reinterpret_cast<f32x4_t*>(o.f + ((long)at.part * o.M + m) * o.ldf + n) = g.acc[tn][tm];
+                } else {
+                    f32x4_t* f = reinterpret_cast<f32x4_t*>(o.f + m * o.ldf + n);
+                    if (!o.first) g.acc[tn][tm] += *f;
+                    if (!o.last) *f = g.acc[tn][tm];
                 }
             }
-            uint16_t* c = o.c + m * o.ldc + n;
-            const uint2 u = make_uint2(f32x2_to_bf16x2(a[0], a[1]), f32x2_to_bf16x2(a[2], a[3]));
-            if (four) {  // (N is a multiple of 4 then too)
-                *reinterpret_cast<uint2*>(c) = u;
-            } else {
-                const uint32_t w[2] = {u.x, u.y};
-                for (int e = 0; e < 4 && n + e < o.N; e++) c[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-            }
         }
+        if (MODE == OutPart || !o.last) return;
     }
+    __syncthreads();
+    const bool eight = (o.ldc & 7) == 0 && ((uintptr_t)o.c & 15) == 0;  // (N = ldc: eight columns are in or out together)
+    store_rows<P>(lds, [&](int tn, int tm) {
+        const f32x4_t a = g.acc[tn][tm];
+        return make_uint2(f32x2_to_bf16x2(a[0], a[1]), f32x2_to_bf16x2(a[2], a[3]));
+    }, [&](int m, int n, uint4 v) {
+        if (m0 + m >= o.M || n0 + n >= o.N) return;
+        uint16_t* c = o.c + (long)(m0 + m) * o.ldc + n0 + n;
+        if (eight) {
+            *reinterpret_cast<uint4*>(c) = v;
+        } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            for (int e = 0; e < 8 && n0 + n + e < o.N; e++) c[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        }
+    });
 }
 // the parts of a contraction added in order, 4 columns a thread
 __global__ __launch_bounds__(256) void add_parts(int M, int N, int splits, const float* f, long ldf, uint16_t* c, long ldc) {
@@ -447,18 +455,22 @@ __global__ __launch_bounds__(256) void pad_rows(long rows, int D, int Dp, const 
     for (long i = blockIdx.y; i < rows; i += gridDim.y) out[i * Dp + c] = c < D ? x[i * ld + c] : 0;
 }
 
-__global__ __launch_bounds__(256) void scale_kernel(uint16_t* x, long n, const float* factor) {
+__global__ __launch_bounds__(256) void scale_kernel(uint16_t* x, long nx, uint16_t* y, long ny, const float* factor) {
     const float f = *factor;
     if (f == 1.f) return;
-    const bool wide = ((uintptr_t)x & 15) == 0;
-    const long n8 = wide ? n / 8 : 0, step = (long)gridDim.x * 256, first = (long)blockIdx.x * 256 + threadIdx.x;
+    const long step = (long)gridDim.x * 256, first = (long)blockIdx.x * 256 + threadIdx.x;
     auto two = [&](uint32_t u) { return f32x2_to_bf16x2(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f); };
-    for (long i = first; i < n8; i += step) {
-        uint4 u = reinterpret_cast<uint4*>(x)[i];
-        u = make_uint4(two(u.x), two(u.y), two(u.z), two(u.w));
-        reinterpret_cast<uint4*>(x)[i] = u;
-    }
-    for (long i = 8 * n8 + first; i < n; i += step) x[i] = f32_to_bf16(bf16_to_f32(x[i]) * f);
+    auto all = [&](uint16_t* v, long n) {
+        const long n8 = ((uintptr_t)v & 15) == 0 ? n / 8 : 0;
+        for (long i = first; i < n8; i += step) {
+            uint4 u = reinterpret_cast<uint4*>(v)[i];
+            u = make_uint4(two(u.x), two(u.y), two(u.z), two(u.w));
+            reinterpret_cast<uint4*>(v)[i] = u;
+        }
+        for (long i = 8 * n8 + first; i < n; i += step) v[i] = f32_to_bf16(bf16_to_f32(v[i]) * f);
+    };
+    all(x, nx);
+    all(y, ny);
 }
 
 __global__ __launch_bounds__(256) void zero_kernel(uint16_t* x, long n) {
@@ -554,7 +566,7 @@ static Tiles tiles(long M, long N, int BM, int BN, long K, int splits) {
     t.all = (int)(K / BK);
     t.steps = (int)ceil_div(t.all, splits);
     t.splits = (int)ceil_div(t.all, t.steps);
-    t.group = t.m < 8 ? t.m : 8;
+    t.group = t.m < 4 ? t.m : 4;
     return t;
 }
 
@@ -575,7 +587,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
     long ldh = a->hidden_stride, ldw = a->weight_stride;
     const float inv_T = 1.f / a->temperature;
     if (p.M == 0) {
-        if (reduce) loss_sum<<<1, 1024, 0, st>>>(0, nullptr, nullptr, a->loss);
+        if (reduce) sums_kernel<<<1, 1024, 0, st>>>(0, nullptr, 0, nullptr, nullptr, a->loss);
         if (a->dweight) zero_kernel<<<1024, 256, 0, st>>>(static_cast<uint16_t*>(a->dweight), p.V * p.D);
         return 0;
     }
@@ -586,13 +598,15 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         pad_rows<<<dim3(gx, (unsigned)(p.V < 32768 ? p.V : 32768)), 256, 0, st>>>(p.V, (int)p.D, (int)p.Dp, W, ldw, w);
         H = h, W = w, ldh = ldw = p.Dp;
     }
-    Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight,
-              a->ignore_index, inv_T, j, q, row};
-    targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
     const long pairs = p.M * p.K;
-    target_logits<<<(unsigned)(ceil_div(pairs, 4) < 65536 ? ceil_div(pairs, 4) : 65536), 256, 0, st>>>(
-        pairs, (int)p.K, (int)p.Dp, H, ldh, W, ldw, j, LOG2E * inv_T, z);
-    if (inv) weight_sum<<<1, 1024, 0, st>>>(p.M, row, inv);
+    const Targets t{pairs, p.V, (int)p.K, (int)p.Dp, a->top_dtype == THESEUS_VOCAB_BF16, H, W, ldh, ldw, a->index, a->top_values,
+                    a->teacher_lse, a->row_weight, a->ignore_index, inv_T, j, q, z, row};
+    targets_kernel<<<(unsigned)ceil_div(pairs, 4), 256, 0, st>>>(t);
+    const bool mean = inv != nullptr;
+    auto sums = [&](float* to, const float* from, float* out) {
+        sums_kernel<<<1, 1024, 0, st>>>(p.M, row, mean, to, from, out);
+    };
+    if (mean && p.grads && p.pieces > 1) sums(inv, nullptr, nullptr);
 
     for (int piece = 0; piece < p.pieces; piece++) {
         const long i0 = piece * p.piece, m = p.M - i0 < p.piece ? p.M - i0 : p.piece;
@@ -610,13 +624,13 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         const Rows rw{m, p.tiles, (int)p.K, part, row + i0, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
                       a->temperature * a->temperature, norm, losses ? losses + i0 : nullptr};
         rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
+        if (p.pieces == 1 && (reduce || (mean && p.grads))) sums(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
         if (!p.grads) continue;
 
         const long mp = up(m, BK);
-        const Probs pr{(int)mp, (int)m, p.tiles, (int)p.K, p.lde, e, part, row + i0, norm, inv,
+        const Probs pr{(int)m, (int)p.K, p.tiles, BN_LOGITS, p.lde, e, part, row + i0, norm, inv,
                        a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, a->temperature};
         probs_kernel<<<dim3((unsigned)ceil_div(p.lde, 2048), (unsigned)mp), 256, 0, st>>>(pr);
-        target_probs<<<(unsigned)ceil_div(m * p.K, 256), 256, 0, st>>>(pr);
         if (a->dhidden) {
             uint16_t* dh = static_cast<uint16_t*>(a->dhidden) + i0 * p.D;
             const Operand GX{e, p.lde, (int)m, (int)p.lde}, WY{W, ldw, (int)p.Dp, (int)p.V};
@@ -639,7 +653,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
             else grad_kernel<Dweight, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
         }
     }
-    if (reduce) loss_sum<<<1, 1024, 0, st>>>(p.M, losses, inv, a->loss);
+    if (reduce && p.pieces > 1) sums(nullptr, losses, a->loss);
     return 0;
 }
 
@@ -660,12 +674,13 @@ int theseus_vocab_loss(const theseus_vocab_loss_args* a, void* workspace, size_t
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }
 
-int theseus_vocab_scale(void* x, long long n, const float* factor, hipStream_t stream) {
-    if (n < 0) return THESEUS_WKV7_ERR_SHAPE;
-    if (!x || !factor) return THESEUS_WKV7_ERR_NULL;
-    if (!n) return THESEUS_WKV7_OK;
-    const long blocks = vocab::ceil_div(n, 8 * 256);
-    vocab::scale_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(static_cast<uint16_t*>(x), n, factor);
+int theseus_vocab_scale(void* x, long long nx, void* y, long long ny, const float* factor, hipStream_t stream) {
+    if (nx < 0 || ny < 0) return THESEUS_WKV7_ERR_SHAPE;
+    if ((nx && !x) || (ny && !y) || !factor) return THESEUS_WKV7_ERR_NULL;
+    if (!nx && !ny) return THESEUS_WKV7_OK;
+    const long blocks = vocab::ceil_div(nx > ny ? nx : ny, 8 * 256);
+    vocab::scale_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(static_cast<uint16_t*>(x), nx,
+                                                                                       static_cast<uint16_t*>(y), ny, factor);
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }
 

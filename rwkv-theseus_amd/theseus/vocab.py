@@ -55,7 +55,7 @@ def _lib():
         lib.theseus_vocab_loss_workspace_size.restype = sz
         lib.theseus_vocab_loss.argtypes = [ctypes.POINTER(LossArgs), vp, sz, vp]
         lib.theseus_vocab_loss.restype = i32
-        lib.theseus_vocab_scale.argtypes = [vp, i64, vp, vp]
+        lib.theseus_vocab_scale.argtypes = [vp, i64, vp, i64, vp, vp]
         lib.theseus_vocab_scale.restype = i32
         lib.theseus_vocab_top_workspace_size.argtypes = [i64, i64, i32, i32]
         lib.theseus_vocab_top_workspace_size.restype = sz
@@ -132,11 +132,9 @@ class _Loss(torch.autograd.Function):
                 call.run(hidden, weight, None, grad, *made)
                 return (*made, None)
             call.run(hidden, weight, None, None, *made)
-        lib = _lib()
+        xy = [v for x in made for v in ((None, 0) if x is None else (x.data_ptr(), x.numel()))]
         with torch.cuda.device(call.device):
-            for x in made:
-                if x is not None and x.numel():
-                    _check(lib.theseus_vocab_scale(x.data_ptr(), x.numel(), grad.data_ptr(), _stream(call.device)))
+            _check(_lib().theseus_vocab_scale(*xy, grad.data_ptr(), _stream(call.device)))
         return (*made, None)
 
 

@@ -462,7 +462,8 @@ def test_c_abi_refuses_without_launching():
     assert call(hidden=None) == 3 and call(index=None) == 3
     assert call(p, size() - 1) == 4 and call(None, size()) == 4
     assert lib.theseus_vocab_loss(None, None, 0, None) == 3
-    assert lib.theseus_vocab_scale(None, 1, p, None) == 3 and lib.theseus_vocab_scale(p, -1, p, None) == 1
+    assert lib.theseus_vocab_scale(None, 1, None, 0, p, None) == 3 and lib.theseus_vocab_scale(p, -1, None, 0, p, None) == 1
+    assert lib.theseus_vocab_scale(None, 0, None, 0, p, None) == 0 and lib.theseus_vocab_scale(p, 1, p, 1, None, None) == 3
     top = lambda M=2, V=100, k=5, dt=1, T=1.0, x=p, ld=100, v=p, i=p, ws=None, n=0: lib.theseus_vocab_top(  # noqa: E731
         M, V, k, dt, T, x, ld, v, i, None, ws, n, None)
     for bad in (dict(M=-1), dict(V=0), dict(k=0), dict(k=101), dict(V=1000, ld=1000, k=257), dict(ld=99), dict(T=0.0), dict(x=p + 2)):
