@@ -1,6 +1,6 @@
 // The operator's autograd functions as native torch nodes (Python module theseus._native).
 //
-// theseus/wkv7.py's _WKV and theseus/gdn.py's _GDN do the same through Python: contiguous
+// theseus/wkv7.py's _WKV, theseus/gdn.py's _GDN and theseus/vocab.py's _Loss do the same through Python: contiguous
 // inputs, the checks of kernels/wkv7_state.cpp:10-15, outputs and workspace from torch's
 // allocator, one C-ABI call on the current stream.  For few tokens that host work is the
 // call: a forward+backward through the Python functions takes 225 us of host time (B=1, T=64,
@@ -15,7 +15,10 @@
 #include <cstdlib>
 #include <cstring>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include "../../include/theseus_gdn_ex.h"
+#include "../../include/theseus_vocab.h"
 #include "../../include/theseus_wkv7.h"
 
 namespace py = pybind11;
@@ -234,10 +237,120 @@ std::pair<Tensor, Tensor> gdn(const Tensor& q, const Tensor& k, const Tensor& v,
     return {o[0], o[1]};
 }
 
+// theseus.vocab's losses: the arguments as theseus/vocab.py's _loss has checked and laid them out
+// (h [M][D] and w [V][D] with rows apart, the others contiguous).
+struct VocabLoss : torch::autograd::Function<VocabLoss> {
+    using Opt = std::optional<Tensor>;
+    static void* optr(const Opt& t) { return t ? t->data_ptr() : nullptr; }
+    static void call(const Tensor& h, const Tensor& w, const Tensor& index, const Opt& top, const Opt& lse, const Opt& weight,
+                     int64_t ignore, double T, int64_t reduction, int64_t piece, const Tensor& loss, const Tensor& row_grad,
+                     const Tensor& dh, const Tensor& dw) {
+        theseus_vocab_loss_args a{};
+        a.rows = h.size(0), a.vocab = w.size(0), a.width = (int)h.size(1), a.targets = top ? (int)top->size(1) : 1;
+        a.hidden = h.data_ptr(), a.weight = w.data_ptr();
+        a.hidden_stride = std::max(h.stride(0), h.size(1)), a.weight_stride = std::max(w.stride(0), w.size(1));
+        a.index = index.data_ptr<int64_t>(), a.top_values = optr(top);
+        a.top_dtype = top && top->scalar_type() == torch::kFloat32 ? THESEUS_VOCAB_FP32 : THESEUS_VOCAB_BF16;
+        a.reduction = (int)reduction, a.teacher_lse = static_cast<float*>(optr(lse)), a.row_weight = static_cast<float*>(optr(weight));
+        a.ignore_index = ignore, a.temperature = (float)T, a.loss = fptr(loss), a.row_grad = fptr(row_grad);
+        a.dhidden = ptr(dh), a.dweight = ptr(dw), a.piece_rows = piece;
+        const size_t need = theseus_vocab_loss_workspace_size(&a);
+        const Tensor ws = scratch(need, h);
+        raise_status(theseus_vocab_loss(&a, ptr(ws), need, stream_of(h)), "theseus_vocab");
+    }
+    static Tensor new_loss(const Tensor& h, int64_t reduction) {
+        const auto f = h.options().dtype(torch::kFloat32);
+        return reduction == THESEUS_VOCAB_NONE ? at::empty({h.size(0)}, f) : at::empty({}, f);
+    }
+    static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& index, const Opt& top, const Opt& lse,
+                          const Opt& weight, int64_t ignore, double T, int64_t reduction, int64_t piece) {
+        c10::OptionalDeviceGuard guard(h.device());
+        const Tensor loss = new_loss(h, reduction);
+        Tensor dh, dw;
+        if (reduction != THESEUS_VOCAB_NONE) {
+            if (h.requires_grad()) dh = at::empty(h.sizes(), h.options());
+            if (w.requires_grad()) dw = at::empty(w.sizes(), w.options());
+            ctx->saved_data["made"] = true;
+            ctx->saved_data["dh"] = dh.defined() ? at::IValue(dh) : at::IValue();
+            ctx->saved_data["dw"] = dw.defined() ? at::IValue(dw) : at::IValue();
+        } else {
+            ctx->saved_data["made"] = false;
+        }
+        call(h, w, index, top, lse, weight, ignore, T, reduction, piece, loss, Tensor(), dh, dw);
+        ctx->save_for_backward({h, w});
+        ctx->saved_data["index"] = index;
+        ctx->saved_data["top"] = top, ctx->saved_data["lse"] = lse, ctx->saved_data["weight"] = weight;
+        ctx->saved_data["ignore"] = ignore, ctx->saved_data["T"] = T, ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["piece"] = piece;
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        auto& d = ctx->saved_data;
+        auto tensor = [](at::IValue& v) { return v.isTensor() ? v.toTensor() : Tensor(); };
+        Tensor dh, dw;
+        const Tensor grad = float_rows(g[0]);
+        const int64_t reduction = d["reduction"].toInt();
+        c10::OptionalDeviceGuard guard(grad.device());
+        const bool made = d["made"].toBool();
+        if (made) {  // the gradients of upstream gradient 1, handed out once
+            dh = tensor(d["dh"]), dw = tensor(d["dw"]);
+            d["made"] = false, d["dh"] = at::IValue(), d["dw"] = at::IValue();
+        } else {
+            const variable_list s = ctx->get_saved_variables();
+            if (ctx->needs_input_grad(0)) dh = at::empty(s[0].sizes(), s[0].options());
+            if (ctx->needs_input_grad(1)) dw = at::empty(s[1].sizes(), s[1].options());
+            auto opt = [&](const char* k) { return d[k].isTensor() ? Opt(d[k].toTensor()) : Opt(); };
+            call(s[0], s[1], d["index"].toTensor(), opt("top"), opt("lse"), opt("weight"), d["ignore"].toInt(), d["T"].toDouble(),
+                 reduction, d["piece"].toInt(), Tensor(), reduction == THESEUS_VOCAB_NONE ? grad : Tensor(), dh, dw);
+        }
+        if (reduction != THESEUS_VOCAB_NONE)
+            raise_status(theseus_vocab_scale(ptr(dh), dh.defined() ? dh.numel() : 0, ptr(dw), dw.defined() ? dw.numel() : 0, fptr(grad),
+                                             stream_of(grad)),
+                         "theseus_vocab");
+        variable_list o{dh, dw};
+        if (at::GradMode::is_enabled()) {  // (create_graph: a later derivative through these raises)
+            for (Tensor& t : o)
+                if (t.defined()) t.requires_grad_();
+            o = (*std::make_shared<torch::autograd::DelayedError>("theseus_vocab: the losses are differentiable once", 2))(std::move(o));
+        }
+        o.resize(10);
+        return o;
+    }
+};
+
+Tensor vocab_loss(const Tensor& h, const Tensor& w, const Tensor& index, const std::optional<Tensor>& top, const std::optional<Tensor>& lse,
+                  const std::optional<Tensor>& weight, int64_t ignore, double T, int64_t reduction, int64_t piece) {
+    py::gil_scoped_release free;
+    if (at::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad()))
+        return VocabLoss::apply(h, w, index, top, lse, weight, ignore, T, reduction, piece);
+    c10::OptionalDeviceGuard guard(h.device());
+    const Tensor loss = VocabLoss::new_loss(h, reduction);
+    VocabLoss::call(h, w, index, top, lse, weight, ignore, T, reduction, piece, loss, Tensor(), Tensor(), Tensor());
+    return loss;
+}
+
+// theseus.vocab.top_logits for x [M][V], checked there: values, indices, lse of M rows
+std::tuple<Tensor, Tensor, Tensor> vocab_top(const Tensor& x, int64_t k, double T) {
+    py::gil_scoped_release free;
+    c10::OptionalDeviceGuard guard(x.device());
+    const int64_t M = x.size(0), V = x.size(1);
+    const int dt = x.scalar_type() == torch::kBFloat16 ? THESEUS_VOCAB_BF16 : THESEUS_VOCAB_FP32;
+    const Tensor values = at::empty({M, k}, x.options()), indices = at::empty({M, k}, x.options().dtype(torch::kInt64)),
+                 lse = at::empty({M}, x.options().dtype(torch::kFloat32));
+    const size_t need = theseus_vocab_top_workspace_size(M, V, (int)k, dt);
+    const Tensor ws = scratch(need, x);
+    raise_status(theseus_vocab_top(M, V, (int)k, dt, (float)T, x.data_ptr(), std::max(x.stride(0), V), values.data_ptr(),
+                                   indices.data_ptr<int64_t>(), fptr(lse), ptr(ws), need, stream_of(x)),
+                 "theseus_vocab");
+    return {values, indices, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("wkv7", &wkv7, "(y, end state) of the recurrence, differentiable");
     m.def("gdn", &gdn, "(o, end state) of the gated delta rule with gradients, differentiable", py::arg("q"),
           py::arg("k"), py::arg("v"), py::arg("g"), py::arg("beta"), py::arg("s0"), py::arg("qk_l2norm") = false);
+    m.def("vocab_loss", &vocab_loss, "a vocabulary loss, differentiable in h and w");
+    m.def("vocab_top", &vocab_top, "(values, indices, log-sum-exp) of the top logits");
 }

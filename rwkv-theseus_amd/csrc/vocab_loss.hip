@@ -37,7 +37,6 @@ using wkv7::f32x2_to_bf16x2;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float E_SHIFT = 15.f;  // kept exponentials are 2^15 e^{z - max}
-constexpr int BN_LOGITS = 256;   // columns of a logits tile
 constexpr int SKIP = -1, BAD = -2;
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -194,6 +193,7 @@ struct LogitsOut {
     int M, N, Ne;     // rows, vocabulary, columns kept (Ne >= N, zero beyond N)
     float scale;      // log2(e) / T
     float2* part;     // [M][tiles] {maximum, sum of 2^15 exp} of a tile, base 2
+    int tiles;
     uint16_t* e;      // [..][lde]
     long lde;
 };
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
                 float sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < P::WN; w++) sum += red[(P::WN + w) * P::BM + m];
-                o.part[(long)(m0 + m) * t.n + at.n] = make_float2(top[tm], sum);
+                o.part[(long)(m0 + m) * o.tiles + at.n] = make_float2(top[tm], sum);
             }
         }
     if constexpr (KEEP) {
@@ -323,7 +323,8 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows p) {
 // ---------------------------------------------------------------------------------- G
 struct Probs {
     int M, K;               // the piece's tokens (its rows up to a multiple of 64 become zeros)
-    int tiles, cols;        // logits tiles of a row, columns of one (a power of two)
+    int tiles;              // logits tiles of a row: main / cols of `cols` columns, then of `rest`
+    int main, cols, rest;
     long lde;
     uint16_t* e;
     const float2* part;
@@ -354,7 +355,8 @@ __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
     const float Q = p.row[i].x;
     const float2 norm = p.norm[i];
     if (n < p.lde) {
-        const float g = f * Q * norm.y * exp2_(p.part[i * p.tiles + n / p.cols].x - norm.x);
+        const int tile = n < p.main ? n / p.cols : p.main / p.cols + (n - p.main) / p.rest;
+        const float g = f * Q * norm.y * exp2_(p.part[i * p.tiles + tile].x - norm.x);
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         uint4 u = *at;
         auto two = [&](uint32_t& x) {
@@ -478,10 +480,31 @@ __global__ __launch_bounds__(256) void zero_kernel(uint16_t* x, long n) {
 }
 
 // ---------------------------------------------------------------------------------- host
-using Logits256 = Product<256, 256, 4, 2, 2, RowK, RowK>;
-using Logits64 = Product<64, 256, 1, 8, 4, RowK, RowK>;
-using Dhidden = Product<256, 256, 4, 2, 2, RowK, RowN>;
-using Dweight = Product<256, 256, 4, 2, 2, RowN, RowN>;
+// The tiles each product can be made in, and what they were measured to cost: us of a step of 64
+// along the contraction and of the rest (first loads, epilogue) for as many tiles as run at
+// once (per_cu on each CU).  From 512 x 32768 logits at D = 1024 and 4096, dhidden of 512 x 4096
+// from 32768 and of 200 x 1024 from 32768, dweight of 16384 x 4096 from 512 and 4096 tokens.
+// plan() takes the cheapest: e.g. 200 x 32768 logits at D = 1024 25.2 us in 256 x 256 tiles and
+// 20.4 in 128 x 256; 64 x 65536 at D = 2560 62 us in 64 x 256 and 80 in 64 x 64; dhidden of
+// 64 x 768 from 8192 31 us in 256 x 256 tiles (8 parts) and 13 in 64 x 64 (16).
+struct Shape {
+    int m, n, per_cu;
+    double step, fixed;
+};
+using Logits0 = Product<256, 256, 4, 2, 2, RowK, RowK>;
+using Logits1 = Product<128, 256, 2, 4, 3, RowK, RowK>;
+using Logits2 = Product<64, 256, 1, 8, 4, RowK, RowK>;
+using Logits3 = Product<64, 64, 2, 4, 4, RowK, RowK>;
+constexpr Shape LOGITS[] = {{256, 256, 1, 1.5, 7}, {128, 256, 1, .83, 5}, {64, 256, 1, .58, 4}, {64, 64, 2, .4, 2.3}};
+using Dhidden0 = Product<256, 256, 4, 2, 2, RowK, RowN>;
+using Dhidden1 = Product<128, 128, 2, 4, 2, RowK, RowN>;
+using Dhidden2 = Product<64, 256, 1, 8, 4, RowK, RowN>;
+using Dhidden3 = Product<64, 64, 2, 4, 4, RowK, RowN>;
+constexpr Shape DHIDDEN[] = {{256, 256, 1, 1.8, 12}, {128, 128, 1, .78, 5}, {64, 256, 1, .78, 8}, {64, 64, 1, .38, 3}};
+using Dweight0 = Product<256, 256, 4, 2, 2, RowN, RowN>;
+using Dweight1 = Product<128, 128, 2, 4, 2, RowN, RowN>;
+constexpr Shape DWEIGHT[] = {{256, 256, 1, 1.62, 7.5}, {128, 128, 2, 1.06, 3.1}};
+constexpr double LAUNCH = 3, BYTES = 5e6;  // us of one more launch; bytes a us
 
 static long up(long x, long to) { return (x + to - 1) / to * to; }
 static long ceil_div(long x, long y) { return (x + y - 1) / y; }
@@ -490,6 +513,8 @@ struct Plan {
     long M, V, D, K, Dp, lde, piece;  // Dp: width in the products; lde: kept columns; piece: rows
     int pieces, tiles;                // row pieces; logits tiles of a row
     bool grads, pad;
+    int logits, rest, dhidden, dweight;  // indices into the shapes
+    long main;                        // columns of the vocabulary in shape `logits`, the others in `rest`
     int splits;                       // of dhidden's contraction
     size_t j, q, row, z, part, norm, loss, inv, e, acc, parts, hidden, weight, bytes;
 };
@@ -515,6 +540,23 @@ static int check(const theseus_vocab_loss_args* a) {
     return THESEUS_WKV7_OK;
 }
 
+// us of a product of M x N outputs and `steps` steps in `splits` parts
+static double cost(const Shape& c, long M, long N, long steps, long splits, int cus) {
+    const long t = ceil_div(M, c.m) * ceil_div(N, c.n) * splits;
+    return (double)ceil_div(t, (long)cus * c.per_cu) * (c.fixed + (double)ceil_div(steps, splits) * c.step);
+}
+// the cheapest shape; none is faster than `least`, where those that do their own part sooner hide more
+template <int N> static int best(const Shape (&c)[N], long M, long cols, long steps, int cus, double least, double* us) {
+    int b = 0;
+    double u = 0;
+    for (int i = 0; i < N; i++) {
+        const double own = cost(c[i], M, cols, steps, 1, cus), x = (own < least ? least : own) + .05 * own;
+        if (i == 0 || x < u) b = i, u = x;
+    }
+    if (us) *us = u;
+    return b;
+}
+
 static Plan plan(const theseus_vocab_loss_args* a) {
     Plan p{};
     p.M = a->rows, p.V = a->vocab, p.D = a->width, p.K = a->targets;
@@ -522,21 +564,39 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     p.pad = p.D != p.Dp || a->hidden_stride % 8 || a->weight_stride % 8 || ((uintptr_t)a->hidden | (uintptr_t)a->weight) % 16;
     p.grads = a->dhidden || a->dweight;
     p.lde = up(p.V, BK);
-    p.tiles = (int)ceil_div(p.V, BN_LOGITS);
     long cap = a->piece_rows ? up(a->piece_rows, 256) : p.grads ? (2l << 30) / (2 * p.lde) / 256 * 256 : MAX_PIECE;
     cap = cap < 256 ? 256 : cap > MAX_PIECE ? MAX_PIECE : cap;
     p.pieces = (int)ceil_div(p.M, cap);
     p.piece = up(ceil_div(p.M, p.pieces ? p.pieces : 1), 256);
     p.pieces = (int)ceil_div(p.M, p.piece ? p.piece : 256);
-    const long rows = p.M < p.piece ? p.M : p.piece;  // of the largest piece
-    if (a->dhidden) {
-        // fill the CUs: dhidden has few tiles (rows x D) and a long contraction (V)
-        const long t = ceil_div(rows, Dhidden::BM) * ceil_div(p.D, Dhidden::BN), steps = p.lde / BK;
-        long s = t >= device_cus() * 4 ? 1 : ceil_div(device_cus() * 4, t);
-        if (s > 16) s = 16;
-        while (s > 1 && steps / s < 16) s--;
-        p.splits = (int)s;
+    const long rows = p.M == 0 ? 1 : p.M < p.piece ? p.M : p.piece;  // of the largest piece (no tokens: nothing is launched for them)
+    const int cus = device_cus();
+    const long steps = p.Dp / BK;
+    // one shape for all columns (no less than the weight's reading), or full rounds of the largest and the remaining columns in another
+    // (1021 x 50001 at D = 2560: 784 tiles of 256 x 256, 3.06 rounds of 256 CUs)
+    double one;
+    p.logits = best(LOGITS, rows, p.V, steps, cus, (double)p.V * p.Dp * 2 / BYTES, &one);
+    p.main = p.V, p.rest = p.logits;
+    const Shape& big = LOGITS[0];
+    const long tm = ceil_div(rows, big.m), rounds = tm * ceil_div(p.V, big.n) / cus, n = rounds * cus / tm * big.n;
+    if (n > 0 && n < p.V) {
+        double us;
+        const int r = best(LOGITS, rows, p.V - n, steps, cus, 0, &us);
+        if (1.05 * cost(big, rows, n, steps, 1, cus) + us + LAUNCH < one) p.logits = 0, p.main = n, p.rest = r;
     }
+    p.tiles = (int)(ceil_div(p.main, LOGITS[p.logits].n) + ceil_div(p.V - p.main, LOGITS[p.rest].n));
+    if (a->dhidden) {
+        // its contraction, the vocabulary, is long and its tiles few: float32 parts that fill the
+        // CUs, added afterwards
+        double least = 0;
+        for (int i = 0; i < (int)(sizeof DHIDDEN / sizeof *DHIDDEN); i++)
+            for (long s = 1; s <= 64 && s <= p.lde / BK; s++) {
+                const double c = cost(DHIDDEN[i], rows, p.D, p.lde / BK, s, cus) +
+                                 (s > 1 ? LAUNCH + (double)s * rows * p.D * 8 / BYTES : 0);
+                if (least == 0 || c < least) least = c, p.dhidden = i, p.splits = (int)s;
+            }
+    }
+    if (a->dweight) p.dweight = best(DWEIGHT, p.V, p.D, ceil_div(rows, BK), cus, 0, nullptr);
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -611,16 +671,26 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
     for (int piece = 0; piece < p.pieces; piece++) {
         const long i0 = piece * p.piece, m = p.M - i0 < p.piece ? p.M - i0 : p.piece;
         const uint16_t* Hp = H + i0 * ldh;
-        const Operand X{Hp, ldh, (int)m, (int)p.Dp}, Y{W, ldw, (int)p.V, (int)p.Dp};
-        const LogitsOut lo{(int)m, (int)p.V, (int)p.lde, LOG2E * inv_T, part, e, p.lde};
-        auto logits = [&](auto tag) {
-            using P = decltype(tag);
-            const Tiles tl = tiles(m, p.V, P::BM, P::BN, p.Dp, 1);
-            if (p.grads) logits_kernel<P, true><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
-            else logits_kernel<P, false><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
+        auto logits = [&](int shape, long n0, long n1, int tile0) {
+            const Operand X{Hp, ldh, (int)m, (int)p.Dp}, Y{W + n0 * ldw, ldw, (int)(n1 - n0), (int)p.Dp};
+            const LogitsOut lo{(int)m, (int)(n1 - n0), (int)((n1 == p.V ? p.lde : n1) - n0), LOG2E * inv_T, part + tile0, p.tiles,
+                               p.grads ? e + n0 : nullptr, p.lde};
+            auto launch = [&](auto tag) {
+                using P = decltype(tag);
+                const Tiles tl = tiles(m, n1 - n0, P::BM, P::BN, p.Dp, 1);
+                if (p.grads) logits_kernel<P, true><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
+                else logits_kernel<P, false><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
+            };
+            switch (shape) {
+                case 0: launch(Logits0{}); break;
+                case 1: launch(Logits1{}); break;
+                case 2: launch(Logits2{}); break;
+                default: launch(Logits3{});
+            }
         };
-        if (m <= 64) logits(Logits64{});
-        else logits(Logits256{});
+        logits(p.logits, 0, p.main, 0);
+        const int main_tiles = (int)ceil_div(p.main, LOGITS[p.logits].n);
+        if (p.main < p.V) logits(p.rest, p.main, p.V, main_tiles);
         const Rows rw{m, p.tiles, (int)p.K, part, row + i0, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
                       a->temperature * a->temperature, norm, losses ? losses + i0 : nullptr};
         rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
@@ -628,29 +698,43 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         if (!p.grads) continue;
 
         const long mp = up(m, BK);
-        const Probs pr{(int)m, (int)p.K, p.tiles, BN_LOGITS, p.lde, e, part, row + i0, norm, inv,
+        const Probs pr{(int)m, (int)p.K, p.tiles, (int)(p.main < p.V ? p.main : p.lde), LOGITS[p.logits].n, LOGITS[p.rest].n, p.lde, e, part, row + i0, norm, inv,
                        a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, a->temperature};
         probs_kernel<<<dim3((unsigned)ceil_div(p.lde, 2048), (unsigned)mp), 256, 0, st>>>(pr);
         if (a->dhidden) {
             uint16_t* dh = static_cast<uint16_t*>(a->dhidden) + i0 * p.D;
             const Operand GX{e, p.lde, (int)m, (int)p.lde}, WY{W, ldw, (int)p.Dp, (int)p.V};
-            const Tiles tl = tiles(m, p.D, Dhidden::BM, Dhidden::BN, p.lde, p.splits);
             float* parts = reinterpret_cast<float*>(at(p.parts));
             const GradOut go{(int)m, (int)p.D, dh, p.D, parts, up(p.D, 4), 0, 0};
-            if (tl.splits > 1) {
-                grad_kernel<Dhidden, OutPart><<<tl.m * tl.n * tl.splits, 512, 0, st>>>(GX, WY, tl, go);
-                add_parts<<<dim3((unsigned)ceil_div(p.D, 1024), (unsigned)m), 256, 0, st>>>((int)m, (int)p.D, tl.splits, parts, up(p.D, 4), dh, p.D);
-            } else {
-                grad_kernel<Dhidden, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, WY, tl, go);
+            auto dhidden = [&](auto tag) {
+                using P = decltype(tag);
+                const Tiles tl = tiles(m, p.D, P::BM, P::BN, p.lde, p.splits);
+                if (tl.splits > 1) {
+                    grad_kernel<P, OutPart><<<tl.m * tl.n * tl.splits, 512, 0, st>>>(GX, WY, tl, go);
+                    add_parts<<<dim3((unsigned)ceil_div(p.D, 1024), (unsigned)m), 256, 0, st>>>((int)m, (int)p.D, tl.splits, parts, up(p.D, 4), dh, p.D);
+                } else {
+                    grad_kernel<P, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, WY, tl, go);
+                }
+            };
+            switch (p.dhidden) {
+                case 0: dhidden(Dhidden0{}); break;
+                case 1: dhidden(Dhidden1{}); break;
+                case 2: dhidden(Dhidden2{}); break;
+                default: dhidden(Dhidden3{});
             }
         }
         if (a->dweight) {
             const Operand GX{e, p.lde, (int)p.lde, (int)mp}, HY{Hp, ldh, (int)p.Dp, (int)m};
-            const Tiles tl = tiles(p.V, p.D, Dweight::BM, Dweight::BN, mp, 1);
             const GradOut go{(int)p.V, (int)p.D, static_cast<uint16_t*>(a->dweight), p.D, reinterpret_cast<float*>(at(p.acc)),
                              up(p.D, 4), piece == 0, piece == p.pieces - 1};
-            if (p.pieces > 1) grad_kernel<Dweight, OutAdd><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
-            else grad_kernel<Dweight, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
+            auto dweight = [&](auto tag) {
+                using P = decltype(tag);
+                const Tiles tl = tiles(p.V, p.D, P::BM, P::BN, mp, 1);
+                if (p.pieces > 1) grad_kernel<P, OutAdd><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
+                else grad_kernel<P, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
+            };
+            if (p.dweight == 0) dweight(Dweight0{});
+            else dweight(Dweight1{});
         }
     }
     if (reduce && p.pieces > 1) sums(nullptr, losses, a->loss);

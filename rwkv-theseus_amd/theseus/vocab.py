@@ -20,10 +20,11 @@ A second backward through the same loss (retain_graph) makes the gradients anew.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
-from .wkv7 import extension
+from .wkv7 import _native, extension
 
 MAX_TOP = 256  # THESEUS_VOCAB_MAX_TOP
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
@@ -119,23 +120,28 @@ class _Loss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        with torch.no_grad():
+            made = _Loss._gradients(ctx, grad.float().contiguous())
+        if torch.is_grad_enabled():  # (create_graph: a later derivative through these raises)
+            made = torch._C._functions.DelayedError("theseus_vocab: the losses are differentiable once", 2)(
+                *(x if x is None else x.requires_grad_() for x in made))
+        return (*made, None)
+
+    @staticmethod
+    def _gradients(ctx, grad):
         call, made, ctx.made = ctx.call, ctx.made, None
-        grad = grad.float().contiguous()
         if made is None:
             hidden, weight = ctx.saved_tensors
             need_h, need_w = ctx.needs_input_grad[:2]
             made = (torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need_h else None,
                     torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None)
-            if call.reduction == "none":
-                call.run(hidden, weight, None, grad, *made)
-                return (*made, None)
-            call.run(hidden, weight, None, None, *made)
-        xy = [v for x in made for v in ((None, 0) if x is None else (x.data_ptr(), x.numel()))]
-        with torch.cuda.device(call.device):
-            _check(_lib().theseus_vocab_scale(*xy, grad.data_ptr(), _stream(call.device)))
-        return (*made, None)
+            call.run(hidden, weight, None, grad if call.reduction == "none" else None, *made)
+        if call.reduction != "none":
+            xy = [v for x in made for v in ((None, 0) if x is None else (x.data_ptr(), x.numel()))]
+            with torch.cuda.device(call.device):
+                _check(_lib().theseus_vocab_scale(*xy, grad.data_ptr(), _stream(call.device)))
+        return made
 
 
 def _rows(x, name, rows, device, dtypes, tail=()):
@@ -144,12 +150,14 @@ def _rows(x, name, rows, device, dtypes, tail=()):
         raise TypeError(f"theseus_vocab: {name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {x.dtype}")
     if x.device != device:
         raise ValueError(f"theseus_vocab: {name} must be on {device}, got {x.device}")
-    if tuple(x.shape) != rows + tail:
+    if x.shape != rows + tail:
         raise ValueError(f"theseus_vocab: {name} must have shape {list(rows + tail)}, got {list(x.shape)}")
-    return x.detach().reshape(-1, *tail).contiguous()
+    if len(rows) != 1:
+        x = x.reshape(math.prod(rows), *tail)
+    return (x.detach() if x.requires_grad else x).contiguous()
 
 
-def _matrix(x, name):
+def _matrix(x):
     """[n][d] with unit stride along d and rows apart (a strided view's rows are read in place)."""
     if x.stride(1) == 1 and x.stride(0) >= x.shape[1] or x.shape[0] == 1 and x.stride(1) == 1:
         return x
@@ -174,7 +182,7 @@ def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_ind
         raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
     if piece_rows < 0:
         raise ValueError(f"theseus_vocab: piece_rows must not be negative, got {piece_rows}")
-    tokens, device = tuple(hidden.shape[:-1]), hidden.device
+    tokens, device = hidden.shape[:-1], hidden.device
     index = _rows(index, "labels" if top_values is None else "top_indices", tokens, device, (torch.int64,),
                   () if top_values is None else (index.shape[-1] if index.dim() else 0,))
     if top_values is not None:
@@ -186,7 +194,12 @@ def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_ind
         teacher_lse = _rows(teacher_lse, "teacher_lse", tokens, device, (torch.float32,))
     if row_weight is not None:
         row_weight = _rows(row_weight, "token_weight", tokens, device, (torch.float32,))
-    h, w = _matrix(hidden.reshape(-1, hidden.shape[-1]), "hidden"), _matrix(weight, "weight")
+    h, w = _matrix(hidden if len(tokens) == 1 else hidden.reshape(math.prod(tokens), hidden.shape[-1])), _matrix(weight)
+    native = _native(h, w)
+    if native is not None:
+        loss = native.vocab_loss(h, w, index, top_values, teacher_lse, row_weight, ignore_index, temperature,
+                                 _REDUCTIONS[reduction], piece_rows)
+        return loss.reshape(tokens) if reduction == "none" and len(tokens) != 1 else loss
     call = _Call(h, w, index, top_values, teacher_lse, row_weight, ignore_index, float(temperature), reduction, piece_rows)
     if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
         loss = _Loss.apply(h, w, call)
@@ -240,7 +253,13 @@ def top_logits(logits, k, *, temperature=1.0):
     if not temperature > 0 or temperature == float("inf"):
         raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
     V, rows = logits.shape[-1], logits.shape[:-1]
-    x = _matrix(logits.detach().reshape(-1, V), "logits")
+    x = _matrix(logits.detach().reshape(math.prod(rows), V))
+    native = _native(x)
+    if native is not None:
+        values, indices, lse = native.vocab_top(x, k, float(temperature))
+        if len(rows) == 1:
+            return values, indices, lse
+        return values.reshape(*rows, k), indices.reshape(*rows, k), lse.reshape(rows)
     n, dt, dev = x.shape[0], _DTYPES[x.dtype], x.device
     values = torch.empty((*rows, k), dtype=x.dtype, device=dev)
     indices = torch.empty((*rows, k), dtype=torch.int64, device=dev)

@@ -475,6 +475,18 @@ def test_c_abi_refuses_without_launching():
     assert extension().lib.theseus_wkv7_error_string(4) == b"workspace too small"
 
 
+def test_sizes_are_planned_for_any_shape_without_a_gpu():
+    """The host's planning divides by tile counts: no size may stop it, 0 tokens among them."""
+    lib = vocab._lib()
+    for M in (0, 1, 3, 255, 256, 257, 5000, 40000, 1 << 20):
+        for V in (1, 2, 63, 65, 255, 257, 50001, 1 << 22):
+            for D in (1, 8, 64, 5120):
+                for grads in ({}, {"dhidden": 16}, {"dhidden": 16, "dweight": 16}):
+                    a = vocab.LossArgs(rows=M, vocab=V, width=D, targets=1, hidden=1 << 20, weight=1 << 20, hidden_stride=D,
+                                       weight_stride=D, index=16, temperature=1.0, reduction=2, loss=16, **grads)
+                    assert lib.theseus_vocab_loss_workspace_size(ctypes.byref(a)) > 0, (M, V, D)
+
+
 def test_workspace_holds_a_piece_not_the_logits():
     """65536 tokens of a vocabulary of 131072: 16 GB of 16-bit probabilities, 2 GiB at a time."""
     a = vocab.LossArgs(rows=65536, vocab=131072, width=4096, targets=1, hidden=1 << 20, weight=1 << 20, hidden_stride=4096,
@@ -484,3 +496,51 @@ def test_workspace_holds_a_piece_not_the_logits():
     assert 2 << 30 <= n < 3.5 * (1 << 30)
     a.dhidden = None
     assert lib.theseus_vocab_loss_workspace_size(ctypes.byref(a)) < 1 << 29
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_the_python_autograd_function_gives_the_native_ones_bits(reduction, monkeypatch):
+    x, w, g = _inputs(70, 64, 300)
+    tv, ti = _teacher(70, 300, 9, g)
+    up = torch.rand(70, generator=g) if reduction == "none" else torch.tensor(.3)
+    f = lambda a, b: vocab.linear_top_distillation(a, b, tv.cuda(), ti.cuda(), temperature=2.0, reduction=reduction)  # noqa: E731
+    native = _run(f, x, w, up, reduction)
+    top = vocab.top_logits(tv.cuda(), 4)
+    quiet = f(x.cuda(), w.cuda())
+    monkeypatch.setattr(vocab, "_native", lambda *xs: None)
+    for p, q in zip(native, _run(f, x, w, up, reduction)):
+        assert torch.equal(p, q)
+    for p, q in zip(top, vocab.top_logits(tv.cuda(), 4)):
+        assert torch.equal(p, q)
+    assert torch.equal(quiet, f(x.cuda(), w.cuda())) and torch.equal(quiet, native[0])
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_second_derivatives_are_refused(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(vocab, "_native", lambda *xs: None)
+    x, w, _ = _inputs(5, 64, 30)
+    x = x.cuda().requires_grad_()
+    loss = vocab.linear_cross_entropy(x, w.cuda(), torch.zeros(5, dtype=torch.int64).cuda())
+    dx, = torch.autograd.grad(loss, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dx.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("M,D,V", [(1021, 64, 50001), (1500, 128, 20011), (130, 64, 33000), (40, 128, 16500)])
+def test_every_tile_shape_matches_float64(M, D, V):
+    """Sizes at which the plan takes other tiles, several shapes for one matrix, parts of the contraction."""
+    print(f"  shapes M={M} D={D} V={V}", flush=True)
+    x, w, g = _inputs(M, D, V, seed=M)
+    labels = torch.randint(V, (M,), generator=g)
+    labels[-1] = V - 1
+    one = torch.ones(M).double()
+    o = _oracle(x.cuda(), w.cuda(), _dense(M, V, labels[:, None], torch.ones(M, 1)).cuda(), 0.0, one.cuda(), 1.0, one.cuda())
+    o = {k: v.cpu() for k, v in o.items()}
+    loss, dx, dw = _run(lambda a, b: vocab.linear_cross_entropy(a, b, labels.cuda(), reduction="none"), x, w, torch.ones(M), "none")
+    assert ((loss.double().cpu() - o["loss"]).abs() <= o["ltol"]).all()
+    _grad_close(dx, o["dx"], o["dx_tol"])
+    _grad_close(dw, o["dw"], o["dw_tol"])
