@@ -4,11 +4,12 @@
 // A workgroup of 1024 threads takes up to SLAB elements of a row into registers (128 KB read once)
 // and selects there:
 //   1. every thread's maximum and, against the row's, its sum of exponentials;
-//   2. the k-th largest of 256 (k <= 128) or 1024 group maxima, to 16 bits and rounded down, is
-//      a bound that the k-th largest element cannot be below: -G ln(1 - k/G) elements (74 of
-//      65536 for k = 64, 295 for k = 256) lie above it in independent data;
+//   2. the k-th largest of 256 (k <= 128) or 512 group maxima, rounded down to 16 bits, is a bound that the k-th largest
+//      element cannot be below: -G ln(1 - k/G) elements (74 of 65536 for k = 64, 355 for k = 256)
+//      are not below it in independent data;
 //   3. the elements not below the bound go to a list in LDS as (key, ~index) in 64 bits, whose
-//      order is the answer's; each one's rank is a count over the list.
+//      order is the answer's; each one's rank is a count over the list (of more than MANY, over
+//      those that are not below its k-th key, found by bisection).
 // With more than CAP elements at the bound (many equal values: a masked vocabulary), the list
 // takes those above it, and of the equal ones those of the lowest indices, found by bisection on
 // the index; should more than CAP lie above it, the exact k-th key is found by bisection first.
@@ -22,17 +23,17 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "wkv7_common.h"
 
 namespace vocab_top {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
-constexpr int WORDS = 32;    // registers of logits per thread
-constexpr int CAP = 1024;    // list entries
+constexpr int THREADS = 1024, SMALL = 256;  // of a workgroup
+constexpr int MOST = 8;                     // 16-byte granules per thread
+constexpr int MANY = 256;                   // list entries worth another selection
 constexpr int MERGE = 16;    // lists joined at a time
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-template <bool BF16> constexpr int SLAB = THREADS * WORDS * (BF16 ? 2 : 1);
 
 __device__ __forceinline__ uint32_t key_of(float f) {
     const uint32_t u = __float_as_uint(f + 0.f);
@@ -45,7 +46,7 @@ __device__ __forceinline__ float base_of(float top) { return fabsf(top) == INFIN
 
 struct Args {
     long rows, vocab, stride;
-    int k, slabs;
+    int k, slabs, each;     // slabs of a row, granules of a slab
     float scale, inv_T;     // log2(e) / temperature, 1 / temperature
     const void* x;
     void* values;           // slabs == 1: the answer
@@ -55,36 +56,44 @@ struct Args {
     float2* sums;           // [rows][slabs] {maximum, sum of exponentials against it}
 };
 
+// (the value comes out of the key, without reading the logit again: -0 as 0, any NaN as one)
 template <bool BF16> __device__ __forceinline__ void emit(const Args& p, long row, int rank, uint64_t c) {
-    const long i = 0xffffffffu - (uint32_t)c, at = row * p.k + rank;
-    p.indices[at] = i;
-    if constexpr (BF16) static_cast<uint16_t*>(p.values)[at] = static_cast<const uint16_t*>(p.x)[row * p.stride + i];
-    else static_cast<float*>(p.values)[at] = static_cast<const float*>(p.x)[row * p.stride + i];
+    const long at = row * p.k + rank;
+    const uint32_t u = __float_as_uint(of_key((uint32_t)(c >> 32)));
+    p.indices[at] = 0xffffffffu - (uint32_t)c;
+    if constexpr (BF16) static_cast<uint16_t*>(p.values)[at] = (uint16_t)(u >> 16);
+    else static_cast<uint32_t*>(p.values)[at] = u;
 }
 
-template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p) {
-    constexpr int PER = BF16 ? 8 : 4, G = WORDS / 4;  // elements of a 16-byte granule, granules per thread
-    __shared__ uint64_t list[CAP];
-    __shared__ float maxima[THREADS];
+// A workgroup of T threads, G granules each: slabs of at most T G granules.  (8 waves a SIMD, 64
+// registers: two workgroups of 1024 on a CU, one loading while the other selects; 4096 rows of
+// 65536 bfloat16 180 -> 126 us.)  T = 1024, or 256 with k <= 128.
+template <bool BF16, int T, int G> __global__ __launch_bounds__(T, 8) void top_part(Args p) {
+    constexpr int PER = BF16 ? 8 : 4;  // elements of a granule
+    constexpr int WAVES = T / 64, CAP = T, GROUPS = T < 512 ? T : 512, KEYS = CAP / 64;
+    __shared__ __attribute__((aligned(16))) uint64_t list[CAP];
+    __shared__ __attribute__((aligned(16))) float maxima[GROUPS];
+    __shared__ int ranks[CAP];
+    __shared__ float shared_bound;
+    __shared__ uint32_t shared_key;
     __shared__ float redf[2][WAVES];
-    __shared__ int count, shared_bits;
+    __shared__ int count;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const long row = blockIdx.x / p.slabs;
     const int slab = blockIdx.x - row * p.slabs;
 
     // Granules are 16-byte aligned in memory, whatever the row's alignment: a row's first and last
     // may hold elements of a neighbour (or of the allocation that the row lies in, which starts
-    // and ends on such a granule), left out below.  Slab s has granules s SG .. of the row.
+    // and ends on such a granule), left out below.  Slab s has granules s each .. of the row.
     const long size = BF16 ? 2 : 4;
     const uint8_t* row0 = static_cast<const uint8_t*>(p.x) + row * p.stride * size;
     const int shift = (int)((uintptr_t)row0 & 15) / (int)size, V = (int)p.vocab;  // elements of the first granule before the row
-    constexpr int SG = SLAB<BF16> / PER;
-    const int g0 = slab * SG, gall = (V + shift + PER - 1) / PER, gend = min(g0 + SG, gall);
+    const int gall = (V + shift + PER - 1) / PER, g0 = slab * p.each, gend = min(g0 + p.each, gall);
     const uint4* gran = reinterpret_cast<const uint4*>(row0 - shift * size);
     uint32_t w[G][4];
 #pragma unroll
     for (int j = 0; j < G; j++) {
-        const uint4 u = gran[min(g0 + j * THREADS + t, gend - 1)];
+        const uint4 u = gran[min(g0 + j * T + t, gend - 1)];
         w[j][0] = u.x, w[j][1] = u.y, w[j][2] = u.z, w[j][3] = u.w;
     }
     if (t == 0) count = 0;
@@ -93,19 +102,21 @@ template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p)
         else return __uint_as_float(u[e]);
     };
     constexpr uint32_t LOW = BF16 ? 0xff80ff80u : 0xff800000u;
+    if ((g0 == 0 && shift) || gend == gall || p.each < T * G) {  // (elsewhere every element is the slab's)
 #pragma unroll
-    for (int j = 0; j < G; j++) {
-        const int g = g0 + j * THREADS + t;
-        const bool out = g >= gend;
+        for (int j = 0; j < G; j++) {
+            const int g = g0 + j * T + t;
+            const bool out = g >= gend;
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[j][i] = out ? LOW : w[j][i];
-        if (g == 0 || g == gall - 1) {
+            for (int i = 0; i < 4; i++) w[j][i] = out ? LOW : w[j][i];
+            if ((g == 0 && shift) || (g == gall - 1 && (V + shift) % PER)) {
 #pragma unroll
-            for (int e = 0; e < PER; e++) {
-                const int i = g * PER + e - shift;
-                if (i < 0 || i >= V) {
-                    if constexpr (BF16) w[j][e >> 1] = e & 1 ? (w[j][e >> 1] & 0xffffu) | 0xff800000u : (w[j][e >> 1] & 0xffff0000u) | 0xff80u;
-                    else w[j][e] = 0xff800000u;
+                for (int e = 0; e < PER; e++) {
+                    const int i = g * PER + e - shift;
+                    if (i < 0 || i >= V) {
+                        if constexpr (BF16) w[j][e >> 1] = e & 1 ? (w[j][e >> 1] & 0xffffu) | 0xff800000u : (w[j][e >> 1] & 0xffff0000u) | 0xff80u;
+                        else w[j][e] = 0xff800000u;
+                    }
                 }
             }
         }
@@ -115,8 +126,13 @@ template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p)
     for (int j = 0; j < G; j++)
 #pragma unroll
         for (int e = 0; e < PER; e++) top = fmaxf(top, val(w[j], e));
-    maxima[t] = top;
+    // groups of four threads, of two for k > 128; the small workgroup's threads
+    const int lg = T == SMALL ? 0 : p.k > 128 ? 1 : 2;
     float all = top;
+    if (lg > 0) all = fmaxf(all, __shfl_xor(all, 1, 64));
+    if (lg == 2) all = fmaxf(all, __shfl_xor(all, 2, 64));
+    if ((t & ((1 << lg) - 1)) == 0) maxima[t >> lg] = all;
+    ranks[t] = 0;
     for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, 64));
     if (lane == 0) redf[0][wave] = all;
     __syncthreads();
@@ -140,26 +156,25 @@ template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p)
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (lane == 0) redf[1][wave] = s;
 
-    if (wave == 0) {  // the k-th largest group maximum, the upper 16 bits of its key
-        const bool fine = p.k > 128;
-        uint32_t key[16];
+    if (wave == 0) {  // the k-th largest group maximum: the upper 16 bits of its key, by bisection
+        uint32_t key[8];
 #pragma unroll
-        for (int i = 0; i < 16; i++) key[i] = key_of(maxima[64 * i + lane]);
-        if (!fine)  // groups of four threads: 64 i .. for i = 4 a .. 4 a + 3
+        for (int i = 0; i < 4; i++) key[i] = key_of(maxima[64 * i + lane]);
 #pragma unroll
-            for (int a = 0; a < 4; a++) key[a] = max(max(key[4 * a], key[4 * a + 1]), max(key[4 * a + 2], key[4 * a + 3]));
-        uint32_t bound = 0;
+        for (int i = 4; i < 8; i++) key[i] = GROUPS == 512 && lg == 1 ? key_of(maxima[(64 * i + lane) & (GROUPS - 1)]) : 0;
+        uint32_t found = 0;
+#pragma unroll 1
         for (int bit = 31; bit >= 16; bit--) {
-            const uint32_t c = bound | (1u << bit);
+            const uint32_t c = found | (1u << bit);
             int n = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) n += __popcll(__ballot(key[i] >= c));
-            if (fine)
+            if (lg == 1)
 #pragma unroll
-                for (int i = 4; i < 16; i++) n += __popcll(__ballot(key[i] >= c));
-            if (n >= p.k) bound = c;
+                for (int i = 4; i < 8; i++) n += __popcll(__ballot(key[i] >= c));
+            if (n >= p.k) found = c;
         }
-        if (lane == 0) shared_bits = (int)bound;
+        if (lane == 0) shared_bound = of_key(max(found, key_of(-INFINITY)));  // (fewer groups than k: everything)
     }
     __syncthreads();
     if (t == 0) {
@@ -168,9 +183,8 @@ template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p)
         if (p.slabs > 1) p.sums[row * p.slabs + slab] = make_float2(base, total);
         else if (p.lse) p.lse[row] = base * p.inv_T + __builtin_amdgcn_logf(total) * LN2;  // (nothing but -inf: log2 0)
     }
-    // (a bound below -inf's key: fewer groups than k)
-    const uint32_t bk = max((uint32_t)shared_bits, key_of(-INFINITY));
-    const float bound = of_key(bk);
+    const float bound = shared_bound;
+    const uint32_t bk = key_of(bound);
 
     auto append = [&](int i, uint32_t key) {
         const int at = atomicAdd(&count, 1);
@@ -187,7 +201,7 @@ template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p)
             hit |= (uint32_t)(nan || !(m < bound)) << j;
         }
         for (; hit; hit &= hit - 1) {
-            const int j = __ffs(hit) - 1, g = g0 + j * THREADS + t;
+            const int j = __ffs(hit) - 1, g = g0 + j * T + t;
             uint32_t u[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) u[i] = w[0][i];
@@ -209,7 +223,7 @@ template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p)
         // f(index, key) for every element of the slab, read again
         auto each = [&](auto f) {
 #pragma unroll 1
-            for (int g = g0 + t; g < gend; g += THREADS) {
+            for (int g = g0 + t; g < gend; g += T) {
                 const uint4 q = gran[g];
                 const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -258,29 +272,61 @@ template <bool BF16> __global__ __launch_bounds__(THREADS) void top_part(Args p)
         __syncthreads();
         n = count;
     }
-    if (t < n) {
-        const uint64_t c = list[t];
-        int rank = 0;
-        for (int i = 0; i < n; i++) rank += list[i] > c;
-        if (rank < p.k) {
-            if (p.slabs > 1) p.lists[((long)row * p.slabs + slab) * p.k + rank] = c;
-            else emit<BF16>(p, row, rank, c);
+    if (n > MANY) {  // (few values of one group are left out where they are fewer than the groups)
+        const uint64_t c = t < n ? list[t] : 0;
+        if (wave == 0) {  // the list's k-th key
+            uint32_t key[KEYS], found = 0;
+#pragma unroll
+            for (int i = 0; i < KEYS; i++) key[i] = 64 * i + lane < n ? (uint32_t)(list[64 * i + lane] >> 32) : 0;
+#pragma unroll 1
+            for (int bit = 31; bit >= 0; bit--) {
+                const uint32_t x = found | (1u << bit);
+                int m = 0;
+#pragma unroll
+                for (int i = 0; i < KEYS; i++) m += __popcll(__ballot(key[i] >= x));
+                if (m >= p.k) found = x;
+            }
+            if (lane == 0) shared_key = found;
         }
+        __syncthreads();
+        if (t == 0) count = 0;
+        __syncthreads();
+        if (t < n && (uint32_t)(c >> 32) >= shared_key) list[atomicAdd(&count, 1)] = c;
+        __syncthreads();
+        n = count;
+    }
+    int lanes = 64, ln = 6;  // threads of one share of the counting: a power of two, n at least
+    while (lanes < n) lanes *= 2, ln++;
+    const int own = t & (lanes - 1);
+    const uint64_t c = own < n ? list[own] : 0;
+    {
+        const int shares = T >> ln, share = ((n + shares - 1) / shares + 1) & ~1, first = (t >> ln) * share;
+        int r = 0;
+        for (int i = first; i < min(n, first + share); i += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + i);
+            r += (two.x > c) + (i + 1 < n && two.y > c);
+        }
+        if (own < n) atomicAdd(ranks + own, r);
+    }
+    __syncthreads();
+    if (t < n && ranks[t] < p.k) {
+        if (p.slabs > 1) p.lists[((long)row * p.slabs + slab) * p.k + ranks[t]] = c;
+        else emit<BF16>(p, row, ranks[t], c);
     }
     if (p.slabs > 1)  // (a short last slab)
-        for (int i = n + t; i < p.k; i += THREADS) p.lists[((long)row * p.slabs + slab) * p.k + i] = 0;
+        for (int i = n + t; i < p.k; i += T) p.lists[((long)row * p.slabs + slab) * p.k + i] = 0;
 }
 
 // Joins up to MERGE sorted lists of a row: an entry's rank is its place in its own list and the
 // numbers of greater entries in the others (bisection).  `last`: the answer, else a list again.
-template <bool BF16> __global__ __launch_bounds__(256) void top_merge(Args p, const uint64_t* in, int lists, uint64_t* out, int groups, int last) {
+template <bool BF16> __global__ __launch_bounds__(THREADS) void top_merge(Args p, const uint64_t* in, int lists, uint64_t* out, int groups, int last) {
     __shared__ uint64_t c[MERGE * THESEUS_VOCAB_MAX_TOP];
     const long row = blockIdx.x / groups;
     const int g = blockIdx.x - row * groups, first = g * MERGE, nl = min(MERGE, lists - first), total = nl * p.k;
     const uint64_t* from = in + (row * lists + first) * p.k;
-    for (int i = threadIdx.x; i < total; i += 256) c[i] = from[i];
+    for (int i = threadIdx.x; i < total; i += THREADS) c[i] = from[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < total; i += 256) {
+    for (int i = threadIdx.x; i < total; i += THREADS) {
         const uint64_t x = c[i];
         const int own = i / p.k;
         int rank = i - own * p.k;
@@ -316,10 +362,22 @@ template <bool BF16> __global__ __launch_bounds__(256) void top_merge(Args p, co
 }
 
 static size_t up(size_t n) { return (n + 255) / 256 * 256; }
-// slabs of a row; `aligned`: every row starts on 16 bytes, else it may have a granule more
-static long slabs_of(long vocab, int dtype, bool aligned) {
-    const long slab = dtype == THESEUS_VOCAB_BF16 ? SLAB<true> : SLAB<false>, per = dtype == THESEUS_VOCAB_BF16 ? 8 : 4;
-    return (vocab + (aligned ? 0 : per - 1) + slab - 1) / slab;
+struct Plan {
+    int threads, granules;  // per thread
+    long slabs, each;       // of a row; granules of one
+};
+// The smallest slab that holds a row, or slabs of one size: a second slab costs its merge (4 us and,
+// for one row of 65536 bfloat16, 12.2 us in two against 10.0 in one).  With enough rows to fill
+// the CUs eight times over, short rows go to workgroups of 256 (4096 rows of 8192).
+static Plan plan(long rows, long vocab, int k, int dtype, bool aligned) {
+    const long per = dtype == THESEUS_VOCAB_BF16 ? 8 : 4;
+    // (a row that does not start on a granule may have one more)
+    const long all = (vocab + (aligned ? 0 : per - 1) + per - 1) / per;
+    const int threads = rows >= 1024 && k <= 128 && all <= SMALL * MOST ? SMALL : THREADS;
+    int g = 1;
+    while (g < MOST && all > (long)threads * g) g *= 2;
+    const long slabs = (all + (long)threads * g - 1) / ((long)threads * g);
+    return {threads, g, slabs, (all + slabs - 1) / slabs};
 }
 static size_t bytes_of(size_t rows, size_t s, int k) {
     if (s == 1) return 0;
@@ -331,21 +389,32 @@ static int check(long long rows, long long vocab, int k, int dtype) {
     if (rows < 0 || rows > (1ll << 30) || vocab < 1 || vocab > (1ll << 30) || k < 1 || k > vocab || k > THESEUS_VOCAB_MAX_TOP)
         return THESEUS_WKV7_ERR_SHAPE;
     if (dtype != THESEUS_VOCAB_BF16 && dtype != THESEUS_VOCAB_FP32) return THESEUS_WKV7_ERR_DTYPE;
-    if (rows * slabs_of(vocab, dtype, false) >= (1ll << 31)) return THESEUS_WKV7_ERR_SHAPE;
+    if (rows * plan(rows, vocab, k, dtype, false).slabs >= (1ll << 31)) return THESEUS_WKV7_ERR_SHAPE;
     return THESEUS_WKV7_OK;
 }
 
-template <bool BF16> static void launch(Args p, uint8_t* ws, hipStream_t st) {
+template <bool BF16> static void launch(Args p, const Plan& pl, uint8_t* ws, hipStream_t st) {
     const size_t lists = up((size_t)p.rows * p.slabs * p.k * 8);
     p.lists = reinterpret_cast<uint64_t*>(ws);
     p.sums = reinterpret_cast<float2*>(ws + lists);
-    top_part<BF16><<<(unsigned)(p.rows * p.slabs), THREADS, 0, st>>>(p);
+    const unsigned n = (unsigned)(p.rows * p.slabs);
+    auto part = [&](auto tag) {
+        constexpr int G = decltype(tag)::value;
+        if (pl.threads == SMALL) top_part<BF16, SMALL, G><<<n, SMALL, 0, st>>>(p);
+        else top_part<BF16, THREADS, G><<<n, THREADS, 0, st>>>(p);
+    };
+    switch (pl.granules) {
+        case 1: part(std::integral_constant<int, 1>{}); break;
+        case 2: part(std::integral_constant<int, 2>{}); break;
+        case 4: part(std::integral_constant<int, 4>{}); break;
+        default: part(std::integral_constant<int, MOST>{});
+    }
     if (p.slabs == 1) return;
     uint64_t* in = p.lists;
     uint64_t* out = reinterpret_cast<uint64_t*>(ws + lists + up((size_t)p.rows * p.slabs * 8));
     for (int n = p.slabs;;) {
         const int groups = (n + MERGE - 1) / MERGE;
-        top_merge<BF16><<<(unsigned)(p.rows * groups), 256, 0, st>>>(p, in, n, out, groups, groups == 1);
+        top_merge<BF16><<<(unsigned)(p.rows * groups), THREADS, 0, st>>>(p, in, n, out, groups, groups == 1);
         if (groups == 1) return;
         uint64_t* t = in;
         in = out, out = t;
@@ -359,7 +428,10 @@ extern "C" {
 
 size_t theseus_vocab_top_workspace_size(long long rows, long long vocab, int k, int dtype) {
     using namespace vocab_top;
-    return check(rows, vocab, k, dtype) ? 0 : bytes_of((size_t)rows, (size_t)slabs_of(vocab, dtype, false), k);
+    if (check(rows, vocab, k, dtype)) return 0;
+    const size_t a = bytes_of((size_t)rows, (size_t)plan(rows, vocab, k, dtype, true).slabs, k);
+    const size_t b = bytes_of((size_t)rows, (size_t)plan(rows, vocab, k, dtype, false).slabs, k);
+    return a > b ? a : b;
 }
 
 int theseus_vocab_top(long long rows, long long vocab, int k, int dtype, float temperature, const void* logits,
@@ -372,12 +444,12 @@ int theseus_vocab_top(long long rows, long long vocab, int k, int dtype, float t
     if (!logits || !values || !indices) return THESEUS_WKV7_ERR_NULL;
     const int size = dtype == THESEUS_VOCAB_BF16 ? 2 : 4;
     if ((uintptr_t)logits % size) return THESEUS_WKV7_ERR_SHAPE;
-    const long slabs = slabs_of(vocab, dtype, ((uintptr_t)logits | (uintptr_t)(row_stride * size)) % 16 == 0);
-    const size_t need = bytes_of((size_t)rows, (size_t)slabs, k);
+    const Plan pl = plan(rows, vocab, k, dtype, ((uintptr_t)logits | (uintptr_t)(row_stride * size)) % 16 == 0);
+    const size_t need = bytes_of((size_t)rows, (size_t)pl.slabs, k);
     if (need && (!workspace || workspace_bytes < need)) return THESEUS_WKV7_ERR_WORKSPACE;
-    Args p{rows, vocab, row_stride, k, (int)slabs, LOG2E / temperature, 1.f / temperature, logits, values, indices, lse, nullptr, nullptr};
-    if (dtype == THESEUS_VOCAB_BF16) launch<true>(p, static_cast<uint8_t*>(workspace), stream);
-    else launch<false>(p, static_cast<uint8_t*>(workspace), stream);
+    Args p{rows, vocab, row_stride, k, (int)pl.slabs, (int)pl.each, LOG2E / temperature, 1.f / temperature, logits, values, indices, lse, nullptr, nullptr};
+    if (dtype == THESEUS_VOCAB_BF16) launch<true>(p, pl, static_cast<uint8_t*>(workspace), stream);
+    else launch<false>(p, pl, static_cast<uint8_t*>(workspace), stream);
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }
 
