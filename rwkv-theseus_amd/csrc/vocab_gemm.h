@@ -42,11 +42,13 @@ enum Lay { RowK, RowN };
 // One operand: rows of `ld` elements.  RowK: outer index -> row, `outer` valid rows, the
 // contraction's `K` elements in every row.  RowN: contraction index -> row, `inner` valid rows,
 // `outer` elements valid in a row (a multiple of 8).  Rows and columns beyond are read from the
-// last valid place; the other operand is zero there, or the output is not stored.
+// last valid place; the other operand is zero there, or the output is not stored.  RowN with
+// `twice`: one step of rows 0 .. 31 and again 0 .. 31.
 struct Operand {
     const uint16_t* p;
     long ld;
     int outer, inner;
+    bool twice = false;
 };
 
 struct Tiles {
@@ -90,6 +92,7 @@ template <Lay L, int B, bool PERM> struct Loader {
     static_assert(B * BK * 2 % 8192 == 0 && (L == RowK || B == 256 || B == 128 || B == 64), "tile");
     const uint8_t* base;
     uint32_t row, col, ld2;
+    uint32_t mask;  // of a row's number (RowN)
     int rows_left;  // RowK: valid rows from the tile's first; RowN: valid rows from the part's first
 
     __device__ __forceinline__ Loader(const Operand& o, int x0, int k0, int wave, int lane) {
@@ -98,6 +101,7 @@ template <Lay L, int B, bool PERM> struct Loader {
             const int r = 8 * wave + (lane >> 3);
             const int c = (lane & 7) ^ (PERM ? (r >> 1) & 7 : r & 7);
             base = reinterpret_cast<const uint8_t*>(o.p + (long)x0 * o.ld + k0);
+            mask = ~0u;
             row = r * ld2;
             col = 16 * c;
             rows_left = o.outer - x0;
@@ -106,7 +110,8 @@ template <Lay L, int B, bool PERM> struct Loader {
             const int r = PER * wave + lane / CH;
             const int c = (lane & (CH - 1)) ^ ((2 * (r & 7)) & (CH - 1));
             base = reinterpret_cast<const uint8_t*>(o.p + (long)k0 * o.ld + x0);
-            row = r * ld2;
+            mask = o.twice ? 31u : ~0u;
+            row = (r & mask) * ld2;
             col = 2 * min(8 * c, o.outer - x0 - 8);
             rows_left = o.inner - k0;
         }
@@ -114,7 +119,7 @@ template <Lay L, int B, bool PERM> struct Loader {
     // piece j of the next step into the tile at `lds`; advance() after the last one
     __device__ __forceinline__ void issue(uint32_t lds, int j, int wave) const {
         const int last = L == RowK ? rows_left - 1 : min(rows_left - 1, BK - 1);
-        const uint32_t r = min(row + (uint32_t)(8 * PER * j) * ld2, (uint32_t)max(last, 0) * ld2);
+        const uint32_t r = min(row + ((uint32_t)(8 * PER * j) & mask) * ld2, (uint32_t)max(last, 0) * ld2);
         dma(lds + (uint32_t)(wave + 8 * j) * 1024, base, r + col);
     }
     // to the next step; past the last one the loader stays there (its pieces are then not used)

@@ -38,6 +38,7 @@ using wkv7::f32x2_to_bf16x2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float E_SHIFT = 15.f;  // kept exponentials are 2^15 e^{z - max}
 constexpr int SKIP = -1, BAD = -2;
+constexpr int TWICE = 32;  // tokens
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
@@ -65,7 +66,7 @@ struct Targets {
     float inv_T;
     int* j;        // [M][K] index, SKIP or BAD
     float* q;      // [M][K] (teacher only)
-    float* z;      // [M][K] z log2(e) / T at the target
+    float* z;      // [M][K] h . w at the target
     float4* row;   // [M] {Q, sum q log q, weight, 0}
 };
 
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(256) void targets_kernel(Targets t) {
         two(u.w, y.w);
     }
     s = wave_sum(s);
-    if (lane == 0) t.z[p] = s * (LOG2E * t.inv_T);
+    if (lane == 0) t.z[p] = s;
 }
 
 // sum over 1024 threads in a fixed order, valid in thread 0
@@ -171,7 +172,7 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
 }
 // MEAN: *inv = 1 / sum of the weights (0 where that is 0); with losses, *out = their sum, times
 // *inv for MEAN.
-__global__ __launch_bounds__(1024) void sums_kernel(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
+__device__ __forceinline__ void sums(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
     __shared__ double red[2][16];
     double w = 0.0, s = 0.0;
 #pragma unroll 4
@@ -187,12 +188,15 @@ __global__ __launch_bounds__(1024) void sums_kernel(long rows, const float4* row
         if (out) *out = (float)(s * f);
     }
 }
+__global__ __launch_bounds__(1024) void sums_kernel(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
+    sums(rows, row, mean, inv, losses, out);
+}
 
 // ---------------------------------------------------------------------------------- logits
 struct LogitsOut {
     int M, N, Ne;     // rows, vocabulary, columns kept (Ne >= N, zero beyond N)
     float scale;      // log2(e) / T
-    float2* part;     // [M][tiles] {maximum, sum of 2^15 exp} of a tile, base 2
+    float2* part;     // [M][tiles] {maximum of h . w, sum of 2^15 exp} of a tile
     int tiles;
     uint16_t* e;      // [..][lde]
     long lde;
@@ -241,14 +245,12 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
         float all = red[m];
 #pragma unroll
         for (int w = 1; w < P::WN; w++) all = fmaxf(all, red[w * P::BM + m]);
-        all *= o.scale;
-        const float shift = E_SHIFT - all;
         float sum = 0.f;
 #pragma unroll
         for (int tn = 0; tn < P::TN; tn++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float x = exp2_(fmaf(g.acc[tn][tm][e], o.scale, shift));
+                const float x = exp2_(fmaf(g.acc[tn][tm][e] - all, o.scale, E_SHIFT));
                 g.acc[tn][tm][e] = x;
                 sum += x;
             }
@@ -283,44 +285,57 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
 
 // ---------------------------------------------------------------------------------- rows
 // One wave a token of the piece: maximum and sum over its tiles, the token's loss.  Nothing is
-// taken from a rounded log-sum-exp: for a confident token, lse - z and p - 1 are small
-// differences of (z - maximum) and of the sum.
+// taken from a rounded log-sum-exp, and products h . w are subtracted before they are scaled: for
+// a confident token, lse - z and p - 1 are small differences of (z - maximum) and of the sum.
 struct Rows {
     long rows;
     int tiles, K;
     const float2* part;
     const float4* row;
     const float *q, *z;
-    float TT;
-    float2* norm;  // {maximum (base 2), 1 / sum of 2^15 exp}
+    float T, scale;
+    float2* norm;  // {maximum of h . w, 1 / sum of 2^15 exp}
     float* loss;
 };
-__global__ __launch_bounds__(256) void rows_kernel(Rows p) {
-    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (i >= p.rows) return;
+__device__ __forceinline__ void one_row(const Rows& p, long i, int lane) {
     const float2* part = p.part + i * p.tiles;
     float top = -INFINITY;
     for (int t = lane; t < p.tiles; t += 64) top = fmaxf(top, part[t].x);
     top = wave_max(top);
     float sum = 0.f;
-    for (int t = lane; t < p.tiles; t += 64) sum += part[t].y * exp2_(part[t].x - top);
+    for (int t = lane; t < p.tiles; t += 64) sum += part[t].y * exp2_((part[t].x - top) * p.scale);
     sum = wave_sum(sum);
     const float lse = logf(sum * exp2_(-E_SHIFT));  // above the maximum
     const float4 row = p.row[i];
     float s = 0.f;
     for (int k = lane; k < p.K; k += 64) {
         const float q = p.q ? p.q[i * p.K + k] : 1.f;
-        if (q != 0.f) s += q * (LN2 * (top - p.z[i * p.K + k]) + lse);
+        if (q != 0.f) s += q * ((top - p.z[i * p.K + k]) * (LN2 * p.scale) + lse);
     }
     s = wave_sum(s);
     if (lane == 0) {
         p.norm[i] = make_float2(top, 1.f / sum);
-        if (p.loss) p.loss[i] = row.z == 0.f ? 0.f : p.TT * row.z * (s + row.y);
+        if (p.loss) p.loss[i] = row.z == 0.f ? 0.f : p.T * p.T * row.z * (s + row.y);
     }
+}
+__global__ __launch_bounds__(256) void rows_kernel(Rows p) {
+    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i < p.rows) one_row(p, i, threadIdx.x & 63);
+}
+// rows and sums of few tokens by one workgroup (64 tokens: 3.9 and 2.9 us in two launches)
+__global__ __launch_bounds__(1024) void rows_sums(Rows p, int mean, float* inv, float* out) {
+    for (long i = threadIdx.x >> 6; i < p.rows; i += 16) one_row(p, i, threadIdx.x & 63);
+    __syncthreads();
+    sums(p.rows, p.row, mean, inv, p.loss, out);
 }
 
 // ---------------------------------------------------------------------------------- G
+// G without its factor common to all tokens (T, and 1 / the sum of the weights for MEAN), which the
+// products' epilogues apply in float32: with it, every label's -1 would become one and the same
+// rounded number, an error of up to 2^-8 of the whole gradient.  For up to TWICE tokens, whose
+// few large entries' roundings would not average out either (one token: the whole error of one
+// number), G is kept as two rows of bfloat16, the rounded one and what rounding left: a step of
+// the contraction over tokens has 64 rows anyway, and dhidden's smallest tile 64.
 struct Probs {
     int M, K;               // the piece's tokens (its rows up to a multiple of 64 become zeros)
     int tiles;              // logits tiles of a row: main / cols of `cols` columns, then of `rest`
@@ -330,44 +345,43 @@ struct Probs {
     const float2* part;
     const float4* row;
     const float2* norm;
-    const float *inv_weight, *row_grad;
+    const float* row_grad;
     const int* j;
     const float *q, *z;
-    float T;
+    float scale;
+    bool twice;             // rows 32 .. 63 take what rounding left of rows 0 .. 31
 };
-__device__ __forceinline__ float row_factor(const Probs& p, long i) {  // T c_i
-    float c = p.row[i].z;
-    if (p.inv_weight) c *= *p.inv_weight;
-    if (p.row_grad) c *= p.row_grad[i];
-    return p.T * c;
-}
 // blockIdx.x: 2048 columns of row blockIdx.y; 8 columns a thread, then the targets among them
 __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
     const long i = blockIdx.y;
     const int n0 = blockIdx.x * 2048, n = n0 + threadIdx.x * 8;
-    uint16_t* row = p.e + i * p.lde;
-    const float f = i < p.M ? row_factor(p, i) : 0.f;
-    uint4* at = reinterpret_cast<uint4*>(row + n);
+    uint16_t *row = p.e + i * p.lde, *rest = row + 32 * p.lde;
+    const float f = i >= p.M ? 0.f : p.row_grad ? p.row[i].z * p.row_grad[i] : p.row[i].z;
     if (f == 0.f) {
-        if (n < p.lde) *at = make_uint4(0, 0, 0, 0);
+        if (n < p.lde) {
+            *reinterpret_cast<uint4*>(row + n) = make_uint4(0, 0, 0, 0);
+            if (p.twice) *reinterpret_cast<uint4*>(rest + n) = make_uint4(0, 0, 0, 0);
+        }
         return;
     }
     const float Q = p.row[i].x;
     const float2 norm = p.norm[i];
     if (n < p.lde) {
         const int tile = n < p.main ? n / p.cols : p.main / p.cols + (n - p.main) / p.rest;
-        const float g = f * Q * norm.y * exp2_(p.part[i * p.tiles + tile].x - norm.x);
+        const float g = f * Q * norm.y * exp2_((p.part[i * p.tiles + tile].x - norm.x) * p.scale);
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        uint4 u = *at;
-        auto two = [&](uint32_t& x) {
-            const h2 h = __builtin_bit_cast(h2, x);
-            x = f32x2_to_bf16x2((float)h[0] * g, (float)h[1] * g);
-        };
-        two(u.x);
-        two(u.y);
-        two(u.z);
-        two(u.w);
-        *at = u;
+        const uint4 u = *reinterpret_cast<const uint4*>(row + n);
+        const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const h2 h = __builtin_bit_cast(h2, in[e]);
+            const float a = (float)h[0] * g, b = (float)h[1] * g;
+            hi[e] = f32x2_to_bf16x2(a, b);
+            lo[e] = f32x2_to_bf16x2(a - __uint_as_float(hi[e] << 16), b - __uint_as_float(hi[e] & 0xffff0000u));
+        }
+        *reinterpret_cast<uint4*>(row + n) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (p.twice) *reinterpret_cast<uint4*>(rest + n) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     __syncthreads();
     if (threadIdx.x < p.K) {  // (equal indices of one token write the same value)
@@ -379,7 +393,9 @@ __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
             else
                 for (int k = 0; k < p.K; k++)
                     if (p.j[i * p.K + k] == v) q += p.q[i * p.K + k];
-            row[v] = f32_to_bf16(f * (Q * (exp2_(p.z[t] - norm.x + E_SHIFT) * norm.y) - q));
+            const float g = f * (Q * (exp2_(fmaf(p.z[t] - norm.x, p.scale, E_SHIFT)) * norm.y) - q);
+            row[v] = f32_to_bf16(g);
+            if (p.twice) rest[v] = f32_to_bf16(g - bf16_to_f32(row[v]));
         }
     }
 }
@@ -394,6 +410,8 @@ struct GradOut {
     float* f;      // OutPart: [splits][M][ldf]; OutAdd: [M][ldf]
     long ldf;
     int first, last;  // OutAdd: of the row pieces
+    float T;              // the common factor T, times *inv where there is one
+    const float* inv;
 };
 
 template <class P, OutMode MODE>
@@ -426,8 +444,9 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
     }
     __syncthreads();
     const bool eight = (o.ldc & 7) == 0 && ((uintptr_t)o.c & 15) == 0;  // (N = ldc: eight columns are in or out together)
+    const float f = o.inv ? o.T * *o.inv : o.T;
     store_rows<P>(lds, [&](int tn, int tm) {
-        const f32x4_t a = g.acc[tn][tm];
+        const f32x4_t a = g.acc[tn][tm] * f;
         return make_uint2(f32x2_to_bf16x2(a[0], a[1]), f32x2_to_bf16x2(a[2], a[3]));
     }, [&](int m, int n, uint4 v) {
         if (m0 + m >= o.M || n0 + n >= o.N) return;
@@ -440,14 +459,17 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
         }
     });
 }
-// the parts of a contraction added in order, 4 columns a thread
-__global__ __launch_bounds__(256) void add_parts(int M, int N, int splits, const float* f, long ldf, uint16_t* c, long ldc) {
+// the parts of a contraction added in order, 4 columns a thread (twice = 32: and row m + 32's)
+__global__ __launch_bounds__(256) void add_parts(GradOut o, int splits, int twice) {
     const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
     const long m = blockIdx.y;
-    if (n >= N) return;
+    if (n >= o.N) return;
     f32x4_t a = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; s++) a += *reinterpret_cast<const f32x4_t*>(f + ((long)s * M + m) * ldf + n);
-    for (int e = 0; e < 4 && n + e < N; e++) c[m * ldc + n + e] = f32_to_bf16(a[e]);
+    for (int r = 0; r <= twice; r += 32)  // (rows 32 .. 63: see above)
+#pragma unroll 8
+        for (int s = 0; s < splits; s++) a += *reinterpret_cast<const f32x4_t*>(o.f + ((long)s * o.M + m + r) * o.ldf + n);
+    a *= o.inv ? o.T * *o.inv : o.T;
+    for (int e = 0; e < 4 && n + e < o.N; e++) o.c[m * o.ldc + n + e] = f32_to_bf16(a[e]);
 }
 
 // copies rows of D elements (any alignment) to rows of Dp, zeros beyond D
@@ -512,7 +534,7 @@ static long ceil_div(long x, long y) { return (x + y - 1) / y; }
 struct Plan {
     long M, V, D, K, Dp, lde, piece;  // Dp: width in the products; lde: kept columns; piece: rows
     int pieces, tiles;                // row pieces; logits tiles of a row
-    bool grads, pad;
+    bool grads, pad, twice;
     int logits, rest, dhidden, dweight;  // indices into the shapes
     long main;                        // columns of the vocabulary in shape `logits`, the others in `rest`
     int splits;                       // of dhidden's contraction
@@ -540,17 +562,17 @@ static int check(const theseus_vocab_loss_args* a) {
     return THESEUS_WKV7_OK;
 }
 
-// us of a product of M x N outputs and `steps` steps in `splits` parts
-static double cost(const Shape& c, long M, long N, long steps, long splits, int cus) {
-    const long t = ceil_div(M, c.m) * ceil_div(N, c.n) * splits;
-    return (double)ceil_div(t, (long)cus * c.per_cu) * (c.fixed + (double)ceil_div(steps, splits) * c.step);
+// us of a product of M x N outputs and `steps` steps
+static double cost(const Shape& c, long M, long N, long steps, int cus) {
+    const long t = ceil_div(M, c.m) * ceil_div(N, c.n);
+    return (double)ceil_div(t, (long)cus * c.per_cu) * (c.fixed + (double)steps * c.step);
 }
 // the cheapest shape; none is faster than `least`, where those that do their own part sooner hide more
 template <int N> static int best(const Shape (&c)[N], long M, long cols, long steps, int cus, double least, double* us) {
     int b = 0;
     double u = 0;
     for (int i = 0; i < N; i++) {
-        const double own = cost(c[i], M, cols, steps, 1, cus), x = (own < least ? least : own) + .05 * own;
+        const double own = cost(c[i], M, cols, steps, cus), x = (own < least ? least : own) + .05 * own;
         if (i == 0 || x < u) b = i, u = x;
     }
     if (us) *us = u;
@@ -570,6 +592,7 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     p.piece = up(ceil_div(p.M, p.pieces ? p.pieces : 1), 256);
     p.pieces = (int)ceil_div(p.M, p.piece ? p.piece : 256);
     const long rows = p.M == 0 ? 1 : p.M < p.piece ? p.M : p.piece;  // of the largest piece (no tokens: nothing is launched for them)
+    p.twice = p.M <= TWICE;
     const int cus = device_cus();
     const long steps = p.Dp / BK;
     // one shape for all columns (no less than the weight's reading), or full rounds of the largest and the remaining columns in another
@@ -582,19 +605,23 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     if (n > 0 && n < p.V) {
         double us;
         const int r = best(LOGITS, rows, p.V - n, steps, cus, 0, &us);
-        if (1.05 * cost(big, rows, n, steps, 1, cus) + us + LAUNCH < one) p.logits = 0, p.main = n, p.rest = r;
+        if (1.05 * cost(big, rows, n, steps, cus) + us + LAUNCH < one) p.logits = 0, p.main = n, p.rest = r;
     }
     p.tiles = (int)(ceil_div(p.main, LOGITS[p.logits].n) + ceil_div(p.V - p.main, LOGITS[p.rest].n));
     if (a->dhidden) {
         // its contraction, the vocabulary, is long and its tiles few: float32 parts that fill the
         // CUs, added afterwards
+        const long all = p.lde / BK, gm = p.twice ? 64 : rows;
         double least = 0;
-        for (int i = 0; i < (int)(sizeof DHIDDEN / sizeof *DHIDDEN); i++)
-            for (long s = 1; s <= 64 && s <= p.lde / BK; s++) {
-                const double c = cost(DHIDDEN[i], rows, p.D, p.lde / BK, s, cus) +
-                                 (s > 1 ? LAUNCH + (double)s * rows * p.D * 8 / BYTES : 0);
-                if (least == 0 || c < least) least = c, p.dhidden = i, p.splits = (int)s;
+        for (int i = 0; i < (int)(sizeof DHIDDEN / sizeof *DHIDDEN); i++) {
+            const Shape& c = DHIDDEN[i];
+            const int t = (int)(ceil_div(gm, c.m) * ceil_div(p.D, c.n));
+            for (int s = 1; s <= 64 && s <= all; s += s < 8 ? 1 : s / 4) {  // (every call comes by here: few candidates)
+                const double us = (t * s + cus * c.per_cu - 1) / (cus * c.per_cu) * (c.fixed + ((int)all + s - 1) / s * c.step) +
+                                  (s > 1 ? LAUNCH + (double)s * gm * p.D * 8 / BYTES : 0);
+                if (least == 0 || us < least) least = us, p.dhidden = i, p.splits = s;
             }
+        }
     }
     if (a->dweight) p.dweight = best(DWEIGHT, p.V, p.D, ceil_div(rows, BK), cus, 0, nullptr);
     size_t at = 0;
@@ -613,7 +640,7 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     p.part = take((size_t)rows * p.tiles * 8);
     p.e = take(p.grads ? (size_t)up(rows, BK) * p.lde * 2 : 0);
     p.acc = take(a->dweight && p.pieces > 1 ? (size_t)p.V * up(p.D, 4) * 4 : 0);
-    p.parts = take(p.splits > 1 ? (size_t)p.splits * rows * up(p.D, 4) * 4 : 0);
+    p.parts = take(p.splits > 1 || p.twice ? (size_t)p.splits * (p.twice ? 64 : rows) * up(p.D, 4) * 4 : 0);
     p.hidden = take(p.pad ? (size_t)p.M * p.Dp * 2 : 0);
     p.weight = take(p.pad ? (size_t)p.V * p.Dp * 2 : 0);
     p.bytes = at;
@@ -692,26 +719,32 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         const int main_tiles = (int)ceil_div(p.main, LOGITS[p.logits].n);
         if (p.main < p.V) logits(p.rest, p.main, p.V, main_tiles);
         const Rows rw{m, p.tiles, (int)p.K, part, row + i0, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
-                      a->temperature * a->temperature, norm, losses ? losses + i0 : nullptr};
-        rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
-        if (p.pieces == 1 && (reduce || (mean && p.grads))) sums(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
+                      a->temperature, LOG2E * inv_T, norm, losses ? losses + i0 : nullptr};
+        const bool now = p.pieces == 1 && (reduce || (mean && p.grads));
+        if (now && m <= 128) {
+            rows_sums<<<1, 1024, 0, st>>>(rw, mean, inv, reduce ? a->loss : nullptr);
+        } else {
+            rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
+            if (now) sums(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
+        }
         if (!p.grads) continue;
 
         const long mp = up(m, BK);
-        const Probs pr{(int)m, (int)p.K, p.tiles, (int)(p.main < p.V ? p.main : p.lde), LOGITS[p.logits].n, LOGITS[p.rest].n, p.lde, e, part, row + i0, norm, inv,
-                       a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, a->temperature};
-        probs_kernel<<<dim3((unsigned)ceil_div(p.lde, 2048), (unsigned)mp), 256, 0, st>>>(pr);
+        const Probs pr{(int)m, (int)p.K, p.tiles, (int)(p.main < p.V ? p.main : p.lde), LOGITS[p.logits].n, LOGITS[p.rest].n, p.lde, e, part, row + i0, norm,
+                       a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, LOG2E * inv_T, p.twice};
+        probs_kernel<<<dim3((unsigned)ceil_div(p.lde, 2048), (unsigned)(p.twice ? 32 : mp)), 256, 0, st>>>(pr);
         if (a->dhidden) {
             uint16_t* dh = static_cast<uint16_t*>(a->dhidden) + i0 * p.D;
-            const Operand GX{e, p.lde, (int)m, (int)p.lde}, WY{W, ldw, (int)p.Dp, (int)p.V};
+            const long gm = p.twice ? 64 : m;  // rows of G
+            const Operand GX{e, p.lde, (int)gm, (int)p.lde}, WY{W, ldw, (int)p.Dp, (int)p.V};
             float* parts = reinterpret_cast<float*>(at(p.parts));
-            const GradOut go{(int)m, (int)p.D, dh, p.D, parts, up(p.D, 4), 0, 0};
+            const GradOut go{(int)gm, (int)p.D, dh, p.D, parts, up(p.D, 4), 0, 0, a->temperature, inv};
             auto dhidden = [&](auto tag) {
                 using P = decltype(tag);
-                const Tiles tl = tiles(m, p.D, P::BM, P::BN, p.lde, p.splits);
-                if (tl.splits > 1) {
+                const Tiles tl = tiles(gm, p.D, P::BM, P::BN, p.lde, p.splits);
+                if (tl.splits > 1 || p.twice) {
                     grad_kernel<P, OutPart><<<tl.m * tl.n * tl.splits, 512, 0, st>>>(GX, WY, tl, go);
-                    add_parts<<<dim3((unsigned)ceil_div(p.D, 1024), (unsigned)m), 256, 0, st>>>((int)m, (int)p.D, tl.splits, parts, up(p.D, 4), dh, p.D);
+                    add_parts<<<dim3((unsigned)ceil_div(p.D, 1024), (unsigned)m), 256, 0, st>>>(go, tl.splits, p.twice ? 32 : 0);
                 } else {
                     grad_kernel<P, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, WY, tl, go);
                 }
@@ -724,9 +757,9 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
             }
         }
         if (a->dweight) {
-            const Operand GX{e, p.lde, (int)p.lde, (int)mp}, HY{Hp, ldh, (int)p.Dp, (int)m};
+            const Operand GX{e, p.lde, (int)p.lde, (int)mp}, HY{Hp, ldh, (int)p.Dp, (int)m, p.twice};
             const GradOut go{(int)p.V, (int)p.D, static_cast<uint16_t*>(a->dweight), p.D, reinterpret_cast<float*>(at(p.acc)),
-                             up(p.D, 4), piece == 0, piece == p.pieces - 1};
+                             up(p.D, 4), piece == 0, piece == p.pieces - 1, a->temperature, inv};
             auto dweight = [&](auto tag) {
                 using P = decltype(tag);
                 const Tiles tl = tiles(p.V, p.D, P::BM, P::BN, mp, 1);

@@ -544,3 +544,24 @@ def test_every_tile_shape_matches_float64(M, D, V):
     assert ((loss.double().cpu() - o["loss"]).abs() <= o["ltol"]).all()
     _grad_close(dx, o["dx"], o["dx_tol"])
     _grad_close(dw, o["dw"], o["dw_tol"])
+
+
+@gpu
+@pytest.mark.parametrize("M,D,V", [(1, 128, 4000), (5, 100, 333), (31, 256, 9000), (32, 64, 50)])
+def test_few_tokens_gradients_are_rounded_once(M, D, V):
+    """Up to 32 tokens: G in two halves (2^-16), its softmax part from float16 exponentials (11 bits: 2^-11), so
+    the gradients are within that of G W and their own rounding, 2^-8."""
+    print(f"  few M={M} D={D} V={V}", flush=True)
+    x, w, g = _inputs(M, D, V, seed=V)
+    labels = torch.randint(V, (M,), generator=g)
+    up = torch.rand(M, generator=g) + .5
+    ones = torch.ones(M).double()
+    o = _oracle(x, w, _dense(M, V, labels[:, None], torch.ones(M, 1)), 0.0, ones, 1.0, up.double())
+    z = x.double() @ w.double().t()
+    P = up.double()[:, None] * torch.softmax(z, -1)
+    G = P - up.double()[:, None] * torch.nn.functional.one_hot(labels, V)
+    ztol = 2.0 ** -24 * (math.sqrt(D) + 8) * (x.double().abs() @ w.double().abs().t()).amax(-1)
+    E = 1.1 * 2.0 ** -11 * P + 2.0 ** -16 * G.abs() + (2 * ztol + 2.0 ** -20)[:, None] * P
+    loss, dx, dw = _run(lambda a, b: vocab.linear_cross_entropy(a, b, labels.cuda(), reduction="none"), x, w, up, "none")
+    _grad_close(dx, o["dx"], E @ w.double().abs())
+    _grad_close(dw, o["dw"], E.t() @ x.double().abs())
