@@ -169,9 +169,14 @@ template <Lay L, int B, bool PERM> struct Reader {
     }
 };
 
+// this wave's LDS reads done and all but its last N DMAs, then everyone's (by the builtins: the
+// compiler counts the reads that are still out, and knows here that none is)
 template <int N> __device__ __forceinline__ void wait_barrier() {
     wkv7::vm_wait_n<N>();
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // A BM x BN tile: WM x WN waves of TM x TN fragments, NST stages.  Leaves acc[tn][tm] (lane:
@@ -225,37 +230,36 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
 #pragma unroll
             for (int tm = 0; tm < TM; tm++) acc[tn][tm] = wkv7::mma32(acc[tn][tm], y[tn], x[tm]);
         };
-        // groups G0 .. TN - 1 with the next half's reads: x in the first groups, y behind its group
+        // groups G0 .. TN - 1; behind each, what there is of a stage's refill and of the next half's
+        // fragments: y as its registers come free, x spread over the groups
         auto groups = [&](const uint4 (&x)[TM], uint4 (&xn)[TM], int stage, int h, auto first, auto fill, int fstage) {
             constexpr int G0 = decltype(first)::value, NG = TN - G0;
-            constexpr int XG = NG >= 4 ? 2 : 1, XPER = (TM + XG - 1) / XG, YPER = (TN + NG - 1) / NG, FPER = (PIECES + NG - 1) / NG;
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
+            for (int g = G0; g < TN; g++) {
+                group(x, g);
+                __builtin_amdgcn_sched_barrier(0);
                 if constexpr (decltype(fill)::value) {
 #pragma unroll
-                    for (int j = g * FPER; j < (g + 1) * FPER && j < PIECES; j++) piece(fstage, j);
+                    for (int j = 0; j < PIECES; j++)
+                        if (G0 + j * NG / PIECES == g) piece(fstage, j);
                 }
 #pragma unroll
-                for (int i = g * XPER; i < (g + 1) * XPER && i < TM; i++) read_x(xn, stage, i, h);
-                group(x, G0 + g);
+                for (int i = 0; i < TM; i++)
+                    if (G0 + i * (NG - 1) / TM == g) read_x(xn, stage, i, h);
 #pragma unroll
                 for (int i = 0; i < TN; i++)
-                    if (i / YPER == g && i <= G0 + g) read_y(stage, i, h);
-                if (g == NG - 1) {
-#pragma unroll
-                    for (int i = 0; i < TN; i++)
-                        if (i / YPER > g || i > G0 + i / YPER) read_y(stage, i, h);
-                }
+                    if ((i > G0 ? i : G0) == g) read_y(stage, i, h);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        constexpr int BG = TN >= 8 ? 1 : 0;  // groups of the second half ahead of the barrier
+        constexpr int BG = TN < 8 || PERM ? 0 : 3;  // groups of the second half ahead of the barrier
         using None = std::integral_constant<int, 0>;
         using Late = std::integral_constant<int, BG>;
 #pragma unroll
         for (int i = 0; i < TM; i++) read_x(x0, 0, i, 0);
 #pragma unroll
         for (int i = 0; i < TN; i++) read_y(0, i, 0);
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // (so that what is out at the loop's start is what its end left)
         int cur = 0;
         for (int s = 0; s < steps; s++) {
             groups(x0, x1, cur, 1, None{}, std::false_type{}, 0);
