@@ -2,17 +2,17 @@
 // include/theseus_vocab.h, where the formulas are).
 //
 // Launches of one call, on the caller's stream:
-//   targets        every token's q, Q, sum q log q and weight from the labels or the teacher's
-//                  logits; z at the target indices, one wave a (token, target)
+//   labels, targets  every token's q, Q, sum q log q and weight
 //   sums           MEAN with several pieces: the sum of the weights (one workgroup, fixed order)
 //   then for each piece of rows
 //     logits       z's tiles on the matrix cores; of each 256-column tile a row's maximum and sum
 //                  of exponentials are kept and, for gradients, the exponentials (float16,
-//                  2^15 e^{z - tile maximum}: 11 significant bits down to e^-20 of the maximum)
+//                  2^15 e^{z - tile maximum}: 11 significant bits down to e^-20 of the maximum);
+//                  z at the targets is taken out of the accumulators
 //     rows         log-sum-exp of a row from its tiles, the row's loss
 //     sums         one piece: the reduced loss and, for MEAN, the sum of the weights
 //     probs        exponentials -> G in place (bfloat16: the one rounding of the gradients' left
-//                  factor); at the target indices from the float32 z of `targets`: p - 1 of a
+//                  factor); at the target indices from their float32 z: p - 1 of a
 //                  confident token would be lost in a rounded p
 //     dhidden, dweight   G W and G^T H (vocab_gemm.h; float32 sums, rounded once)
 //   sums           several pieces: the reduced loss
@@ -54,10 +54,8 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // ---------------------------------------------------------------------------------- targets
 struct Targets {
-    long pairs, vocab;
-    int K, D, top_bf16;
-    const uint16_t *x, *w;    // rows of D elements, a multiple of 64, 16-byte aligned
-    long ldx, ldw;
+    long rows, vocab;
+    int K, top_bf16;
     const int64_t* index;
     const void* top;          // null: labels
     const float* teacher_lse;
@@ -66,98 +64,66 @@ struct Targets {
     float inv_T;
     int* j;        // [M][K] index, SKIP or BAD
     float* q;      // [M][K] (teacher only)
-    float* z;      // [M][K] h . w at the target
     float4* row;   // [M] {Q, sum q log q, weight, 0}
 };
+__device__ __forceinline__ int place(const Targets& t, int64_t v) { return v < 0 || v >= t.vocab ? BAD : (int)v; }
 
-// One wave a (token, target): the token's q (again for each of its targets: K values against the
-// D of the dot product), then z at its own target.  The first target's wave writes the token's.
-__global__ __launch_bounds__(256) void targets_kernel(Targets t) {
-    const long p = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (p >= t.pairs) return;
-    const long i = t.top ? p / t.K : p;
-    const int k0 = (int)(p - i * t.K);
-    auto place = [&](int64_t v) { return v < 0 || v >= t.vocab ? BAD : (int)v; };
+// labels: one thread a token
+__global__ __launch_bounds__(256) void labels_kernel(Targets t) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= t.rows) return;
+    const int64_t y = t.index[i];
     const float weight = t.row_weight ? t.row_weight[i] : 1.f;
-    int v;
-    if (!t.top) {
-        const int64_t y = t.index[i];
-        v = y == t.ignore ? SKIP : place(y);
-        if (lane == 0) {
-            t.j[i] = v;
-            t.row[i] = make_float4(1.f, 0.f, y == t.ignore ? 0.f : weight, 0.f);
+    t.j[i] = y == t.ignore ? SKIP : place(t, y);
+    t.row[i] = make_float4(1.f, 0.f, y == t.ignore ? 0.f : weight, 0.f);
+}
+
+// a teacher's logits: one wave a token
+__global__ __launch_bounds__(256) void targets_kernel(Targets t) {
+    constexpr int S = THESEUS_VOCAB_MAX_TOP / 64;
+    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (i >= t.rows) return;
+    const float weight = t.row_weight ? t.row_weight[i] : 1.f;
+    float x[S], top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const int k = 64 * s + lane;
+        x[s] = -INFINITY;
+        if (64 * s < t.K && k < t.K) {
+            const long at = i * t.K + k;
+            x[s] = (t.top_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(t.top)[at]) : static_cast<const float*>(t.top)[at]) * t.inv_T;
         }
+        top = fmaxf(top, x[s]);
+    }
+    float base;
+    if (t.teacher_lse) {
+        base = t.teacher_lse[i];
     } else {
-        constexpr int S = THESEUS_VOCAB_MAX_TOP / 64;
-        float x[S], top = -INFINITY;
+        // (a token of whom the teacher kept nothing has q = 0 throughout)
+        top = wave_max(top);
+        float sum = 0.f;
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            const int k = 64 * s + lane;
-            x[s] = -INFINITY;
-            if (64 * s < t.K && k < t.K) {
-                const long at = i * t.K + k;
-                x[s] = (t.top_bf16 ? bf16_to_f32(static_cast<const uint16_t*>(t.top)[at]) : static_cast<const float*>(t.top)[at]) * t.inv_T;
-            }
-            top = fmaxf(top, x[s]);
-        }
-        float base;
-        if (t.teacher_lse) {
-            base = t.teacher_lse[i];
-        } else {
-            // (a token of whom the teacher kept nothing has q = 0 throughout)
-            top = wave_max(top);
-            float sum = 0.f;
-#pragma unroll
-            for (int s = 0; s < S; s++)
-                if (64 * s < t.K) sum += x[s] == -INFINITY ? 0.f : expf(x[s] - top);
-            base = top + logf(wave_sum(sum));
-        }
-        if (k0 == 0) {
-            float Q = 0.f, H = 0.f;
-#pragma unroll
-            for (int s = 0; s < S; s++) {
-                const int k = 64 * s + lane;
-                if (k < t.K) {
-                    const float lq = x[s] - base, q = x[s] == -INFINITY ? 0.f : expf(lq);
-                    const long at = i * t.K + k;
-                    t.q[at] = q;
-                    t.j[at] = q == 0.f ? SKIP : place(t.index[at]);
-                    Q += q;
-                    H += q == 0.f ? 0.f : q * lq;
-                }
-            }
-            Q = wave_sum(Q);
-            H = wave_sum(H);
-            if (lane == 0) t.row[i] = make_float4(Q, H, weight, 0.f);
-        }
-        float own = x[0];
-#pragma unroll
-        for (int s = 1; s < S; s++) own = s == k0 >> 6 ? x[s] : own;
-        own = __shfl(own, k0 & 63, 64);
-        v = own == -INFINITY || expf(own - base) == 0.f ? SKIP : place(t.index[p]);
+        for (int s = 0; s < S; s++)
+            if (64 * s < t.K) sum += x[s] == -INFINITY ? 0.f : expf(x[s] - top);
+        base = top + logf(wave_sum(sum));
     }
-    if (v < 0) {
-        if (lane == 0) t.z[p] = v == BAD ? NAN : 0.f;
-        return;
+    float Q = 0.f, H = 0.f;
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const int k = 64 * s + lane;
+        if (k < t.K) {
+            const float lq = x[s] - base, q = x[s] == -INFINITY ? 0.f : expf(lq);
+            const long at = i * t.K + k;
+            t.q[at] = q;
+            t.j[at] = q == 0.f ? SKIP : place(t, t.index[at]);
+            Q += q;
+            H += q == 0.f ? 0.f : q * lq;
+        }
     }
-    const uint4* a = reinterpret_cast<const uint4*>(t.x + i * t.ldx);
-    const uint4* b = reinterpret_cast<const uint4*>(t.w + (long)v * t.ldw);
-    float s = 0.f;
-#pragma unroll 4
-    for (int c = lane; c < t.D / 8; c += 64) {
-        const uint4 u = a[c], y = b[c];
-        auto two = [&](uint32_t m, uint32_t n) {
-            s += __uint_as_float(m << 16) * __uint_as_float(n << 16);
-            s += __uint_as_float(m & 0xffff0000u) * __uint_as_float(n & 0xffff0000u);
-        };
-        two(u.x, y.x);
-        two(u.y, y.y);
-        two(u.z, y.z);
-        two(u.w, y.w);
-    }
-    s = wave_sum(s);
-    if (lane == 0) t.z[p] = s;
+    Q = wave_sum(Q);
+    H = wave_sum(H);
+    if (lane == 0) t.row[i] = make_float4(Q, H, weight, 0.f);
 }
 
 // sum over 1024 threads in a fixed order, valid in thread 0
@@ -172,7 +138,7 @@ __device__ __forceinline__ double block_sum(double x, double* red) {
 }
 // MEAN: *inv = 1 / sum of the weights (0 where that is 0); with losses, *out = their sum, times
 // *inv for MEAN.
-__device__ __forceinline__ void sums(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
+__global__ __launch_bounds__(1024) void sums_kernel(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
     __shared__ double red[2][16];
     double w = 0.0, s = 0.0;
 #pragma unroll 4
@@ -188,9 +154,6 @@ __device__ __forceinline__ void sums(long rows, const float4* row, int mean, flo
         if (out) *out = (float)(s * f);
     }
 }
-__global__ __launch_bounds__(1024) void sums_kernel(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
-    sums(rows, row, mean, inv, losses, out);
-}
 
 // ---------------------------------------------------------------------------------- logits
 struct LogitsOut {
@@ -200,7 +163,72 @@ struct LogitsOut {
     int tiles;
     uint16_t* e;      // [..][lde]
     long lde;
+    const int* j;     // [M][K] targets
+    float* z;         // [M][K] their h . w
+    int K;
+    int n0;           // the product's first column
 };
+
+// acc[tn][tm] of fragment code = tn TM + tm, the same for the whole wave (no indexed registers)
+template <class P, int LO, int HI> __device__ __forceinline__ f32x4_t fragment(const P& g, int code) {
+    if constexpr (HI - LO == 1) {
+        f32x4_t a = g.acc[LO / P::TM][LO % P::TM];
+        asm("" : "+v"(a));  // (a value here: joined as addresses, the accumulators would have to lie in memory)
+        return a;
+    }
+    else if (code < (LO + HI) / 2) return fragment<P, LO, (LO + HI) / 2>(g, code);
+    else return fragment<P, (LO + HI) / 2, HI>(g, code);
+}
+// h . w at the targets that lie in the workgroup's tile, out of the accumulators: the tile's tokens'
+// targets are looked through (8192 at a time), those in its columns listed in LDS, and each wave
+// goes down the list for its own.  The list's order, which the atomics leave open, changes nothing.
+// (About 3 us a tile of 256 x 256 with 32 targets a token, 96 us of 8192 x 65536 logits; dot products
+// in a kernel of their own, D values of weight a target: 460 us.  With labels equal.)
+template <class P> __device__ __forceinline__ void pick_targets(const P& g, uint8_t* lds, const LogitsOut& o, int m0, int n0) {
+    constexpr int CHUNK = P::THREADS * 16;
+    uint32_t* list = reinterpret_cast<uint32_t*>(lds);
+    int* count = reinterpret_cast<int*>(lds + CHUNK * 4 + 256);
+    static_assert(P::LDS >= CHUNK * 4 + 4 + 256, "list");  // (64 entries are read at a time)
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int total = min(P::BM, o.M - m0) * o.K, first = o.n0 + n0;
+    const int* j = o.j + (long)m0 * o.K;
+    for (int c0 = 0; c0 < total; c0 += CHUNK) {
+        int4 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {  // (what a last four reads past the targets lies in the workspace)
+            const int i = c0 + (r * P::THREADS + t) * 4;
+            v[r] = i < total ? *reinterpret_cast<const int4*>(j + i) : make_int4(-1, -1, -1, -1);
+        }
+        __syncthreads();
+        if (t == 0) *count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int i = c0 + (r * P::THREADS + t) * 4, x[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (i + e < total && (uint32_t)(x[e] - first) < (uint32_t)P::BN) {
+                    const int m = (i + e) / o.K;
+                    list[atomicAdd(count, 1)] = (uint32_t)m << 16 | (uint32_t)(x[e] - first) << 8 | (uint32_t)(i + e - m * o.K);
+                }
+        }
+        __syncthreads();
+        const int n = *count;
+        for (int i = 0; i < n; i += 64) {
+            const uint32_t own = list[i + lane];
+            uint64_t mine = __ballot(i + lane < n && (int)(own >> 16) / (16 * P::TM) == wave / P::WN &&
+                                     (int)((own >> 8) & 255) / (16 * P::TN) == wave % P::WN);
+            for (; mine; mine &= mine - 1) {
+                const uint32_t e = __builtin_amdgcn_readlane(own, __builtin_ctzll(mine));
+                const int m = e >> 16, c = (e >> 8) & 255;
+                const f32x4_t a = fragment<P, 0, P::TM * P::TN>(g, c / 16 % P::TN * P::TM + m / 16 % P::TM);
+                const float z = (c & 2) ? (c & 1) ? a[3] : a[2] : (c & 1) ? a[1] : a[0];
+                if ((lane & 15) == (m & 15) && lane >> 4 == ((c >> 2) & 3)) o.z[(long)(m0 + m) * o.K + (e & 255)] = z;
+            }
+        }
+    }
+    __syncthreads();
+}
 
 template <class P, bool KEEP>
 __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y, Tiles t, LogitsOut o) {
@@ -209,6 +237,7 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
     const int m0 = at.m * P::BM, n0 = at.n * P::BN;
     P g;
     g.run(lds, X, Y, m0, n0, 0, t.all);
+    pick_targets(g, lds, o, m0, n0);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
     const int wm = wave / P::WN, wn = wave % P::WN;
@@ -292,12 +321,16 @@ struct Rows {
     int tiles, K;
     const float2* part;
     const float4* row;
+    const int* j;
     const float *q, *z;
     float T, scale;
     float2* norm;  // {maximum of h . w, 1 / sum of 2^15 exp}
     float* loss;
 };
-__device__ __forceinline__ void one_row(const Rows& p, long i, int lane) {
+__global__ __launch_bounds__(256) void rows_kernel(Rows p) {
+    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (i >= p.rows) return;
     const float2* part = p.part + i * p.tiles;
     float top = -INFINITY;
     for (int t = lane; t < p.tiles; t += 64) top = fmaxf(top, part[t].x);
@@ -310,23 +343,14 @@ __device__ __forceinline__ void one_row(const Rows& p, long i, int lane) {
     float s = 0.f;
     for (int k = lane; k < p.K; k += 64) {
         const float q = p.q ? p.q[i * p.K + k] : 1.f;
-        if (q != 0.f) s += q * ((top - p.z[i * p.K + k]) * (LN2 * p.scale) + lse);
+        const int v = p.j[i * p.K + k];
+        if (q != 0.f) s += v == BAD ? NAN : q * ((top - p.z[i * p.K + k]) * (LN2 * p.scale) + lse);
     }
     s = wave_sum(s);
     if (lane == 0) {
         p.norm[i] = make_float2(top, 1.f / sum);
         if (p.loss) p.loss[i] = row.z == 0.f ? 0.f : p.T * p.T * row.z * (s + row.y);
     }
-}
-__global__ __launch_bounds__(256) void rows_kernel(Rows p) {
-    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i < p.rows) one_row(p, i, threadIdx.x & 63);
-}
-// rows and sums of few tokens by one workgroup (64 tokens: 3.9 and 2.9 us in two launches)
-__global__ __launch_bounds__(1024) void rows_sums(Rows p, int mean, float* inv, float* out) {
-    for (long i = threadIdx.x >> 6; i < p.rows; i += 16) one_row(p, i, threadIdx.x & 63);
-    __syncthreads();
-    sums(p.rows, p.row, mean, inv, p.loss, out);
 }
 
 // ---------------------------------------------------------------------------------- G
@@ -685,10 +709,10 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         pad_rows<<<dim3(gx, (unsigned)(p.V < 32768 ? p.V : 32768)), 256, 0, st>>>(p.V, (int)p.D, (int)p.Dp, W, ldw, w);
         H = h, W = w, ldh = ldw = p.Dp;
     }
-    const long pairs = p.M * p.K;
-    const Targets t{pairs, p.V, (int)p.K, (int)p.Dp, a->top_dtype == THESEUS_VOCAB_BF16, H, W, ldh, ldw, a->index, a->top_values,
-                    a->teacher_lse, a->row_weight, a->ignore_index, inv_T, j, q, z, row};
-    targets_kernel<<<(unsigned)ceil_div(pairs, 4), 256, 0, st>>>(t);
+    const Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight,
+                    a->ignore_index, inv_T, j, q, row};
+    if (a->top_values) targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
+    else labels_kernel<<<(unsigned)ceil_div(p.M, 256), 256, 0, st>>>(t);
     const bool mean = inv != nullptr;
     auto sums = [&](float* to, const float* from, float* out) {
         sums_kernel<<<1, 1024, 0, st>>>(p.M, row, mean, to, from, out);
@@ -701,7 +725,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         auto logits = [&](int shape, long n0, long n1, int tile0) {
             const Operand X{Hp, ldh, (int)m, (int)p.Dp}, Y{W + n0 * ldw, ldw, (int)(n1 - n0), (int)p.Dp};
             const LogitsOut lo{(int)m, (int)(n1 - n0), (int)((n1 == p.V ? p.lde : n1) - n0), LOG2E * inv_T, part + tile0, p.tiles,
-                               p.grads ? e + n0 : nullptr, p.lde};
+                               p.grads ? e + n0 : nullptr, p.lde, j + i0 * p.K, z + i0 * p.K, (int)p.K, (int)n0};
             auto launch = [&](auto tag) {
                 using P = decltype(tag);
                 const Tiles tl = tiles(m, n1 - n0, P::BM, P::BN, p.Dp, 1);
@@ -718,15 +742,10 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         logits(p.logits, 0, p.main, 0);
         const int main_tiles = (int)ceil_div(p.main, LOGITS[p.logits].n);
         if (p.main < p.V) logits(p.rest, p.main, p.V, main_tiles);
-        const Rows rw{m, p.tiles, (int)p.K, part, row + i0, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
+        const Rows rw{m, p.tiles, (int)p.K, part, row + i0, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
                       a->temperature, LOG2E * inv_T, norm, losses ? losses + i0 : nullptr};
-        const bool now = p.pieces == 1 && (reduce || (mean && p.grads));
-        if (now && m <= 128) {
-            rows_sums<<<1, 1024, 0, st>>>(rw, mean, inv, reduce ? a->loss : nullptr);
-        } else {
-            rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
-            if (now) sums(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
-        }
+        rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
+        if (p.pieces == 1 && (reduce || (mean && p.grads))) sums(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
         if (!p.grads) continue;
 
         const long mp = up(m, BK);

@@ -565,3 +565,21 @@ def test_few_tokens_gradients_are_rounded_once(M, D, V):
     loss, dx, dw = _run(lambda a, b: vocab.linear_cross_entropy(a, b, labels.cuda(), reduction="none"), x, w, up, "none")
     _grad_close(dx, o["dx"], E @ w.double().abs())
     _grad_close(dw, o["dw"], E.t() @ x.double().abs())
+
+
+@gpu
+@pytest.mark.parametrize("M,K,V", [(300, 200, 260), (256, 64, 64), (70, 256, 1000)])
+def test_many_targets_in_one_tile(M, K, V):
+    """Every token has the same K targets side by side: all in one or two tiles' columns."""
+    print(f"  crowded M={M} K={K} V={V}", flush=True)
+    x, w, g = _inputs(M, 64, V, seed=K)
+    tv = torch.randn(M, K, generator=g)
+    ti = torch.arange(K).repeat(M, 1)
+    q = torch.softmax(tv.double(), -1)
+    one = torch.ones(M).double()
+    o = _oracle(x, w, _dense(M, V, ti, q), (q * q.log()).sum(-1), one, 1.0, one)
+    loss, dx, dw = _run(lambda a, b: vocab.linear_top_distillation(a, b, tv.cuda(), ti.cuda(), reduction="none"), x, w, torch.ones(M), "none")
+    qtol = 2.0 ** -19 * (q * q.log().abs()).sum(-1)  # (float32 exponentials and logarithms of q)
+    assert ((loss.double().cpu() - o["loss"]).abs() <= o["ltol"] + qtol).all()
+    _grad_close(dx, o["dx"], o["dx_tol"] + 2.0 ** -19 * q.sum(-1, keepdim=True) * w.double().abs().amax(0))
+    _grad_close(dw, o["dw"], o["dw_tol"] + 2.0 ** -19 * x.double().abs().sum(0))
