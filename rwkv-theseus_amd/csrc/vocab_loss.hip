@@ -375,32 +375,54 @@ struct Probs {
     float scale;
     bool twice;             // rows 32 .. 63 take what rounding left of rows 0 .. 31
 };
-// blockIdx.x: 2048 columns of row blockIdx.y; 8 columns a thread, then the targets among them
+// blockIdx.x: PROBS columns of a row, 8 at a time a thread, then the targets among them; the rows
+// backwards, from those that the logits wrote last to those that dhidden reads first
+constexpr int PROBS = 4096;
 __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
-    const long i = blockIdx.y;
-    const int n0 = blockIdx.x * 2048, n = n0 + threadIdx.x * 8;
+    __shared__ int js[THESEUS_VOCAB_MAX_TOP];
+    __shared__ float qs[THESEUS_VOCAB_MAX_TOP];
+    const long i = gridDim.y - 1 - blockIdx.y;
+    const int t = threadIdx.x, n0 = blockIdx.x * PROBS;
     uint16_t *row = p.e + i * p.lde, *rest = row + 32 * p.lde;
     const float f = i >= p.M ? 0.f : p.row_grad ? p.row[i].z * p.row_grad[i] : p.row[i].z;
+    constexpr int G = PROBS / 2048;
     if (f == 0.f) {
-        if (n < p.lde) {
-            *reinterpret_cast<uint4*>(row + n) = make_uint4(0, 0, 0, 0);
-            if (p.twice) *reinterpret_cast<uint4*>(rest + n) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int n = n0 + (g * 256 + t) * 8;
+            if (n < p.lde) {
+                *reinterpret_cast<uint4*>(row + n) = make_uint4(0, 0, 0, 0);
+                if (p.twice) *reinterpret_cast<uint4*>(rest + n) = make_uint4(0, 0, 0, 0);
+            }
         }
         return;
     }
+    uint4 u[G];
+    float top[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int n = min(n0 + (g * 256 + t) * 8, (int)p.lde - 8);
+        u[g] = *reinterpret_cast<const uint4*>(row + n);
+        top[g] = p.part[i * p.tiles + (n < p.main ? n / p.cols : p.main / p.cols + (n - p.main) / p.rest)].x;
+    }
+    if (t < p.K) {
+        js[t] = p.j[i * p.K + t];
+        qs[t] = p.q ? p.q[i * p.K + t] : 1.f;
+    }
     const float Q = p.row[i].x;
     const float2 norm = p.norm[i];
-    if (n < p.lde) {
-        const int tile = n < p.main ? n / p.cols : p.main / p.cols + (n - p.main) / p.rest;
-        const float g = f * Q * norm.y * exp2_((p.part[i * p.tiles + tile].x - norm.x) * p.scale);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int n = n0 + (g * 256 + t) * 8;
+        if (n >= p.lde) continue;
+        const float c = f * Q * norm.y * exp2_((top[g] - norm.x) * p.scale);
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        const uint4 u = *reinterpret_cast<const uint4*>(row + n);
-        const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t in[4] = {u[g].x, u[g].y, u[g].z, u[g].w};
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const h2 h = __builtin_bit_cast(h2, in[e]);
-            const float a = (float)h[0] * g, b = (float)h[1] * g;
+            const float a = (float)h[0] * c, b = (float)h[1] * c;
             hi[e] = f32x2_to_bf16x2(a, b);
             lo[e] = f32x2_to_bf16x2(a - __uint_as_float(hi[e] << 16), b - __uint_as_float(hi[e] & 0xffff0000u));
         }
@@ -408,18 +430,14 @@ __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
         if (p.twice) *reinterpret_cast<uint4*>(rest + n) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     __syncthreads();
-    if (threadIdx.x < p.K) {  // (equal indices of one token write the same value)
-        const long t = i * p.K + threadIdx.x;
-        const int v = p.j[t];
-        if (v >= n0 && v < n0 + 2048) {
+    if (t < p.K) {  // (equal indices of one token write the same value)
+        const int v = js[t];
+        if (v >= n0 && v < n0 + PROBS) {
             float q = 0.f;
-            if (!p.q) q = 1.f;
-            else
-                for (int k = 0; k < p.K; k++)
-                    if (p.j[i * p.K + k] == v) q += p.q[i * p.K + k];
-            const float g = f * (Q * (exp2_(fmaf(p.z[t] - norm.x, p.scale, E_SHIFT)) * norm.y) - q);
+            for (int k = 0; k < p.K; k++) q += js[k] == v ? qs[k] : 0.f;
+            const float g = f * (Q * (exp2_(fmaf(p.z[i * p.K + t] - norm.x, p.scale, E_SHIFT)) * norm.y) - q);
             row[v] = f32_to_bf16(g);
-            if (p.twice) rest[v] = f32_to_bf16(g - bf16_to_f32(row[v]));
+            if (p.twice) rest[v] = f32_to_bf16(g - bf16_to_f32(f32_to_bf16(g)));
         }
     }
 }
@@ -751,7 +769,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         const long mp = up(m, BK);
         const Probs pr{(int)m, (int)p.K, p.tiles, (int)(p.main < p.V ? p.main : p.lde), LOGITS[p.logits].n, LOGITS[p.rest].n, p.lde, e, part, row + i0, norm,
                        a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, LOG2E * inv_T, p.twice};
-        probs_kernel<<<dim3((unsigned)ceil_div(p.lde, 2048), (unsigned)(p.twice ? 32 : mp)), 256, 0, st>>>(pr);
+        probs_kernel<<<dim3((unsigned)ceil_div(p.lde, PROBS), (unsigned)(p.twice ? 32 : mp)), 256, 0, st>>>(pr);
         if (a->dhidden) {
             uint16_t* dh = static_cast<uint16_t*>(a->dhidden) + i0 * p.D;
             const long gm = p.twice ? 64 : m;  // rows of G
