@@ -546,11 +546,11 @@ __global__ __launch_bounds__(256) void zero_kernel(uint16_t* x, long n) {
 // ---------------------------------------------------------------------------------- host
 // The tiles each product can be made in, and what they were measured to cost: us of a step of 64
 // along the contraction and of the rest (first loads, epilogue) for as many tiles as run at
-// once (per_cu on each CU).  From 512 x 32768 logits at D = 1024 and 4096, dhidden of 512 x 4096
-// from 32768 and of 200 x 1024 from 32768, dweight of 16384 x 4096 from 512 and 4096 tokens.
-// plan() takes the cheapest: e.g. 200 x 32768 logits at D = 1024 25.2 us in 256 x 256 tiles and
-// 20.4 in 128 x 256; 64 x 65536 at D = 2560 62 us in 64 x 256 and 80 in 64 x 64; dhidden of
-// 64 x 768 from 8192 31 us in 256 x 256 tiles (8 parts) and 13 in 64 x 64 (16).
+// once (per_cu on each CU).  From logits of 64 .. 1024 x 131072 at D = 1280 and 2560, dhidden of as
+// many x 2560 from 131072, dweight of 131072 x 2560 from 64 .. 1024 tokens, and small ones.
+// plan() takes the cheapest: e.g. 128 tokens' logits there take 152, 127, 176 and 234 us in the
+// four shapes, 512 tokens' 273, 346, 564 and 734; dhidden of 64 x 768 from 8192 31 us in 256 x 256
+// tiles (8 parts) and 13 in 64 x 64 (16).
 struct Shape {
     int m, n, per_cu;
     double step, fixed;
@@ -559,16 +559,17 @@ using Logits0 = Product<256, 256, 4, 2, 2, RowK, RowK>;
 using Logits1 = Product<128, 256, 2, 4, 3, RowK, RowK>;
 using Logits2 = Product<64, 256, 1, 8, 4, RowK, RowK>;
 using Logits3 = Product<64, 64, 2, 4, 4, RowK, RowK>;
-constexpr Shape LOGITS[] = {{256, 256, 1, 1.5, 7}, {128, 256, 1, .83, 5}, {64, 256, 1, .58, 4}, {64, 64, 2, .4, 2.3}};
+constexpr Shape LOGITS[] = {{256, 256, 1, 1.5, 7}, {128, 256, 1, .95, 5}, {64, 256, 1, .78, 4}, {64, 64, 2, .5, 2.3}};
 using Dhidden0 = Product<256, 256, 4, 2, 2, RowK, RowN>;
 using Dhidden1 = Product<128, 128, 2, 4, 2, RowK, RowN>;
 using Dhidden2 = Product<64, 256, 1, 8, 4, RowK, RowN>;
 using Dhidden3 = Product<64, 64, 2, 4, 4, RowK, RowN>;
-constexpr Shape DHIDDEN[] = {{256, 256, 1, 1.8, 12}, {128, 128, 1, .78, 5}, {64, 256, 1, .78, 8}, {64, 64, 1, .38, 3}};
+constexpr Shape DHIDDEN[] = {{256, 256, 1, 1.75, 12}, {128, 128, 1, .8, 5}, {64, 256, 1, .85, 8}, {64, 64, 1, .45, 3}};
 using Dweight0 = Product<256, 256, 4, 2, 2, RowN, RowN>;
 using Dweight1 = Product<128, 128, 2, 4, 2, RowN, RowN>;
-constexpr Shape DWEIGHT[] = {{256, 256, 1, 1.62, 7.5}, {128, 128, 2, 1.06, 3.1}};
+constexpr Shape DWEIGHT[] = {{256, 256, 1, 1.62, 6.7}, {128, 128, 2, 1.03, 4.1}};
 constexpr double LAUNCH = 3, BYTES = 5e6;  // us of one more launch; bytes a us
+constexpr int TOGETHER = 1024;             // rows of a product whose tiles run together (see tiles())
 
 static long up(long x, long to) { return (x + to - 1) / to * to; }
 static long ceil_div(long x, long y) { return (x + y - 1) / y; }
@@ -604,20 +605,21 @@ static int check(const theseus_vocab_loss_args* a) {
     return THESEUS_WKV7_OK;
 }
 
-// us of a product of M x N outputs and `steps` steps
-static double cost(const Shape& c, long M, long N, long steps, int cus) {
+// us of a product of M x N outputs: rounds of tiles, or the reading of the weight behind it (`bytes`,
+// once for TOGETHER rows), whichever is longer, and a little of the other
+static double both(double a, double b) { return a > b ? a + .1 * b : b + .1 * a; }
+static double cost(const Shape& c, long M, long N, long steps, double bytes, int cus) {
     const long t = ceil_div(M, c.m) * ceil_div(N, c.n);
-    return (double)ceil_div(t, (long)cus * c.per_cu) * (c.fixed + (double)steps * c.step);
+    return both((double)ceil_div(t, (long)cus * c.per_cu) * (c.fixed + (double)steps * c.step), ceil_div(M, TOGETHER) * bytes / BYTES);
 }
-// the cheapest shape; none is faster than `least`, where those that do their own part sooner hide more
-template <int N> static int best(const Shape (&c)[N], long M, long cols, long steps, int cus, double least, double* us) {
+template <int N> static int best(const Shape (&c)[N], long M, long cols, long steps, double bytes, int cus, double* us) {
     int b = 0;
     double u = 0;
     for (int i = 0; i < N; i++) {
-        const double own = cost(c[i], M, cols, steps, cus), x = (own < least ? least : own) + .05 * own;
+        const double x = cost(c[i], M, cols, steps, bytes, cus);
         if (i == 0 || x < u) b = i, u = x;
     }
-    if (us) *us = u;
+    *us = u;
     return b;
 }
 
@@ -637,35 +639,38 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     p.twice = p.M <= TWICE;
     const int cus = device_cus();
     const long steps = p.Dp / BK;
-    // one shape for all columns (no less than the weight's reading), or full rounds of the largest and the remaining columns in another
-    // (1021 x 50001 at D = 2560: 784 tiles of 256 x 256, 3.06 rounds of 256 CUs)
-    double one;
-    p.logits = best(LOGITS, rows, p.V, steps, cus, (double)p.V * p.Dp * 2 / BYTES, &one);
-    p.main = p.V, p.rest = p.logits;
-    const Shape& big = LOGITS[0];
-    const long tm = ceil_div(rows, big.m), rounds = tm * ceil_div(p.V, big.n) / cus, n = rounds * cus / tm * big.n;
-    if (n > 0 && n < p.V) {
-        double us;
-        const int r = best(LOGITS, rows, p.V - n, steps, cus, 0, &us);
-        if (1.05 * cost(big, rows, n, steps, cus) + us + LAUNCH < one) p.logits = 0, p.main = n, p.rest = r;
+    // one shape for all columns, or full rounds of one and the remaining columns in another
+    // (1021 x 50001 at D = 2560: 784 tiles of 256 x 256, 3.06 rounds of 256 CUs; 296 -> 241 us)
+    double us, least;
+    const double column = (double)p.Dp * 2;
+    p.logits = p.rest = best(LOGITS, rows, p.V, steps, p.V * column, cus, &least);
+    p.main = p.V;
+    for (int i = 0; i < (int)(sizeof LOGITS / sizeof *LOGITS); i++) {
+        const Shape& c = LOGITS[i];
+        const long tm = ceil_div(rows, c.m), slots = (long)cus * c.per_cu, n = tm * ceil_div(p.V, c.n) / slots * slots / tm * c.n;
+        if (n <= 0 || n >= p.V) continue;
+        const int r = best(LOGITS, rows, p.V - n, steps, (p.V - n) * column, cus, &us);
+        us += cost(c, rows, n, steps, n * column, cus) + LAUNCH;
+        if (us < least) least = us, p.logits = i, p.main = n, p.rest = r;
     }
     p.tiles = (int)(ceil_div(p.main, LOGITS[p.logits].n) + ceil_div(p.V - p.main, LOGITS[p.rest].n));
     if (a->dhidden) {
         // its contraction, the vocabulary, is long and its tiles few: float32 parts that fill the
         // CUs, added afterwards
         const long all = p.lde / BK, gm = p.twice ? 64 : rows;
-        double least = 0;
+        const double read = (double)ceil_div(gm, TOGETHER) * p.V * column / BYTES;
+        least = 0;
         for (int i = 0; i < (int)(sizeof DHIDDEN / sizeof *DHIDDEN); i++) {
             const Shape& c = DHIDDEN[i];
             const int t = (int)(ceil_div(gm, c.m) * ceil_div(p.D, c.n));
             for (int s = 1; s <= 64 && s <= all; s += s < 8 ? 1 : s / 4) {  // (every call comes by here: few candidates)
-                const double us = (t * s + cus * c.per_cu - 1) / (cus * c.per_cu) * (c.fixed + ((int)all + s - 1) / s * c.step) +
-                                  (s > 1 ? LAUNCH + (double)s * gm * p.D * 8 / BYTES : 0);
+                us = both((t * s + cus * c.per_cu - 1) / (cus * c.per_cu) * (c.fixed + ((int)all + s - 1) / s * c.step), read) +
+                     (s > 1 ? LAUNCH + (double)s * gm * p.D * 8 / BYTES : 0);
                 if (least == 0 || us < least) least = us, p.dhidden = i, p.splits = s;
             }
         }
     }
-    if (a->dweight) p.dweight = best(DWEIGHT, p.V, p.D, ceil_div(rows, BK), cus, 0, nullptr);
+    if (a->dweight) p.dweight = best(DWEIGHT, p.V, p.D, ceil_div(rows, BK), 0, cus, &us);
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -695,7 +700,10 @@ static Tiles tiles(long M, long N, int BM, int BN, long K, int splits) {
     t.all = (int)(K / BK);
     t.steps = (int)ceil_div(t.all, splits);
     t.splits = (int)ceil_div(t.all, t.steps);
-    t.group = t.m < 4 ? t.m : 4;
+    // m tiles that run together, 1024 rows: with 256 x 256 tiles and 8192 rows 4 tiles took 4.46 ms for
+    // dweight, 8 4.63 and 2 4.51; smaller tiles of few rows would read the other operand again
+    const int group = TOGETHER / BM;
+    t.group = t.m < group ? t.m : group;
     return t;
 }
 
