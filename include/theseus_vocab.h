@@ -66,7 +66,18 @@ typedef struct theseus_vocab_loss_args {
     long long piece_rows;    /* tokens whose probabilities (V 16-bit values each) are in the
                                 workspace at a time, 0: as many as 2 GiB hold.  Rounded up to
                                 a multiple of 256                                              */
+    void* kept;              /* theseus_vocab_loss_kept_size bytes: what the forward of a call with
+                                reduction NONE leaves for its gradients                        */
+    int phase;               /* theseus_vocab_phase                                            */
 } theseus_vocab_loss_args;
+
+/* ALL: the losses and, where asked for, the gradients.  With kept of the size given, reduction
+ * NONE and gradients that are wanted later: FORWARD writes the losses and kept (dhidden, dweight
+ * and row_grad are not looked at), GRADIENTS with the same other arguments reads kept (and
+ * destroys it) and writes the gradients without forming the logits again. */
+enum theseus_vocab_phase { THESEUS_VOCAB_ALL = 0, THESEUS_VOCAB_FORWARD = 1, THESEUS_VOCAB_GRADIENTS = 2 };
+/* most that is kept: a call with more in its row pieces (V 16-bit values a token) keeps nothing */
+#define THESEUS_VOCAB_MAX_KEPT (256ll << 20)
 
 /* c_i of the gradients is row_grad_i row_weight_i, over the sum of the weights for MEAN.  A
  * token whose c_i (loss: row_weight_i) is 0 adds nothing (its hidden state has to be finite all
@@ -74,6 +85,7 @@ typedef struct theseus_vocab_loss_args {
  * Target entries with q = 0 (a teacher's -inf) are not looked at; one with q != 0 whose index is
  * outside the vocabulary makes the token's loss NaN (and adds nothing to the gradients but p). */
 size_t theseus_vocab_loss_workspace_size(const theseus_vocab_loss_args* args);
+size_t theseus_vocab_loss_kept_size(const theseus_vocab_loss_args* args); /* 0: nothing can be kept */
 int theseus_vocab_loss(const theseus_vocab_loss_args* args, void* workspace, size_t workspace_bytes,
                        hipStream_t stream);
 

@@ -244,7 +244,7 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
     static void* optr(const Opt& t) { return t ? t->data_ptr() : nullptr; }
     static void call(const Tensor& h, const Tensor& w, const Tensor& index, const Opt& top, const Opt& lse, const Opt& weight,
                      int64_t ignore, double T, int64_t reduction, int64_t piece, const Tensor& loss, const Tensor& row_grad,
-                     const Tensor& dh, const Tensor& dw) {
+                     const Tensor& dh, const Tensor& dw, Tensor* kept = nullptr) {
         theseus_vocab_loss_args a{};
         a.rows = h.size(0), a.vocab = w.size(0), a.width = (int)h.size(1), a.targets = top ? (int)top->size(1) : 1;
         a.hidden = h.data_ptr(), a.weight = w.data_ptr();
@@ -254,6 +254,14 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
         a.reduction = (int)reduction, a.teacher_lse = static_cast<float*>(optr(lse)), a.row_weight = static_cast<float*>(optr(weight));
         a.ignore_index = ignore, a.temperature = (float)T, a.loss = fptr(loss), a.row_grad = fptr(row_grad);
         a.dhidden = ptr(dh), a.dweight = ptr(dw), a.piece_rows = piece;
+        if (kept) {  // an empty tensor: the forward, into what it can keep; else the gradients from it
+            a.phase = kept->defined() ? THESEUS_VOCAB_GRADIENTS : THESEUS_VOCAB_FORWARD;
+            if (!kept->defined()) {
+                *kept = scratch(theseus_vocab_loss_kept_size(&a), h);
+                if (!kept->defined()) a.phase = THESEUS_VOCAB_ALL;
+            }
+            a.kept = ptr(*kept);
+        }
         const size_t need = theseus_vocab_loss_workspace_size(&a);
         const Tensor ws = scratch(need, h);
         raise_status(theseus_vocab_loss(&a, ptr(ws), need, stream_of(h)), "theseus_vocab");
@@ -266,7 +274,7 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
                           const Opt& weight, int64_t ignore, double T, int64_t reduction, int64_t piece) {
         c10::OptionalDeviceGuard guard(h.device());
         const Tensor loss = new_loss(h, reduction);
-        Tensor dh, dw;
+        Tensor dh, dw, kept;
         if (reduction != THESEUS_VOCAB_NONE) {
             if (h.requires_grad()) dh = at::empty(h.sizes(), h.options());
             if (w.requires_grad()) dw = at::empty(w.sizes(), w.options());
@@ -276,7 +284,9 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
         } else {
             ctx->saved_data["made"] = false;
         }
-        call(h, w, index, top, lse, weight, ignore, T, reduction, piece, loss, Tensor(), dh, dw);
+        call(h, w, index, top, lse, weight, ignore, T, reduction, piece, loss, Tensor(), dh, dw,
+             reduction == THESEUS_VOCAB_NONE ? &kept : nullptr);
+        ctx->saved_data["kept"] = kept.defined() ? at::IValue(kept) : at::IValue();
         ctx->save_for_backward({h, w});
         ctx->saved_data["index"] = index;
         ctx->saved_data["top"] = top, ctx->saved_data["lse"] = lse, ctx->saved_data["weight"] = weight;
@@ -300,8 +310,10 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
             if (ctx->needs_input_grad(0)) dh = at::empty(s[0].sizes(), s[0].options());
             if (ctx->needs_input_grad(1)) dw = at::empty(s[1].sizes(), s[1].options());
             auto opt = [&](const char* k) { return d[k].isTensor() ? Opt(d[k].toTensor()) : Opt(); };
+            Tensor kept = tensor(d["kept"]);
+            d["kept"] = at::IValue();
             call(s[0], s[1], d["index"].toTensor(), opt("top"), opt("lse"), opt("weight"), d["ignore"].toInt(), d["T"].toDouble(),
-                 reduction, d["piece"].toInt(), Tensor(), reduction == THESEUS_VOCAB_NONE ? grad : Tensor(), dh, dw);
+                 reduction, d["piece"].toInt(), Tensor(), reduction == THESEUS_VOCAB_NONE ? grad : Tensor(), dh, dw, kept.defined() ? &kept : nullptr);
         }
         if (reduction != THESEUS_VOCAB_NONE)
             raise_status(theseus_vocab_scale(ptr(dh), dh.defined() ? dh.numel() : 0, ptr(dw), dw.defined() ? dw.numel() : 0, fptr(grad),

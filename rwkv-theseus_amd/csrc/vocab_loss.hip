@@ -19,7 +19,9 @@
 //
 // The gradients take three products of 2 M V D operations, not the four of a backward that
 // forms the logits again: with SUM and MEAN the upstream gradient is one number, applied to the
-// results (theseus_vocab_scale).
+// results (theseus_vocab_scale); with NONE, up to THESEUS_VOCAB_MAX_KEPT bytes of exponentials are
+// kept for the backward (1021 tokens of 50001 at width 2560: 990 -> 760 us), which otherwise makes them
+// again.
 #include "../../include/theseus_vocab.h"
 #include "../../include/theseus_wkv7.h"
 
@@ -581,7 +583,7 @@ struct Plan {
     int logits, rest, dhidden, dweight;  // indices into the shapes
     long main;                        // columns of the vocabulary in shape `logits`, the others in `rest`
     int splits;                       // of dhidden's contraction
-    size_t j, q, row, z, part, norm, loss, inv, e, acc, parts, hidden, weight, bytes;
+    size_t j, q, row, z, part, norm, loss, inv, e, kept, acc, parts, hidden, weight, bytes;
 };
 
 constexpr long MAX_PIECE = 32768;  // rows: a grid's y dimension
@@ -601,7 +603,9 @@ static int check(const theseus_vocab_loss_args* a) {
     // (a tile's rows are addressed by 32-bit byte offsets)
     if (a->hidden_stride > (1ll << 21) || a->weight_stride > (1ll << 21)) return THESEUS_WKV7_ERR_SHAPE;
     if (a->top_dtype != THESEUS_VOCAB_BF16 && a->top_dtype != THESEUS_VOCAB_FP32) return THESEUS_WKV7_ERR_DTYPE;
-    if (a->reduction < THESEUS_VOCAB_NONE || a->reduction > THESEUS_VOCAB_MEAN) return THESEUS_WKV7_ERR_FLAGS;
+    if (a->reduction < THESEUS_VOCAB_NONE || a->reduction > THESEUS_VOCAB_MEAN || a->phase < THESEUS_VOCAB_ALL ||
+        a->phase > THESEUS_VOCAB_GRADIENTS || (a->phase != THESEUS_VOCAB_ALL && a->reduction != THESEUS_VOCAB_NONE))
+        return THESEUS_WKV7_ERR_FLAGS;
     return THESEUS_WKV7_OK;
 }
 
@@ -628,7 +632,7 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     p.M = a->rows, p.V = a->vocab, p.D = a->width, p.K = a->targets;
     p.Dp = up(p.D, BK);
     p.pad = p.D != p.Dp || a->hidden_stride % 8 || a->weight_stride % 8 || ((uintptr_t)a->hidden | (uintptr_t)a->weight) % 16;
-    p.grads = a->dhidden || a->dweight;
+    p.grads = a->dhidden || a->dweight || a->phase != THESEUS_VOCAB_ALL;
     p.lde = up(p.V, BK);
     long cap = a->piece_rows ? up(a->piece_rows, 256) : p.grads ? (2l << 30) / (2 * p.lde) / 256 * 256 : MAX_PIECE;
     cap = cap < 256 ? 256 : cap > MAX_PIECE ? MAX_PIECE : cap;
@@ -686,11 +690,14 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     p.norm = take(rows * 8);
     p.part = take((size_t)rows * p.tiles * 8);
     p.e = take(p.grads ? (size_t)up(rows, BK) * p.lde * 2 : 0);
+    p.kept = at;
+    if (a->phase != THESEUS_VOCAB_ALL) at = 0;  // (what is above lies in a->kept)
     p.acc = take(a->dweight && p.pieces > 1 ? (size_t)p.V * up(p.D, 4) * 4 : 0);
     p.parts = take(p.splits > 1 || p.twice ? (size_t)p.splits * (p.twice ? 64 : rows) * up(p.D, 4) * 4 : 0);
     p.hidden = take(p.pad ? (size_t)p.M * p.Dp * 2 : 0);
     p.weight = take(p.pad ? (size_t)p.V * p.Dp * 2 : 0);
     p.bytes = at;
+    if (a->phase == THESEUS_VOCAB_FORWARD && !p.pad) p.bytes = 0;
     return p;
 }
 
@@ -708,7 +715,9 @@ static Tiles tiles(long M, long N, int BM, int BN, long K, int splits) {
 }
 
 static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hipStream_t st) {
-    auto at = [&](size_t off) { return ws + off; };
+    uint8_t* first = a->phase != THESEUS_VOCAB_ALL ? static_cast<uint8_t*>(a->kept) : ws;
+    auto at = [&](size_t off) { return first + off; };
+    const bool forward = a->phase != THESEUS_VOCAB_GRADIENTS, gradients = p.grads && a->phase != THESEUS_VOCAB_FORWARD;
     int* j = reinterpret_cast<int*>(at(p.j));
     float* q = a->top_values ? reinterpret_cast<float*>(at(p.q)) : nullptr;
     float4* row = reinterpret_cast<float4*>(at(p.row));
@@ -729,7 +738,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         return 0;
     }
     if (p.pad) {
-        uint16_t *h = reinterpret_cast<uint16_t*>(at(p.hidden)), *w = reinterpret_cast<uint16_t*>(at(p.weight));
+        uint16_t *h = reinterpret_cast<uint16_t*>((ws + p.hidden)), *w = reinterpret_cast<uint16_t*>((ws + p.weight));
         const unsigned gx = (unsigned)ceil_div(p.Dp, 256);
         pad_rows<<<dim3(gx, (unsigned)(p.M < 32768 ? p.M : 32768)), 256, 0, st>>>(p.M, (int)p.D, (int)p.Dp, H, ldh, h);
         pad_rows<<<dim3(gx, (unsigned)(p.V < 32768 ? p.V : 32768)), 256, 0, st>>>(p.V, (int)p.D, (int)p.Dp, W, ldw, w);
@@ -737,7 +746,8 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
     }
     const Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight,
                     a->ignore_index, inv_T, j, q, row};
-    if (a->top_values) targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
+    if (!forward) {
+    } else if (a->top_values) targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
     else labels_kernel<<<(unsigned)ceil_div(p.M, 256), 256, 0, st>>>(t);
     const bool mean = inv != nullptr;
     auto sums = [&](float* to, const float* from, float* out) {
@@ -765,14 +775,15 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
                 default: launch(Logits3{});
             }
         };
-        logits(p.logits, 0, p.main, 0);
-        const int main_tiles = (int)ceil_div(p.main, LOGITS[p.logits].n);
-        if (p.main < p.V) logits(p.rest, p.main, p.V, main_tiles);
+        if (forward) {
+            logits(p.logits, 0, p.main, 0);
+            if (p.main < p.V) logits(p.rest, p.main, p.V, (int)ceil_div(p.main, LOGITS[p.logits].n));
+        }
         const Rows rw{m, p.tiles, (int)p.K, part, row + i0, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
                       a->temperature, LOG2E * inv_T, norm, losses ? losses + i0 : nullptr};
-        rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
+        if (forward) rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
         if (p.pieces == 1 && (reduce || (mean && p.grads))) sums(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
-        if (!p.grads) continue;
+        if (!gradients) continue;
 
         const long mp = up(m, BK);
         const Probs pr{(int)m, (int)p.K, p.tiles, (int)(p.main < p.V ? p.main : p.lde), LOGITS[p.logits].n, LOGITS[p.rest].n, p.lde, e, part, row + i0, norm,
@@ -782,7 +793,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
             uint16_t* dh = static_cast<uint16_t*>(a->dhidden) + i0 * p.D;
             const long gm = p.twice ? 64 : m;  // rows of G
             const Operand GX{e, p.lde, (int)gm, (int)p.lde}, WY{W, ldw, (int)p.Dp, (int)p.V};
-            float* parts = reinterpret_cast<float*>(at(p.parts));
+            float* parts = reinterpret_cast<float*>((ws + p.parts));
             const GradOut go{(int)gm, (int)p.D, dh, p.D, parts, up(p.D, 4), 0, 0, a->temperature, inv};
             auto dhidden = [&](auto tag) {
                 using P = decltype(tag);
@@ -803,7 +814,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         }
         if (a->dweight) {
             const Operand GX{e, p.lde, (int)p.lde, (int)mp}, HY{Hp, ldh, (int)p.Dp, (int)m, p.twice};
-            const GradOut go{(int)p.V, (int)p.D, static_cast<uint16_t*>(a->dweight), p.D, reinterpret_cast<float*>(at(p.acc)),
+            const GradOut go{(int)p.V, (int)p.D, static_cast<uint16_t*>(a->dweight), p.D, reinterpret_cast<float*>((ws + p.acc)),
                              up(p.D, 4), piece == 0, piece == p.pieces - 1, a->temperature, inv};
             auto dweight = [&](auto tag) {
                 using P = decltype(tag);
@@ -827,9 +838,21 @@ size_t theseus_vocab_loss_workspace_size(const theseus_vocab_loss_args* args) {
     return vocab::check(args) ? 0 : vocab::plan(args).bytes;
 }
 
+size_t theseus_vocab_loss_kept_size(const theseus_vocab_loss_args* args) {
+    if (vocab::check(args) || !args->rows || args->reduction != THESEUS_VOCAB_NONE) return 0;
+    theseus_vocab_loss_args a = *args;
+    a.phase = THESEUS_VOCAB_FORWARD;
+    const vocab::Plan p = vocab::plan(&a);
+    return p.pieces == 1 && p.kept <= (size_t)THESEUS_VOCAB_MAX_KEPT ? p.kept : 0;
+}
+
 int theseus_vocab_loss(const theseus_vocab_loss_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (int e = vocab::check(a)) return e;
     if (a->rows && (!a->hidden || !a->weight || !a->index)) return THESEUS_WKV7_ERR_NULL;
+    if (a->phase != THESEUS_VOCAB_ALL) {
+        if (!theseus_vocab_loss_kept_size(a)) return THESEUS_WKV7_ERR_SHAPE;
+        if (!a->kept) return THESEUS_WKV7_ERR_NULL;
+    }
     const vocab::Plan p = vocab::plan(a);
     if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return THESEUS_WKV7_ERR_WORKSPACE;
     vocab::run(a, p, static_cast<uint8_t*>(workspace), stream);

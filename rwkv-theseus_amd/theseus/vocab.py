@@ -14,7 +14,8 @@ training the whole student takes next: losses on the head's output that never ho
 The losses are differentiable in ``hidden`` and ``weight`` (bfloat16; under autocast other types
 are cast as ``torch.nn.functional.linear`` casts them).  With ``reduction="mean"`` or ``"sum"``
 the gradients are made together with the loss, in three products, and the backward multiplies
-them by the upstream gradient; with ``"none"`` the backward forms the probabilities again.
+them by the upstream gradient; with ``"none"`` the backward makes them, from 16-bit exponentials
+that the forward keeps where they take at most 256 MiB, and else from the logits formed again.
 A second backward through the same loss (retain_graph) makes the gradients anew.
 """
 from __future__ import annotations
@@ -41,7 +42,7 @@ class LossArgs(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("teacher_lse", "row_weight")]
                 + [("ignore_index", ctypes.c_longlong), ("temperature", ctypes.c_float)]
                 + [(n, ctypes.c_void_p) for n in ("loss", "row_grad", "dhidden", "dweight")]
-                + [("piece_rows", ctypes.c_longlong)])
+                + [("piece_rows", ctypes.c_longlong), ("kept", ctypes.c_void_p), ("phase", ctypes.c_int)])
 
 
 _bound = None
@@ -54,6 +55,8 @@ def _lib():
         vp, i32, i64, sz, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t, ctypes.c_float
         lib.theseus_vocab_loss_workspace_size.argtypes = [ctypes.POINTER(LossArgs)]
         lib.theseus_vocab_loss_workspace_size.restype = sz
+        lib.theseus_vocab_loss_kept_size.argtypes = [ctypes.POINTER(LossArgs)]
+        lib.theseus_vocab_loss_kept_size.restype = sz
         lib.theseus_vocab_loss.argtypes = [ctypes.POINTER(LossArgs), vp, sz, vp]
         lib.theseus_vocab_loss.restype = i32
         lib.theseus_vocab_scale.argtypes = [vp, i64, vp, i64, vp, vp]
@@ -86,19 +89,32 @@ class _Call:
         self.rows, self.vocab, self.width = hidden.shape[0], weight.shape[0], hidden.shape[1]
         self.device = hidden.device
 
-    def run(self, hidden, weight, loss, row_grad, dhidden, dweight):
-        lib = _lib()
+    def args(self, hidden, weight, loss, row_grad, dhidden, dweight):
         p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        a = LossArgs(self.rows, self.vocab, self.width, self.targets, p(hidden), p(weight),
-                     max(hidden.stride(0), self.width), max(weight.stride(0), self.width),
-                     p(self.index), p(self.top_values),
-                     0 if self.top_values is None else _DTYPES[self.top_values.dtype], _REDUCTIONS[self.reduction],
-                     p(self.teacher_lse), p(self.row_weight), self.ignore_index, self.temperature, p(loss), p(row_grad),
-                     p(dhidden), p(dweight), self.piece_rows)
+        return LossArgs(self.rows, self.vocab, self.width, self.targets, p(hidden), p(weight),
+                        max(hidden.stride(0), self.width), max(weight.stride(0), self.width),
+                        p(self.index), p(self.top_values),
+                        0 if self.top_values is None else _DTYPES[self.top_values.dtype], _REDUCTIONS[self.reduction],
+                        p(self.teacher_lse), p(self.row_weight), self.ignore_index, self.temperature, p(loss), p(row_grad),
+                        p(dhidden), p(dweight), self.piece_rows, None, 0)
+
+    def run(self, hidden, weight, loss=None, row_grad=None, dhidden=None, dweight=None, kept=None):
+        """``kept`` None: the whole call; True: the forward, returning what it keeps for the gradients
+        (None where that is too much); a tensor: the gradients from what the forward kept."""
+        lib = _lib()
+        a = self.args(hidden, weight, loss, row_grad, dhidden, dweight)
         with torch.cuda.device(self.device):
+            if kept is True:
+                nbytes = int(lib.theseus_vocab_loss_kept_size(ctypes.byref(a)))
+                kept = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+                a.phase = 0 if kept is None else 1
+            elif kept is not None:
+                a.phase = 2
+            a.kept = None if kept is None else kept.data_ptr()
             nbytes = int(lib.theseus_vocab_loss_workspace_size(ctypes.byref(a)))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             _check(lib.theseus_vocab_loss(ctypes.byref(a), ws.data_ptr(), nbytes, _stream(self.device)))
+        return kept
 
     def new_loss(self):
         return torch.empty(self.rows if self.reduction == "none" else (), dtype=torch.float32, device=self.device)
@@ -109,13 +125,12 @@ class _Loss(torch.autograd.Function):
     def forward(ctx, hidden, weight, call):
         loss = call.new_loss()
         need_h, need_w = ctx.needs_input_grad[:2]
-        ctx.call, ctx.made = call, None
-        dh = dw = None
-        if call.reduction != "none":
-            dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need_h else None
-            dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None
-            ctx.made = (dh, dw)
-        call.run(hidden, weight, loss, None, dh, dw)
+        ctx.call, ctx.made, ctx.kept = call, None, None
+        if call.reduction == "none":
+            ctx.kept = call.run(hidden, weight, loss, kept=True)
+        else:
+            ctx.made = _Loss._like(hidden, need_h), _Loss._like(weight, need_w)
+            call.run(hidden, weight, loss, None, *ctx.made)
         ctx.save_for_backward(hidden, weight)
         return loss
 
@@ -129,14 +144,18 @@ class _Loss(torch.autograd.Function):
         return (*made, None)
 
     @staticmethod
+    def _like(x, wanted):
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device) if wanted else None
+
+    @staticmethod
     def _gradients(ctx, grad):
-        call, made, ctx.made = ctx.call, ctx.made, None
+        call, made, kept = ctx.call, ctx.made, ctx.kept
+        ctx.made = ctx.kept = None
         if made is None:
             hidden, weight = ctx.saved_tensors
             need_h, need_w = ctx.needs_input_grad[:2]
-            made = (torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need_h else None,
-                    torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need_w else None)
-            call.run(hidden, weight, None, grad if call.reduction == "none" else None, *made)
+            made = _Loss._like(hidden, need_h), _Loss._like(weight, need_w)
+            call.run(hidden, weight, None, grad if call.reduction == "none" else None, *made, kept=kept)
         if call.reduction != "none":
             xy = [v for x in made for v in ((None, 0) if x is None else (x.data_ptr(), x.numel()))]
             with torch.cuda.device(call.device):
@@ -205,7 +224,7 @@ def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_ind
         loss = _Loss.apply(h, w, call)
     else:
         loss = call.new_loss()
-        call.run(h, w, loss, None, None, None)
+        call.run(h, w, loss)
     return loss.reshape(tokens) if reduction == "none" else loss
 
 

@@ -583,3 +583,39 @@ def test_many_targets_in_one_tile(M, K, V):
     assert ((loss.double().cpu() - o["loss"]).abs() <= o["ltol"] + qtol).all()
     _grad_close(dx, o["dx"], o["dx_tol"] + 2.0 ** -19 * q.sum(-1, keepdim=True) * w.double().abs().amax(0))
     _grad_close(dw, o["dw"], o["dw_tol"] + 2.0 ** -19 * x.double().abs().sum(0))
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_kept_exponentials_give_the_same_gradients(native, monkeypatch):
+    """reduction="none": the first backward from what the forward kept, the second from the logits formed again;
+    a piece of the tokens at a time nothing is kept."""
+    if not native:
+        monkeypatch.setattr(vocab, "_native", lambda *xs: None)
+    x, w, g = _inputs(300, 72, 700)  # (72: padded copies in both)
+    labels = torch.randint(700, (300,), generator=g).cuda()
+    up = torch.rand(300, generator=g).cuda()
+    a, b = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    loss = vocab.linear_cross_entropy(a, b, labels, reduction="none")
+    g1 = torch.autograd.grad(loss, (a, b), up, retain_graph=True)
+    g2 = torch.autograd.grad(loss, (a, b), up)
+    for p, q in zip(g1, g2):
+        assert torch.equal(p, q)
+    cut = vocab.linear_cross_entropy(a, b, labels, reduction="none", piece_rows=256)
+    assert torch.equal(cut, loss)
+    o = _oracle(x, w, _dense(300, 700, labels.cpu()[:, None], torch.ones(300, 1)), 0.0, torch.ones(300).double(), 1.0, up.double().cpu())
+    for got in (g1, torch.autograd.grad(cut, (a, b), up)):
+        _grad_close(got[0], o["dx"], o["dx_tol"])
+        _grad_close(got[1], o["dw"], o["dw_tol"])
+
+
+def test_kept_sizes_and_phases_are_refused_without_launching():
+    lib, p = vocab._lib(), 1 << 20
+    base = dict(rows=1000, vocab=50000, width=64, targets=1, hidden=p, weight=p, hidden_stride=64, weight_stride=64, index=p,
+                temperature=1.0, reduction=0, loss=p)
+    kept = lambda **kw: lib.theseus_vocab_loss_kept_size(ctypes.byref(vocab.LossArgs(**{**base, **kw})))  # noqa: E731
+    call = lambda **kw: lib.theseus_vocab_loss(ctypes.byref(vocab.LossArgs(**{**base, **kw})), p, 1 << 40, None)  # noqa: E731
+    assert 1000 * 50000 * 2 <= kept() <= 256 << 20
+    assert kept(rows=0) == kept(reduction=2) == kept(vocab=200000) == kept(piece_rows=256) == kept(vocab=0) == 0
+    assert call(phase=3) == 7 and call(phase=1, reduction=1, kept=p) == 7
+    assert call(phase=1) == 3 and call(phase=1, vocab=200000, kept=p) == 1
