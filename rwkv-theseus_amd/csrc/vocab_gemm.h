@@ -118,7 +118,7 @@ template <Lay L, int B, bool PERM> struct Loader {
     }
     // piece j of the next step into the tile at `lds`; advance() after the last one
     __device__ __forceinline__ void issue(uint32_t lds, int j, int wave) const {
-        const int last = L == RowK ? rows_left - 1 : min(rows_left - 1, BK - 1);
+        const int last = min(rows_left, L == RowK ? B : BK) - 1;  // (of the tile: 32 bits hold its rows' offsets)
         const uint32_t r = min(row + ((uint32_t)(8 * PER * j) & mask) * ld2, (uint32_t)max(last, 0) * ld2);
         dma(lds + (uint32_t)(wave + 8 * j) * 1024, base, r + col);
     }
