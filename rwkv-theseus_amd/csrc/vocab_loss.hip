@@ -487,6 +487,8 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
         if (MODE == OutPart || !o.last) return;
     }
     __syncthreads();
+    // (dweight is as large as the weight and not read again here: streamed past the caches it leaves them
+    // to the weight and its own writing to the memory; 33 tokens, 56136 x 5120: the call 429 -> 374 us)
     const bool eight = (o.ldc & 7) == 0 && ((uintptr_t)o.c & 15) == 0;  // (N = ldc: eight columns are in or out together)
     const float f = o.inv ? o.T * *o.inv : o.T;
     store_rows<P>(lds, [&](int tn, int tm) {
@@ -496,7 +498,9 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
         if (m0 + m >= o.M || n0 + n >= o.N) return;
         uint16_t* c = o.c + (long)(m0 + m) * o.ldc + n0 + n;
         if (eight) {
-            *reinterpret_cast<uint4*>(c) = v;
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            if constexpr (P::LX == RowN) __builtin_nontemporal_store(__builtin_bit_cast(u4, v), reinterpret_cast<u4*>(c));
+            else *reinterpret_cast<uint4*>(c) = v;
         } else {
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
             for (int e = 0; e < 8 && n0 + n + e < o.N; e++) c[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
@@ -566,7 +570,7 @@ using Dhidden0 = Product<256, 256, 4, 2, 2, RowK, RowN>;
 using Dhidden1 = Product<128, 128, 2, 4, 2, RowK, RowN>;
 using Dhidden2 = Product<64, 256, 1, 8, 4, RowK, RowN>;
 using Dhidden3 = Product<64, 64, 2, 4, 4, RowK, RowN>;
-constexpr Shape DHIDDEN[] = {{256, 256, 1, 1.75, 12}, {128, 128, 1, .8, 5}, {64, 256, 1, .85, 8}, {64, 64, 1, .45, 3}};
+constexpr Shape DHIDDEN[] = {{256, 256, 1, 1.75, 12}, {128, 128, 1, .8, 5}, {64, 256, 1, .85, 8}, {64, 64, 1, .45, 3}, {128, 128, 2, 1.45, 7}};
 using Dweight0 = Product<256, 256, 4, 2, 2, RowN, RowN>;
 using Dweight1 = Product<128, 128, 2, 4, 2, RowN, RowN>;
 constexpr Shape DWEIGHT[] = {{256, 256, 1, 1.62, 6.7}, {128, 128, 2, 1.03, 4.1}};
@@ -609,12 +613,14 @@ static int check(const theseus_vocab_loss_args* a) {
     return THESEUS_WKV7_OK;
 }
 
-// us of a product of M x N outputs: rounds of tiles, or the reading of the weight behind it (`bytes`,
-// once for TOGETHER rows), whichever is longer, and a little of the other
+// us of a product of M x N outputs: its full rounds of tiles and a last one with fewer, each the
+// tiles' own time or the reading of the weight behind them (`bytes` in all, once for TOGETHER
+// rows), whichever is longer, and a little of the other
 static double both(double a, double b) { return a > b ? a + .1 * b : b + .1 * a; }
 static double cost(const Shape& c, long M, long N, long steps, double bytes, int cus) {
-    const long t = ceil_div(M, c.m) * ceil_div(N, c.n);
-    return both((double)ceil_div(t, (long)cus * c.per_cu) * (c.fixed + (double)steps * c.step), ceil_div(M, TOGETHER) * bytes / BYTES);
+    const long t = ceil_div(M, c.m) * ceil_div(N, c.n), slots = (long)cus * c.per_cu, full = t / slots;
+    const double tile = c.fixed + (double)steps * c.step, read = ceil_div(M, TOGETHER) * bytes / BYTES / t;
+    return (full ? full * both(tile, slots * read) : 0) + (t % slots ? both(tile, t % slots * read) : 0);
 }
 template <int N> static int best(const Shape (&c)[N], long M, long cols, long steps, double bytes, int cus, double* us) {
     int b = 0;
@@ -666,11 +672,14 @@ static Plan plan(const theseus_vocab_loss_args* a) {
         least = 0;
         for (int i = 0; i < (int)(sizeof DHIDDEN / sizeof *DHIDDEN); i++) {
             const Shape& c = DHIDDEN[i];
-            const int t = (int)(ceil_div(gm, c.m) * ceil_div(p.D, c.n));
-            for (int s = 1; s <= 64 && s <= all; s += s < 8 ? 1 : s / 4) {  // (every call comes by here: few candidates)
-                us = both((t * s + cus * c.per_cu - 1) / (cus * c.per_cu) * (c.fixed + ((int)all + s - 1) / s * c.step), read) +
+            const long t = ceil_div(gm, c.m) * ceil_div(p.D, c.n);
+            const long slots = (long)cus * c.per_cu;
+            for (int r = 1; r <= 12; r++) {  // few parts, or as many as fit 1 .. 4 rounds (every call comes by here: few candidates)
+                const long s = r <= 8 ? r : (r - 8) * slots / t;
+                if (s > all || s > 64 || (r > 8 && s <= 8)) continue;
+                us = both(ceil_div(t * s, slots) * (c.fixed + ceil_div(all, s) * c.step), read) +
                      (s > 1 ? LAUNCH + (double)s * gm * p.D * 8 / BYTES : 0);
-                if (least == 0 || us < least) least = us, p.dhidden = i, p.splits = s;
+                if (least == 0 || us < least) least = us, p.dhidden = i, p.splits = (int)s;
             }
         }
     }
@@ -807,7 +816,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
             };
             switch (p.dhidden) {
                 case 0: dhidden(Dhidden0{}); break;
-                case 1: dhidden(Dhidden1{}); break;
+                case 1: case 4: dhidden(Dhidden1{}); break;
                 case 2: dhidden(Dhidden2{}); break;
                 default: dhidden(Dhidden3{});
             }
