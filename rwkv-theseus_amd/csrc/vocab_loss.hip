@@ -2,7 +2,7 @@
 // include/theseus_vocab.h, where the formulas are).
 //
 // Launches of one call, on the caller's stream:
-//   labels, targets  every token's q, Q, sum q log q and weight
+//   targets        a teacher's: every token's q, Q, sum q log q and weight (a label's are made in rows)
 //   sums           MEAN with several pieces: the sum of the weights (one workgroup, fixed order)
 //   then for each piece of rows
 //     logits       z's tiles on the matrix cores; of each 256-column tile a row's maximum and sum
@@ -10,7 +10,8 @@
 //                  2^15 e^{z - tile maximum}: 11 significant bits down to e^-20 of the maximum);
 //                  z at the targets is taken out of the accumulators
 //     rows         log-sum-exp of a row from its tiles, the row's loss
-//     sums         one piece: the reduced loss and, for MEAN, the sum of the weights
+//     sums         one piece: the reduced loss and, for MEAN, the sum of the weights; with gradients
+//                  a workgroup of the next launch
 //     probs        exponentials -> G in place (bfloat16: the one rounding of the gradients' left
 //                  factor); at the target indices from their float32 z: p - 1 of a
 //                  confident token would be lost in a rounded p
@@ -59,25 +60,32 @@ struct Targets {
     long rows, vocab;
     int K, top_bf16;
     const int64_t* index;
-    const void* top;          // null: labels
+    const void* top;
     const float* teacher_lse;
     const float* row_weight;
-    long long ignore;
     float inv_T;
     int* j;        // [M][K] index, SKIP or BAD
-    float* q;      // [M][K] (teacher only)
+    float* q;      // [M][K]
     float4* row;   // [M] {Q, sum q log q, weight, 0}
 };
-__device__ __forceinline__ int place(const Targets& t, int64_t v) { return v < 0 || v >= t.vocab ? BAD : (int)v; }
 
-// labels: one thread a token
-__global__ __launch_bounds__(256) void labels_kernel(Targets t) {
+// labels: q = Q = 1
+struct Labels {
+    const int64_t* y;         // null: a teacher's targets
+    const float* row_weight;
+    long long ignore, vocab;
+    __device__ __forceinline__ float4 row(long i) const {
+        return make_float4(1.f, 0.f, y[i] == ignore ? 0.f : row_weight ? row_weight[i] : 1.f, 0.f);
+    }
+    __device__ __forceinline__ int place(long i) const {
+        const int64_t v = y[i];
+        return v == ignore ? SKIP : v < 0 || v >= vocab ? BAD : (int)v;
+    }
+};
+// their weights ahead of the pieces; one thread a token
+__global__ __launch_bounds__(256) void labels_kernel(Labels t, long rows, float4* row) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= t.rows) return;
-    const int64_t y = t.index[i];
-    const float weight = t.row_weight ? t.row_weight[i] : 1.f;
-    t.j[i] = y == t.ignore ? SKIP : place(t, y);
-    t.row[i] = make_float4(1.f, 0.f, y == t.ignore ? 0.f : weight, 0.f);
+    if (i < rows) row[i] = t.row(i);
 }
 
 // a teacher's logits: one wave a token
@@ -118,7 +126,8 @@ __global__ __launch_bounds__(256) void targets_kernel(Targets t) {
             const float lq = x[s] - base, q = x[s] == -INFINITY ? 0.f : expf(lq);
             const long at = i * t.K + k;
             t.q[at] = q;
-            t.j[at] = q == 0.f ? SKIP : place(t, t.index[at]);
+            const int64_t v = t.index[at];
+            t.j[at] = q == 0.f ? SKIP : v < 0 || v >= t.vocab ? BAD : (int)v;
             Q += q;
             H += q == 0.f ? 0.f : q * lq;
         }
@@ -128,34 +137,42 @@ __global__ __launch_bounds__(256) void targets_kernel(Targets t) {
     if (lane == 0) t.row[i] = make_float4(Q, H, weight, 0.f);
 }
 
-// sum over 1024 threads in a fixed order, valid in thread 0
-__device__ __forceinline__ double block_sum(double x, double* red) {
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double s = 0.0;
-    if (threadIdx.x == 0)
-        for (int k = 0; k < 16; k++) s += red[k];
-    return s;
-}
 // MEAN: *inv = 1 / sum of the weights (0 where that is 0); with losses, *out = their sum, times
-// *inv for MEAN.
-__global__ __launch_bounds__(1024) void sums_kernel(long rows, const float4* row, int mean, float* inv, const float* losses, float* out) {
+// *inv for MEAN.  One workgroup; 1024 partial sums, whatever its threads, added in a fixed order.
+struct Sums {
+    long rows;
+    const float4* row;
+    int mean;
+    float* inv;
+    const float* losses;
+    float* out;
+};
+template <int THREADS> __device__ __forceinline__ void sums(const Sums& p) {
     __shared__ double red[2][16];
-    double w = 0.0, s = 0.0;
+    const int t = threadIdx.x;
+    for (int v = 0; v < 1024; v += THREADS) {
+        double w = 0.0, s = 0.0;
 #pragma unroll 4
-    for (long i = threadIdx.x; i < rows; i += 1024) {
-        if (mean) w += row[i].z;
-        if (losses) s += losses[i];
+        for (long i = v + t; i < p.rows; i += 1024) {
+            if (p.mean) w += p.row[i].z;
+            if (p.losses) s += p.losses[i];
+        }
+        for (int o = 32; o > 0; o >>= 1) {
+            w += __shfl_xor(w, o, 64);
+            s += __shfl_xor(s, o, 64);
+        }
+        if ((t & 63) == 0) red[0][(v + t) >> 6] = w, red[1][(v + t) >> 6] = s;
     }
-    if (mean) w = block_sum(w, red[0]);
-    s = block_sum(s, red[1]);
-    if (threadIdx.x == 0) {
-        const double f = !mean ? 1.0 : w == 0.0 ? 0.0 : 1.0 / w;
-        if (inv) *inv = (float)f;
-        if (out) *out = (float)(s * f);
+    __syncthreads();
+    if (t == 0) {
+        double w = 0.0, s = 0.0;
+        for (int k = 0; k < 16; k++) w += red[0][k], s += red[1][k];
+        const double f = !p.mean ? 1.0 : w == 0.0 ? 0.0 : 1.0 / w;
+        if (p.inv) *p.inv = (float)f;
+        if (p.out) *p.out = (float)(s * f);
     }
 }
+__global__ __launch_bounds__(1024) void sums_kernel(Sums p) { sums<1024>(p); }
 
 // ---------------------------------------------------------------------------------- logits
 struct LogitsOut {
@@ -165,6 +182,7 @@ struct LogitsOut {
     int tiles;
     uint16_t* e;      // [..][lde]
     long lde;
+    Labels labels;    // or
     const int* j;     // [M][K] targets
     float* z;         // [M][K] their h . w
     int K;
@@ -196,10 +214,20 @@ template <class P> __device__ __forceinline__ void pick_targets(const P& g, uint
     const int* j = o.j + (long)m0 * o.K;
     for (int c0 = 0; c0 < total; c0 += CHUNK) {
         int4 v[4];
+        if (o.labels.y) {  // (one a token, at most 256)
+            v[0] = v[1] = v[2] = v[3] = make_int4(-1, -1, -1, -1);
+            if (4 * t < total) {
+                int x[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {  // (what a last four reads past the targets lies in the workspace)
-            const int i = c0 + (r * P::THREADS + t) * 4;
-            v[r] = i < total ? *reinterpret_cast<const int4*>(j + i) : make_int4(-1, -1, -1, -1);
+                for (int e = 0; e < 4; e++) x[e] = o.labels.place(m0 + min(4 * t + e, total - 1));
+                v[0] = make_int4(x[0], x[1], x[2], x[3]);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {  // (what a last four reads past the targets lies in the workspace)
+                const int i = c0 + (r * P::THREADS + t) * 4;
+                v[r] = i < total ? *reinterpret_cast<const int4*>(j + i) : make_int4(-1, -1, -1, -1);
+            }
         }
         __syncthreads();
         if (t == 0) *count = 0;
@@ -322,8 +350,9 @@ struct Rows {
     long rows;
     int tiles, K;
     const float2* part;
-    const float4* row;
-    const int* j;
+    Labels labels;  // their rows and places are written here
+    float4* row;
+    int* j;
     const float *q, *z;
     float T, scale;
     float2* norm;  // {maximum of h . w, 1 / sum of 2^15 exp}
@@ -341,15 +370,16 @@ __global__ __launch_bounds__(256) void rows_kernel(Rows p) {
     for (int t = lane; t < p.tiles; t += 64) sum += part[t].y * exp2_((part[t].x - top) * p.scale);
     sum = wave_sum(sum);
     const float lse = logf(sum * exp2_(-E_SHIFT));  // above the maximum
-    const float4 row = p.row[i];
+    const float4 row = p.labels.y ? p.labels.row(i) : p.row[i];
     float s = 0.f;
     for (int k = lane; k < p.K; k += 64) {
         const float q = p.q ? p.q[i * p.K + k] : 1.f;
-        const int v = p.j[i * p.K + k];
+        const int v = p.labels.y ? p.labels.place(i) : p.j[i * p.K + k];
         if (q != 0.f) s += v == BAD ? NAN : q * ((top - p.z[i * p.K + k]) * (LN2 * p.scale) + lse);
     }
     s = wave_sum(s);
     if (lane == 0) {
+        if (p.labels.y) p.row[i] = row, p.j[i] = p.labels.place(i);
         p.norm[i] = make_float2(top, 1.f / sum);
         if (p.loss) p.loss[i] = row.z == 0.f ? 0.f : p.T * p.T * row.z * (s + row.y);
     }
@@ -376,13 +406,20 @@ struct Probs {
     const float *q, *z;
     float scale;
     bool twice;             // rows 32 .. 63 take what rounding left of rows 0 .. 31
+    bool sum;               // one row of workgroups more, whose first one makes `sums`
+    Sums sums;
 };
 // blockIdx.x: PROBS columns of a row, 8 at a time a thread, then the targets among them; the rows
-// backwards, from those that the logits wrote last to those that dhidden reads first
+// backwards, from those that the logits wrote last to those that dhidden reads first.  (The sums are
+// wanted by the products' epilogues only, and cost a launch of 4 us alone.)
 constexpr int PROBS = 4096;
 __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
     __shared__ int js[THESEUS_VOCAB_MAX_TOP];
     __shared__ float qs[THESEUS_VOCAB_MAX_TOP];
+    if (p.sum && blockIdx.y == 0) {
+        if (blockIdx.x == 0) sums<256>(p.sums);
+        return;
+    }
     const long i = gridDim.y - 1 - blockIdx.y;
     const int t = threadIdx.x, n0 = blockIdx.x * PROBS;
     uint16_t *row = p.e + i * p.lde, *rest = row + 32 * p.lde;
@@ -742,7 +779,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
     long ldh = a->hidden_stride, ldw = a->weight_stride;
     const float inv_T = 1.f / a->temperature;
     if (p.M == 0) {
-        if (reduce) sums_kernel<<<1, 1024, 0, st>>>(0, nullptr, 0, nullptr, nullptr, a->loss);
+        if (reduce) sums_kernel<<<1, 1024, 0, st>>>(Sums{0, nullptr, 0, nullptr, nullptr, a->loss});
         if (a->dweight) zero_kernel<<<1024, 256, 0, st>>>(static_cast<uint16_t*>(a->dweight), p.V * p.D);
         return 0;
     }
@@ -753,16 +790,19 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         pad_rows<<<dim3(gx, (unsigned)(p.V < 32768 ? p.V : 32768)), 256, 0, st>>>(p.V, (int)p.D, (int)p.Dp, W, ldw, w);
         H = h, W = w, ldh = ldw = p.Dp;
     }
-    const Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight,
-                    a->ignore_index, inv_T, j, q, row};
-    if (!forward) {
-    } else if (a->top_values) targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
-    else labels_kernel<<<(unsigned)ceil_div(p.M, 256), 256, 0, st>>>(t);
-    const bool mean = inv != nullptr;
-    auto sums = [&](float* to, const float* from, float* out) {
-        sums_kernel<<<1, 1024, 0, st>>>(p.M, row, mean, to, from, out);
+    if (forward && a->top_values) {
+        const Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight, inv_T, j, q, row};
+        targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
+    }
+    auto labels = [&](long i0) {
+        return Labels{a->top_values ? nullptr : a->index + i0, a->row_weight ? a->row_weight + i0 : nullptr, a->ignore_index, p.V};
     };
-    if (mean && p.grads && p.pieces > 1) sums(inv, nullptr, nullptr);
+    const bool mean = inv != nullptr;
+    auto sums_of = [&](float* to, const float* from, float* out) { return Sums{p.M, row, mean, to, from, out}; };
+    if (mean && p.grads && p.pieces > 1) {
+        if (!a->top_values) labels_kernel<<<(unsigned)ceil_div(p.M, 256), 256, 0, st>>>(labels(0), p.M, row);
+        sums_kernel<<<1, 1024, 0, st>>>(sums_of(inv, nullptr, nullptr));
+    }
 
     for (int piece = 0; piece < p.pieces; piece++) {
         const long i0 = piece * p.piece, m = p.M - i0 < p.piece ? p.M - i0 : p.piece;
@@ -770,7 +810,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
         auto logits = [&](int shape, long n0, long n1, int tile0) {
             const Operand X{Hp, ldh, (int)m, (int)p.Dp}, Y{W + n0 * ldw, ldw, (int)(n1 - n0), (int)p.Dp};
             const LogitsOut lo{(int)m, (int)(n1 - n0), (int)((n1 == p.V ? p.lde : n1) - n0), LOG2E * inv_T, part + tile0, p.tiles,
-                               p.grads ? e + n0 : nullptr, p.lde, j + i0 * p.K, z + i0 * p.K, (int)p.K, (int)n0};
+                               p.grads ? e + n0 : nullptr, p.lde, labels(i0), j + i0 * p.K, z + i0 * p.K, (int)p.K, (int)n0};
             auto launch = [&](auto tag) {
                 using P = decltype(tag);
                 const Tiles tl = tiles(m, n1 - n0, P::BM, P::BN, p.Dp, 1);
@@ -788,16 +828,18 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
             logits(p.logits, 0, p.main, 0);
             if (p.main < p.V) logits(p.rest, p.main, p.V, (int)ceil_div(p.main, LOGITS[p.logits].n));
         }
-        const Rows rw{m, p.tiles, (int)p.K, part, row + i0, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
+        const Rows rw{m, p.tiles, (int)p.K, part, labels(i0), row + i0, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K,
                       a->temperature, LOG2E * inv_T, norm, losses ? losses + i0 : nullptr};
         if (forward) rows_kernel<<<(unsigned)ceil_div(m, 4), 256, 0, st>>>(rw);
-        if (p.pieces == 1 && (reduce || (mean && p.grads))) sums(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
+        const bool sum = p.pieces == 1 && (reduce || (mean && p.grads));
+        const Sums su = sums_of(inv, reduce ? losses : nullptr, reduce ? a->loss : nullptr);
+        if (sum && !gradients) sums_kernel<<<1, 1024, 0, st>>>(su);
         if (!gradients) continue;
 
         const long mp = up(m, BK);
         const Probs pr{(int)m, (int)p.K, p.tiles, (int)(p.main < p.V ? p.main : p.lde), LOGITS[p.logits].n, LOGITS[p.rest].n, p.lde, e, part, row + i0, norm,
-                       a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, LOG2E * inv_T, p.twice};
-        probs_kernel<<<dim3((unsigned)ceil_div(p.lde, PROBS), (unsigned)(p.twice ? 32 : mp)), 256, 0, st>>>(pr);
+                       a->row_grad ? a->row_grad + i0 : nullptr, j + i0 * p.K, q ? q + i0 * p.K : nullptr, z + i0 * p.K, LOG2E * inv_T, p.twice, sum, su};
+        probs_kernel<<<dim3((unsigned)ceil_div(p.lde, PROBS), (unsigned)((p.twice ? 32 : mp) + sum)), 256, 0, st>>>(pr);
         if (a->dhidden) {
             uint16_t* dh = static_cast<uint16_t*>(a->dhidden) + i0 * p.D;
             const long gm = p.twice ? 64 : m;  // rows of G
@@ -835,7 +877,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
             else dweight(Dweight1{});
         }
     }
-    if (reduce && p.pieces > 1) sums(nullptr, losses, a->loss);
+    if (reduce && p.pieces > 1) sums_kernel<<<1, 1024, 0, st>>>(sums_of(inv, losses, a->loss));
     return 0;
 }
 
