@@ -592,8 +592,10 @@ __global__ __launch_bounds__(256) void zero_kernel(uint16_t* x, long n) {
 // once (per_cu on each CU).  From logits of 64 .. 1024 x 131072 at D = 1280 and 2560, dhidden of as
 // many x 2560 from 131072, dweight of 131072 x 2560 from 64 .. 1024 tokens, and small ones.
 // plan() takes the cheapest: e.g. 128 tokens' logits there take 152, 127, 176 and 234 us in the
-// four shapes, 512 tokens' 273, 346, 564 and 734; dhidden of 64 x 768 from 8192 31 us in 256 x 256
-// tiles (8 parts) and 13 in 64 x 64 (16).
+// first four shapes, 512 tokens' 273, 346, 564 and 734, 384 tokens' 279 in tiles of 256 rows and 258 of
+// 192; dhidden of 64 x 768 from 8192 31 us in 256 x 256 tiles (8 parts) and 13 in 64 x 64 (16), of
+// 285 x 2048 from 101681 167 in 256 x 256 and 151 in 192 x 256 (16), of 100 x 5120 from 72799 198 in
+// 128 x 128 one a CU and 168 two a CU.
 struct Shape {
     int m, n, per_cu;
     double step, fixed;
@@ -602,12 +604,14 @@ using Logits0 = Product<256, 256, 4, 2, 2, RowK, RowK>;
 using Logits1 = Product<128, 256, 2, 4, 3, RowK, RowK>;
 using Logits2 = Product<64, 256, 1, 8, 4, RowK, RowK>;
 using Logits3 = Product<64, 64, 2, 4, 4, RowK, RowK>;
-constexpr Shape LOGITS[] = {{256, 256, 1, 1.5, 7}, {128, 256, 1, .95, 5}, {64, 256, 1, .78, 4}, {64, 64, 2, .5, 2.3}};
+using Logits4 = Product<192, 256, 4, 2, 2, RowK, RowK>;
+constexpr Shape LOGITS[] = {{256, 256, 1, 1.5, 7}, {128, 256, 1, .95, 5}, {64, 256, 1, .78, 4}, {64, 64, 2, .5, 2.3}, {192, 256, 1, 1.27, 5.5}};
 using Dhidden0 = Product<256, 256, 4, 2, 2, RowK, RowN>;
 using Dhidden1 = Product<128, 128, 2, 4, 2, RowK, RowN>;
 using Dhidden2 = Product<64, 256, 1, 8, 4, RowK, RowN>;
 using Dhidden3 = Product<64, 64, 2, 4, 4, RowK, RowN>;
-constexpr Shape DHIDDEN[] = {{256, 256, 1, 1.75, 12}, {128, 128, 1, .8, 5}, {64, 256, 1, .85, 8}, {64, 64, 1, .45, 3}, {128, 128, 2, 1.45, 7}};
+using Dhidden5 = Product<192, 256, 4, 2, 2, RowK, RowN>;
+constexpr Shape DHIDDEN[] = {{256, 256, 1, 1.75, 12}, {128, 128, 1, .8, 5}, {64, 256, 1, .85, 8}, {64, 64, 1, .45, 3}, {128, 128, 2, 1.45, 7}, {192, 256, 1, 1.5, 8.5}};
 using Dweight0 = Product<256, 256, 4, 2, 2, RowN, RowN>;
 using Dweight1 = Product<128, 128, 2, 4, 2, RowN, RowN>;
 constexpr Shape DWEIGHT[] = {{256, 256, 1, 1.62, 6.7}, {128, 128, 2, 1.03, 4.1}};
@@ -621,8 +625,9 @@ struct Plan {
     long M, V, D, K, Dp, lde, piece;  // Dp: width in the products; lde: kept columns; piece: rows
     int pieces, tiles;                // row pieces; logits tiles of a row
     bool grads, pad, twice;
-    int logits, rest, dhidden, dweight;  // indices into the shapes
+    int logits, rest, dhidden, dweight, wrest;  // indices into the shapes
     long main;                        // columns of the vocabulary in shape `logits`, the others in `rest`
+    long wmain;                       // rows of dweight in shape `dweight`, the others in `wrest`
     int splits;                       // of dhidden's contraction
     size_t j, q, row, z, part, norm, loss, inv, e, kept, acc, parts, hidden, weight, bytes;
 };
@@ -652,12 +657,13 @@ static int check(const theseus_vocab_loss_args* a) {
 
 // us of a product of M x N outputs: its full rounds of tiles and a last one with fewer, each the
 // tiles' own time or the reading of the weight behind them (`bytes` in all, once for TOGETHER
-// rows), whichever is longer, and a little of the other
+// rows), whichever is longer, and a little of the other.  A last round's tiles run faster, the fewer
+// the more (the clock; 3088 tokens' dweight of 25163 x 2048, 24 tiles of 256: 44 us for 86)
 static double both(double a, double b) { return a > b ? a + .1 * b : b + .1 * a; }
 static double cost(const Shape& c, long M, long N, long steps, double bytes, int cus) {
-    const long t = ceil_div(M, c.m) * ceil_div(N, c.n), slots = (long)cus * c.per_cu, full = t / slots;
+    const long t = ceil_div(M, c.m) * ceil_div(N, c.n), slots = (long)cus * c.per_cu, full = t / slots, left = t % slots;
     const double tile = c.fixed + (double)steps * c.step, read = ceil_div(M, TOGETHER) * bytes / BYTES / t;
-    return (full ? full * both(tile, slots * read) : 0) + (t % slots ? both(tile, t % slots * read) : 0);
+    return (full ? full * both(tile, slots * read) : 0) + (left ? both(full ? tile * (.6 + .4 * left / slots) : tile, left * read) : 0);
 }
 template <int N> static int best(const Shape (&c)[N], long M, long cols, long steps, double bytes, int cus, double* us) {
     int b = 0;
@@ -720,7 +726,20 @@ static Plan plan(const theseus_vocab_loss_args* a) {
             }
         }
     }
-    if (a->dweight) p.dweight = best(DWEIGHT, p.V, p.D, ceil_div(rows, BK), 0, cus, &us);
+    if (a->dweight) {
+        const long k = ceil_div(rows, BK);
+        p.dweight = p.wrest = best(DWEIGHT, p.V, p.D, k, 0, cus, &least);
+        p.wmain = p.V;
+        // (as the logits' columns; 2604 tokens, 53714 x 768: 2.46 rounds of 256 x 256 tiles, 207 -> 195 us;
+        // the smaller tiles are slower in full rounds)
+        const Shape& c = DWEIGHT[0];
+        const long tn = ceil_div(p.D, c.n), m = ceil_div(p.V, c.m) * tn / cus * cus / tn * c.m;
+        if (m > 0 && m < p.V) {
+            const int r = best(DWEIGHT, p.V - m, p.D, k, 0, cus, &us);
+            us += cost(c, m, p.D, k, 0, cus) + LAUNCH;
+            if (us < least) p.dweight = 0, p.wmain = m, p.wrest = r;
+        }
+    }
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -821,6 +840,7 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
                 case 0: launch(Logits0{}); break;
                 case 1: launch(Logits1{}); break;
                 case 2: launch(Logits2{}); break;
+                case 4: launch(Logits4{}); break;
                 default: launch(Logits3{});
             }
         };
@@ -860,21 +880,28 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
                 case 0: dhidden(Dhidden0{}); break;
                 case 1: case 4: dhidden(Dhidden1{}); break;
                 case 2: dhidden(Dhidden2{}); break;
+                case 5: dhidden(Dhidden5{}); break;
                 default: dhidden(Dhidden3{});
             }
         }
         if (a->dweight) {
-            const Operand GX{e, p.lde, (int)p.lde, (int)mp}, HY{Hp, ldh, (int)p.Dp, (int)m, p.twice};
-            const GradOut go{(int)p.V, (int)p.D, static_cast<uint16_t*>(a->dweight), p.D, reinterpret_cast<float*>((ws + p.acc)),
-                             up(p.D, 4), piece == 0, piece == p.pieces - 1, a->temperature, inv};
-            auto dweight = [&](auto tag) {
+            const Operand HY{Hp, ldh, (int)p.Dp, (int)m, p.twice};
+            auto dweight = [&](auto tag, long v0, long v1) {
                 using P = decltype(tag);
-                const Tiles tl = tiles(p.V, p.D, P::BM, P::BN, mp, 1);
+                const Operand GX{e + v0, p.lde, (int)((v1 == p.V ? p.lde : v1) - v0), (int)mp};
+                const GradOut go{(int)(v1 - v0), (int)p.D, static_cast<uint16_t*>(a->dweight) + v0 * p.D, p.D,
+                                 reinterpret_cast<float*>((ws + p.acc)) + v0 * up(p.D, 4), up(p.D, 4), piece == 0, piece == p.pieces - 1,
+                                 a->temperature, inv};
+                const Tiles tl = tiles(v1 - v0, p.D, P::BM, P::BN, mp, 1);
                 if (p.pieces > 1) grad_kernel<P, OutAdd><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
                 else grad_kernel<P, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
             };
-            if (p.dweight == 0) dweight(Dweight0{});
-            else dweight(Dweight1{});
+            if (p.dweight == 0) dweight(Dweight0{}, 0, p.wmain);
+            else dweight(Dweight1{}, 0, p.wmain);
+            if (p.wmain < p.V) {
+                if (p.wrest == 0) dweight(Dweight0{}, p.wmain, p.V);
+                else dweight(Dweight1{}, p.wmain, p.V);
+            }
         }
     }
     if (reduce && p.pieces > 1) sums_kernel<<<1, 1024, 0, st>>>(sums_of(inv, losses, a->loss));

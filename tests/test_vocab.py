@@ -547,6 +547,23 @@ def test_every_tile_shape_matches_float64(M, D, V):
 
 
 @gpu
+@pytest.mark.parametrize("M,D,V,piece", [(300, 128, 50000, 0), (1000, 768, 30000, 0), (70, 2560, 40000, 0), (600, 768, 30000, 256)])
+def test_tiles_of_192_rows_and_split_weight_gradients_match_float64(M, D, V, piece):
+    """Sizes planned with tiles of 192 rows, dhidden two tiles a CU, dweight in full rounds and a rest (one piece, several)."""
+    print(f"  shapes M={M} D={D} V={V} piece={piece}", flush=True)
+    x, w, g = _inputs(M, D, V, seed=M)
+    labels = torch.randint(V, (M,), generator=g)
+    labels[0], labels[-1] = 0, V - 1
+    one = torch.ones(M).double()
+    o = _oracle(x.cuda(), w.cuda(), _dense(M, V, labels[:, None], torch.ones(M, 1)).cuda(), 0.0, one.cuda(), 1.0, (one / M).cuda())
+    o = {k: v.cpu() for k, v in o.items()}
+    loss, dx, dw = _run(lambda a, b: vocab.linear_cross_entropy(a, b, labels.cuda(), piece_rows=piece), x, w, torch.tensor(1.), "mean")
+    assert abs(float(loss) - float(o["loss"].mean())) <= float(o["ltol"].mean())
+    _grad_close(dx, o["dx"], o["dx_tol"])
+    _grad_close(dw, o["dw"], o["dw_tol"])
+
+
+@gpu
 @pytest.mark.parametrize("M,D,V", [(1, 128, 4000), (5, 100, 333), (31, 256, 9000), (32, 64, 50)])
 def test_few_tokens_gradients_are_rounded_once(M, D, V):
     """Up to 32 tokens: G in two halves (2^-16), its softmax part from float16 exponentials (11 bits: 2^-11), so
