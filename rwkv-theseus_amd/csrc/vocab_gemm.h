@@ -57,15 +57,16 @@ struct Tiles {
     int steps;    // steps of one part (the last may have fewer)
     int all;      // steps in all
     int group;    // m tiles that run together
+    int total;    // tiles in all: m n splits
 };
 
 struct Where {
     int m, n, part;
 };
-// Workgroup b runs on XCD b % 8: each XCD takes a run of consecutive tiles, ordered in groups of
+// Workgroup b % (the grid, where that is smaller, a multiple of 8) runs on XCD b % 8: each XCD takes a run of consecutive tiles, ordered in groups of
 // `group` m tiles that share the n tiles they walk over, so that an XCD's L2 serves both operands.
-__device__ __forceinline__ Where tile_of(const Tiles& t, int b, int total) {
-    const int each = total >> 3;
+__device__ __forceinline__ Where tile_of(const Tiles& t, int b) {
+    const int each = t.total >> 3;
     int id = b < each * 8 ? (b & 7) * each + (b >> 3) : b;
     const int mn = t.m * t.n;
     Where w;
@@ -93,7 +94,8 @@ template <Lay L, int B, bool PERM> struct Loader {
     const uint8_t* base;
     uint32_t row, col, ld2;
     uint32_t mask;  // of a row's number (RowN)
-    int rows_left;  // RowK: valid rows from the tile's first; RowN: valid rows from the part's first
+    uint32_t limit; // RowK: offset of the tile's last valid row
+    int rows_left;  // RowN: valid rows from the step's first
 
     __device__ __forceinline__ Loader(const Operand& o, int x0, int k0, int wave, int lane) {
         ld2 = (uint32_t)(o.ld * 2);
@@ -104,7 +106,8 @@ template <Lay L, int B, bool PERM> struct Loader {
             mask = ~0u;
             row = r * ld2;
             col = 16 * c;
-            rows_left = o.outer - x0;
+            limit = (uint32_t)max(min(o.outer - x0, B) - 1, 0) * ld2;  // (of the tile: 32 bits hold its rows' offsets)
+            rows_left = 0;
         } else {
             constexpr int CH = B / 8;  // chunks in a row
             const int r = PER * wave + lane / CH;
@@ -114,20 +117,32 @@ template <Lay L, int B, bool PERM> struct Loader {
             row = (r & mask) * ld2;
             col = 2 * min(8 * c, o.outer - x0 - 8);
             rows_left = o.inner - k0;
+            limit = 0;
         }
     }
     // piece j of the next step into the tile at `lds`; advance() after the last one
     __device__ __forceinline__ void issue(uint32_t lds, int j, int wave) const {
-        const int last = min(rows_left, L == RowK ? B : BK) - 1;  // (of the tile: 32 bits hold its rows' offsets)
-        const uint32_t r = min(row + ((uint32_t)(8 * PER * j) & mask) * ld2, (uint32_t)max(last, 0) * ld2);
+        const uint32_t last = L == RowK ? limit : (uint32_t)max(min(rows_left, BK) - 1, 0) * ld2;
+        const uint32_t r = min(row + ((uint32_t)(8 * PER * j) & mask) * ld2, last);
         dma(lds + (uint32_t)(wave + 8 * j) * 1024, base, r + col);
     }
-    // to the next step; past the last one the loader stays there (its pieces are then not used)
+    // to the next step (behind a workgroup's last one the loader stays: its pieces are then not used)
     __device__ __forceinline__ void advance(bool more) {
         if constexpr (L == RowK) base += more ? BK * 2 : 0;
         else {
             base += more ? (long)BK * ld2 : 0;
             rows_left -= more ? BK : 0;
+        }
+    }
+    // or to another tile's first step
+    __device__ __forceinline__ void move(bool more, bool jump, const Loader& to) {
+        advance(more);
+        base = jump ? to.base : base;
+        if constexpr (L == RowK) {
+            limit = jump ? to.limit : limit;
+        } else {
+            rows_left = jump ? to.rows_left : rows_left;
+            col = jump ? to.col : col;
         }
     }
 };
@@ -179,29 +194,51 @@ template <int N> __device__ __forceinline__ void wait_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// A BM x BN tile: WM x WN waves of TM x TN fragments, NST stages.  Leaves acc[tn][tm] (lane:
-// n = 16 tn + 4 (lane / 16) + e, m = 16 tm + lane % 16 from the wave's first) and every DMA
-// landed; the caller puts a barrier before it writes to LDS.
+// threadIdx.x where a tile is finished: what follows from it is made there again, not held in registers
+// through the multiplication
+__device__ __forceinline__ int thread_here() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+struct Place {
+    int m0, n0, step0, steps;
+};
+
+// BM x BN tiles: WM x WN waves of TM x TN fragments, NST stages.  go() makes a workgroup's tiles one
+// after the other: next(place) says which (false: no more), done(place) is called with each tile's
+// acc[tn][tm] (lane: n = 16 tn + 4 (lane / 16) + e, m = 16 tm + lane % 16 from the wave's first).
+// While a tile's last steps are multiplied and done() works in LDS of its own (epilogue()), the
+// next tile's first stages are on their way (a workgroup's tiles have more than NST steps, or it has one;
+// one tile a workgroup throughout: 2604 tokens' logits of 53714 at D = 768 336 us for 295, 365 tokens'
+// dweight of 60000 x 2560 159 for 144, with 80 steps and more, at the power limit, the same).  Shapes whose
+// stages leave no LDS for that (KEPT false) make one tile, and done() writes where the stages were.
 template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct Product {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NST = NST_;
     static constexpr Lay LX = LX_, LY = LY_;
     static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
     static constexpr bool PERM = LX == RowN || LY == RowN;
     static constexpr int STAGE = (BM + BN) * BK * 2;
-    static constexpr int LDS = NST * STAGE;
+    static constexpr int EPILOGUE = TN * 4096 > 9216 ? TN * 4096 : 9216;
+    static constexpr bool KEPT = NST * STAGE + EPILOGUE <= 163840;
+    static constexpr int LDS = NST * STAGE + (KEPT ? EPILOGUE : 0);
     static constexpr int THREADS = 512;
     static_assert(WM * WN == 8, "eight waves");
     using LoadX = Loader<LX, BM, PERM>;
     using LoadY = Loader<LY, BN, PERM>;
     static constexpr int PIECES = LoadX::PIECES + LoadY::PIECES;
 
+    __device__ static __forceinline__ uint8_t* epilogue(uint8_t* lds) { return lds + (KEPT ? NST * STAGE : 0); }
+
     f32x4_t acc[TN][TM];
 
-    __device__ __forceinline__ void run(uint8_t* lds, const Operand& X, const Operand& Y, int m0, int n0, int step0, int steps) {
+    template <class Next, class Done>
+    __device__ __forceinline__ void go(uint8_t* lds, const Operand& X, const Operand& Y, Place at, Next next, Done done) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-        LoadX lx(X, m0, step0 * BK, wave, lane);
-        LoadY ly(Y, n0, step0 * BK, wave, lane);
+        LoadX lx(X, at.m0, at.step0 * BK, wave, lane);
+        LoadY ly(Y, at.n0, at.step0 * BK, wave, lane);
         const Reader<LX, BM, PERM> rx((wave / WN) * TM * 16, lane);
         const Reader<LY, BN, PERM> ry((wave % WN) * TN * 16, lane);
         auto piece = [&](int stage, int j) {
@@ -209,15 +246,11 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
             else ly.issue(lds0 + stage * STAGE + BM * BK * 2, j - LoadX::PIECES, wave);
         };
 #pragma unroll
-        for (int tn = 0; tn < TN; tn++)
-#pragma unroll
-            for (int tm = 0; tm < TM; tm++) acc[tn][tm] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
         for (int s = 0; s < NST; s++) {
 #pragma unroll
             for (int j = 0; j < PIECES; j++) piece(s, j);
-            lx.advance(s + 1 < steps);
-            ly.advance(s + 1 < steps);
+            lx.advance(s + 1 < at.steps);
+            ly.advance(s + 1 < at.steps);
         }
         wait_barrier<(NST - 1) * PIECES>();
 
@@ -255,51 +288,88 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
         constexpr int BG = TN < 8 || PERM ? 0 : 3;  // groups of the second half ahead of the barrier
         using None = std::integral_constant<int, 0>;
         using Late = std::integral_constant<int, BG>;
-#pragma unroll
-        for (int i = 0; i < TM; i++) read_x(x0, 0, i, 0);
-#pragma unroll
-        for (int i = 0; i < TN; i++) read_y(0, i, 0);
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // (so that what is out at the loop's start is what its end left)
         int cur = 0;
-        for (int s = 0; s < steps; s++) {
-            groups(x0, x1, cur, 1, None{}, std::false_type{}, 0);
-            // (the stage's last reads complete under these)
+        for (;;) {
+            Place to;
+            const bool more = KEPT && next(to);
+            if (!more) to = at;
+            const LoadX tx(X, to.m0, to.step0 * BK, wave, lane);
+            const LoadY ty(Y, to.n0, to.step0 * BK, wave, lane);
 #pragma unroll
-            for (int g = 0; g < BG; g++) group(x1, g);
-            __builtin_amdgcn_sched_barrier(0);
-            // the next stage has landed, and every wave has read all of this one
-            wait_barrier<(NST - 2) * PIECES>();
-            const int next = cur + 1 == NST ? 0 : cur + 1;
-            groups(x1, x0, next, 0, Late{}, std::true_type{}, cur);
-            lx.advance(s + 1 + NST < steps);
-            ly.advance(s + 1 + NST < steps);
-            cur = next;
+            for (int tn = 0; tn < TN; tn++)
+#pragma unroll
+                for (int tm = 0; tm < TM; tm++) acc[tn][tm] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < TM; i++) read_x(x0, cur, i, 0);
+#pragma unroll
+            for (int i = 0; i < TN; i++) read_y(cur, i, 0);
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // (so that what is out at the loop's start is what its end left)
+            auto step = [&](auto move) {
+                groups(x0, x1, cur, 1, None{}, std::false_type{}, 0);
+                // (the stage's last reads complete under these)
+#pragma unroll
+                for (int g = 0; g < BG; g++) group(x1, g);
+                __builtin_amdgcn_sched_barrier(0);
+                // the next stage has landed, and every wave has read all of this one
+                wait_barrier<(NST - 2) * PIECES>();
+                const int then = cur + 1 == NST ? 0 : cur + 1;
+                groups(x1, x0, then, 0, Late{}, std::true_type{}, cur);
+                move();
+                cur = then;
+            };
+            // step s loads step s + NST; the last ones, which load the next tile's, in a loop of their own
+            // (the choice in the long one costs 2 %)
+            int s = 0;
+            for (; s < at.steps - NST - 1; s++)
+                step([&] {
+                    lx.advance(true);
+                    ly.advance(true);
+                });
+            for (; s < at.steps; s++)
+                step([&] {
+                    const int left = at.steps - NST - 1 - s;
+                    lx.move(more && left < 0, more && left == 0, tx);
+                    ly.move(more && left < 0, more && left == 0, ty);
+                });
+            if constexpr (!KEPT) {
+                wkv7::vm_wait_n<0>();
+                __syncthreads();
+            }
+            done(at);
+            if (!more) break;
+            at = to;
         }
-        wkv7::vm_wait_n<0>();
+        wkv7::vm_wait_n<0>();  // (before the workgroup's LDS is another's)
     }
 };
 
 // The workgroup's tile of 16-bit values to memory, whole rows at a time: an accumulator lane holds
 // 8 bytes of a row, which stored as they are reach memory as 32-byte pieces of 16 rows (8192 x
 // 65536 exponentials at D = 640: 1080 us, and 920 by whole rows; a weight gradient of 65536 x
-// 5120 from 64 tokens 233 and 158).  Each wave turns its own tile in its own part of LDS (16-byte chunk c of row r at
-// c ^ (r mod chunks)).  pack(tn, tm): the lane's four values; put(m, n, v): eight values of row m
-// from column n, both from the workgroup's first.  The caller puts a barrier before.
+// 5120 from 64 tokens 233 and 158).  Each wave turns its own tile, 16 rows at a time, in its own part of
+// the epilogue's LDS (16-byte chunk c of row r at c ^ (r mod chunks)).  pack(tn, tm): the lane's four
+// values; put(m, n, v): eight values of row m from column n, both from the workgroup's first.
 template <class P, class Pack, class Put> __device__ __forceinline__ void store_rows(uint8_t* lds, Pack pack, Put put) {
     constexpr int CH = P::TN * 2, ROW = CH * 16;  // chunks and bytes of a row of the wave's tile
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
-    uint8_t* mine = lds + wave * (P::TM * 16 * ROW);
-#pragma unroll
-    for (int tm = 0; tm < P::TM; tm++)
-#pragma unroll
-        for (int tn = 0; tn < P::TN; tn++)
-            *reinterpret_cast<uint2*>(mine + (16 * tm + r16) * ROW + (((2 * tn + (q >> 1)) ^ (r16 & (CH - 1))) << 4) + 8 * (q & 1)) = pack(tn, tm);
-    wkv7::wave_lds_fence();
+    constexpr int EACH = CH < 4 ? 2 : 1;          // fragments of 16 rows at a time: 64 chunks or more
+    static_assert(P::TM % EACH == 0 && 8 * EACH * 16 * ROW <= P::EPILOGUE, "tile");
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6, r16 = lane & 15, q = lane >> 4;
+    uint8_t* mine = P::epilogue(lds) + wave * (EACH * 16 * ROW);
     const int c = lane & (CH - 1), m0 = (wave / P::WN) * P::TM * 16, n = (wave % P::WN) * P::TN * 16 + 8 * c;
 #pragma unroll
-    for (int i = 0; i < P::TM * 16 * CH / 64; i++) {
-        const int r = i * (64 / CH) + lane / CH;
-        put(m0 + r, n, *reinterpret_cast<const uint4*>(mine + r * ROW + ((c ^ (r & (CH - 1))) << 4)));
+    for (int t0 = 0; t0 < P::TM; t0 += EACH) {
+#pragma unroll
+        for (int t = 0; t < EACH; t++)
+#pragma unroll
+            for (int tn = 0; tn < P::TN; tn++)
+                *reinterpret_cast<uint2*>(mine + (16 * t + r16) * ROW + (((2 * tn + (q >> 1)) ^ (r16 & (CH - 1))) << 4) + 8 * (q & 1)) = pack(tn, t0 + t);
+        wkv7::wave_lds_fence();
+#pragma unroll
+        for (int i = 0; i < EACH * 16 * CH / 64; i++) {
+            const int r = i * (64 / CH) + lane / CH;
+            put(m0 + 16 * t0 + r, n, *reinterpret_cast<const uint4*>(mine + r * ROW + ((c ^ (r & (CH - 1))) << 4)));
+        }
+        wkv7::wave_lds_fence();
     }
 }
 

@@ -174,6 +174,24 @@ template <int THREADS> __device__ __forceinline__ void sums(const Sums& p) {
 }
 __global__ __launch_bounds__(1024) void sums_kernel(Sums p) { sums<1024>(p); }
 
+// a workgroup's tiles: every gridDim.x-th
+template <class P> struct Places {
+    const Tiles& t;
+    int b = blockIdx.x;
+    __device__ __forceinline__ explicit Places(const Tiles& tiles) : t(tiles) {}
+    __device__ __forceinline__ Place place() const {
+        const Where w = tile_of(t, b);
+        const int s0 = w.part * t.steps;
+        return Place{w.m * P::BM, w.n * P::BN, s0, min(t.steps, t.all - s0)};
+    }
+    __device__ __forceinline__ bool operator()(Place& p) {
+        b += gridDim.x;
+        if (b >= t.total) return false;
+        p = place();
+        return true;
+    }
+};
+
 // ---------------------------------------------------------------------------------- logits
 struct LogitsOut {
     int M, N, Ne;     // rows, vocabulary, columns kept (Ne >= N, zero beyond N)
@@ -200,22 +218,22 @@ template <class P, int LO, int HI> __device__ __forceinline__ f32x4_t fragment(c
     else return fragment<P, (LO + HI) / 2, HI>(g, code);
 }
 // h . w at the targets that lie in the workgroup's tile, out of the accumulators: the tile's tokens'
-// targets are looked through (8192 at a time), those in its columns listed in LDS, and each wave
+// targets are looked through (some thousand at a time), those in its columns listed in LDS, and each wave
 // goes down the list for its own.  The list's order, which the atomics leave open, changes nothing.
 // (About 3 us a tile of 256 x 256 with 32 targets a token, 96 us of 8192 x 65536 logits; dot products
 // in a kernel of their own, D values of weight a target: 460 us.  With labels equal.)
 template <class P> __device__ __forceinline__ void pick_targets(const P& g, uint8_t* lds, const LogitsOut& o, int m0, int n0) {
-    constexpr int CHUNK = P::THREADS * 16;
-    uint32_t* list = reinterpret_cast<uint32_t*>(lds);
-    int* count = reinterpret_cast<int*>(lds + CHUNK * 4 + 256);
-    static_assert(P::LDS >= CHUNK * 4 + 4 + 256, "list");  // (64 entries are read at a time)
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    constexpr int READ = (P::EPILOGUE - 260) / (P::THREADS * 16), CHUNK = P::THREADS * 4 * READ;  // (fours a thread)
+    uint32_t* list = reinterpret_cast<uint32_t*>(P::epilogue(lds));  // (64 entries are read at a time)
+    int* count = reinterpret_cast<int*>(P::epilogue(lds) + CHUNK * 4 + 256);
+    const int t = thread_here(), lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int total = min(P::BM, o.M - m0) * o.K, first = o.n0 + n0;
     const int* j = o.j + (long)m0 * o.K;
     for (int c0 = 0; c0 < total; c0 += CHUNK) {
-        int4 v[4];
+        int4 v[READ];
         if (o.labels.y) {  // (one a token, at most 256)
-            v[0] = v[1] = v[2] = v[3] = make_int4(-1, -1, -1, -1);
+#pragma unroll
+            for (int r = 0; r < READ; r++) v[r] = make_int4(-1, -1, -1, -1);
             if (4 * t < total) {
                 int x[4];
 #pragma unroll
@@ -224,7 +242,7 @@ template <class P> __device__ __forceinline__ void pick_targets(const P& g, uint
             }
         } else {
 #pragma unroll
-            for (int r = 0; r < 4; r++) {  // (what a last four reads past the targets lies in the workspace)
+            for (int r = 0; r < READ; r++) {  // (what a last four reads past the targets lies in the workspace)
                 const int i = c0 + (r * P::THREADS + t) * 4;
                 v[r] = i < total ? *reinterpret_cast<const int4*>(j + i) : make_int4(-1, -1, -1, -1);
             }
@@ -233,7 +251,7 @@ template <class P> __device__ __forceinline__ void pick_targets(const P& g, uint
         if (t == 0) *count = 0;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
+        for (int r = 0; r < READ; r++) {
             const int i = c0 + (r * P::THREADS + t) * 4, x[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -260,19 +278,13 @@ template <class P> __device__ __forceinline__ void pick_targets(const P& g, uint
     __syncthreads();
 }
 
-template <class P, bool KEEP>
-__global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y, Tiles t, LogitsOut o) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
-    const Where at = tile_of(t, blockIdx.x, gridDim.x);
-    const int m0 = at.m * P::BM, n0 = at.n * P::BN;
-    P g;
-    g.run(lds, X, Y, m0, n0, 0, t.all);
+template <class P, bool KEEP> __device__ __forceinline__ void logits_done(P& g, uint8_t* lds, const LogitsOut& o, int m0, int n0) {
     pick_targets(g, lds, o, m0, n0);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6, r16 = lane & 15, q = lane >> 4;
     const int wm = wave / P::WN, wn = wave % P::WN;
     const int mw = wm * P::TM * 16 + r16, nw = n0 + wn * P::TN * 16 + 4 * q;
-    float* red = reinterpret_cast<float*>(lds);  // [2][WN][BM]
+    float* red = reinterpret_cast<float*>(P::epilogue(lds));  // [2][WN][BM]
     if (n0 + P::BN > o.N) {
 #pragma unroll
         for (int tn = 0; tn < P::TN; tn++)
@@ -327,7 +339,7 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
                 float sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < P::WN; w++) sum += red[(P::WN + w) * P::BM + m];
-                o.part[(long)(m0 + m) * o.tiles + at.n] = make_float2(top[tm], sum);
+                o.part[(long)(m0 + m) * o.tiles + n0 / P::BN] = make_float2(top[tm], sum);
             }
         }
     if constexpr (KEEP) {
@@ -340,6 +352,13 @@ __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y
             if (m0 + m < o.M && n0 + n < o.Ne) *reinterpret_cast<uint4*>(o.e + (long)(m0 + m) * o.lde + n0 + n) = v;
         });
     }
+}
+
+template <class P, bool KEEP>
+__global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y, Tiles t, LogitsOut o) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
+    P g;
+    g.go(lds, X, Y, Places<P>(t).place(), Places<P>(t), [&](const Place& at) { logits_done<P, KEEP>(g, lds, o, at.m0, at.n0); });
 }
 
 // ---------------------------------------------------------------------------------- rows
@@ -495,14 +514,8 @@ struct GradOut {
     const float* inv;
 };
 
-template <class P, OutMode MODE>
-__global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, Tiles t, GradOut o) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
-    const Where at = tile_of(t, blockIdx.x, gridDim.x);
-    const int m0 = at.m * P::BM, n0 = at.n * P::BN, s0 = at.part * t.steps;
-    P g;
-    g.run(lds, X, Y, m0, n0, s0, min(t.steps, t.all - s0));
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+template <class P, OutMode MODE> __device__ __forceinline__ void grad_done(P& g, uint8_t* lds, const GradOut& o, int m0, int n0, int part) {
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6, r16 = lane & 15, q = lane >> 4;
     const int mw = m0 + (wave / P::WN) * P::TM * 16 + r16, nw = n0 + (wave % P::WN) * P::TN * 16 + 4 * q;
     if constexpr (MODE != OutBf16) {
 #pragma unroll
@@ -513,7 +526,7 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
                 const int n = nw + 16 * tn;
                 if (m >= o.M || n >= o.N) continue;
                 if constexpr (MODE == OutPart) {
-                    *reinterpret_cast<f32x4_t*>(o.f + ((long)at.part * o.M + m) * o.ldf + n) = g.acc[tn][tm];
+                    *reinterpret_cast<f32x4_t*>(o.f + ((long)part * o.M + m) * o.ldf + n) = g.acc[tn][tm];
                 } else {
                     f32x4_t* f = reinterpret_cast<f32x4_t*>(o.f + m * o.ldf + n);
                     if (!o.first) g.acc[tn][tm] += *f;
@@ -523,7 +536,6 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
         }
         if (MODE == OutPart || !o.last) return;
     }
-    __syncthreads();
     // (dweight is as large as the weight and not read again here: streamed past the caches it leaves them
     // to the weight and its own writing to the memory; 33 tokens, 56136 x 5120: the call 429 -> 374 us)
     const bool eight = (o.ldc & 7) == 0 && ((uintptr_t)o.c & 15) == 0;  // (N = ldc: eight columns are in or out together)
@@ -543,6 +555,12 @@ __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, 
             for (int e = 0; e < 8 && n0 + n + e < o.N; e++) c[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
         }
     });
+}
+template <class P, OutMode MODE>
+__global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, Tiles t, GradOut o) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
+    P g;
+    g.go(lds, X, Y, Places<P>(t).place(), Places<P>(t), [&](const Place& at) { grad_done<P, MODE>(g, lds, o, at.m0, at.n0, at.step0 / t.steps); });
 }
 // the parts of a contraction added in order, 4 columns a thread (twice = 32: and row m + 32's)
 __global__ __launch_bounds__(256) void add_parts(GradOut o, int splits, int twice) {
@@ -772,6 +790,7 @@ static Tiles tiles(long M, long N, int BM, int BN, long K, int splits) {
     t.all = (int)(K / BK);
     t.steps = (int)ceil_div(t.all, splits);
     t.splits = (int)ceil_div(t.all, t.steps);
+    t.total = t.m * t.n * t.splits;
     // m tiles that run together, 1024 rows: with 256 x 256 tiles and 8192 rows 4 tiles took 4.46 ms for
     // dweight, 8 4.63 and 2 4.51; smaller tiles of few rows would read the other operand again
     const int group = TOGETHER / BM;
@@ -779,7 +798,14 @@ static Tiles tiles(long M, long N, int BM, int BN, long K, int splits) {
     return t;
 }
 
+// workgroups of a product: as many as run at once, each with its tiles, or (few steps) one a tile
+template <class P> static unsigned groups(const Tiles& t, int cus) {
+    const int slots = cus * (163840 / P::LDS < 2 ? 1 : 2) / 8 * 8;
+    return P::KEPT && t.all - (t.splits - 1) * t.steps > P::NST && slots > 0 && t.total > slots ? slots : t.total;
+}
+
 static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hipStream_t st) {
+    const int cus = device_cus();
     uint8_t* first = a->phase != THESEUS_VOCAB_ALL ? static_cast<uint8_t*>(a->kept) : ws;
     auto at = [&](size_t off) { return first + off; };
     const bool forward = a->phase != THESEUS_VOCAB_GRADIENTS, gradients = p.grads && a->phase != THESEUS_VOCAB_FORWARD;
@@ -833,8 +859,8 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
             auto launch = [&](auto tag) {
                 using P = decltype(tag);
                 const Tiles tl = tiles(m, n1 - n0, P::BM, P::BN, p.Dp, 1);
-                if (p.grads) logits_kernel<P, true><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
-                else logits_kernel<P, false><<<tl.m * tl.n, P::THREADS, 0, st>>>(X, Y, tl, lo);
+                if (p.grads) logits_kernel<P, true><<<groups<P>(tl, cus), P::THREADS, 0, st>>>(X, Y, tl, lo);
+                else logits_kernel<P, false><<<groups<P>(tl, cus), P::THREADS, 0, st>>>(X, Y, tl, lo);
             };
             switch (shape) {
                 case 0: launch(Logits0{}); break;
@@ -870,10 +896,10 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
                 using P = decltype(tag);
                 const Tiles tl = tiles(gm, p.D, P::BM, P::BN, p.lde, p.splits);
                 if (tl.splits > 1 || p.twice) {
-                    grad_kernel<P, OutPart><<<tl.m * tl.n * tl.splits, 512, 0, st>>>(GX, WY, tl, go);
+                    grad_kernel<P, OutPart><<<groups<P>(tl, cus), 512, 0, st>>>(GX, WY, tl, go);
                     add_parts<<<dim3((unsigned)ceil_div(p.D, 1024), (unsigned)m), 256, 0, st>>>(go, tl.splits, p.twice ? 32 : 0);
                 } else {
-                    grad_kernel<P, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, WY, tl, go);
+                    grad_kernel<P, OutBf16><<<groups<P>(tl, cus), 512, 0, st>>>(GX, WY, tl, go);
                 }
             };
             switch (p.dhidden) {
@@ -893,8 +919,8 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
                                  reinterpret_cast<float*>((ws + p.acc)) + v0 * up(p.D, 4), up(p.D, 4), piece == 0, piece == p.pieces - 1,
                                  a->temperature, inv};
                 const Tiles tl = tiles(v1 - v0, p.D, P::BM, P::BN, mp, 1);
-                if (p.pieces > 1) grad_kernel<P, OutAdd><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
-                else grad_kernel<P, OutBf16><<<tl.m * tl.n, 512, 0, st>>>(GX, HY, tl, go);
+                if (p.pieces > 1) grad_kernel<P, OutAdd><<<groups<P>(tl, cus), 512, 0, st>>>(GX, HY, tl, go);
+                else grad_kernel<P, OutBf16><<<groups<P>(tl, cus), 512, 0, st>>>(GX, HY, tl, go);
             };
             if (p.dweight == 0) dweight(Dweight0{}, 0, p.wmain);
             else dweight(Dweight1{}, 0, p.wmain);

@@ -564,6 +564,44 @@ def test_tiles_of_192_rows_and_split_weight_gradients_match_float64(M, D, V, pie
 
 
 @gpu
+@pytest.mark.parametrize("M,D,V,piece", [(1000, 192, 30000, 0), (1000, 128, 30000, 0), (130, 320, 120000, 0), (100, 320, 90001, 0),
+                                         (64, 384, 80000, 0), (250, 384, 60001, 0), (1025, 1280, 20003, 512), (4096, 4608, 3000, 0)])
+def test_workgroups_that_make_several_tiles_match_float64(M, D, V, piece):
+    """More tiles than run at once, of one step more than the stages hold and of many, of just as many (one tile a
+    workgroup), in parts and pieces."""
+    print(f"  several tiles M={M} D={D} V={V} piece={piece}", flush=True)
+    x, w, g = _inputs(M, D, V, seed=D)
+    labels = torch.randint(V, (M,), generator=g)
+    one = torch.ones(M).double()
+    o = _oracle(x.cuda(), w.cuda(), _dense(M, V, labels[:, None], torch.ones(M, 1)).cuda(), 0.0, one.cuda(), 1.0, (one / M).cuda())
+    o = {k: v.cpu() for k, v in o.items()}
+    loss, dx, dw = _run(lambda a, b: vocab.linear_cross_entropy(a, b, labels.cuda(), piece_rows=piece), x, w, torch.tensor(1.), "mean")
+    assert abs(float(loss) - float(o["loss"].mean())) <= float(o["ltol"].mean())
+    _grad_close(dx, o["dx"], o["dx_tol"])
+    _grad_close(dw, o["dw"], o["dw_tol"])
+    each = vocab.linear_cross_entropy(x.cuda(), w.cuda(), labels.cuda(), reduction="none")
+    assert ((each.double().cpu() - o["loss"]).abs() <= o["ltol"]).all()
+
+
+@gpu
+def test_many_targets_of_several_tiles_match_float64():
+    M, D, V, K = 300, 320, 80001, 100
+    x, w, g = _inputs(M, D, V, seed=5)
+    tv, ti = 2 * torch.randn(M, K, generator=g), torch.randint(V, (M, K), generator=g)
+    q = torch.softmax(tv.double() / 2, -1)
+    one = torch.ones(M).double()
+    o = _oracle(x.cuda(), w.cuda(), _dense(M, V, ti, q).cuda(), (q * q.log()).sum(-1).cuda(), one.cuda(), 2.0, one.cuda())
+    o = {k: v.cpu() for k, v in o.items()}
+    loss, dx, dw = _run(lambda a, b: vocab.linear_top_distillation(a, b, tv.cuda(), ti.cuda(), temperature=2.0, reduction="none"),
+                        x, w, torch.ones(M), "none")
+    # (q itself: float32 exponentials of |t / T - lse| < 20, 2^-20 of each term)
+    qtol = 4 * 2.0 ** -19 * (q * q.log().abs()).sum(-1)
+    assert ((loss.double().cpu() - o["loss"]).abs() <= o["ltol"] + qtol + 1e-6 * o["loss"].abs()).all()
+    _grad_close(dx, o["dx"], o["dx_tol"])
+    _grad_close(dw, o["dw"], o["dw_tol"])
+
+
+@gpu
 @pytest.mark.parametrize("M,D,V", [(1, 128, 4000), (5, 100, 333), (31, 256, 9000), (32, 64, 50)])
 def test_few_tokens_gradients_are_rounded_once(M, D, V):
     """Up to 32 tokens: G in two halves (2^-16), its softmax part from float16 exponentials (11 bits: 2^-11), so
