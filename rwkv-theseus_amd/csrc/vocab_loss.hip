@@ -218,10 +218,11 @@ template <class P, int LO, int HI> __device__ __forceinline__ f32x4_t fragment(c
     else return fragment<P, (LO + HI) / 2, HI>(g, code);
 }
 // h . w at the targets that lie in the workgroup's tile, out of the accumulators: the tile's tokens'
-// targets are looked through (some thousand at a time), those in its columns listed in LDS, and each wave
-// goes down the list for its own.  The list's order, which the atomics leave open, changes nothing.
-// (About 3 us a tile of 256 x 256 with 32 targets a token, 96 us of 8192 x 65536 logits; dot products
-// in a kernel of their own, D values of weight a target: 460 us.  With labels equal.)
+// targets are looked through (some thousand at a time), those in its columns listed in LDS, and each
+// wave goes down the list for its own.  The list's order, which the atomics leave open, changes
+// nothing.  (2048 x 131072 logits at D = 4096 and their gradient: 3412 us with 1 or 16 targets a token,
+// 3497 with 64; dot products in a kernel of their own, D values of weight a target, 460 us for 32
+// targets each of 8192 tokens, D = 5120.)
 template <class P> __device__ __forceinline__ void pick_targets(const P& g, uint8_t* lds, const LogitsOut& o, int m0, int n0) {
     constexpr int READ = (P::EPILOGUE - 260) / (P::THREADS * 16), CHUNK = P::THREADS * 4 * READ;  // (fours a thread)
     uint32_t* list = reinterpret_cast<uint32_t*>(P::epilogue(lds));  // (64 entries are read at a time)
