@@ -237,7 +237,10 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
 
     f32x4_t acc[TN][TM];
 
-    template <class Next, class Done>
+    // SHORT, for tiles of few steps: what is loaded ahead lies any number of tiles ahead; else no further
+    // than in the next tile.  (33 tokens' dweight of 56136 x 5120, one step a tile: 142 us with one tile a
+    // workgroup, 113 so, 5.1 TB/s)
+    template <bool SHORT, class Next, class Done>
     __device__ __forceinline__ void go(uint8_t* lds, const Operand& X, const Operand& Y, Place at, Next next, Done done) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
@@ -245,6 +248,20 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
         LoadY ly(Y, at.n0, at.step0 * BK, wave, lane);
         const Reader<LX, BM, PERM> rx((wave / WN) * TM * 16, lane);
         const Reader<LY, BN, PERM> ry((wave % WN) * TN * 16, lane);
+        Place far = at;  // (SHORT: where the loaders are)
+        Next beyond = next;
+        int step = 0;
+        auto forward = [&] {
+            if (step + 1 < far.steps) {
+                step++;
+                lx.advance(true);
+                ly.advance(true);
+            } else if (Place to; beyond(to)) {
+                far = to, step = 0;
+                lx = LoadX(X, to.m0, to.step0 * BK, wave, lane);
+                ly = LoadY(Y, to.n0, to.step0 * BK, wave, lane);
+            }
+        };
         auto piece = [&](int stage, int j) {
             if (j < LoadX::PIECES) lx.issue(lds0 + stage * STAGE, j, wave);
             else ly.issue(lds0 + stage * STAGE + BM * BK * 2, j - LoadX::PIECES, wave);
@@ -253,8 +270,12 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
         for (int s = 0; s < NST; s++) {
 #pragma unroll
             for (int j = 0; j < PIECES; j++) piece(s, j);
-            lx.advance(s + 1 < at.steps);
-            ly.advance(s + 1 < at.steps);
+            if constexpr (SHORT) {
+                forward();
+            } else {
+                lx.advance(s + 1 < at.steps);
+                ly.advance(s + 1 < at.steps);
+            }
         }
         wait_barrier<(NST - 1) * PIECES>();
 
@@ -308,7 +329,7 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
 #pragma unroll
             for (int i = 0; i < TN; i++) read_y(cur, i, 0);
             __builtin_amdgcn_s_waitcnt(0xc07f);  // (so that what is out at the loop's start is what its end left)
-            auto step = [&](auto move) {
+            auto multiply = [&](auto move) {
                 groups(x0, x1, cur, 1, None{}, std::false_type{}, 0);
                 // (the stage's last reads complete under these)
 #pragma unroll
@@ -323,18 +344,22 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
             };
             // step s loads step s + NST; the last ones, which load the next tile's, in a loop of their own
             // (the choice in the long one costs 2 %)
-            int s = 0;
-            for (; s < at.steps - NST - 1; s++)
-                step([&] {
-                    lx.advance(true);
-                    ly.advance(true);
-                });
-            for (; s < at.steps; s++)
-                step([&] {
-                    const int left = at.steps - NST - 1 - s;
-                    lx.move(more && left < 0, more && left == 0, tx);
-                    ly.move(more && left < 0, more && left == 0, ty);
-                });
+            if constexpr (SHORT) {
+                for (int s = 0; s < at.steps; s++) multiply(forward);
+            } else {
+                int s = 0;
+                for (; s < at.steps - NST - 1; s++)
+                    multiply([&] {
+                        lx.advance(true);
+                        ly.advance(true);
+                    });
+                for (; s < at.steps; s++)
+                    multiply([&] {
+                        const int left = at.steps - NST - 1 - s;
+                        lx.move(more && left < 0, more && left == 0, tx);
+                        ly.move(more && left < 0, more && left == 0, ty);
+                    });
+            }
             if constexpr (!KEPT) {
                 wkv7::vm_wait_n<0>();
                 __syncthreads();

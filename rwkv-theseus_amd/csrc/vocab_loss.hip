@@ -359,7 +359,7 @@ template <class P, bool KEEP>
 __global__ __launch_bounds__(P::THREADS) void logits_kernel(Operand X, Operand Y, Tiles t, LogitsOut o) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
     P g;
-    g.go(lds, X, Y, Places<P>(t).place(), Places<P>(t), [&](const Place& at) { logits_done<P, KEEP>(g, lds, o, at.m0, at.n0); });
+    g.template go<false>(lds, X, Y, Places<P>(t).place(), Places<P>(t), [&](const Place& at) { logits_done<P, KEEP>(g, lds, o, at.m0, at.n0); });
 }
 
 // ---------------------------------------------------------------------------------- rows
@@ -557,11 +557,11 @@ template <class P, OutMode MODE> __device__ __forceinline__ void grad_done(P& g,
         }
     });
 }
-template <class P, OutMode MODE>
+template <class P, OutMode MODE, bool SHORT = false>
 __global__ __launch_bounds__(P::THREADS) void grad_kernel(Operand X, Operand Y, Tiles t, GradOut o) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
     P g;
-    g.go(lds, X, Y, Places<P>(t).place(), Places<P>(t), [&](const Place& at) { grad_done<P, MODE>(g, lds, o, at.m0, at.n0, at.step0 / t.steps); });
+    g.template go<SHORT>(lds, X, Y, Places<P>(t).place(), Places<P>(t), [&](const Place& at) { grad_done<P, MODE>(g, lds, o, at.m0, at.n0, at.step0 / t.steps); });
 }
 // the parts of a contraction added in order, 4 columns a thread (twice = 32: and row m + 32's)
 __global__ __launch_bounds__(256) void add_parts(GradOut o, int splits, int twice) {
@@ -799,10 +799,11 @@ static Tiles tiles(long M, long N, int BM, int BN, long K, int splits) {
     return t;
 }
 
-// workgroups of a product: as many as run at once, each with its tiles, or (few steps) one a tile
-template <class P> static unsigned groups(const Tiles& t, int cus) {
+// workgroups of a product: as many as run at once, each with its tiles, or (few steps, and not go()'s
+// SHORT form) one a tile
+template <class P> static unsigned groups(const Tiles& t, int cus, bool few = false) {
     const int slots = cus * (163840 / P::LDS < 2 ? 1 : 2) / 8 * 8;
-    return P::KEPT && t.all - (t.splits - 1) * t.steps > P::NST && slots > 0 && t.total > slots ? slots : t.total;
+    return P::KEPT && (few || t.all - (t.splits - 1) * t.steps > P::NST) && slots > 0 && t.total > slots ? slots : t.total;
 }
 
 static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hipStream_t st) {
@@ -920,7 +921,9 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
                                  reinterpret_cast<float*>((ws + p.acc)) + v0 * up(p.D, 4), up(p.D, 4), piece == 0, piece == p.pieces - 1,
                                  a->temperature, inv};
                 const Tiles tl = tiles(v1 - v0, p.D, P::BM, P::BN, mp, 1);
+                const bool few = tl.all <= P::NST;  // up to 128 tokens
                 if (p.pieces > 1) grad_kernel<P, OutAdd><<<groups<P>(tl, cus), 512, 0, st>>>(GX, HY, tl, go);
+                else if (few) grad_kernel<P, OutBf16, true><<<groups<P>(tl, cus, true), 512, 0, st>>>(GX, HY, tl, go);
                 else grad_kernel<P, OutBf16><<<groups<P>(tl, cus), 512, 0, st>>>(GX, HY, tl, go);
             };
             if (p.dweight == 0) dweight(Dweight0{}, 0, p.wmain);

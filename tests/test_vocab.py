@@ -565,7 +565,8 @@ def test_tiles_of_192_rows_and_split_weight_gradients_match_float64(M, D, V, pie
 
 @gpu
 @pytest.mark.parametrize("M,D,V,piece", [(1000, 192, 30000, 0), (1000, 128, 30000, 0), (130, 320, 120000, 0), (100, 320, 90001, 0),
-                                         (64, 384, 80000, 0), (250, 384, 60001, 0), (1025, 1280, 20003, 512), (4096, 4608, 3000, 0)])
+                                         (64, 384, 80000, 0), (250, 384, 60001, 0), (8, 768, 30152, 0), (64, 1280, 20000, 0),
+                                         (128, 1280, 20001, 0), (90, 1100, 30000, 0), (1025, 1280, 20003, 512), (4096, 4608, 3000, 0)])
 def test_workgroups_that_make_several_tiles_match_float64(M, D, V, piece):
     """More tiles than run at once, of one step more than the stages hold and of many, of just as many (one tile a
     workgroup), in parts and pieces."""
