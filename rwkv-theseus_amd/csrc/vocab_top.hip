@@ -140,12 +140,16 @@ template <bool BF16, int T, int G> __global__ __launch_bounds__(T, 8) void top_p
 
     const float base = base_of(all), b = base * p.scale;
     float sum = 0.f;
-    if (fabsf(b) < 1e30f) {
+    // x scale - b is one fma, whose exponents are all off by b's rounding, as the lse is by that of its own
+    // largest part: up to 2^12 that shift is below 2^-12.  Beyond, where it would reach whole powers of two (and the
+    // products overflow at the type's ends), the difference is taken first: the maximum's term is 1.  (One operation
+    // more for each element.)
+    if (fabsf(b) < 4096.f) {
 #pragma unroll
         for (int j = 0; j < G; j++)
 #pragma unroll
             for (int e = 0; e < PER; e++) sum += __builtin_amdgcn_exp2f(val(w[j], e) * p.scale - b);
-    } else {  // (a row at the type's lowest or highest values: their products with the scale would overflow)
+    } else {
 #pragma unroll
         for (int j = 0; j < G; j++)
 #pragma unroll
