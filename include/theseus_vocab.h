@@ -46,7 +46,9 @@ typedef struct theseus_vocab_loss_args {
     int targets;             /* K in 1 .. THESEUS_VOCAB_MAX_TOP (labels: 1)                    */
     const void* hidden;      /* bfloat16 [M][D], hidden_stride elements from row to row        */
     const void* weight;      /* bfloat16 [V][D], weight_stride elements from row to row        */
-    long long hidden_stride, weight_stride;
+    long long hidden_stride, weight_stride; /* at least D (of one row: not used); weight_stride up to 2^21.
+                                Rows that are not 16-byte aligned, not whole multiples of 64 wide or (hidden)
+                                more than 2^21 elements apart are copied in the workspace            */
     const int64_t* index;    /* [M][K]: the labels, or the teacher's top indices               */
     const void* top_values;  /* [M][K] the teacher's logits; NULL: index holds labels (K = 1,
                                 q = 1, rows with ignore_index left out)                        */

@@ -643,7 +643,7 @@ static long ceil_div(long x, long y) { return (x + y - 1) / y; }
 struct Plan {
     long M, V, D, K, Dp, lde, piece;  // Dp: width in the products; lde: kept columns; piece: rows
     int pieces, tiles;                // row pieces; logits tiles of a row
-    bool grads, pad, twice;
+    bool grads, padh, padw, twice;    // padh, padw: hidden, weight copied to rows of Dp
     int logits, rest, dhidden, dweight, wrest;  // indices into the shapes
     long main;                        // columns of the vocabulary in shape `logits`, the others in `rest`
     long wmain;                       // rows of dweight in shape `dweight`, the others in `wrest`
@@ -652,6 +652,9 @@ struct Plan {
 };
 
 constexpr long MAX_PIECE = 32768;  // rows: a grid's y dimension
+// Elements from row to row in the products, which address a tile's rows by 32-bit byte offsets.  Hidden
+// states further apart (the last token of each of several long sequences) are copied, a weight is refused.
+constexpr long MAX_STRIDE = 1l << 21;
 
 static int device_cus() {
     int dev = 0, n = 0;
@@ -665,8 +668,7 @@ static int check(const theseus_vocab_loss_args* a) {
         a->targets < 1 || a->targets > THESEUS_VOCAB_MAX_TOP || (!a->top_values && a->targets != 1) || a->hidden_stride < a->width ||
         a->weight_stride < a->width || a->piece_rows < 0 || !(a->temperature > 0.f) || !isfinite(a->temperature))
         return THESEUS_WKV7_ERR_SHAPE;
-    // (a tile's rows are addressed by 32-bit byte offsets)
-    if (a->hidden_stride > (1ll << 21) || a->weight_stride > (1ll << 21)) return THESEUS_WKV7_ERR_SHAPE;
+    if (a->vocab > 1 && a->weight_stride > MAX_STRIDE) return THESEUS_WKV7_ERR_SHAPE;
     if (a->top_dtype != THESEUS_VOCAB_BF16 && a->top_dtype != THESEUS_VOCAB_FP32) return THESEUS_WKV7_ERR_DTYPE;
     if (a->reduction < THESEUS_VOCAB_NONE || a->reduction > THESEUS_VOCAB_MEAN || a->phase < THESEUS_VOCAB_ALL ||
         a->phase > THESEUS_VOCAB_GRADIENTS || (a->phase != THESEUS_VOCAB_ALL && a->reduction != THESEUS_VOCAB_NONE))
@@ -699,7 +701,11 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     Plan p{};
     p.M = a->rows, p.V = a->vocab, p.D = a->width, p.K = a->targets;
     p.Dp = up(p.D, BK);
-    p.pad = p.D != p.Dp || a->hidden_stride % 8 || a->weight_stride % 8 || ((uintptr_t)a->hidden | (uintptr_t)a->weight) % 16;
+    // (the products read rows of whole steps, 16 bytes at a time; the stride of one row is not used)
+    auto pad = [&](const void* x, long rows, long stride) {
+        return p.D != p.Dp || (uintptr_t)x % 16 || (rows > 1 && (stride % 8 || stride > MAX_STRIDE));
+    };
+    p.padh = pad(a->hidden, p.M, a->hidden_stride), p.padw = pad(a->weight, p.V, a->weight_stride);
     p.grads = a->dhidden || a->dweight || a->phase != THESEUS_VOCAB_ALL;
     p.lde = up(p.V, BK);
     long cap = a->piece_rows ? up(a->piece_rows, 256) : p.grads ? (2l << 30) / (2 * p.lde) / 256 * 256 : MAX_PIECE;
@@ -778,10 +784,10 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     if (a->phase != THESEUS_VOCAB_ALL) at = 0;  // (what is above lies in a->kept)
     p.acc = take(a->dweight && p.pieces > 1 ? (size_t)p.V * up(p.D, 4) * 4 : 0);
     p.parts = take(p.splits > 1 || p.twice ? (size_t)p.splits * (p.twice ? 64 : rows) * up(p.D, 4) * 4 : 0);
-    p.hidden = take(p.pad ? (size_t)p.M * p.Dp * 2 : 0);
-    p.weight = take(p.pad ? (size_t)p.V * p.Dp * 2 : 0);
+    p.hidden = take(p.padh ? (size_t)p.M * p.Dp * 2 : 0);
+    p.weight = take(p.padw ? (size_t)p.V * p.Dp * 2 : 0);
     p.bytes = at;
-    if (a->phase == THESEUS_VOCAB_FORWARD && !p.pad) p.bytes = 0;
+    if (a->phase == THESEUS_VOCAB_FORWARD && !p.padh && !p.padw) p.bytes = 0;
     return p;
 }
 
@@ -823,20 +829,21 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
     float* losses = reduce ? reinterpret_cast<float*>(at(p.loss)) : a->loss;
     const uint16_t* H = static_cast<const uint16_t*>(a->hidden);
     const uint16_t* W = static_cast<const uint16_t*>(a->weight);
-    long ldh = a->hidden_stride, ldw = a->weight_stride;
+    long ldh = p.M == 1 ? p.Dp : a->hidden_stride, ldw = p.V == 1 ? p.Dp : a->weight_stride;
     const float inv_T = 1.f / a->temperature;
     if (p.M == 0) {
         if (reduce) sums_kernel<<<1, 1024, 0, st>>>(Sums{0, nullptr, 0, nullptr, nullptr, a->loss});
         if (a->dweight) zero_kernel<<<1024, 256, 0, st>>>(static_cast<uint16_t*>(a->dweight), p.V * p.D);
         return 0;
     }
-    if (p.pad) {
-        uint16_t *h = reinterpret_cast<uint16_t*>((ws + p.hidden)), *w = reinterpret_cast<uint16_t*>((ws + p.weight));
-        const unsigned gx = (unsigned)ceil_div(p.Dp, 256);
-        pad_rows<<<dim3(gx, (unsigned)(p.M < 32768 ? p.M : 32768)), 256, 0, st>>>(p.M, (int)p.D, (int)p.Dp, H, ldh, h);
-        pad_rows<<<dim3(gx, (unsigned)(p.V < 32768 ? p.V : 32768)), 256, 0, st>>>(p.V, (int)p.D, (int)p.Dp, W, ldw, w);
-        H = h, W = w, ldh = ldw = p.Dp;
-    }
+    auto padded = [&](const uint16_t* x, long rows, long& ld, size_t to) {
+        uint16_t* out = reinterpret_cast<uint16_t*>(ws + to);
+        pad_rows<<<dim3((unsigned)ceil_div(p.Dp, 256), (unsigned)(rows < 32768 ? rows : 32768)), 256, 0, st>>>(rows, (int)p.D, (int)p.Dp, x, ld, out);
+        ld = p.Dp;
+        return static_cast<const uint16_t*>(out);
+    };
+    if (p.padh) H = padded(H, p.M, ldh, p.hidden);
+    if (p.padw) W = padded(W, p.V, ldw, p.weight);
     if (forward && a->top_values) {
         const Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight, inv_T, j, q, row};
         targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);

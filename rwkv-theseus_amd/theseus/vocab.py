@@ -28,6 +28,7 @@ import torch
 from .wkv7 import _native, extension
 
 MAX_TOP = 256  # THESEUS_VOCAB_MAX_TOP
+MAX_STRIDE = 1 << 21  # elements from row to row of a weight (include/theseus_vocab.h)
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
@@ -214,6 +215,8 @@ def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_ind
     if row_weight is not None:
         row_weight = _rows(row_weight, "token_weight", tokens, device, (torch.float32,))
     h, w = _matrix(hidden if len(tokens) == 1 else hidden.reshape(math.prod(tokens), hidden.shape[-1])), _matrix(weight)
+    if w.stride(0) > MAX_STRIDE:
+        w = w.contiguous()
     native = _native(h, w)
     if native is not None:
         loss = native.vocab_loss(h, w, index, top_values, teacher_lse, row_weight, ignore_index, temperature,

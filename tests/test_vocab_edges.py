@@ -47,3 +47,69 @@ def test_log_sum_exp_with_one_slab_of_large_values(dtype, V, T):
     values, _, lse = vocab.top_logits(x.cuda(), 5, temperature=T)
     _lse_close(lse, x, T)
     assert torch.equal(values.cpu(), x.topk(5, -1).values)
+
+
+# ------------------------------------------------------------------------------ rows far apart
+def _inputs(M, D, V, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(M, D, generator=g).bfloat16(), (torch.randn(V, D, generator=g) * (2 / D ** .5)).bfloat16(), g
+
+
+def _python_path(monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(vocab, "_native", lambda *xs: None)
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("B,T,D", [(1, 410, 5120), (3, 410, 5120), (1, 33000, 64), (40, 33000, 64), (2, 30000, 72)])
+def test_last_tokens_of_long_sequences(B, T, D, native, monkeypatch):
+    """hidden[:, -1] of [B,T,D] with T D > 2^21: the loss and gradients of a contiguous copy."""
+    _python_path(monkeypatch, native)
+    print(f"  last of {B} x {T} x {D}", flush=True)
+    x, w, g = _inputs(B, D, 700)
+    labels = torch.randint(700, (B,), generator=g).cuda()
+    full = torch.full((B, T, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+    full[:, -1] = x.cuda()
+    for reduction in ("mean", "none"):
+        got, want = [], []
+        for out, h in ((got, full.clone().requires_grad_()), (want, x.cuda().requires_grad_())):
+            wt = w.cuda().requires_grad_()
+            loss = vocab.linear_cross_entropy(h[:, -1] if h.dim() == 3 else h, wt, labels, reduction=reduction)
+            dh, dw = torch.autograd.grad(loss.sum(), (h, wt))
+            out += [loss.detach(), dh[:, -1] if dh.dim() == 3 else dh, dw]
+            assert dh.dim() == 2 or not dh[:, :-1].any()
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+        assert torch.equal(vocab.linear_cross_entropy(full[:, -1], w.cuda(), labels, reduction=reduction), want[0])
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_weight_rows_far_apart(native, monkeypatch):
+    _python_path(monkeypatch, native)
+    x, w, g = _inputs(9, 64, 5)
+    labels = torch.randint(5, (9,), generator=g).cuda()
+    want = vocab.linear_cross_entropy(x.cuda(), w.cuda(), labels)
+    wide = torch.full((5, (1 << 21) + 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[:, :64] = w.cuda()
+    assert torch.equal(vocab.linear_cross_entropy(x.cuda(), wide[:, :64], labels), want)
+    one = vocab.linear_cross_entropy(x.cuda(), wide[2:3, :64], torch.zeros(9, dtype=torch.int64).cuda(), reduction="none")
+    assert one.abs().max() <= 1e-5  # (a vocabulary of one word)
+
+
+def test_strides_are_sized_without_a_gpu():
+    """Hidden rows at any distance; of one row no stride is used, of a weight's rows 2^21 is the limit;
+    only what needs it is copied."""
+    lib, p = vocab._lib(), 1 << 20
+    ok = dict(rows=4, vocab=1000, width=64, targets=1, hidden=p, weight=p, hidden_stride=64, weight_stride=64, index=p,
+              temperature=1.0, reduction=0, loss=p)
+    size = lambda **kw: lib.theseus_vocab_loss_workspace_size(vocab.LossArgs(**{**ok, **kw}))  # noqa: E731
+    far = 1 << 21
+    assert size(hidden_stride=far) == size()
+    copied = size(hidden_stride=far + 8)
+    assert size() < copied <= size() + 4 * 64 * 2 + 256 and size(hidden_stride=1 << 40) == size(hidden=p + 2) == copied
+    assert size(rows=1, hidden_stride=1 << 40) == size(rows=1) > 0
+    assert size(weight_stride=far) == size() and size(weight_stride=far + 8) == 0
+    assert size(vocab=1, weight_stride=far + 8) == size(vocab=1) > 0
+    assert size(weight=p + 2) >= size() + 1000 * 64 * 2
