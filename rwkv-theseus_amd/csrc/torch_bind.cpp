@@ -241,6 +241,7 @@ std::pair<Tensor, Tensor> gdn(const Tensor& q, const Tensor& k, const Tensor& v,
 // (h [M][D] and w [V][D] with rows apart, the others contiguous).
 struct VocabLoss : torch::autograd::Function<VocabLoss> {
     using Opt = std::optional<Tensor>;
+    static constexpr const char *INDEX = "labels (or top_indices)", *TOP = "top_values", *LSE = "teacher_lse", *WEIGHT = "token_weight";
     static void* optr(const Opt& t) { return t ? t->data_ptr() : nullptr; }
     static void call(const Tensor& h, const Tensor& w, const Tensor& index, const Opt& top, const Opt& lse, const Opt& weight,
                      int64_t ignore, double T, int64_t reduction, int64_t piece, const Tensor& loss, const Tensor& row_grad,
@@ -270,6 +271,24 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
         const auto f = h.options().dtype(torch::kFloat32);
         return reduction == THESEUS_VOCAB_NONE ? at::empty({h.size(0)}, f) : at::empty({}, f);
     }
+    // What a backward that forms the logits again reads of the targets, and that it was not changed since: the
+    // others (gradients made with the loss, kept exponentials) do not look at these, so they are not saved
+    // variables, whose unpacking would ask of every backward what only this one needs.  Tensors of inference
+    // mode have no version: a copy.
+    static void hold(AutogradContext* ctx, const char* name, const Opt& t) {
+        if (!t) return;
+        const Tensor own = t->is_inference() ? t->clone() : *t;
+        ctx->saved_data[name] = own;
+        ctx->saved_data[std::string(name) + " version"] = (int64_t)own._version();
+    }
+    static Opt held(AutogradContext* ctx, const char* name) {
+        const auto at = ctx->saved_data.find(name);
+        if (at == ctx->saved_data.end()) return Opt();
+        const Tensor t = at->second.toTensor();
+        TORCH_CHECK((int64_t)t._version() == ctx->saved_data[std::string(name) + " version"].toInt(), "theseus_vocab: the ", name,
+                    " have been modified by an inplace operation after the loss whose gradients need them");
+        return t;
+    }
     static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& index, const Opt& top, const Opt& lse,
                           const Opt& weight, int64_t ignore, double T, int64_t reduction, int64_t piece) {
         c10::OptionalDeviceGuard guard(h.device());
@@ -288,8 +307,7 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
              reduction == THESEUS_VOCAB_NONE ? &kept : nullptr);
         ctx->saved_data["kept"] = kept.defined() ? at::IValue(kept) : at::IValue();
         ctx->save_for_backward({h, w});
-        ctx->saved_data["index"] = index;
-        ctx->saved_data["top"] = top, ctx->saved_data["lse"] = lse, ctx->saved_data["weight"] = weight;
+        hold(ctx, INDEX, index), hold(ctx, TOP, top), hold(ctx, LSE, lse), hold(ctx, WEIGHT, weight);
         ctx->saved_data["ignore"] = ignore, ctx->saved_data["T"] = T, ctx->saved_data["reduction"] = reduction;
         ctx->saved_data["piece"] = piece;
         return loss;
@@ -309,10 +327,14 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
             const variable_list s = ctx->get_saved_variables();
             if (ctx->needs_input_grad(0)) dh = at::empty(s[0].sizes(), s[0].options());
             if (ctx->needs_input_grad(1)) dw = at::empty(s[1].sizes(), s[1].options());
-            auto opt = [&](const char* k) { return d[k].isTensor() ? Opt(d[k].toTensor()) : Opt(); };
             Tensor kept = tensor(d["kept"]);
             d["kept"] = at::IValue();
-            call(s[0], s[1], d["index"].toTensor(), opt("top"), opt("lse"), opt("weight"), d["ignore"].toInt(), d["T"].toDouble(),
+            auto target = [&](const char* name) {  // (with exponentials, their targets were kept too)
+                if (!kept.defined()) return held(ctx, name);
+                const auto at = d.find(name);
+                return at == d.end() ? Opt() : Opt(at->second.toTensor());
+            };
+            call(s[0], s[1], *target(INDEX), target(TOP), target(LSE), target(WEIGHT), d["ignore"].toInt(), d["T"].toDouble(),
                  reduction, d["piece"].toInt(), Tensor(), reduction == THESEUS_VOCAB_NONE ? grad : Tensor(), dh, dw, kept.defined() ? &kept : nullptr);
         }
         if (reduction != THESEUS_VOCAB_NONE)

@@ -16,7 +16,8 @@ are cast as ``torch.nn.functional.linear`` casts them).  With ``reduction="mean"
 the gradients are made together with the loss, in three products, and the backward multiplies
 them by the upstream gradient; with ``"none"`` the backward makes them, from 16-bit exponentials
 that the forward keeps where they take at most 256 MiB, and else from the logits formed again.
-A second backward through the same loss (retain_graph) makes the gradients anew.
+A second backward through the same loss (retain_graph) makes the gradients anew.  Where a backward
+reads labels or a teacher's tensors again, it raises if they were changed in place since the call.
 """
 from __future__ import annotations
 
@@ -90,6 +91,24 @@ class _Call:
         self.rows, self.vocab, self.width = hidden.shape[0], weight.shape[0], hidden.shape[1]
         self.device = hidden.device
 
+    _HELD = {"index": "labels (or top_indices)", "top_values": "top_values", "teacher_lse": "teacher_lse", "row_weight": "token_weight"}
+
+    def hold(self):
+        """For a backward that forms the logits again: what it reads of the targets and that it was not changed
+        since (unchanged).  Not saved_tensors, whose unpacking would ask that of every backward.  Tensors of
+        inference mode have no version: a copy."""
+        for name in self._HELD:
+            t = getattr(self, name)
+            if t is not None and t.is_inference():
+                setattr(self, name, t.clone())
+        self.versions = {name: getattr(self, name)._version for name in self._HELD if getattr(self, name) is not None}
+
+    def unchanged(self):
+        for name, version in self.versions.items():
+            if getattr(self, name)._version != version:
+                raise RuntimeError(f"theseus_vocab: the {self._HELD[name]} have been modified by an inplace operation after "
+                                   "the loss whose gradients need them")
+
     def args(self, hidden, weight, loss, row_grad, dhidden, dweight):
         p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         return LossArgs(self.rows, self.vocab, self.width, self.targets, p(hidden), p(weight),
@@ -133,6 +152,7 @@ class _Loss(torch.autograd.Function):
             ctx.made = _Loss._like(hidden, need_h), _Loss._like(weight, need_w)
             call.run(hidden, weight, loss, None, *ctx.made)
         ctx.save_for_backward(hidden, weight)
+        call.hold()
         return loss
 
     @staticmethod
@@ -156,6 +176,8 @@ class _Loss(torch.autograd.Function):
             hidden, weight = ctx.saved_tensors
             need_h, need_w = ctx.needs_input_grad[:2]
             made = _Loss._like(hidden, need_h), _Loss._like(weight, need_w)
+            if kept is None:  # (with exponentials, their targets were kept too)
+                call.unchanged()
             call.run(hidden, weight, None, grad if call.reduction == "none" else None, *made, kept=kept)
         if call.reduction != "none":
             xy = [v for x in made for v in ((None, 0) if x is None else (x.data_ptr(), x.numel()))]

@@ -113,3 +113,66 @@ def test_strides_are_sized_without_a_gpu():
     assert size(weight_stride=far) == size() and size(weight_stride=far + 8) == 0
     assert size(vocab=1, weight_stride=far + 8) == size(vocab=1) > 0
     assert size(weight=p + 2) >= size() + 1000 * 64 * 2
+
+
+# ------------------------------------------------------------------------------ targets changed before the backward
+def _targets(g, M=300, V=700, K=6):
+    return {"labels": torch.randint(V, (M,), generator=g).cuda(), "top_indices": torch.randint(V, (M, K), generator=g).cuda(),
+            "top_values": torch.randn(M, K, generator=g).cuda(), "teacher_lse": torch.full((M,), 2.0).cuda(),
+            "token_weight": torch.rand(M, generator=g).cuda()}
+
+
+def _loss_of(name, h, w, t, **more):
+    if name == "labels":
+        return vocab.linear_cross_entropy(h, w, t["labels"], **more)
+    return vocab.linear_top_distillation(h, w, t["top_values"], t["top_indices"], teacher_lse=t["teacher_lse"],
+                                         token_weight=t["token_weight"], **more)
+
+
+NAMES = ["labels", "top_indices", "top_values", "teacher_lse", "token_weight"]
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("name", NAMES)
+def test_changed_targets_never_give_other_gradients(name, native, monkeypatch):
+    """A backward that reads the targets again raises once they were changed; the others give the call's."""
+    _python_path(monkeypatch, native)
+    x, w, g = _inputs(300, 64, 700)
+    t = _targets(g)
+    h, wt = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    for more, again in ((dict(reduction="none", piece_rows=256), True), (dict(reduction="none"), False), (dict(reduction="mean"), False)):
+        want = torch.autograd.grad(_loss_of(name, h, wt, t, **more).sum(), (h, wt))
+        old = t[name].clone()
+        loss = _loss_of(name, h, wt, t, **more).sum()
+        t[name].zero_()
+        if not again:
+            got = torch.autograd.grad(loss, (h, wt), retain_graph=True)
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, (h, wt))
+        t[name].copy_(old)
+    loss = _loss_of(name, h, wt, t, reduction="none", piece_rows=256).sum()
+    assert all(torch.isfinite(p).all() for p in torch.autograd.grad(loss, (h, wt)))
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_targets_of_inference_mode(native, monkeypatch):
+    """A teacher's tensors from torch.inference_mode, written again before a backward that reads the targets anew."""
+    _python_path(monkeypatch, native)
+    x, w, g = _inputs(300, 64, 700)
+    t = _targets(g)
+    h, wt = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    for name in ("labels", "top_values"):
+        for more in (dict(reduction="none", piece_rows=256), dict(reduction="mean")):
+            want = torch.autograd.grad(_loss_of(name, h, wt, t, **more).sum(), (h, wt))
+            with torch.inference_mode():
+                u = {k: v.clone() for k, v in t.items()}
+            loss = _loss_of(name, h, wt, u, **more).sum()
+            with torch.inference_mode():
+                for v in u.values():
+                    v.zero_()
+            for _ in range(2):
+                got = torch.autograd.grad(loss, (h, wt), retain_graph=True)
+                assert all(torch.equal(p, q) for p, q in zip(got, want))
