@@ -26,6 +26,7 @@ import math
 
 import torch
 
+from .fused import _direct
 from .wkv7 import _native, extension
 
 MAX_TOP = 256  # THESEUS_VOCAB_MAX_TOP
@@ -142,12 +143,15 @@ class _Call:
 
 class _Loss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, call):
+    def forward(ctx, hidden, weight, *targets_and_constants):
+        # (a trace replays this with tensors that nothing else has looked at)
+        hidden, weight, *targets = _laid_out(hidden, weight, *targets_and_constants[:4])
+        call = _Call(hidden, weight, *targets, *targets_and_constants[4:])
         loss = call.new_loss()
         need_h, need_w = ctx.needs_input_grad[:2]
         ctx.call, ctx.made, ctx.kept = call, None, None
         if call.reduction == "none":
-            ctx.kept = call.run(hidden, weight, loss, kept=True)
+            ctx.kept = call.run(hidden, weight, loss, kept=True if need_h or need_w else None)
         else:
             ctx.made = _Loss._like(hidden, need_h), _Loss._like(weight, need_w)
             call.run(hidden, weight, loss, None, *ctx.made)
@@ -162,7 +166,7 @@ class _Loss(torch.autograd.Function):
         if torch.is_grad_enabled():  # (create_graph: a later derivative through these raises)
             made = torch._C._functions.DelayedError("theseus_vocab: the losses are differentiable once", 2)(
                 *(x if x is None else x.requires_grad_() for x in made))
-        return (*made, None)
+        return (*made, *(None,) * 8)
 
     @staticmethod
     def _like(x, wanted):
@@ -206,24 +210,16 @@ def _matrix(x):
     return x.contiguous()
 
 
-def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_index, temperature, reduction, piece_rows):
-    if reduction not in _REDUCTIONS:
-        raise ValueError(f"theseus_vocab: unknown reduction {reduction!r} (none, sum or mean)")
+def _laid_out(hidden, weight, index, top_values, teacher_lse, row_weight):
+    """A loss's tensors, checked: hidden [M][D] and weight [V][D] with rows apart, the targets contiguous."""
     if not (hidden.is_cuda and weight.is_cuda):
         raise ValueError("theseus_vocab: hidden and weight must be CUDA tensors")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"theseus_vocab: expected hidden [..., D] and weight [V, D], got {list(hidden.shape)} and {list(weight.shape)}")
     if weight.device != hidden.device:
         raise ValueError(f"theseus_vocab: weight must be on {hidden.device}, got {weight.device}")
-    if torch.is_autocast_enabled("cuda"):
-        dt = torch.get_autocast_dtype("cuda")
-        hidden, weight = hidden.to(dt), weight.to(dt)
     if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise TypeError(f"theseus_vocab: hidden and weight must be bfloat16 (or cast by autocast), got {hidden.dtype} and {weight.dtype}")
-    if not temperature > 0 or temperature == float("inf"):
-        raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
-    if piece_rows < 0:
-        raise ValueError(f"theseus_vocab: piece_rows must not be negative, got {piece_rows}")
     tokens, device = hidden.shape[:-1], hidden.device
     index = _rows(index, "labels" if top_values is None else "top_indices", tokens, device, (torch.int64,),
                   () if top_values is None else (index.shape[-1] if index.dim() else 0,))
@@ -239,17 +235,32 @@ def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_ind
     h, w = _matrix(hidden if len(tokens) == 1 else hidden.reshape(math.prod(tokens), hidden.shape[-1])), _matrix(weight)
     if w.stride(0) > MAX_STRIDE:
         w = w.contiguous()
+    return h, w, index, top_values, teacher_lse, row_weight
+
+
+def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_index, temperature, reduction, piece_rows):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"theseus_vocab: unknown reduction {reduction!r} (none, sum or mean)")
+    if not temperature > 0 or temperature == float("inf"):
+        raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
+    if piece_rows < 0:
+        raise ValueError(f"theseus_vocab: piece_rows must not be negative, got {piece_rows}")
+    if hidden.is_cuda and weight.is_cuda and torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(dt), weight.to(dt)
+    tokens = hidden.shape[:-1]
+    h, w, *targets = _laid_out(hidden, weight, index, top_values, teacher_lse, row_weight)
     native = _native(h, w)
     if native is not None:
-        loss = native.vocab_loss(h, w, index, top_values, teacher_lse, row_weight, ignore_index, temperature,
-                                 _REDUCTIONS[reduction], piece_rows)
+        loss = native.vocab_loss(h, w, *targets, ignore_index, temperature, _REDUCTIONS[reduction], piece_rows)
         return loss.reshape(tokens) if reduction == "none" and len(tokens) != 1 else loss
-    call = _Call(h, w, index, top_values, teacher_lse, row_weight, ignore_index, float(temperature), reduction, piece_rows)
-    if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
-        loss = _Loss.apply(h, w, call)
-    else:
+    constants = ignore_index, float(temperature), reduction, piece_rows
+    if _direct(h, w, *targets):
+        call = _Call(h, w, *targets, *constants)
         loss = call.new_loss()
         call.run(h, w, loss)
+    else:
+        loss = _Loss.apply(h, w, *targets, *constants)
     return loss.reshape(tokens) if reduction == "none" else loss
 
 

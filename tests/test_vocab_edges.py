@@ -176,3 +176,53 @@ def test_targets_of_inference_mode(native, monkeypatch):
             for _ in range(2):
                 got = torch.autograd.grad(loss, (h, wt), retain_graph=True)
                 assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+# ------------------------------------------------------------------------------ traces and forward mode
+CALLS = {"cross_entropy": lambda h, w, y, tv, ti, lse, wt, **kw: vocab.linear_cross_entropy(h, w, y, **kw),
+         "distillation": lambda h, w, y, tv, ti, lse, wt, **kw: vocab.linear_top_distillation(
+             h, w, tv, ti, temperature=2.0, teacher_lse=lse, token_weight=wt, **kw)}
+
+
+def _call_tensors(seed, M=40, V=300):
+    x, w, g = _inputs(M, 64, V, seed)
+    t = _targets(g, M, V)
+    return x.cuda(), w.cuda(), t["labels"], t["top_values"], t["top_indices"], t["teacher_lse"], t["token_weight"]
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("name", list(CALLS))
+def test_traced_losses_run_again(name, reduction):
+    """torch.jit.trace, without gradients and with them: a replay computes the loss of its own inputs."""
+    f = lambda *a: CALLS[name](*a, reduction=reduction)  # noqa: E731
+    args, other = _call_tensors(1), _call_tensors(2)
+    traced = torch.jit.trace(f, args, check_trace=False)
+    for a in (args, other):
+        assert torch.equal(traced(*a), f(*a))
+    # (hidden states whose rows lie otherwise than the traced ones'; labels of other tokens)
+    turned = (other[0].t().contiguous().t(), *other[1:])
+    assert torch.equal(traced(*turned), f(*other))
+    with pytest.raises(Exception, match="must have shape"):
+        traced(*other[:2], *(t[:7] for t in other[2:]))
+    args, other = ([x.requires_grad_() for x in a[:2]] + list(a[2:]) for a in (args, other))
+    traced = torch.jit.trace(f, tuple(args), check_trace=False)
+    got, want = traced(*other).sum(), f(*other).sum()
+    assert torch.equal(got.detach(), want.detach())
+    for p, q in zip(torch.autograd.grad(got, other[:2]), torch.autograd.grad(want, other[:2])):
+        assert torch.equal(p, q)
+    batch = [x.detach() if i == 1 else x.detach().reshape(2, 20, *x.shape[1:]) for i, x in enumerate(args)]
+    traced = torch.jit.trace(f, tuple(batch), check_trace=False)
+    assert torch.equal(traced(*batch), f(*batch))
+
+
+@gpu
+@pytest.mark.parametrize("at", [0, 1, 3, 5, 6])
+def test_losses_refuse_a_tangent(at):
+    """Forward mode is not supported: no derivative of 0 by leaving a tangent behind."""
+    args = list(_call_tensors(3))
+    with torch.autograd.forward_ad.dual_level():
+        args[at] = torch.autograd.forward_ad.make_dual(args[at], torch.ones_like(args[at]))
+        for name in CALLS if at < 2 else ["distillation"]:
+            with pytest.raises(NotImplementedError, match="jvp"):
+                CALLS[name](*args)
