@@ -291,6 +291,42 @@ def linear_top_distillation(hidden, weight, top_values, top_indices, *, temperat
                  int(piece_rows))
 
 
+class _Top(torch.autograd.Function):
+    """What a trace runs again (its tensors checked and laid out here once more)."""
+
+    @staticmethod
+    def forward(ctx, x, k, temperature):
+        out = _top(_matrix(_top_checked(x, k)), k, temperature)
+        ctx.mark_non_differentiable(*out)
+        return out
+
+
+def _top(x, k, temperature):
+    """The C call for x [M][V], rows apart."""
+    (n, V), dt, dev = x.shape, _DTYPES[x.dtype], x.device
+    values = torch.empty((n, k), dtype=x.dtype, device=dev)
+    indices = torch.empty((n, k), dtype=torch.int64, device=dev)
+    lse = torch.empty(n, dtype=torch.float32, device=dev)
+    lib = _lib()
+    with torch.cuda.device(dev):
+        nbytes = int(lib.theseus_vocab_top_workspace_size(n, V, k, dt))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _check(lib.theseus_vocab_top(n, V, k, dt, temperature, x.data_ptr(), max(x.stride(0), V), values.data_ptr(),
+                                     indices.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                                     _stream(dev)))
+    return values, indices, lse
+
+
+def _top_checked(logits, k):
+    if not logits.is_cuda:
+        raise ValueError("theseus_vocab: logits must be a CUDA tensor")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"theseus_vocab: logits must be bfloat16 or float32, got {logits.dtype}")
+    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], MAX_TOP):
+        raise ValueError(f"theseus_vocab: k must be in 1..min(V, {MAX_TOP}), got {k} for logits {list(logits.shape)}")
+    return logits
+
+
 @torch.no_grad()
 def top_logits(logits, k, *, temperature=1.0):
     """The k largest logits of each row: (values [..., k] in the logits' type, indices [..., k]
@@ -299,31 +335,17 @@ def top_logits(logits, k, *, temperature=1.0):
 
     logits [..., V] bfloat16 or float32 (rows may lie apart: a slice of a wider tensor is read in
     place), 1 <= k <= min(V, 256).  Not differentiable."""
-    if not logits.is_cuda:
-        raise ValueError("theseus_vocab: logits must be a CUDA tensor")
-    if logits.dtype not in _DTYPES:
-        raise TypeError(f"theseus_vocab: logits must be bfloat16 or float32, got {logits.dtype}")
-    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], MAX_TOP):
-        raise ValueError(f"theseus_vocab: k must be in 1..min(V, {MAX_TOP}), got {k} for logits {list(logits.shape)}")
+    _top_checked(logits, k)
     if not temperature > 0 or temperature == float("inf"):
         raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
     V, rows = logits.shape[-1], logits.shape[:-1]
     x = _matrix(logits.detach().reshape(math.prod(rows), V))
     native = _native(x)
     if native is not None:
-        values, indices, lse = native.vocab_top(x, k, float(temperature))
-        if len(rows) == 1:
-            return values, indices, lse
-        return values.reshape(*rows, k), indices.reshape(*rows, k), lse.reshape(rows)
-    n, dt, dev = x.shape[0], _DTYPES[x.dtype], x.device
-    values = torch.empty((*rows, k), dtype=x.dtype, device=dev)
-    indices = torch.empty((*rows, k), dtype=torch.int64, device=dev)
-    lse = torch.empty(rows, dtype=torch.float32, device=dev)
-    lib = _lib()
-    with torch.cuda.device(dev):
-        nbytes = int(lib.theseus_vocab_top_workspace_size(n, V, k, dt))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _check(lib.theseus_vocab_top(n, V, k, dt, float(temperature), x.data_ptr(), max(x.stride(0), V), values.data_ptr(),
-                                     indices.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
-                                     _stream(dev)))
-    return values, indices, lse
+        out = native.vocab_top(x, k, float(temperature))
+    else:
+        out = (_top if _direct(x) else _Top.apply)(x, k, float(temperature))
+    if len(rows) == 1:
+        return out
+    values, indices, lse = out
+    return values.reshape(*rows, k), indices.reshape(*rows, k), lse.reshape(rows)

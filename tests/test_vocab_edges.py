@@ -226,3 +226,25 @@ def test_losses_refuse_a_tangent(at):
         for name in CALLS if at < 2 else ["distillation"]:
             with pytest.raises(NotImplementedError, match="jvp"):
                 CALLS[name](*args)
+
+
+@gpu
+def test_traced_top_logits_run_again():
+    g = torch.Generator().manual_seed(4)
+    f = lambda z: vocab.top_logits(z, 7, temperature=2.0)  # noqa: E731
+    a, b = (torch.randn(6, 500, generator=g).cuda() for _ in range(2))
+    traced = torch.jit.trace(f, (a,), check_trace=False)
+    for z in (a, b, b.t().contiguous().t()):
+        for p, q in zip(traced(z), f(b if z is not a else a)):
+            assert torch.equal(p, q)
+    with pytest.raises(Exception, match="k must be"):
+        traced(b[:, :5])
+    for shape in ((2, 3, 500), (500,)):
+        z = torch.randn(shape, generator=g).cuda()
+        traced = torch.jit.trace(f, (z,), check_trace=False)
+        for p, q in zip(traced(2 * z), f(2 * z)):
+            assert torch.equal(p, q)
+    want = f(a)
+    with torch.autograd.forward_ad.dual_level():  # (no tangent: the call itself)
+        for p, q in zip(f(a), want):
+            assert torch.equal(p, q)
