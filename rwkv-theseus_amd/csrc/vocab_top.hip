@@ -451,9 +451,15 @@ int theseus_vocab_top(long long rows, long long vocab, int k, int dtype, float t
     const Plan pl = plan(rows, vocab, k, dtype, ((uintptr_t)logits | (uintptr_t)(row_stride * size)) % 16 == 0);
     const size_t need = bytes_of((size_t)rows, (size_t)pl.slabs, k);
     if (need && (!workspace || workspace_bytes < need)) return THESEUS_WKV7_ERR_WORKSPACE;
-    Args p{rows, vocab, row_stride, k, (int)pl.slabs, (int)pl.each, LOG2E / temperature, 1.f / temperature, logits, values, indices, lse, nullptr, nullptr};
-    if (dtype == THESEUS_VOCAB_BF16) launch<true>(p, pl, static_cast<uint8_t*>(workspace), stream);
-    else launch<false>(p, pl, static_cast<uint8_t*>(workspace), stream);
+    // A launch has fewer than 2^32 threads: more rows than that (4 million of one slab) in several, in one workspace.
+    const long most = (long)(0xffffffffu / THREADS) / pl.slabs;
+    for (long r0 = 0; r0 < rows; r0 += most) {
+        Args p{rows - r0 < most ? rows - r0 : most, vocab, row_stride, k, (int)pl.slabs, (int)pl.each, LOG2E / temperature, 1.f / temperature,
+               static_cast<const uint8_t*>(logits) + r0 * row_stride * size, static_cast<uint8_t*>(values) + r0 * k * size,
+               indices + r0 * k, lse ? lse + r0 : nullptr, nullptr, nullptr};
+        if (dtype == THESEUS_VOCAB_BF16) launch<true>(p, pl, static_cast<uint8_t*>(workspace), stream);
+        else launch<false>(p, pl, static_cast<uint8_t*>(workspace), stream);
+    }
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }
 

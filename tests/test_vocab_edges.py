@@ -248,3 +248,31 @@ def test_traced_top_logits_run_again():
     with torch.autograd.forward_ad.dual_level():  # (no tangent: the call itself)
         for p, q in zip(f(a), want):
             assert torch.equal(p, q)
+
+
+# ------------------------------------------------------------------------------ sizes past one launch's
+@gpu
+@pytest.mark.parametrize("rows,V,k,dtype", [((1 << 22) + 5, 256, 129, torch.bfloat16), ((1 << 24) + 7, 16, 3, torch.float32)])
+def test_top_logits_of_more_rows_than_one_launch_takes(rows, V, k, dtype):
+    """Every row holds 0 .. V - 1 turned by its number: the answers are known."""
+    print(f"  top of {rows} x {V}", flush=True)
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB")
+    col = torch.arange(V, device="cuda", dtype=torch.int32)
+    x = torch.empty(rows, V, dtype=dtype, device="cuda")
+    piece = 1 << 18
+    for r in range(0, rows, piece):
+        n = min(piece, rows - r)
+        x[r:r + n] = (col[None] * 5 + torch.arange(r, r + n, device="cuda", dtype=torch.int32)[:, None]) % V
+    values, indices, lse = vocab.top_logits(x, k)
+    want = torch.arange(V - 1, V - 1 - k, -1, device="cuda", dtype=torch.int64)
+    inverse = pow(5, -1, V)
+    assert torch.equal(values[0].long(), want) and bool((values == values[0]).all()) and bool((lse == lse[0]).all())
+    for r in range(0, rows, piece):
+        n = min(piece, rows - r)
+        row = torch.arange(r, r + n, device="cuda", dtype=torch.int64)[:, None]
+        assert torch.equal(indices[r:r + n], (want[None] - row) * inverse % V), r
+    _lse_close(lse[:1], x[:1].cpu(), 1.0)
+    del x, values, indices, lse
+    torch.cuda.empty_cache()
