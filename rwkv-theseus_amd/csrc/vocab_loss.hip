@@ -845,8 +845,14 @@ static int run(const theseus_vocab_loss_args* a, const Plan& p, uint8_t* ws, hip
     if (p.padh) H = padded(H, p.M, ldh, p.hidden);
     if (p.padw) W = padded(W, p.V, ldw, p.weight);
     if (forward && a->top_values) {
-        const Targets t{p.M, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index, a->top_values, a->teacher_lse, a->row_weight, inv_T, j, q, row};
-        targets_kernel<<<(unsigned)ceil_div(p.M, 4), 256, 0, st>>>(t);
+        // (a launch has fewer than 2^32 threads, 64 a token)
+        const long most = 1l << 25, size = a->top_dtype == THESEUS_VOCAB_BF16 ? 2 : 4;
+        for (long i = 0; i < p.M; i += most) {
+            const long n = p.M - i < most ? p.M - i : most;
+            const Targets t{n, p.V, (int)p.K, a->top_dtype == THESEUS_VOCAB_BF16, a->index + i * p.K, static_cast<const uint8_t*>(a->top_values) + i * p.K * size,
+                            a->teacher_lse ? a->teacher_lse + i : nullptr, a->row_weight ? a->row_weight + i : nullptr, inv_T, j + i * p.K, q + i * p.K, row + i};
+            targets_kernel<<<(unsigned)ceil_div(n, 4), 256, 0, st>>>(t);
+        }
     }
     auto labels = [&](long i0) {
         return Labels{a->top_values ? nullptr : a->index + i0, a->row_weight ? a->row_weight + i0 : nullptr, a->ignore_index, p.V};

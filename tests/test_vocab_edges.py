@@ -276,3 +276,30 @@ def test_top_logits_of_more_rows_than_one_launch_takes(rows, V, k, dtype):
     _lse_close(lse[:1], x[:1].cpu(), 1.0)
     del x, values, indices, lse
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("top", [torch.float32, torch.bfloat16])
+def test_distillation_of_more_tokens_than_one_launch_takes(top):
+    """2^26 + 9 tokens of width 1 and a vocabulary of 3, two targets each: every token's loss."""
+    M, K = (1 << 26) + 9, 2
+    print(f"  distillation of {M} tokens", flush=True)
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB")
+    h = (torch.arange(M, device="cuda", dtype=torch.int32) % 97 - 48)[:, None].to(torch.bfloat16) / 16
+    w = torch.tensor([[1.0], [-.5], [.25]], device="cuda").bfloat16()
+    tv = torch.stack([(torch.arange(M, device="cuda", dtype=torch.int32) % p).to(top) / 8 for p in (31, 23)], 1)
+    ti = torch.stack([torch.arange(M, device="cuda") % 3, (torch.arange(M, device="cuda") + 1) % 3], 1)
+    weight = (torch.arange(M, device="cuda", dtype=torch.int32) % 5).float()
+    loss = vocab.linear_top_distillation(h, w, tv, ti, token_weight=weight, reduction="none")
+    piece = 1 << 23
+    for i in range(0, M, piece):
+        r = slice(i, i + piece)
+        logp = torch.log_softmax(h[r].double() * w.double().t(), -1)
+        q = torch.softmax(tv[r].double(), -1)
+        want = weight[r] * (q * (q.log() - logp.gather(1, ti[r]))).sum(-1)
+        # (losses of a few units of float32 exponentials and logarithms: 2^-20 of each of the terms, at most 10)
+        assert ((loss[r] - want).abs() <= 2.0 ** -20 * 10 * (weight[r] + 1)).all(), i
+    del h, tv, ti, weight, loss, logp, q, want
+    torch.cuda.empty_cache()
