@@ -82,8 +82,9 @@ enum theseus_vocab_phase { THESEUS_VOCAB_ALL = 0, THESEUS_VOCAB_FORWARD = 1, THE
 #define THESEUS_VOCAB_MAX_KEPT (256ll << 20)
 
 /* c_i of the gradients is row_grad_i row_weight_i, over the sum of the weights for MEAN.  A
- * token whose c_i (loss: row_weight_i) is 0 adds nothing (its hidden state has to be finite all
- * the same where dweight is asked for: 0 times it is added).
+ * token whose row_weight_i is 0 or whose label is ignored adds nothing, whatever its row_grad_i, nor to the
+ * gradients one whose c_i is 0 (its hidden state has to be finite all the same where dweight is asked for:
+ * 0 times it is added).
  * Target entries with q = 0 (a teacher's -inf) are not looked at; one with q != 0 whose index is
  * outside the vocabulary makes the token's loss NaN (and adds nothing to the gradients but p). */
 size_t theseus_vocab_loss_workspace_size(const theseus_vocab_loss_args* args);

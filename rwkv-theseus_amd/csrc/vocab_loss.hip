@@ -443,7 +443,8 @@ __global__ __launch_bounds__(256) void probs_kernel(Probs p) {
     const long i = gridDim.y - 1 - blockIdx.y;
     const int t = threadIdx.x, n0 = blockIdx.x * PROBS;
     uint16_t *row = p.e + i * p.lde, *rest = row + 32 * p.lde;
-    const float f = i >= p.M ? 0.f : p.row_grad ? p.row[i].z * p.row_grad[i] : p.row[i].z;
+    const float weight = i >= p.M ? 0.f : p.row[i].z;  // (0: whatever its upstream gradient, which may be infinite or NaN there)
+    const float f = p.row_grad && weight != 0.f ? weight * p.row_grad[i] : weight;
     constexpr int G = PROBS / 2048;
     if (f == 0.f) {
 #pragma unroll

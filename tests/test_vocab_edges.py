@@ -303,3 +303,26 @@ def test_distillation_of_more_tokens_than_one_launch_takes(top):
         assert ((loss[r] - want).abs() <= 2.0 ** -20 * 10 * (weight[r] + 1)).all(), i
     del h, tv, ti, weight, loss, logp, q, want
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------ tokens that do not count
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("M,piece", [(20, 0), (300, 0), (300, 256)])
+def test_upstream_gradients_of_tokens_that_do_not_count_are_not_looked_at(M, piece, native, monkeypatch):
+    """NaN and infinite upstream gradients (of a branch not taken) at ignored labels and weights of 0: 0, as
+    torch.nn.functional.cross_entropy has it."""
+    _python_path(monkeypatch, native)
+    x, w, g = _inputs(M, 64, 700)
+    t = _targets(g, M)
+    out = torch.arange(M, device="cuda") % 3 == 0
+    t["labels"][out] = -100
+    t["token_weight"][out] = 0
+    up = torch.rand(M, generator=g).cuda()
+    bad = torch.where(out, torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda")[torch.arange(M, device="cuda") % 3], up)
+    bad[::6] = float("inf")
+    h, wt = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    for name in ("labels", "top_values"):
+        loss = lambda: _loss_of(name, h, wt, t, reduction="none", piece_rows=piece)  # noqa: E731
+        for p, q in zip(torch.autograd.grad(loss(), (h, wt), bad), torch.autograd.grad(loss(), (h, wt), torch.where(out, 0., up))):
+            assert torch.isfinite(q).all() and torch.equal(p, q)
