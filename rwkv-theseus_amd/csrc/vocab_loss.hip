@@ -709,7 +709,7 @@ static Plan plan(const theseus_vocab_loss_args* a) {
     p.padh = pad(a->hidden, p.M, a->hidden_stride), p.padw = pad(a->weight, p.V, a->weight_stride);
     p.grads = a->dhidden || a->dweight || a->phase != THESEUS_VOCAB_ALL;
     p.lde = up(p.V, BK);
-    long cap = a->piece_rows ? up(a->piece_rows, 256) : p.grads ? (2l << 30) / (2 * p.lde) / 256 * 256 : MAX_PIECE;
+    long cap = a->piece_rows ? up(a->piece_rows < MAX_PIECE ? a->piece_rows : MAX_PIECE, 256) : p.grads ? (2l << 30) / (2 * p.lde) / 256 * 256 : MAX_PIECE;
     cap = cap < 256 ? 256 : cap > MAX_PIECE ? MAX_PIECE : cap;
     p.pieces = (int)ceil_div(p.M, cap);
     p.piece = up(ceil_div(p.M, p.pieces ? p.pieces : 1), 256);

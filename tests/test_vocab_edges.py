@@ -326,3 +326,12 @@ def test_upstream_gradients_of_tokens_that_do_not_count_are_not_looked_at(M, pie
         loss = lambda: _loss_of(name, h, wt, t, reduction="none", piece_rows=piece)  # noqa: E731
         for p, q in zip(torch.autograd.grad(loss(), (h, wt), bad), torch.autograd.grad(loss(), (h, wt), torch.where(out, 0., up))):
             assert torch.isfinite(q).all() and torch.equal(p, q)
+
+
+def test_any_number_of_piece_rows_is_taken():
+    """"All of them" in one piece, however that is written."""
+    lib, p = vocab._lib(), 1 << 20
+    size = lambda piece: lib.theseus_vocab_loss_workspace_size(vocab.LossArgs(  # noqa: E731
+        rows=100000, vocab=500, width=64, targets=1, hidden=p, weight=p, hidden_stride=64, weight_stride=64, index=p,
+        temperature=1.0, reduction=2, loss=p, dhidden=p, piece_rows=piece))
+    assert size(256) < size(32768) == size(100000) == size(2 ** 62) == size(2 ** 63 - 1)
