@@ -216,6 +216,9 @@ def _laid_out(hidden, weight, index, top_values, teacher_lse, row_weight):
         raise ValueError("theseus_vocab: hidden and weight must be CUDA tensors")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"theseus_vocab: expected hidden [..., D] and weight [V, D], got {list(hidden.shape)} and {list(weight.shape)}")
+    if weight.shape[0] > 1 << 22 or weight.shape[1] > 1 << 17 or hidden.numel() > weight.shape[1] << 30:
+        raise ValueError("theseus_vocab: at most 2^22 words, a width of 2^17 and 2^30 tokens, got "
+                         f"hidden {list(hidden.shape)} and weight {list(weight.shape)}")
     if weight.device != hidden.device:
         raise ValueError(f"theseus_vocab: weight must be on {hidden.device}, got {weight.device}")
     if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
@@ -324,6 +327,8 @@ def _top_checked(logits, k):
         raise TypeError(f"theseus_vocab: logits must be bfloat16 or float32, got {logits.dtype}")
     if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], MAX_TOP):
         raise ValueError(f"theseus_vocab: k must be in 1..min(V, {MAX_TOP}), got {k} for logits {list(logits.shape)}")
+    if logits.shape[-1] > 1 << 30:
+        raise ValueError(f"theseus_vocab: at most 2^30 logits in a row, got {list(logits.shape)}")
     return logits
 
 

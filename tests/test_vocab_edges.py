@@ -335,3 +335,15 @@ def test_any_number_of_piece_rows_is_taken():
         rows=100000, vocab=500, width=64, targets=1, hidden=p, weight=p, hidden_stride=64, weight_stride=64, index=p,
         temperature=1.0, reduction=2, loss=p, dhidden=p, piece_rows=piece))
     assert size(256) < size(32768) == size(100000) == size(2 ** 62) == size(2 ** 63 - 1)
+
+
+@gpu
+def test_sizes_out_of_range_are_named():
+    y = torch.zeros(2, dtype=torch.int64, device="cuda")
+    one = torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda")
+    for h, w in ((one.expand(2, 1), one.expand((1 << 22) + 1, 1)), (one.expand(2, (1 << 17) + 1), one.expand(3, (1 << 17) + 1)),
+                 (one.expand((1 << 30) + 1, 1), one)):
+        with pytest.raises(ValueError, match="at most"):
+            vocab.linear_cross_entropy(h, w, y)
+    with pytest.raises(ValueError, match="at most"):
+        vocab.top_logits(one.expand(1, (1 << 30) + 1), 2)
