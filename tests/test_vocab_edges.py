@@ -5,6 +5,7 @@ past a launch's, gradients of tokens that do not count.
 import pytest
 import torch
 
+from test_vocab import _dense, _grad_close, _oracle
 from theseus import vocab
 
 gpu = pytest.mark.gpu
@@ -347,3 +348,45 @@ def test_sizes_out_of_range_are_named():
             vocab.linear_cross_entropy(h, w, y)
     with pytest.raises(ValueError, match="at most"):
         vocab.top_logits(one.expand(1, (1 << 30) + 1), 2)
+
+
+# ------------------------------------------------------------------------------ distillation in pieces
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("M,D,V,K,own_lse", [(700, 72, 900, 9, False), (513, 64, 500, 64, True), (1025, 128, 3001, 3, True)])
+def test_distillation_in_pieces_matches_float64(M, D, V, K, own_lse, reduction):
+    """Tokens in pieces of 256: targets, weights and their sum of every piece, the bounds of one piece."""
+    print(f"  kd pieces M={M} D={D} V={V} K={K} lse={own_lse} {reduction}", flush=True)
+    T = 2.0
+    x, w, g = _inputs(M, D, V, M)
+    tv = 2 * torch.randn(M, K, generator=g)
+    tv[torch.rand(M, K, generator=g) < .1] = -float("inf")
+    tv[:, 0] = 1.0
+    ti = torch.randint(V, (M, K), generator=g)
+    weight = torch.rand(M, generator=g)
+    weight[::5] = 0
+    up = torch.rand(M, generator=g) if reduction == "none" else torch.tensor(1.0)
+    tz = tv.double() / T
+    lse = torch.logsumexp(tz, -1).float() + (.25 if own_lse else 0.)
+    q = torch.exp(tz - lse[:, None].double()) if own_lse else torch.softmax(tz, -1)
+    logq = (tz - lse[:, None].double()) if own_lse else torch.log_softmax(tz, -1)
+    H = torch.where(q > 0, q * logq, 0.).nan_to_num(0.).sum(-1)
+    wd = weight.double()
+    total = wd.sum() if reduction == "mean" else torch.tensor(1.0).double()
+    o = _oracle(x, w, _dense(M, V, ti, q), H, wd, T, wd * up.double() / total)
+    call = lambda a, b, **kw: vocab.linear_top_distillation(  # noqa: E731
+        a, b, tv.cuda(), ti.cuda(), temperature=T, teacher_lse=lse.cuda() if own_lse else None, token_weight=weight.cuda(),
+        reduction=reduction, **kw)
+    # (q itself: float32 exponentials of |t / T - lse| < 20, 2^-20 of each term)
+    qtol = T * T * wd * 2.0 ** -19 * (q * logq.abs().nan_to_num(0., 0., 0.)).sum(-1) + 1e-6 * o["loss"].abs()
+    h, wt = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    loss = call(h, wt, piece_rows=256)
+    assert torch.equal(loss.detach(), call(x.cuda(), w.cuda(), piece_rows=256))
+    for got in (loss.detach().double().cpu(), call(x.cuda(), w.cuda()).double().cpu()):  # (whole: other tiles, other sums)
+        if reduction == "none":
+            assert ((got - o["loss"]).abs() <= o["ltol"] + qtol).all()
+        else:
+            assert abs(float(got) - float(o["loss"].sum() / total)) <= float((o["ltol"] + qtol).sum() / total)
+    dx, dw = torch.autograd.grad(loss, (h, wt), up.cuda())
+    _grad_close(dx, o["dx"], o["dx_tol"])
+    _grad_close(dw, o["dw"], o["dw_tol"])
