@@ -214,16 +214,17 @@ def _laid_out(hidden, weight, index, top_values, teacher_lse, row_weight):
     """A loss's tensors, checked: hidden [M][D] and weight [V][D] with rows apart, the targets contiguous."""
     if not (hidden.is_cuda and weight.is_cuda):
         raise ValueError("theseus_vocab: hidden and weight must be CUDA tensors")
-    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"theseus_vocab: expected hidden [..., D] and weight [V, D], got {list(hidden.shape)} and {list(weight.shape)}")
-    if weight.shape[0] > 1 << 22 or weight.shape[1] > 1 << 17 or hidden.numel() > weight.shape[1] << 30:
+    shape, size, device = hidden.shape, weight.shape, hidden.device
+    if len(shape) < 1 or len(size) != 2 or shape[-1] != size[1] or size[0] < 1 or size[1] < 1:
+        raise ValueError(f"theseus_vocab: expected hidden [..., D] and weight [V, D], got {list(shape)} and {list(size)}")
+    if size[0] > 1 << 22 or size[1] > 1 << 17 or hidden.numel() > size[1] << 30:
         raise ValueError("theseus_vocab: at most 2^22 words, a width of 2^17 and 2^30 tokens, got "
-                         f"hidden {list(hidden.shape)} and weight {list(weight.shape)}")
-    if weight.device != hidden.device:
-        raise ValueError(f"theseus_vocab: weight must be on {hidden.device}, got {weight.device}")
+                         f"hidden {list(shape)} and weight {list(size)}")
+    if weight.device != device:
+        raise ValueError(f"theseus_vocab: weight must be on {device}, got {weight.device}")
     if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise TypeError(f"theseus_vocab: hidden and weight must be bfloat16 (or cast by autocast), got {hidden.dtype} and {weight.dtype}")
-    tokens, device = hidden.shape[:-1], hidden.device
+    tokens = shape[:-1]
     index = _rows(index, "labels" if top_values is None else "top_indices", tokens, device, (torch.int64,),
                   () if top_values is None else (index.shape[-1] if index.dim() else 0,))
     if top_values is not None:
@@ -235,7 +236,7 @@ def _laid_out(hidden, weight, index, top_values, teacher_lse, row_weight):
         teacher_lse = _rows(teacher_lse, "teacher_lse", tokens, device, (torch.float32,))
     if row_weight is not None:
         row_weight = _rows(row_weight, "token_weight", tokens, device, (torch.float32,))
-    h, w = _matrix(hidden if len(tokens) == 1 else hidden.reshape(math.prod(tokens), hidden.shape[-1])), _matrix(weight)
+    h, w = _matrix(hidden if len(tokens) == 1 else hidden.reshape(math.prod(tokens), shape[-1])), _matrix(weight)
     if w.stride(0) > MAX_STRIDE:
         w = w.contiguous()
     return h, w, index, top_values, teacher_lse, row_weight
@@ -248,15 +249,14 @@ def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_ind
         raise ValueError(f"theseus_vocab: temperature must be positive, got {temperature}")
     if piece_rows < 0:
         raise ValueError(f"theseus_vocab: piece_rows must not be negative, got {piece_rows}")
-    if hidden.is_cuda and weight.is_cuda and torch.is_autocast_enabled("cuda"):
+    if torch.is_autocast_enabled("cuda") and hidden.is_cuda and weight.is_cuda:
         dt = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dt), weight.to(dt)
-    tokens = hidden.shape[:-1]
     h, w, *targets = _laid_out(hidden, weight, index, top_values, teacher_lse, row_weight)
     native = _native(h, w)
     if native is not None:
         loss = native.vocab_loss(h, w, *targets, ignore_index, temperature, _REDUCTIONS[reduction], piece_rows)
-        return loss.reshape(tokens) if reduction == "none" and len(tokens) != 1 else loss
+        return loss.reshape(hidden.shape[:-1]) if reduction == "none" and hidden.dim() != 2 else loss
     constants = ignore_index, float(temperature), reduction, piece_rows
     if _direct(h, w, *targets):
         call = _Call(h, w, *targets, *constants)
@@ -264,7 +264,7 @@ def _loss(hidden, weight, index, top_values, teacher_lse, row_weight, ignore_ind
         call.run(h, w, loss)
     else:
         loss = _Loss.apply(h, w, *targets, *constants)
-    return loss.reshape(tokens) if reduction == "none" else loss
+    return loss.reshape(hidden.shape[:-1]) if reduction == "none" else loss
 
 
 def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, reduction="mean", piece_rows=0):
