@@ -17,8 +17,9 @@
  *   dhidden = G weight,  dweight = G^T hidden
  *
  * Pointers are device memory on the current device; hidden, weight and their gradients are
- * bfloat16, all sums float32 or wider.  Nothing is allocated or synchronised; results are
- * deterministic (no atomics).  Status codes are those of theseus_wkv7.h: sizes out of range
+ * bfloat16, all sums float32 or wider.  Nothing is allocated or synchronised.  Results are
+ * deterministic: sums run in a fixed order, and only counts and places in lists whose order changes
+ * nothing come from (LDS) atomics.  Status codes are those of theseus_wkv7.h: sizes out of range
  * THESEUS_WKV7_ERR_SHAPE, an unknown type _ERR_DTYPE, an unknown kind or reduction _ERR_FLAGS.
  */
 #ifndef THESEUS_VOCAB_H
@@ -78,7 +79,10 @@ typedef struct theseus_vocab_loss_args {
  * and row_grad are not looked at), GRADIENTS with the same other arguments reads kept (and
  * destroys it) and writes the gradients without forming the logits again. */
 enum theseus_vocab_phase { THESEUS_VOCAB_ALL = 0, THESEUS_VOCAB_FORWARD = 1, THESEUS_VOCAB_GRADIENTS = 2 };
-/* most that is kept: a call with more in its row pieces (V 16-bit values a token) keeps nothing */
+/* most that is kept: a call with more in its row pieces (V 16-bit values a token) keeps nothing and forms its
+ * logits twice.  A bound on memory held from the forward to the backward, which costs a fourth product
+ * beyond it: 65536 words, width 5120, both gradients, 1984 tokens (kept) 1607 ns a token, 2112 (not kept) 2256,
+ * 4096 2027; reduced losses of as many 1606, 1718, 1559 */
 #define THESEUS_VOCAB_MAX_KEPT (256ll << 20)
 
 /* c_i of the gradients is row_grad_i row_weight_i, over the sum of the weights for MEAN.  A
@@ -99,7 +103,9 @@ int theseus_vocab_scale(void* x, long long nx, void* y, long long ny, const floa
 /* logits [M][V] bfloat16 or float32, row_stride elements from row to row, M >= 0, V in
  * 1 .. 2^30, k in 1 .. min(V, THESEUS_VOCAB_MAX_TOP).  values [M][k] in the logits' type and
  * indices [M][k], largest first, equal values by the lowest index, NaN above every number;
- * lse [M] = log sum exp(logits / temperature), may be NULL. */
+ * lse [M] = log sum exp(logits / temperature), may be NULL.  Rows are read in whole granules of 16 aligned
+ * bytes: up to 15 bytes on either side of the first and last row are read too (never across such a
+ * boundary, so never beyond a page) and not looked at. */
 size_t theseus_vocab_top_workspace_size(long long rows, long long vocab, int k, int dtype);
 int theseus_vocab_top(long long rows, long long vocab, int k, int dtype, float temperature, const void* logits,
                       long long row_stride, void* values, int64_t* indices, float* lse, void* workspace,

@@ -26,9 +26,9 @@
 //   rows along the output ("RowN"): [64][BN], chunk c of row r at c ^ (2 (r & 7)), read by
 //                 ds_read_b64_tr_b16.
 //
-// 8192 x 65536 x 5120: 4.1-4.3 ms in the three layouts (1.28-1.34 PFLOP/s), the card at its power limit
+// 8192 x 65536 x 5120: 4.0-4.2 ms in the three layouts (1.32-1.38 PFLOP/s), the card at its power limit
 // (1.85 GHz; the matrix cores busy 65 % of the time, no bank conflicts, 81 % L2 hits).  64 tokens'
-// logits read a weight of 0.34 GB in 60 us (5.6 TB/s).
+// logits read a weight of 0.34 GB in 61 us (5.5 TB/s).
 #pragma once
 
 #include <type_traits>

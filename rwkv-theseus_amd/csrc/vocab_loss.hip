@@ -5,8 +5,8 @@
 //   targets        a teacher's: every token's q, Q, sum q log q and weight (a label's are made in rows)
 //   sums           MEAN with several pieces: the sum of the weights (one workgroup, fixed order)
 //   then for each piece of rows
-//     logits       z's tiles on the matrix cores; of each 256-column tile a row's maximum and sum
-//                  of exponentials are kept and, for gradients, the exponentials (float16,
+//     logits       z's tiles on the matrix cores; of each tile (64 or 256 columns) a row's maximum and
+//                  sum of exponentials are kept and, for gradients, the exponentials (float16,
 //                  2^15 e^{z - tile maximum}: 11 significant bits down to e^-20 of the maximum);
 //                  z at the targets is taken out of the accumulators
 //     rows         log-sum-exp of a row from its tiles, the row's loss
@@ -22,7 +22,7 @@
 // forms the logits again: with SUM and MEAN the upstream gradient is one number, applied to the
 // results (theseus_vocab_scale); with NONE, up to THESEUS_VOCAB_MAX_KEPT bytes of exponentials are
 // kept for the backward (1021 tokens of 50001 at width 2560: 990 -> 760 us), which otherwise makes them
-// again.
+// again (what that costs: beside the limit).
 #include "../../include/theseus_vocab.h"
 #include "../../include/theseus_wkv7.h"
 
