@@ -1,5 +1,6 @@
 """What a language model's head is trained on and answers with, over a large vocabulary
-(C ABI: include/theseus_vocab.h).
+(C ABI: include/theseus_vocab.h), and the embedding that its tokens come in by
+(include/theseus_embed.h).
 
 The reference distils its student layers against hidden states and checks the converted model by
 a divergence over full logits (theseus/losses.py:5-30, validate.py).  These operators are what
@@ -9,7 +10,9 @@ training the whole student takes next: losses on the head's output that never ho
 * ``linear_cross_entropy(hidden, weight, labels)``: softmax cross entropy of hidden @ weight.T;
 * ``linear_top_distillation(hidden, weight, top_values, top_indices)``: the divergence of the
   student's softmax from a teacher of whom each token's top logits are known;
-* ``top_logits(logits, k)``: those top logits and indices, and the row's log-sum-exp.
+* ``top_logits(logits, k)``: those top logits and indices, and the row's log-sum-exp;
+* ``embedding(ids, weight)``: rows of a table times a factor, rounded to the layers' type in the
+  same pass, with the table's gradient by sorted tokens.
 
 The losses are differentiable in ``hidden`` and ``weight`` (bfloat16; under autocast other types
 are cast as ``torch.nn.functional.linear`` casts them).  With ``reduction="mean"`` or ``"sum"``
@@ -68,6 +71,12 @@ def _lib():
         lib.theseus_vocab_top_workspace_size.restype = sz
         lib.theseus_vocab_top.argtypes = [i64, i64, i32, i32, f32, vp, i64, vp, vp, vp, vp, sz, vp]
         lib.theseus_vocab_top.restype = i32
+        lib.theseus_embed_lookup.argtypes = [i64, i64, i32, i32, i32, vp, vp, i64, f32, vp, vp]
+        lib.theseus_embed_lookup.restype = i32
+        lib.theseus_embed_grad_workspace_size.argtypes = [i64, i64, i32]
+        lib.theseus_embed_grad_workspace_size.restype = sz
+        lib.theseus_embed_grad.argtypes = [i64, i64, i32, i32, i32, vp, i64, vp, i64, f32, vp, vp, sz, vp]
+        lib.theseus_embed_grad.restype = i32
         _bound = True
     return lib
 
@@ -354,3 +363,99 @@ def top_logits(logits, k, *, temperature=1.0):
         return out
     values, indices, lse = out
     return values.reshape(*rows, k), indices.reshape(*rows, k), lse.reshape(rows)
+
+
+# ------------------------------------------------------------------------------ embedding
+class _Embedding(torch.autograd.Function):
+    """``embedding`` for ids [M] (a trace replays this with tensors that nothing else has looked at)."""
+
+    @staticmethod
+    def forward(ctx, weight, ids, scale, skip, dtype):
+        w, ids = _table(weight, ids)
+        ctx.save_for_backward(ids)
+        ctx.table, ctx.constants = (w.shape[0], w.shape[1], w.dtype), (scale, skip)
+        return _lookup(w, ids, scale, dtype)
+
+    @staticmethod
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        with torch.no_grad():
+            dweight = _table_grad(grad, ids, *ctx.table, *ctx.constants)
+        if torch.is_grad_enabled():  # (create_graph: a later derivative through this raises)
+            dweight = torch._C._functions.DelayedError("theseus_vocab: embedding is differentiable once", 1)(dweight.requires_grad_())
+        return dweight, None, None, None, None
+
+
+def _lookup(w, ids, scale, dtype):
+    out = torch.empty((ids.shape[0], w.shape[1]), dtype=dtype, device=w.device)
+    with torch.cuda.device(w.device):
+        _check(_lib().theseus_embed_lookup(ids.shape[0], *w.shape, _DTYPES[w.dtype], _DTYPES[dtype], ids.data_ptr(), w.data_ptr(),
+                                           max(w.stride(0), w.shape[1]), scale, out.data_ptr(), _stream(w.device)))
+    return out
+
+
+def _table_grad(grad, ids, V, D, dtype, scale, skip):
+    if grad.dtype not in _DTYPES:
+        grad = grad.float()
+    if grad.stride(1) != 1 or grad.stride(0) < D and grad.stride(0) != 0:
+        grad = grad.contiguous()
+    dweight = torch.empty((V, D), dtype=dtype, device=grad.device)
+    lib = _lib()
+    with torch.cuda.device(grad.device):
+        nbytes = int(lib.theseus_embed_grad_workspace_size(ids.shape[0], V, D))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
+        _check(lib.theseus_embed_grad(ids.shape[0], V, D, _DTYPES[grad.dtype], _DTYPES[dtype], ids.data_ptr(), skip, grad.data_ptr(),
+                                      grad.stride(0), scale, dweight.data_ptr(), ws.data_ptr(), nbytes, _stream(grad.device)))
+    return dweight
+
+
+def _table(weight, ids):
+    """The table with rows apart and the indices in one row, checked."""
+    if not (weight.is_cuda and ids.is_cuda):
+        raise ValueError("theseus_vocab: ids and weight must be CUDA tensors")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"theseus_vocab: expected weight [V, D], got {list(weight.shape)}")
+    if weight.shape[0] > 1 << 22 or weight.shape[1] > 1 << 17 or ids.numel() > 1 << 30:
+        raise ValueError("theseus_vocab: at most 2^22 words, a width of 2^17 and 2^30 tokens, got "
+                         f"ids {list(ids.shape)} and weight {list(weight.shape)}")
+    if ids.device != weight.device:
+        raise ValueError(f"theseus_vocab: ids must be on {weight.device}, got {ids.device}")
+    if weight.dtype not in _DTYPES:
+        raise TypeError(f"theseus_vocab: weight must be bfloat16 or float32, got {weight.dtype}")
+    if ids.dtype != torch.int64:
+        raise TypeError(f"theseus_vocab: ids must be int64, got {ids.dtype}")
+    return _matrix(weight), ids.reshape(-1).contiguous()
+
+
+def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
+    """``scale * weight[ids]`` in ``dtype`` (the weight's own if None), and the weight's gradient.
+
+    ids [...] int64, weight [V, D] bfloat16 or float32 (rows may lie apart), dtype one of the same
+    two: a float32 table gives bfloat16 rows in one pass, product and rounding once.  An index
+    outside the vocabulary makes its row NaN and has no part in the gradient (the device is not
+    asked before the call returns).  ``padding_idx`` (negative: from the end): tokens of this index
+    get the table's row like the others, but add nothing to its gradient.  Returns [..., D].
+
+    The gradient has the weight's type and is written whole, rows without tokens as 0.  Each row is
+    the float32 sum over its tokens in their order, times ``scale``, rounded once: the same bits on
+    every run.  Differentiable once; raises if the ids were changed in place before the backward."""
+    w, flat = _table(weight, ids)
+    scale = float(scale)
+    if not math.isfinite(scale) or abs(scale) > 3.4028234663852886e38:
+        raise ValueError(f"theseus_vocab: scale must be finite in float32, got {scale}")
+    V, skip = w.shape[0], -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"theseus_vocab: padding_idx must be in -V .. V-1, got {padding_idx} for weight {list(weight.shape)}")
+        skip = int(padding_idx) % V
+    dtype = weight.dtype if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"theseus_vocab: dtype must be bfloat16 or float32, got {dtype}")
+    native = _native(w, flat)
+    if native is not None:
+        out = native.embedding(w, flat, scale, skip, dtype == torch.float32)
+    elif _direct(w):
+        out = _lookup(w, flat, scale, dtype)
+    else:
+        out = _Embedding.apply(w, flat, scale, skip, dtype)
+    return out if ids.dim() == 1 else out.reshape(*ids.shape, w.shape[1])
