@@ -329,48 +329,47 @@ __global__ __launch_bounds__(THREADS) void place_digits(Pass p) {
 // ------------------------------------------------------------------------------ sums
 struct Runs {
     long M, V;
-    int D, each, slabs;        // each: tokens of a run; slabs: of 256 N columns
-    const uint32_t *keys, *places;
+    int D, each, slabs;  // each: tokens of a run; slabs: of a workgroup's columns
     long ldg;
     float scale;
-    float* parts;  // [run][2][D]: of the stretch that a run begins inside of, of the one that it begins and does not end
 };
 struct Run {
     long from, to;
     bool inside, open;  // begins inside a stretch; ends inside one
 };
-__device__ __forceinline__ Run run_at(const Runs& s, long c) {
+__device__ __forceinline__ Run run_at(const Runs& s, const uint32_t* __restrict__ keys, long c) {
     Run r;
     r.from = c * s.each, r.to = min(r.from + s.each, s.M);
-    r.inside = r.from > 0 && s.keys[r.from - 1] == s.keys[r.from];
-    r.open = r.to < s.M && s.keys[r.to - 1] == s.keys[r.to];
+    r.inside = r.from > 0 && keys[r.from - 1] == keys[r.from];
+    r.open = r.to < s.M && keys[r.to - 1] == keys[r.to];
     return r;
 }
 
-template <int N, typename G, typename W>
-__global__ __launch_bounds__(256) void sum_runs(Runs s, const G* __restrict__ grad, W* __restrict__ dweight) {
-    const long c = blockIdx.x / s.slabs;
-    const int chunk = (int)(blockIdx.x - c * s.slabs) * blockDim.x + threadIdx.x;
+// (keys and places through pointers of their own: scalar loads, the same for a whole workgroup)
+// parts: [run][2][D], of the stretch that a run begins inside of, of the one that it begins and does not end
+template <int N, int BATCH, typename G, typename W>
+__global__ __launch_bounds__(256) void sum_runs(Runs s, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places,
+                                                const G* __restrict__ grad, float* __restrict__ parts, W* __restrict__ dweight) {
+    const int c = blockIdx.x / s.slabs, chunk = (blockIdx.x - c * s.slabs) * blockDim.x + threadIdx.x;
     if (chunk * N >= s.D) return;
     const int col = column<N>(chunk, s.D);
-    const Run r = run_at(s, c);
-    if (s.keys[r.from] >= s.V) return;  // (sorted: nothing in this run counts)
+    const Run r = run_at(s, keys, c);
+    if (keys[r.from] >= s.V) return;  // (sorted: nothing in this run counts)
     bool inside = r.inside;
-    constexpr int BATCH = 8;
     float sum[N];
 #pragma unroll
     for (int e = 0; e < N; e++) sum[e] = 0.f;
     for (long i0 = r.from; i0 < r.to; i0 += BATCH) {
-        float x[BATCH][N];
         uint32_t key[BATCH + 1];
+        float x[BATCH][N];
 #pragma unroll
         for (int j = 0; j < BATCH; j++) {
             const long i = min(i0 + j, r.to - 1);
-            key[j] = s.keys[i];
+            key[j] = keys[i];
             // (a token that adds nothing is not loaded: the run's first one is instead)
-            load<N>(x[j], grad + (long)(key[j] < s.V ? s.places[i] : s.places[r.from]) * s.ldg + col);
+            load<N>(x[j], grad + (long)(key[j] < s.V ? places[i] : places[r.from]) * s.ldg + col);
         }
-        key[BATCH] = s.keys[min(i0 + BATCH, s.M - 1)];
+        key[BATCH] = keys[min(i0 + BATCH, s.M - 1)];
 #pragma unroll
         for (int j = 0; j < BATCH; j++) {
             if (i0 + j >= r.to || key[j] >= s.V) return;
@@ -379,7 +378,7 @@ __global__ __launch_bounds__(256) void sum_runs(Runs s, const G* __restrict__ gr
             const bool end = i0 + j + 1 == r.to;
             if (!end && key[j + 1] == key[j]) continue;
             if (inside || (end && r.open)) {
-                store<N>(s.parts + (2 * c + !inside) * s.D + col, sum);
+                store<N>(parts + (2l * c + !inside) * s.D + col, sum);
             } else {
 #pragma unroll
                 for (int e = 0; e < N; e++) sum[e] *= s.scale;
@@ -392,28 +391,30 @@ __global__ __launch_bounds__(256) void sum_runs(Runs s, const G* __restrict__ gr
     }
 }
 
-template <int N, typename W> __global__ __launch_bounds__(256) void add_parts(Runs s, W* __restrict__ dweight) {
-    const long c = blockIdx.x / s.slabs;
-    const int chunk = (int)(blockIdx.x - c * s.slabs) * blockDim.x + threadIdx.x;
-    if (chunk * N >= s.D) return;
-    const Run r = run_at(s, c);
-    const uint32_t key = s.keys[r.to - 1];
-    if (!r.open || key >= s.V || (r.inside && s.keys[r.from] == key)) return;  // no stretch begins here and goes on
-    const int col = column<N>(chunk, s.D);
-    long lo = r.to, hi = s.M;  // the first token behind the stretch
-    while (lo < hi) {
-        const long mid = (lo + hi) >> 1;
-        if (s.keys[mid] == key) lo = mid + 1;
-        else hi = mid;
+template <int N, typename W>
+__global__ __launch_bounds__(256) void add_parts(Runs s, const uint32_t* __restrict__ keys, const float* __restrict__ parts,
+                                                 W* __restrict__ dweight) {
+    const int c = blockIdx.x / s.slabs, chunk = (blockIdx.x - c * s.slabs) * blockDim.x + threadIdx.x;
+    const Run r = run_at(s, keys, c);
+    const uint32_t key = keys[r.to - 1];
+    if (!r.open || key >= s.V || (r.inside && keys[r.from] == key)) return;  // no stretch begins here and goes on
+    // the last run that begins inside the stretch: 64 of them looked at together
+    const int runs = (int)((s.M + s.each - 1) / s.each);
+    int last = c;
+    for (uint64_t same = ~0ull; same == ~0ull;) {
+        const int d = last + 1 + (threadIdx.x & 63);
+        same = __ballot(d < runs && keys[(long)d * s.each] == key);
+        last += same == ~0ull ? 64 : __builtin_ctzll(~same);  // (sorted: those of the stretch come first)
     }
-    const long last = (lo - 1) / s.each;
+    if (chunk * N >= s.D) return;
+    const int col = column<N>(chunk, s.D);
     float sum[N];
-    load<N>(sum, s.parts + (2 * c + 1) * s.D + col);
+    load<N>(sum, parts + (2l * c + 1) * s.D + col);
     constexpr int BATCH = 8;
-    for (long d0 = c + 1; d0 <= last; d0 += BATCH) {
+    for (int d0 = c + 1; d0 <= last; d0 += BATCH) {
         float x[BATCH][N];
 #pragma unroll
-        for (int j = 0; j < BATCH; j++) load<N>(x[j], s.parts + 2 * min(d0 + j, last) * s.D + col);
+        for (int j = 0; j < BATCH; j++) load<N>(x[j], parts + 2l * min(d0 + j, last) * s.D + col);
 #pragma unroll
         for (int j = 0; j < BATCH; j++)
             if (d0 + j <= last)
@@ -473,13 +474,14 @@ static void launch_lookup(long M, long V, int D, const int64_t* ids, const void*
 }
 
 template <int N, typename G, typename W>
-static void launch_sums(Runs s, long runs, const void* grad, void* dweight, hipStream_t st) {
+static void launch_sums(Runs s, long runs, const uint32_t* keys, const uint32_t* places, const void* grad, float* parts, void* dweight,
+                        hipStream_t st) {
     const long chunks = ceil_div(s.D, N);
     const int threads = chunks >= 256 ? 256 : (int)(ceil_div(chunks, 64) * 64);
     s.slabs = (int)ceil_div(chunks, threads);
     const unsigned grid = (unsigned)(runs * s.slabs);
-    sum_runs<N, G, W><<<grid, threads, 0, st>>>(s, static_cast<const G*>(grad), static_cast<W*>(dweight));
-    if (runs > 1) add_parts<N, W><<<grid, threads, 0, st>>>(s, static_cast<W*>(dweight));
+    sum_runs<N, 32 / sizeof(G), G, W><<<grid, threads, 0, st>>>(s, keys, places, static_cast<const G*>(grad), parts, static_cast<W*>(dweight));
+    if (runs > 1) add_parts<N, W><<<grid, threads, 0, st>>>(s, keys, parts, static_cast<W*>(dweight));
 }
 
 }  // namespace embed
@@ -534,6 +536,7 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
             sort_fill<decltype(rounds)::value><<<(unsigned)(1 + fills), THREADS, 0, stream>>>((int)M, V, skip, dg, ids, at(p.keys), at(p.places), f);
         };
         if (M <= 2 * THREADS) sort(std::integral_constant<int, 2>{});
+        else if (M <= 6 * THREADS) sort(std::integral_constant<int, 6>{});
         else sort(std::integral_constant<int, ONE / THREADS>{});
     } else {
         Pass q{M, V, skip, dg.bits, 0, (int)p.blocks, ids, nullptr, nullptr, at(p.keys), at(p.places), at(p.counts), at(p.totals)};
@@ -549,12 +552,13 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
         }
     }
     if (M) {
-        const Runs s{M, V, D, p.each, 0, keys, places, grad_stride, scale, reinterpret_cast<float*>(ws + p.parts)};
+        const Runs s{M, V, D, p.each, 0, grad_stride, scale};
+        float* parts = reinterpret_cast<float*>(ws + p.parts);
         auto go = [&](auto g, auto w) {
             using G = decltype(g);
             using W = decltype(w);
-            if (D >= 8) launch_sums<8, G, W>(s, p.runs, grad, dweight, stream);
-            else launch_sums<1, G, W>(s, p.runs, grad, dweight, stream);
+            if (D >= 8) launch_sums<8, G, W>(s, p.runs, keys, places, grad, parts, dweight, stream);
+            else launch_sums<1, G, W>(s, p.runs, keys, places, grad, parts, dweight, stream);
         };
         if (grad_dtype == THESEUS_EMBED_BF16) {
             if (weight_dtype == THESEUS_EMBED_BF16) go(uint16_t{}, uint16_t{});
