@@ -20,8 +20,8 @@
 // The tensor list travels in kernel arguments (32 tensors per launch, under
 // the 4 KB argument limit), so nothing is copied to the device per step and
 // the sequence can be captured into a graph.
-#include "../../include/theseus_optim.h"
 #include "../../include/theseus_wkv7.h"
+#include "optim_norm.h"
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -232,6 +232,18 @@ static bool next_batch(const theseus_adamw_tensor* ts, int nt, int& next, long l
     return bt.count > 0;
 }
 
+// The norm pass of a step (optim_norm.h)
+void launch_sumsq(const theseus_adamw_tensor* ts, int nt, long long& chunks, long long keep_from, double* partial, hipStream_t stream) {
+    Batch bt;
+    bt.keep_from = (int)keep_from;
+    int next = 0;
+    while (next_batch(ts, nt, next, chunks, bt))
+        hipLaunchKernelGGL(grad_sumsq, dim3(bt.chunk0[bt.count]), dim3(THREADS), 0, stream, bt, partial);
+}
+void launch_norm(const double* partial, long long chunks, float grad_scale, float max_norm, float* result, hipStream_t stream) {
+    hipLaunchKernelGGL(norm_finish, dim3(1), dim3(1024), 0, stream, partial, (int)chunks, grad_scale, max_norm, result);
+}
+
 }  // namespace optim
 
 extern "C" {
@@ -261,20 +273,16 @@ int theseus_adamw_step(const theseus_adamw_tensor* tensors, int ntensors, float 
     if (norm && nchunks && (!workspace || workspace_bytes < (size_t)nchunks * sizeof(double)))
         return THESEUS_WKV7_ERR_WORKSPACE;
     double* partial = static_cast<double*>(workspace);
-    optim::Batch bt;
     constexpr long long CHUNK_BYTES = optim::CHUNK * (long long)sizeof(float);
     const long long keep = nchunks - optim::KEEP_BYTES / CHUNK_BYTES;
     const bool back = nchunks > optim::L2_BYTES / CHUNK_BYTES;
-    bt.keep_from = !back ? (int)nchunks : keep > 0 ? (int)keep : 0;
-    int next = 0;
     long long base = 0;
-    while (norm && optim::next_batch(tensors, ntensors, next, base, bt))
-        hipLaunchKernelGGL(optim::grad_sumsq, dim3(bt.chunk0[bt.count]), dim3(optim::THREADS), 0, stream, bt,
-                           partial);
-    hipLaunchKernelGGL(optim::norm_finish, dim3(1), dim3(1024), 0, stream, partial, norm ? (int)nchunks : 0,
-                       grad_scale, max_norm, result);
+    if (norm) optim::launch_sumsq(tensors, ntensors, base, !back ? nchunks : keep > 0 ? keep : 0, partial, stream);
+    optim::launch_norm(partial, norm ? nchunks : 0, grad_scale, max_norm, result, stream);
     const optim::Hyper h{beta1, beta2, eps, skip_nonfinite};
-    next = 0;
+    optim::Batch bt;
+    bt.keep_from = 0;
+    int next = 0;
     base = 0;
     while (optim::next_batch(tensors, ntensors, next, base, bt, back))
         hipLaunchKernelGGL(back ? optim::adamw<true> : optim::adamw<false>, dim3(bt.chunk0[bt.count]),

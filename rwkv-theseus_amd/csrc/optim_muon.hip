@@ -1,0 +1,703 @@
+// Orthogonalised updates (C ABI: include/theseus_muon.h), gfx950.
+//
+// X_0 = s u / max(|u|_F, eps) and, `steps` times with p the short side,
+//
+//   A = X X^T (X^T X where X is tall)      the lower triangle's tiles, each stored on both sides
+//   B = b A + (c / s^2) A^2                the same: A commutes with itself, so A^2 = A A^T
+//   X = a X + (1 / s^2) B X (X B)
+//
+// p^2 q + p^3 + 2 p^2 q products and sums a step instead of 2 p^2 q + 2 p^3 + 2 p^2 q, on the matrix
+// cores with vocab_gemm.h's tiles: a wide X is read along its rows for A and along its columns for
+// B X, a tall one the other way round, so no matrix is ever transposed in memory.  The list's
+// matrices share every launch: workgroups find their matrix in the kernel's arguments.
+//
+// Numerics.  Operands are float16: bfloat16 has 8 times their rounding, and the polynomial magnifies
+// it (a Gaussian 768 x 768: 1.0e-2 from the exact result instead of 1.3e-3, where rounding the result
+// to bfloat16 costs 1.7e-3).  s, a power of two near sqrt(p), keeps their values (X near 1 / sqrt(q),
+// A near 1 after the first steps and s^2 / p before) inside float16's range.  Where u has few strong directions, rounding X itself
+// would add to it a matrix outside of its row and column spaces, which the polynomials raise by a
+// each step, 485 in five, while the strong directions stay at 1 (rank 64: 2.3e-2 off, rank 1:
+// 0.15).  Products with a rounded factor have their errors inside these spaces, which grow as X does; so
+// X is held in two halves, hi + lo / 2048, hi alone goes into the products, and both into a X: at most 1.7e-3 on all
+// spectra that were tried.
+#include "../../include/theseus_muon.h"
+#include "../../include/theseus_wkv7.h"
+
+#include <math.h>
+
+#include "optim_norm.h"
+#include "vocab_gemm.h"
+
+namespace muon {
+
+using namespace vocab;
+using wkv7::bf16_to_f32;
+using wkv7::f32x2_to_bf16x2;
+
+constexpr int MAX = 32;         // matrices of a launch
+constexpr int TOGETHER = 1024;  // rows of a product whose tiles run together
+constexpr int PIECE = 8192;     // elements of a workgroup of the norm's pass
+constexpr float LO = 2048.f;    // of X's second half, so that it is no subnormal
+
+// One matrix.  Its part of the workspace: X hi, X lo, the next X hi and lo ([mp][np] each, zero
+// beyond m and n), A and B ([pp][pp], pp the padded short side).
+struct Matrix {
+    const void* src;  // the gradient, or X
+    long ld;          // of src
+    float* momentum;  // null: orthogonalize
+    void* dst;        // float32 param, or bfloat16 out
+    uint16_t* ws;
+    int m, n, mp, np;  // and padded to steps of the products
+    int piece0, pieces;  // of the norm's partial sums
+    float s;
+    float keep, step;
+    int fp32;  // src
+    __device__ __host__ bool tall() const { return m > n; }
+    __device__ __host__ int pp() const { return tall() ? np : mp; }
+    __device__ long size() const { return (long)mp * np; }
+    __device__ uint16_t* hi(int which) const { return ws + 2 * which * size(); }
+    __device__ uint16_t* lo(int which) const { return hi(which) + size(); }
+    __device__ uint16_t* gram() const { return ws + 4 * size(); }
+    __device__ uint16_t* square() const { return gram() + (long)pp() * pp(); }
+};
+struct List {
+    int count;
+    int first[MAX + 1];  // of each matrix' workgroups in this launch
+    Matrix x[MAX];
+};
+static_assert(sizeof(List) < 4000, "kernel arguments");
+
+__device__ __forceinline__ int which(const List& l, int b) {
+    int i = 0;
+    while (i + 1 < l.count && l.first[i + 1] <= b) i++;
+    return i;
+}
+
+__device__ __forceinline__ uint32_t half2_of(float x, float y) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
+}
+__device__ __forceinline__ float2 floats_of(uint32_t u) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 h = __builtin_bit_cast(h2, u);
+    return make_float2((float)h[0], (float)h[1]);
+}
+// x, y -> hi; what that rounds away, times LO -> lo
+__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = half2_of(x, y);
+    const float2 h = floats_of(hi);
+    lo = half2_of((x - h.x) * LO, (y - h.y) * LO);
+}
+
+// ------------------------------------------------------------------------------ u, its norm, X_0
+struct Update {
+    float mu;
+    int nesterov;
+    float factor;         // of the gradients, where result is null
+    const float* result;  // of the norm pass: the factor, and whether nothing may change
+    int skip;
+    float eps;
+};
+__device__ __forceinline__ bool skipped(const Update& u) { return u.result && u.skip && u.result[2] != 0.f; }
+
+template <typename T> struct Eight {
+    typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));  // (rows may begin anywhere)
+};
+__device__ __forceinline__ void load8(float (&x)[8], const void* p, long at, int count, bool fp32) {
+    if (count >= 8) {
+        if (fp32) {
+            const auto v = *reinterpret_cast<const Eight<float>::type*>(static_cast<const float*>(p) + at);
+            for (int e = 0; e < 8; e++) x[e] = v[e];
+        } else {
+            const auto v = *reinterpret_cast<const Eight<uint16_t>::type*>(static_cast<const uint16_t*>(p) + at);
+            for (int e = 0; e < 8; e++) x[e] = bf16_to_f32(v[e]);
+        }
+    } else {
+        for (int e = 0; e < 8; e++)
+            x[e] = e >= count ? 0.f : fp32 ? static_cast<const float*>(p)[at + e] : bf16_to_f32(static_cast<const uint16_t*>(p)[at + e]);
+    }
+}
+__device__ __forceinline__ double block_sum(double x, double* red) {  // in every thread
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+// momentum, and the sum of u^2 of a workgroup's rows: float32 values, float64 squares and sums (their squares may
+// leave float32's range, and there are up to 2^34 of them)
+__global__ __launch_bounds__(256) void momentum_norm(List l, Update u, double* __restrict__ sums) {
+    __shared__ double red[4];
+    if (skipped(u)) return;
+    const int i = which(l, blockIdx.x), k = blockIdx.x - l.first[i];
+    const Matrix& x = l.x[i];
+    const float f = u.result ? u.result[1] : u.factor;
+    const int per = (x.n + 7) / 8;
+    const long all = (long)x.m * per;
+    double sum = 0;
+    for (int j = 0; j < PIECE / 2048; j++) {
+        const long c = (long)k * (PIECE / 8) + j * 256 + threadIdx.x;
+        if (c >= all) break;
+        const long row = c / per;
+        const int col = (int)(c - row * per) * 8, count = x.n - col;
+        float g[8];
+        load8(g, x.src, row * x.ld + col, count, x.fp32);
+        if (x.momentum) {
+            float m[8];
+            const long at = row * x.n + col;
+            load8(m, x.momentum, at, count, true);
+            for (int e = 0; e < 8; e++) {
+                g[e] *= f;
+                m[e] = u.mu * m[e] + (1.f - u.mu) * g[e];
+            }
+            if (count >= 8) {
+                Eight<float>::type v;
+                for (int e = 0; e < 8; e++) v[e] = m[e];
+                *reinterpret_cast<Eight<float>::type*>(x.momentum + at) = v;
+            } else {
+                for (int e = 0; e < count; e++) x.momentum[at + e] = m[e];
+            }
+            for (int e = 0; e < 8; e++) g[e] = u.nesterov ? u.mu * m[e] + (1.f - u.mu) * g[e] : m[e];
+        }
+        for (int e = 0; e < 8; e++) sum += (double)g[e] * g[e];
+    }
+    sum = block_sum(sum, red);
+    if (threadIdx.x == 0) sums[x.piece0 + k] = sum;
+}
+
+// X_0 in two halves, with zeros around it
+__global__ __launch_bounds__(256) void scale_split(List l, Update u, const double* __restrict__ sums) {
+    __shared__ double red[4];
+    const int i = which(l, blockIdx.x), k = blockIdx.x - l.first[i];
+    const Matrix& x = l.x[i];
+    double sum = 0;
+    for (int j = threadIdx.x; j < x.pieces; j += 256) sum += sums[x.piece0 + j];
+    const double norm = sqrt(block_sum(sum, red));
+    const float by = (float)(x.s / (norm < u.eps ? (double)u.eps : norm));  // (a NaN stays one)
+    const float f = u.result ? u.result[1] : u.factor;
+    const int per = x.np / 8;
+    const long all = (long)x.mp * per;
+    for (int j = 0; j < PIECE / 2048; j++) {
+        const long c = (long)k * (PIECE / 8) + j * 256 + threadIdx.x;
+        if (c >= all) break;
+        const long row = c / per;
+        const int col = (int)(c - row * per) * 8, count = row < x.m ? x.n - col : 0;
+        float g[8];
+        load8(g, x.src, row * x.ld + col, count, x.fp32);
+        if (x.momentum) {
+            float m[8];
+            load8(m, x.momentum, row * x.n + col, count, true);
+            for (int e = 0; e < 8; e++) g[e] = u.nesterov ? u.mu * m[e] + (1.f - u.mu) * (g[e] * f) : m[e];
+        }
+        uint4 hi, lo;
+        split(g[0] * by, g[1] * by, hi.x, lo.x);
+        split(g[2] * by, g[3] * by, hi.y, lo.y);
+        split(g[4] * by, g[5] * by, hi.z, lo.z);
+        split(g[6] * by, g[7] * by, hi.w, lo.w);
+        *reinterpret_cast<uint4*>(x.hi(0) + row * x.np + col) = hi;
+        *reinterpret_cast<uint4*>(x.lo(0) + row * x.np + col) = lo;
+    }
+}
+
+// ------------------------------------------------------------------------------ products
+// A launch's workgroup b -> its place in the order of tiles: each XCD (b % 8) takes a run of
+// consecutive tiles, so that its L2 serves both operands.
+__device__ __forceinline__ int place_of(const List& l) {
+    const int total = l.first[l.count], each = total >> 3, b = blockIdx.x;
+    return b < each * 8 ? (b & 7) * each + (b >> 3) : b;
+}
+// tile k of the lower triangle of T x T, in groups of G rows that walk over the columns together
+__device__ __forceinline__ void lower_tile(int T, int G, int k, int& i, int& j) {
+    int f = 0, size;
+    for (;;) {
+        size = min(G, T - f);
+        const int all = size * f + size * (size + 1) / 2;
+        if (k < all) break;
+        k -= all;
+        f += size;
+    }
+    if (k < size * f) {
+        j = k / size, i = f + (k - j * size);
+        return;
+    }
+    k -= size * f;
+    j = 0;
+    while (k >= size - j) k -= size - j, j++;
+    i = f + j + k, j += f;
+}
+__device__ __forceinline__ int tiles_of(int x, int by) { return (x + by - 1) / by; }
+
+// a tile's values as float16 to its place and, where it lies below the diagonal, to the mirrored one: v[tn][tm] holds
+// a lane's four consecutive columns of a row
+template <class P> __device__ __forceinline__ void store_both(uint8_t* lds, const uint2 (&v)[P::TN][P::TM], uint16_t* c, int ld, int m0, int n0) {
+    store_rows<P>(
+        lds, [&](int tn, int tm) { return v[tn][tm]; },
+        [&](int m, int n, const uint4& x) {
+            if (m0 + m < ld && n0 + n < ld) *reinterpret_cast<uint4*>(c + (long)(m0 + m) * ld + n0 + n) = x;
+        });
+    if (m0 == n0) return;
+    // the mirrored tile's rows are this one's columns: 16 at a time through the wave's part of LDS
+    constexpr int CH = P::TM * 2, ROW = CH * 16;
+    static_assert(8 * 16 * ROW <= P::EPILOGUE && CH <= 8, "tile");
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6, r16 = lane & 15, q = lane >> 4;
+    uint8_t* mine = P::epilogue(lds) + wave * (16 * ROW);
+    const int m = m0 + (wave / P::WN) * P::TM * 16 + 8 * (lane & (CH - 1)), nw = n0 + (wave % P::WN) * P::TN * 16;
+#pragma unroll
+    for (int tn = 0; tn < P::TN; tn++) {
+#pragma unroll
+        for (int tm = 0; tm < P::TM; tm++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int n = 4 * q + e, at = n * ROW + (((2 * tm + (r16 >> 3)) ^ ((n >> 1) & (CH - 1))) << 4) + 2 * (r16 & 7);
+                const uint32_t w = e < 2 ? v[tn][tm].x : v[tn][tm].y;
+                *reinterpret_cast<uint16_t*>(mine + at) = (uint16_t)(e & 1 ? w >> 16 : w);
+            }
+        wkv7::wave_lds_fence();
+#pragma unroll
+        for (int i = 0; i < 16 * CH / 64; i++) {
+            const int r = i * (64 / CH) + lane / CH, n = nw + 16 * tn + r;
+            const uint4 x = *reinterpret_cast<const uint4*>(mine + r * ROW + (((lane & (CH - 1)) ^ ((r >> 1) & (CH - 1))) << 4));
+            if (m < ld && n < ld) *reinterpret_cast<uint4*>(c + (long)n * ld + m) = x;
+        }
+        wkv7::wave_lds_fence();
+    }
+}
+
+template <class P> __device__ __forceinline__ uint2 halves(const P& g, int tn, int tm) {
+    const f32x4_t& a = g.acc[tn][tm];
+    return make_uint2(half2_of(a[0], a[1]), half2_of(a[2], a[3]));
+}
+struct OneTile {
+    __device__ __forceinline__ bool operator()(Place&) const { return false; }
+};
+
+// A of the current X
+template <class PW, class PT> __global__ __launch_bounds__(512) void gram(List l, int now) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[PW::LDS > PT::LDS ? PW::LDS : PT::LDS];
+    const int at = place_of(l), k = which(l, at);
+    const Matrix& x = l.x[k];
+    const int pp = x.pp();
+    int i, j;
+    lower_tile(tiles_of(pp, PW::BM), TOGETHER / PW::BM, at - l.first[k], i, j);
+    auto go = [&](auto tag, const Operand& o, int inner) {
+        using P = decltype(tag);
+        P g;
+        g.template go<false>(lds, o, o, Place{i * P::BM, j * P::BN, 0, inner / BK}, OneTile{}, [&](const Place& t) {
+            uint2 v[P::TN][P::TM];
+#pragma unroll
+            for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+                for (int tm = 0; tm < P::TM; tm++) v[tn][tm] = halves(g, tn, tm);
+            store_both<P>(lds, v, x.gram(), pp, t.m0, t.n0);
+        });
+    };
+    if (x.tall()) go(PT{}, Operand{x.hi(now), x.np, x.np, x.mp}, x.mp);
+    else go(PW{}, Operand{x.hi(now), x.np, x.mp, x.np}, x.np);
+}
+
+// B of A
+template <class P> __global__ __launch_bounds__(512) void square(List l, float b, float c) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
+    const int at = place_of(l), k = which(l, at);
+    const Matrix& x = l.x[k];
+    const int pp = x.pp();
+    int i, j;
+    lower_tile(tiles_of(pp, P::BM), TOGETHER / P::BM, at - l.first[k], i, j);
+    const Operand o{x.gram(), pp, pp, pp};
+    P g;
+    g.template go<false>(lds, o, o, Place{i * P::BM, j * P::BN, 0, pp / BK}, OneTile{}, [&](const Place& t) {
+        const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
+        const int m = t.m0 + (wave / P::WN) * P::TM * 16 + (lane & 15), n = t.n0 + (wave % P::WN) * P::TN * 16 + 4 * (lane >> 4);
+        const float cs = c / (x.s * x.s);
+        const uint16_t* a = x.gram();
+        uint2 v[P::TN][P::TM];
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+            for (int tm = 0; tm < P::TM; tm++)  // (places beyond the matrix are not stored: any valid ones)
+                v[tn][tm] = *reinterpret_cast<const uint2*>(a + (long)min(m + 16 * tm, pp - 1) * pp + min(n + 16 * tn, pp - 4));
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+            for (int tm = 0; tm < P::TM; tm++) {
+                const float2 x0 = floats_of(v[tn][tm].x), x1 = floats_of(v[tn][tm].y);
+                const f32x4_t& z = g.acc[tn][tm];
+                v[tn][tm] = make_uint2(half2_of(b * x0.x + cs * z[0], b * x0.y + cs * z[1]), half2_of(b * x1.x + cs * z[2], b * x1.y + cs * z[3]));
+            }
+        store_both<P>(lds, v, x.square(), pp, t.m0, t.n0);
+    });
+}
+
+// 16 (EACH = 2: 32) rows of a wave's tile of 16-bit values through its part of LDS, as store_rows
+template <class P, int EACH, class Put> __device__ __forceinline__ void store_strip(uint8_t* lds, int t0, const uint2 (&v)[EACH][P::TN], Put put) {
+    constexpr int CH = P::TN * 2, ROW = CH * 16;
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6, r16 = lane & 15, q = lane >> 4;
+    uint8_t* mine = P::epilogue(lds) + wave * (EACH * 16 * ROW);
+    const int c = lane & (CH - 1), m0 = (wave / P::WN) * P::TM * 16, n = (wave % P::WN) * P::TN * 16 + 8 * c;
+#pragma unroll
+    for (int t = 0; t < EACH; t++)
+#pragma unroll
+        for (int tn = 0; tn < P::TN; tn++)
+            *reinterpret_cast<uint2*>(mine + (16 * t + r16) * ROW + (((2 * tn + (q >> 1)) ^ (r16 & (CH - 1))) << 4) + 8 * (q & 1)) = v[t][tn];
+    wkv7::wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < EACH * 16 * CH / 64; i++) {
+        const int r = i * (64 / CH) + lane / CH;
+        put(m0 + 16 * t0 + r, n, *reinterpret_cast<const uint4*>(mine + r * ROW + ((c ^ (r & (CH - 1))) << 4)));
+    }
+    wkv7::wave_lds_fence();
+}
+
+// the next X, or what the call is for
+template <class P> __device__ __forceinline__ void update_done(P& g, uint8_t* lds, const Matrix& x, int now, bool last, float a, int tm0, int tn0) {
+    constexpr int EACH = P::TN < 2 ? 2 : 1, STRIPS = P::TM / EACH;
+    static_assert(P::TM % EACH == 0 && 8 * EACH * 16 * P::TN * 32 <= P::EPILOGUE, "tile");
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
+    const int m = tm0 + (wave / P::WN) * P::TM * 16 + (lane & 15), n = tn0 + (wave % P::WN) * P::TN * 16 + 4 * (lane >> 4);
+    const uint16_t *hi = x.hi(now), *lo = x.lo(now);
+    const float by = 1.f / (x.s * x.s), is = 1.f / x.s;
+    uint2 h[2][EACH][P::TN], o[2][EACH][P::TN];  // a strip's, and the next one's on their way
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int t = 0; t < EACH; t++)
+#pragma unroll
+            for (int tn = 0; tn < P::TN; tn++) {
+                const long at = (long)min(m + 16 * (s * EACH + t), x.mp - 1) * x.np + min(n + 16 * tn, x.np - 4);
+                h[s & 1][t][tn] = *reinterpret_cast<const uint2*>(hi + at);
+                o[s & 1][t][tn] = *reinterpret_cast<const uint2*>(lo + at);
+            }
+    };
+    fetch(0);
+#pragma unroll
+    for (int s = 0; s < STRIPS; s++) {
+        if (s + 1 < STRIPS) fetch(s + 1);
+#pragma unroll
+        for (int t = 0; t < EACH; t++)
+#pragma unroll
+            for (int tn = 0; tn < P::TN; tn++) {
+                uint2 &vh = h[s & 1][t][tn], &vo = o[s & 1][t][tn];
+                const float2 h0 = floats_of(vh.x), h1 = floats_of(vh.y), o0 = floats_of(vo.x), o1 = floats_of(vo.y);
+                const f32x4_t& z = g.acc[tn][s * EACH + t];
+                float y[4] = {a * (h0.x + o0.x * (1.f / LO)) + by * z[0], a * (h0.y + o0.y * (1.f / LO)) + by * z[1],
+                              a * (h1.x + o1.x * (1.f / LO)) + by * z[2], a * (h1.y + o1.y * (1.f / LO)) + by * z[3]};
+                if (!last) {
+                    split(y[0], y[1], vh.x, vo.x);
+                    split(y[2], y[3], vh.y, vo.y);
+                } else if (!x.momentum) {
+                    vh = make_uint2(f32x2_to_bf16x2(y[0] * is, y[1] * is), f32x2_to_bf16x2(y[2] * is, y[3] * is));
+                } else {
+                    const int row = m + 16 * (s * EACH + t), col = n + 16 * tn;
+                    if (row < x.m && col < x.n) {
+                        float* p = static_cast<float*>(x.dst) + (long)row * x.n + col;
+                        const float by2 = x.step * is;
+                        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+                        if (col + 4 <= x.n) {
+                            f4 v = *reinterpret_cast<f4*>(p);
+                            for (int e = 0; e < 4; e++) v[e] = v[e] * x.keep - by2 * y[e];
+                            *reinterpret_cast<f4*>(p) = v;
+                        } else {
+                            for (int e = 0; e < 4; e++)
+                                if (col + e < x.n) p[e] = p[e] * x.keep - by2 * y[e];
+                        }
+                    }
+                }
+            }
+        if (!last) {
+            uint16_t *nh = x.hi(now ^ 1), *no = x.lo(now ^ 1);
+            auto put = [&](uint16_t* to) {
+                return [&x, to, tm0, tn0](int i, int j, const uint4& v) {
+                    if (tm0 + i < x.mp && tn0 + j < x.np) *reinterpret_cast<uint4*>(to + (long)(tm0 + i) * x.np + tn0 + j) = v;
+                };
+            };
+            store_strip<P, EACH>(lds, s * EACH, h[s & 1], put(nh));
+            store_strip<P, EACH>(lds, s * EACH, o[s & 1], put(no));
+        } else if (!x.momentum) {
+            store_strip<P, EACH>(lds, s * EACH, h[s & 1], [&](int i, int j, const uint4& v) {
+                const int row = tm0 + i, col = tn0 + j;
+                if (row >= x.m || col >= x.n) return;
+                uint16_t* to = static_cast<uint16_t*>(x.dst) + (long)row * x.n + col;
+                typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+                if (col + 8 <= x.n) *reinterpret_cast<u4*>(to) = u4{v.x, v.y, v.z, v.w};
+                else
+                    for (int e = 0; e < 8 && col + e < x.n; e++) {
+                        const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+                        to[e] = (uint16_t)(e & 1 ? w >> 16 : w);
+                    }
+            });
+        }
+    }
+}
+
+template <class PW, class PT> __global__ __launch_bounds__(512) void update(List l, Update u, int now, bool last, float a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[PW::LDS > PT::LDS ? PW::LDS : PT::LDS];
+    if (last && skipped(u)) return;
+    const int at = place_of(l), k = which(l, at);
+    const Matrix& x = l.x[k];
+    const int pp = x.pp(), id = at - l.first[k];
+    const int tm = tiles_of(x.mp, PW::BM), tn = tiles_of(x.np, PW::BN), G = min(tm, TOGETHER / PW::BM);
+    const int per = G * tn, f = id / per * G, size = min(tm - f, G), r = id - id / per * per, j = r / size, i = f + (r - j * size);
+    const Operand B{x.square(), pp, pp, pp};
+    auto go = [&](auto tag, const Operand& X, const Operand& Y) {
+        using P = decltype(tag);
+        P g;
+        g.template go<false>(lds, X, Y, Place{i * P::BM, j * P::BN, 0, pp / BK}, OneTile{},
+                             [&](const Place& t) { update_done<P>(g, lds, x, now, last, a, t.m0, t.n0); });
+    };
+    // (B is symmetric: its rows serve as columns)
+    if (x.tall()) go(PT{}, Operand{x.hi(now), x.np, x.mp, x.np}, B);
+    else go(PW{}, B, Operand{x.hi(now), x.np, x.np, x.mp});
+}
+
+// ------------------------------------------------------------------------------ host
+static long up(long x, long to) { return (x + to - 1) / to * to; }
+static long ceil_div(long x, long y) { return (x + y - 1) / y; }
+
+template <int BM, int WM, int WN, int NST> struct Shape {
+    using KK = Product<BM, BM, WM, WN, NST, RowK, RowK, true>;
+    using NN = Product<BM, BM, WM, WN, NST, RowN, RowN, true>;
+    using KN = Product<BM, BM, WM, WN, NST, RowK, RowN, true>;
+};
+using Large = Shape<256, 4, 2, 2>;
+using Middle = Shape<128, 4, 2, 2>;
+using Small = Shape<64, 2, 4, 4>;
+// side, workgroups on a CU, us of a step of 64 along the contraction and of the rest
+struct Cost {
+    int side, per_cu;
+    double step, fixed;
+};
+constexpr Cost COSTS[] = {{256, 1, 1.6, 8}, {128, 2, 1.05, 5}, {64, 2, .5, 3}};
+
+static int device_cus() {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
+    return n > 0 ? n : 256;
+}
+
+constexpr size_t MOST = 4ull << 30;  // bytes of the matrices of a launch together, if it has more than one
+
+static size_t bytes_of(const Matrix& x) { return 2 * (4 * (size_t)x.mp * x.np + 2 * (size_t)x.pp() * x.pp()); }
+
+static Matrix matrix(int m, int n) {
+    Matrix x{};
+    x.m = m, x.n = n, x.mp = (int)up(m, BK), x.np = (int)up(n, BK);
+    const int p = m < n ? m : n;
+    x.s = 1.f;
+    while (4.f * x.s * x.s <= (float)(p < 16384 ? p : 16384)) x.s *= 2.f;
+    x.pieces = (int)ceil_div((long)m * ceil_div(n, 8), PIECE / 8);
+    x.ld = n;
+    return x;
+}
+
+// The list's matrices from `next` on that one set of launches takes.
+template <class Get> static bool take(int count, int& next, Get get, List& l, size_t& bytes, long& pieces) {
+    l.count = 0;
+    bytes = 0, pieces = 0;
+    while (next < count && l.count < MAX) {
+        Matrix x = get(next);
+        if (x.m && x.n) {
+            const size_t size = bytes_of(x);
+            if (l.count && bytes + size > MOST) break;
+            x.piece0 = (int)pieces;
+            pieces += x.pieces;
+            bytes += size;
+            l.x[l.count++] = x;
+        }
+        next++;
+    }
+    return l.count > 0;
+}
+static size_t sums_bytes(long pieces) { return up(pieces * sizeof(double), 256); }
+
+template <class Get> static size_t workspace(int count, Get get) {
+    size_t most = 0, bytes;
+    long pieces;
+    int next = 0;
+    List l;
+    while (take(count, next, get, l, bytes, pieces)) most = most > bytes + sums_bytes(pieces) ? most : bytes + sums_bytes(pieces);
+    return most;
+}
+
+// tiles of matrix x in a product: 0 gram or square, 1 update
+static long tiles(const Matrix& x, int kind, int side) {
+    const long p = ceil_div(x.pp(), side);
+    return kind == 0 ? p * (p + 1) / 2 : ceil_div(x.mp, side) * ceil_div(x.np, side);
+}
+// The shape that a product of the whole list is quickest in: tiles of 256 where they fill the CUs, smaller
+// ones (twice the operands' traffic for each halving) where there are few.
+static int shape(const List& l, int kind, bool gram, int cus) {
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < 3; i++) {
+        const Cost& c = COSTS[i];
+        double work = 0, longest = 0, n = 0;
+        for (int k = 0; k < l.count; k++) {
+            const Matrix& x = l.x[k];
+            const double steps = (gram ? (x.tall() ? x.mp : x.np) : x.pp()) / BK, t = c.fixed + steps * c.step, w = (double)tiles(x, kind, c.side);
+            work += t * w, n += w;
+            longest = longest > t ? longest : t;
+        }
+        double us = work / n * ceil(n / (cus * c.per_cu));
+        us = us > longest ? us : longest;
+        if (i == 0 || us < least) least = us, best = i;
+    }
+    return best;
+}
+
+template <class Set> static unsigned prefix(List& l, Set groups) {
+    long at = 0;
+    for (int k = 0; k < l.count; k++) {
+        l.first[k] = (int)at;
+        at += groups(l.x[k]);
+    }
+    l.first[l.count] = (int)at;
+    return (unsigned)at;
+}
+
+static void run(List& l, const Update& u, const theseus_newton_schulz* ns, uint8_t* ws, long pieces, hipStream_t st) {
+    double* sums = reinterpret_cast<double*>(ws);
+    uint8_t* at = ws + sums_bytes(pieces);
+    for (int k = 0; k < l.count; k++) {
+        l.x[k].ws = reinterpret_cast<uint16_t*>(at);
+        at += bytes_of(l.x[k]);
+    }
+    const int cus = device_cus();
+    momentum_norm<<<prefix(l, [](const Matrix& x) { return (long)x.pieces; }), 256, 0, st>>>(l, u, sums);
+    const unsigned scale = prefix(l, [](const Matrix& x) { return ceil_div((long)x.mp * x.np, PIECE); });
+    scale_split<<<scale, 256, 0, st>>>(l, u, sums);
+    const int sg = shape(l, 0, true, cus), ss = shape(l, 0, false, cus), su = shape(l, 1, false, cus);
+    auto with = [](int which, auto go) {
+        if (which == 0) go(Large{});
+        else if (which == 1) go(Middle{});
+        else go(Small{});
+    };
+    for (int i = 0; i < ns->steps; i++) {
+        const int now = i & 1;
+        with(sg, [&](auto s) {
+            using S = decltype(s);
+            const unsigned n = prefix(l, [&](const Matrix& x) { return tiles(x, 0, COSTS[sg].side); });
+            gram<typename S::KK, typename S::NN><<<n, 512, 0, st>>>(l, now);
+        });
+        with(ss, [&](auto s) {
+            using S = decltype(s);
+            const unsigned n = prefix(l, [&](const Matrix& x) { return tiles(x, 0, COSTS[ss].side); });
+            square<typename S::KK><<<n, 512, 0, st>>>(l, ns->b, ns->c);
+        });
+        with(su, [&](auto s) {
+            using S = decltype(s);
+            const unsigned n = prefix(l, [&](const Matrix& x) { return tiles(x, 1, COSTS[su].side); });
+            update<typename S::KN, typename S::KK><<<n, 512, 0, st>>>(l, u, now, i + 1 == ns->steps, ns->a);
+        });
+    }
+}
+
+static int check(const theseus_newton_schulz* ns) {
+    if (!ns) return THESEUS_WKV7_ERR_NULL;
+    if (ns->steps < 1 || ns->steps > 100 || !isfinite(ns->a) || !isfinite(ns->b) || !isfinite(ns->c) || !(ns->eps >= 0.f) || !isfinite(ns->eps))
+        return THESEUS_WKV7_ERR_SHAPE;
+    return THESEUS_WKV7_OK;
+}
+static bool fits(long long m, long long n) { return m >= 0 && n >= 0 && m <= 1 << 17 && n <= 1 << 17; }
+
+static Matrix get_orth(const theseus_orthogonalize_matrix& s) {
+    Matrix x = matrix(s.rows, s.cols);
+    x.src = s.x, x.ld = s.row_stride, x.dst = s.out, x.fp32 = s.dtype == THESEUS_MUON_FP32;
+    return x;
+}
+static Matrix get_muon(const theseus_muon_matrix& s) {
+    Matrix x = matrix(s.rows, s.cols);
+    x.src = s.grad, x.momentum = s.momentum, x.dst = s.param, x.keep = s.keep, x.step = s.step, x.fp32 = 1;
+    return x;
+}
+static int check(const theseus_orthogonalize_matrix* ms, int count) {
+    if (count < 0) return THESEUS_WKV7_ERR_SHAPE;
+    if (count && !ms) return THESEUS_WKV7_ERR_NULL;
+    for (int i = 0; i < count; i++) {
+        const theseus_orthogonalize_matrix& s = ms[i];
+        if (!fits(s.rows, s.cols) || (s.rows > 1 && s.row_stride < s.cols)) return THESEUS_WKV7_ERR_SHAPE;
+        if (s.dtype != THESEUS_MUON_BF16 && s.dtype != THESEUS_MUON_FP32) return THESEUS_WKV7_ERR_DTYPE;
+        if (s.rows && s.cols && (!s.x || !s.out)) return THESEUS_WKV7_ERR_NULL;
+    }
+    return THESEUS_WKV7_OK;
+}
+static int check(const theseus_muon_matrix* ms, int count) {
+    if (count < 0) return THESEUS_WKV7_ERR_SHAPE;
+    if (count && !ms) return THESEUS_WKV7_ERR_NULL;
+    for (int i = 0; i < count; i++) {
+        const theseus_muon_matrix& s = ms[i];
+        if (!fits(s.rows, s.cols)) return THESEUS_WKV7_ERR_SHAPE;
+        if (s.rows && s.cols && (!s.param || !s.grad || !s.momentum)) return THESEUS_WKV7_ERR_NULL;
+    }
+    return THESEUS_WKV7_OK;
+}
+
+// The norm pass over the gradients, a launch's tensors at a time; partial == nullptr: its doubles alone.
+static long long norm_pass(const theseus_muon_matrix* ms, int count, double* partial, hipStream_t st) {
+    theseus_adamw_tensor t[MAX];
+    long long chunks = 0;
+    for (int i = 0; i < count; i += MAX) {
+        const int n = count - i < MAX ? count - i : MAX;
+        for (int k = 0; k < n; k++) {
+            t[k] = theseus_adamw_tensor{};
+            t[k].grad = ms[i + k].grad, t[k].numel = (long long)ms[i + k].rows * ms[i + k].cols;
+            if (!partial) chunks += (t[k].numel + THESEUS_ADAMW_CHUNK - 1) / THESEUS_ADAMW_CHUNK;
+        }
+        if (partial) optim::launch_sumsq(t, n, chunks, 0, partial, st);
+    }
+    return chunks;
+}
+
+}  // namespace muon
+
+extern "C" {
+
+size_t theseus_orthogonalize_workspace_size(const theseus_orthogonalize_matrix* ms, int count) {
+    if (muon::check(ms, count)) return 0;
+    return muon::workspace(count, [&](int i) { return muon::get_orth(ms[i]); });
+}
+
+int theseus_orthogonalize(const theseus_orthogonalize_matrix* ms, int count, const theseus_newton_schulz* ns, void* workspace,
+                          size_t workspace_bytes, hipStream_t stream) {
+    if (int e = muon::check(ns)) return e;
+    if (int e = muon::check(ms, count)) return e;
+    auto get = [&](int i) { return muon::get_orth(ms[i]); };
+    const size_t need = muon::workspace(count, get);
+    if (need && (!workspace || workspace_bytes < need)) return THESEUS_WKV7_ERR_WORKSPACE;
+    const muon::Update u{0.f, 0, 1.f, nullptr, 0, ns->eps};
+    muon::List l;
+    size_t bytes;
+    long pieces;
+    int next = 0;
+    while (muon::take(count, next, get, l, bytes, pieces)) muon::run(l, u, ns, static_cast<uint8_t*>(workspace), pieces, stream);
+    return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
+}
+
+size_t theseus_muon_workspace_size(const theseus_muon_matrix* ms, int count) {
+    if (muon::check(ms, count)) return 0;
+    const size_t norm = (size_t)muon::norm_pass(ms, count, nullptr, nullptr) * sizeof(double), step = muon::workspace(count, [&](int i) { return muon::get_muon(ms[i]); });
+    return norm > step ? norm : step;
+}
+
+int theseus_muon_step(const theseus_muon_matrix* ms, int count, const theseus_newton_schulz* ns, float momentum, int nesterov,
+                      float grad_scale, float max_norm, int skip_nonfinite, float* result, void* workspace, size_t workspace_bytes,
+                      hipStream_t stream) {
+    if (int e = muon::check(ns)) return e;
+    if (int e = muon::check(ms, count)) return e;
+    const bool norm = max_norm >= 0.f;
+    if (norm && !result) return THESEUS_WKV7_ERR_NULL;
+    const size_t need = theseus_muon_workspace_size(ms, count);
+    if (need && (!workspace || workspace_bytes < need)) return THESEUS_WKV7_ERR_WORKSPACE;
+    if (norm) {
+        double* partial = static_cast<double*>(workspace);
+        optim::launch_norm(partial, muon::norm_pass(ms, count, partial, stream), grad_scale, max_norm, result, stream);
+    }
+    const muon::Update u{momentum, nesterov, grad_scale, norm ? result : nullptr, skip_nonfinite, ns->eps};
+    auto get = [&](int i) { return muon::get_muon(ms[i]); };
+    muon::List l;
+    size_t bytes;
+    long pieces;
+    int next = 0;
+    while (muon::take(count, next, get, l, bytes, pieces)) muon::run(l, u, ns, static_cast<uint8_t*>(workspace), pieces, stream);
+    return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
+}
+
+}  // extern "C"

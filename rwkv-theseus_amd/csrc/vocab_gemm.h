@@ -1,5 +1,6 @@
-// Matrix product of the vocabulary losses (gfx950): C[m][n] = sum_k X(m, k) Y(n, k), bfloat16
-// operands, float32 sums, for the three products of a vocabulary head:
+// Matrix product of the vocabulary losses and of the orthogonalised updates (gfx950):
+// C[m][n] = sum_k X(m, k) Y(n, k), bfloat16 (or float16) operands, float32 sums, for the three
+// products of a vocabulary head:
 //
 //   logits   Z = H W^T      X = H [m][k], Y = W [n][k]      both rows run along the contraction
 //   dhidden  G W            X = G [m][k], Y = W [k][n]      Y's rows run along the output
@@ -218,7 +219,8 @@ struct Place {
 // one tile a workgroup throughout: 2604 tokens' logits of 53714 at D = 768 336 us for 295, 365 tokens'
 // dweight of 60000 x 2560 159 for 144, with 80 steps and more, at the power limit, the same).  Shapes whose
 // stages leave no LDS for that (KEPT false) make one tile, and done() writes where the stages were.
-template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct Product {
+// HALF: float16 operands.
+template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_, bool HALF = false> struct Product {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NST = NST_;
     static constexpr Lay LX = LX_, LY = LY_;
     static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
@@ -286,7 +288,7 @@ template <int BM_, int BN_, int WM_, int WN_, int NST_, Lay LX_, Lay LY_> struct
         auto read_y = [&](int stage, int i, int h) { y[i] = ry.get(lds, stage * STAGE + BM * BK * 2, i, h); };
         auto group = [&](const uint4 (&x)[TM], int tn) {
 #pragma unroll
-            for (int tm = 0; tm < TM; tm++) acc[tn][tm] = wkv7::mma32(acc[tn][tm], y[tn], x[tm]);
+            for (int tm = 0; tm < TM; tm++) acc[tn][tm] = HALF ? wkv7::mma32h(acc[tn][tm], y[tn], x[tm]) : wkv7::mma32(acc[tn][tm], y[tn], x[tm]);
         };
         // groups G0 .. TN - 1; behind each, what there is of a stage's refill and of the next half's
         // fragments: y as its registers come free, x spread over the groups

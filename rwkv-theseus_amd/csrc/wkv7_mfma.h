@@ -25,6 +25,11 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ f32x4_t zero4() { return f32x4_t{0.f, 0.f, 0.f, 0.f}; }
 
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+// the same shape and lanes with float16 operands
+__device__ __forceinline__ f32x4_t mma32h(f32x4_t acc, uint4 a, uint4 b) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), acc, 0, 0, 0);
+}
 __device__ __forceinline__ f32x4_t mma32(f32x4_t acc, uint4 a, uint4 b) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                    __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);
