@@ -237,10 +237,11 @@ template <class P> __device__ __forceinline__ void store_both(uint8_t* lds, cons
         });
     if (m0 == n0) return;
     // the mirrored tile's rows are this one's columns: 16 at a time through the wave's part of LDS
-    constexpr int CH = P::TM * 2, ROW = CH * 16;
-    static_assert(8 * 16 * ROW <= P::EPILOGUE && CH <= 8, "tile");
+    // (store_rows' part, so that no other wave is still in it)
+    constexpr int CH = P::TM * 2, ROW = CH * 16, MINE = P::TN * 512 * (P::TN < 2 ? 2 : 1);
+    static_assert(16 * ROW <= MINE && 8 * MINE <= P::EPILOGUE && CH <= 8, "tile");
     const int thread = thread_here(), lane = thread & 63, wave = thread >> 6, r16 = lane & 15, q = lane >> 4;
-    uint8_t* mine = P::epilogue(lds) + wave * (16 * ROW);
+    uint8_t* mine = P::epilogue(lds) + wave * MINE;
     const int m = m0 + (wave / P::WN) * P::TM * 16 + 8 * (lane & (CH - 1)), nw = n0 + (wave % P::WN) * P::TN * 16;
 #pragma unroll
     for (int tn = 0; tn < P::TN; tn++) {
