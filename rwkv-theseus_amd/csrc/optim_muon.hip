@@ -3,8 +3,8 @@
 // X_0 = s u / max(|u|_F, eps) and, `steps` times with p the short side,
 //
 //   A = X X^T (X^T X where X is tall)      the lower triangle's tiles, each stored on both sides
-//   B = b A + (c / s^2) A^2                the same: A commutes with itself, so A^2 = A A^T
-//   X = a X + (1 / s^2) B X (X B)
+//   B = s^2 a I + b A + (c / s^2) A^2      the same: A is symmetric, so A^2 = A A^T
+//   X = (1 / s^2) B X (X B)
 //
 // p^2 q + p^3 + 2 p^2 q products and sums a step instead of 2 p^2 q + 2 p^3 + 2 p^2 q, on the matrix
 // cores with vocab_gemm.h's tiles: a wide X is read along its rows for A and along its columns for
@@ -200,11 +200,16 @@ __global__ __launch_bounds__(256) void scale_split(List l, Update u, const doubl
 }
 
 // ------------------------------------------------------------------------------ products
-// A launch's workgroup b -> its place in the order of tiles: each XCD (b % 8) takes a run of
-// consecutive tiles, so that its L2 serves both operands.
-__device__ __forceinline__ int place_of(const List& l) {
-    const int total = l.first[l.count], each = total >> 3, b = blockIdx.x;
-    return b < each * 8 ? (b & 7) * each + (b >> 3) : b;
+// A launch makes tiles from, from + 1, .. of the list, its workgroups one after the other: t-th of
+// the launch -> its number, each XCD (t % 8) a run of consecutive ones, so that its L2 serves
+// both operands.
+struct Span {
+    int from, count;
+    bool quarters;  // of tiles of twice the side
+};
+__device__ __forceinline__ int number_of(const Span& s, int t) {
+    const int each = s.count >> 3;
+    return t < each * 8 ? (t & 7) * each + (t >> 3) : t;
 }
 // tile k of the lower triangle of T x T, in groups of G rows that walk over the columns together
 __device__ __forceinline__ void lower_tile(int T, int G, int k, int& i, int& j) {
@@ -225,7 +230,54 @@ __device__ __forceinline__ void lower_tile(int T, int G, int k, int& i, int& j) 
     while (k >= size - j) k -= size - j, j++;
     i = f + j + k, j += f;
 }
+// tile k of TM x TN likewise
+__device__ __forceinline__ void any_tile(int TM, int TN, int G, int k, int& i, int& j) {
+    const int per = min(G, TM) * TN, f = k / per * min(G, TM), size = min(TM - f, G);
+    k -= k / per * per;
+    j = k / size, i = f + (k - j * size);
+}
 __device__ __forceinline__ int tiles_of(int x, int by) { return (x + by - 1) / by; }
+
+struct Tile {
+    int matrix, m0, n0;
+    bool none;  // a quarter beyond the matrix, or above the diagonal
+};
+template <int SIDE, bool LOWER> __device__ __forceinline__ Tile tile_at(const List& l, const Span& s, int t) {
+    int id = number_of(s, t), part = 0;
+    if (s.quarters) part = id & 3, id >>= 2;
+    id += s.from;
+    Tile r;
+    r.matrix = which(l, id);
+    const Matrix& x = l.x[r.matrix];
+    const int side = s.quarters ? 2 * SIDE : SIDE, M = LOWER ? x.pp() : x.mp, N = LOWER ? M : x.np;
+    int i, j;
+    if constexpr (LOWER) lower_tile(tiles_of(M, side), TOGETHER / side, id - l.first[r.matrix], i, j);
+    else any_tile(tiles_of(M, side), tiles_of(N, side), TOGETHER / side, id - l.first[r.matrix], i, j);
+    r.m0 = i * side + (part & 1) * SIDE, r.n0 = j * side + (part >> 1) * SIDE;
+    r.none = r.m0 >= M || r.n0 >= N || (LOWER && r.m0 < r.n0);
+    return r;
+}
+
+// A workgroup's tiles.  As long as they are of one matrix, and long enough for it, a tile's first
+// stages are loaded under the last steps and the epilogue of the one before it.
+template <int SIDE, bool LOWER, class Make> __device__ __forceinline__ void each_tile(const List& l, const Span& s, Make make) {
+    for (int t = blockIdx.x; t < s.count; t += gridDim.x) {
+        const Tile at = tile_at<SIDE, LOWER>(l, s, t);
+        if (at.none) continue;
+        make(l.x[at.matrix], at, [&](int steps, int NST) {
+            return [&l, &s, &t, at, steps, NST](Place& p) {
+                const int then = t + gridDim.x;
+                if (steps <= NST || then >= s.count) return false;
+                const Tile to = tile_at<SIDE, LOWER>(l, s, then);
+                if (to.matrix != at.matrix || to.none) return false;
+                t = then;
+                p = Place{to.m0, to.n0, 0, steps};
+                return true;
+            };
+        });
+        __syncthreads();
+    }
+}
 
 // a tile's values as float16 to its place and, where it lies below the diagonal, to the mirrored one: v[tn][tm] holds
 // a lane's four consecutive columns of a row
@@ -268,64 +320,59 @@ template <class P> __device__ __forceinline__ uint2 halves(const P& g, int tn, i
     const f32x4_t& a = g.acc[tn][tm];
     return make_uint2(half2_of(a[0], a[1]), half2_of(a[2], a[3]));
 }
-struct OneTile {
-    __device__ __forceinline__ bool operator()(Place&) const { return false; }
-};
 
 // A of the current X
-template <class PW, class PT> __global__ __launch_bounds__(512) void gram(List l, int now) {
+template <class PW, class PT> __global__ __launch_bounds__(512) void gram(List l, Span s, int now) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[PW::LDS > PT::LDS ? PW::LDS : PT::LDS];
-    const int at = place_of(l), k = which(l, at);
-    const Matrix& x = l.x[k];
-    const int pp = x.pp();
-    int i, j;
-    lower_tile(tiles_of(pp, PW::BM), TOGETHER / PW::BM, at - l.first[k], i, j);
-    auto go = [&](auto tag, const Operand& o, int inner) {
-        using P = decltype(tag);
+    each_tile<PW::BM, true>(l, s, [&](const Matrix& x, const Tile& at, auto more) {
+        auto go = [&](auto tag, const Operand& o, int inner) {
+            using P = decltype(tag);
+            P g;
+            g.template go<false>(lds, o, o, Place{at.m0, at.n0, 0, inner / BK}, more(inner / BK, P::NST), [&](const Place& t) {
+                uint2 v[P::TN][P::TM];
+#pragma unroll
+                for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+                    for (int tm = 0; tm < P::TM; tm++) v[tn][tm] = halves(g, tn, tm);
+                store_both<P>(lds, v, x.gram(), x.pp(), t.m0, t.n0);
+            });
+        };
+        if (x.tall()) go(PT{}, Operand{x.hi(now), x.np, x.np, x.mp}, x.mp);
+        else go(PW{}, Operand{x.hi(now), x.np, x.mp, x.np}, x.np);
+    });
+}
+
+// s^2 (a I + b A + c A^2) of A, with s^2 A in memory
+template <class P> __global__ __launch_bounds__(512) void square(List l, Span s, float a, float b, float c) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
+    each_tile<P::BM, true>(l, s, [&](const Matrix& x, const Tile& at, auto more) {
+        const int pp = x.pp();
+        const Operand o{x.gram(), pp, pp, pp};
         P g;
-        g.template go<false>(lds, o, o, Place{i * P::BM, j * P::BN, 0, inner / BK}, OneTile{}, [&](const Place& t) {
+        g.template go<false>(lds, o, o, Place{at.m0, at.n0, 0, pp / BK}, more(pp / BK, P::NST), [&](const Place& t) {
+            const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
+            const int m = t.m0 + (wave / P::WN) * P::TM * 16 + (lane & 15), n = t.n0 + (wave % P::WN) * P::TN * 16 + 4 * (lane >> 4);
+            const float cs = c / (x.s * x.s), as = a * (x.s * x.s);
+            const uint16_t* gram = x.gram();
             uint2 v[P::TN][P::TM];
 #pragma unroll
             for (int tn = 0; tn < P::TN; tn++)
 #pragma unroll
-                for (int tm = 0; tm < P::TM; tm++) v[tn][tm] = halves(g, tn, tm);
-            store_both<P>(lds, v, x.gram(), pp, t.m0, t.n0);
+                for (int tm = 0; tm < P::TM; tm++)  // (places beyond the matrix are not stored: any valid ones)
+                    v[tn][tm] = *reinterpret_cast<const uint2*>(gram + (long)min(m + 16 * tm, pp - 1) * pp + min(n + 16 * tn, pp - 4));
+#pragma unroll
+            for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+                for (int tm = 0; tm < P::TM; tm++) {
+                    const float2 x0 = floats_of(v[tn][tm].x), x1 = floats_of(v[tn][tm].y);
+                    const f32x4_t& z = g.acc[tn][tm];
+                    float y[4] = {b * x0.x + cs * z[0], b * x0.y + cs * z[1], b * x1.x + cs * z[2], b * x1.y + cs * z[3]};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] += m + 16 * tm == n + 16 * tn + e ? as : 0.f;
+                    v[tn][tm] = make_uint2(half2_of(y[0], y[1]), half2_of(y[2], y[3]));
+                }
+            store_both<P>(lds, v, x.square(), pp, t.m0, t.n0);
         });
-    };
-    if (x.tall()) go(PT{}, Operand{x.hi(now), x.np, x.np, x.mp}, x.mp);
-    else go(PW{}, Operand{x.hi(now), x.np, x.mp, x.np}, x.np);
-}
-
-// B of A
-template <class P> __global__ __launch_bounds__(512) void square(List l, float b, float c) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
-    const int at = place_of(l), k = which(l, at);
-    const Matrix& x = l.x[k];
-    const int pp = x.pp();
-    int i, j;
-    lower_tile(tiles_of(pp, P::BM), TOGETHER / P::BM, at - l.first[k], i, j);
-    const Operand o{x.gram(), pp, pp, pp};
-    P g;
-    g.template go<false>(lds, o, o, Place{i * P::BM, j * P::BN, 0, pp / BK}, OneTile{}, [&](const Place& t) {
-        const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
-        const int m = t.m0 + (wave / P::WN) * P::TM * 16 + (lane & 15), n = t.n0 + (wave % P::WN) * P::TN * 16 + 4 * (lane >> 4);
-        const float cs = c / (x.s * x.s);
-        const uint16_t* a = x.gram();
-        uint2 v[P::TN][P::TM];
-#pragma unroll
-        for (int tn = 0; tn < P::TN; tn++)
-#pragma unroll
-            for (int tm = 0; tm < P::TM; tm++)  // (places beyond the matrix are not stored: any valid ones)
-                v[tn][tm] = *reinterpret_cast<const uint2*>(a + (long)min(m + 16 * tm, pp - 1) * pp + min(n + 16 * tn, pp - 4));
-#pragma unroll
-        for (int tn = 0; tn < P::TN; tn++)
-#pragma unroll
-            for (int tm = 0; tm < P::TM; tm++) {
-                const float2 x0 = floats_of(v[tn][tm].x), x1 = floats_of(v[tn][tm].y);
-                const f32x4_t& z = g.acc[tn][tm];
-                v[tn][tm] = make_uint2(half2_of(b * x0.x + cs * z[0], b * x0.y + cs * z[1]), half2_of(b * x1.x + cs * z[2], b * x1.y + cs * z[3]));
-            }
-        store_both<P>(lds, v, x.square(), pp, t.m0, t.n0);
     });
 }
 
@@ -349,71 +396,71 @@ template <class P, int EACH, class Put> __device__ __forceinline__ void store_st
     wkv7::wave_lds_fence();
 }
 
-// the next X, or what the call is for
-template <class P> __device__ __forceinline__ void update_done(P& g, uint8_t* lds, const Matrix& x, int now, bool last, float a, int tm0, int tn0) {
+// What an update makes of its sums: the next X in two halves, its first half alone (the step before the
+// last, whose X goes nowhere but into products), or what the call is for.
+enum Stage { BOTH, FIRST, LAST };
+template <class P, Stage ST> __device__ __forceinline__ void update_done(P& g, uint8_t* lds, const Matrix& x, int now, float a, int tm0, int tn0) {
     constexpr int EACH = P::TN < 2 ? 2 : 1, STRIPS = P::TM / EACH;
     static_assert(P::TM % EACH == 0 && 8 * EACH * 16 * P::TN * 32 <= P::EPILOGUE, "tile");
     const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
     const int m = tm0 + (wave / P::WN) * P::TM * 16 + (lane & 15), n = tn0 + (wave % P::WN) * P::TN * 16 + 4 * (lane >> 4);
-    const uint16_t *hi = x.hi(now), *lo = x.lo(now);
-    const float by = 1.f / (x.s * x.s), is = 1.f / x.s;
-    uint2 h[2][EACH][P::TN], o[2][EACH][P::TN];  // a strip's, and the next one's on their way
+    const float by = 1.f / (x.s * x.s), al = a * (1.f / LO);
+    uint2 o[2][EACH][P::TN];  // the second halves of a strip, and the next one's on their way
     auto fetch = [&](int s) {
 #pragma unroll
         for (int t = 0; t < EACH; t++)
 #pragma unroll
-            for (int tn = 0; tn < P::TN; tn++) {
-                const long at = (long)min(m + 16 * (s * EACH + t), x.mp - 1) * x.np + min(n + 16 * tn, x.np - 4);
-                h[s & 1][t][tn] = *reinterpret_cast<const uint2*>(hi + at);
-                o[s & 1][t][tn] = *reinterpret_cast<const uint2*>(lo + at);
-            }
+            for (int tn = 0; tn < P::TN; tn++)
+                o[s & 1][t][tn] = *reinterpret_cast<const uint2*>(x.lo(now) + (long)min(m + 16 * (s * EACH + t), x.mp - 1) * x.np + min(n + 16 * tn, x.np - 4));
     };
-    fetch(0);
+    if constexpr (ST != LAST) fetch(0);
+    auto put = [&](uint16_t* to) {
+        return [&x, to, tm0, tn0](int i, int j, const uint4& v) {
+            if (tm0 + i < x.mp && tn0 + j < x.np) *reinterpret_cast<uint4*>(to + (long)(tm0 + i) * x.np + tn0 + j) = v;
+        };
+    };
 #pragma unroll
     for (int s = 0; s < STRIPS; s++) {
-        if (s + 1 < STRIPS) fetch(s + 1);
+        if constexpr (ST != LAST) {
+            if (s + 1 < STRIPS) fetch(s + 1);
+        }
+        uint2 h[EACH][P::TN];
 #pragma unroll
         for (int t = 0; t < EACH; t++)
 #pragma unroll
             for (int tn = 0; tn < P::TN; tn++) {
-                uint2 &vh = h[s & 1][t][tn], &vo = o[s & 1][t][tn];
-                const float2 h0 = floats_of(vh.x), h1 = floats_of(vh.y), o0 = floats_of(vo.x), o1 = floats_of(vo.y);
                 const f32x4_t& z = g.acc[tn][s * EACH + t];
-                float y[4] = {a * (h0.x + o0.x * (1.f / LO)) + by * z[0], a * (h0.y + o0.y * (1.f / LO)) + by * z[1],
-                              a * (h1.x + o1.x * (1.f / LO)) + by * z[2], a * (h1.y + o1.y * (1.f / LO)) + by * z[3]};
-                if (!last) {
-                    split(y[0], y[1], vh.x, vo.x);
-                    split(y[2], y[3], vh.y, vo.y);
-                } else if (!x.momentum) {
-                    vh = make_uint2(f32x2_to_bf16x2(y[0] * is, y[1] * is), f32x2_to_bf16x2(y[2] * is, y[3] * is));
+                if constexpr (ST != LAST) {
+                    uint2& lo = o[s & 1][t][tn];
+                    const float2 o0 = floats_of(lo.x), o1 = floats_of(lo.y);
+                    split(al * o0.x + by * z[0], al * o0.y + by * z[1], h[t][tn].x, lo.x);
+                    split(al * o1.x + by * z[2], al * o1.y + by * z[3], h[t][tn].y, lo.y);
                 } else {
+                    const float is = by / x.s;
+                    if (!x.momentum) {
+                        h[t][tn] = make_uint2(f32x2_to_bf16x2(z[0] * is, z[1] * is), f32x2_to_bf16x2(z[2] * is, z[3] * is));
+                        continue;
+                    }
                     const int row = m + 16 * (s * EACH + t), col = n + 16 * tn;
-                    if (row < x.m && col < x.n) {
-                        float* p = static_cast<float*>(x.dst) + (long)row * x.n + col;
-                        const float by2 = x.step * is;
-                        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-                        if (col + 4 <= x.n) {
-                            f4 v = *reinterpret_cast<f4*>(p);
-                            for (int e = 0; e < 4; e++) v[e] = v[e] * x.keep - by2 * y[e];
-                            *reinterpret_cast<f4*>(p) = v;
-                        } else {
-                            for (int e = 0; e < 4; e++)
-                                if (col + e < x.n) p[e] = p[e] * x.keep - by2 * y[e];
-                        }
+                    if (row >= x.m || col >= x.n) continue;
+                    float* p = static_cast<float*>(x.dst) + (long)row * x.n + col;
+                    const float step = x.step * is;
+                    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+                    if (col + 4 <= x.n) {
+                        f4 v = *reinterpret_cast<f4*>(p);
+                        for (int e = 0; e < 4; e++) v[e] = v[e] * x.keep - step * z[e];
+                        *reinterpret_cast<f4*>(p) = v;
+                    } else {
+                        for (int e = 0; e < 4; e++)
+                            if (col + e < x.n) p[e] = p[e] * x.keep - step * z[e];
                     }
                 }
             }
-        if (!last) {
-            uint16_t *nh = x.hi(now ^ 1), *no = x.lo(now ^ 1);
-            auto put = [&](uint16_t* to) {
-                return [&x, to, tm0, tn0](int i, int j, const uint4& v) {
-                    if (tm0 + i < x.mp && tn0 + j < x.np) *reinterpret_cast<uint4*>(to + (long)(tm0 + i) * x.np + tn0 + j) = v;
-                };
-            };
-            store_strip<P, EACH>(lds, s * EACH, h[s & 1], put(nh));
-            store_strip<P, EACH>(lds, s * EACH, o[s & 1], put(no));
+        if constexpr (ST != LAST) {
+            store_strip<P, EACH>(lds, s * EACH, h, put(x.hi(now ^ 1)));
+            if constexpr (ST == BOTH) store_strip<P, EACH>(lds, s * EACH, o[s & 1], put(x.lo(now ^ 1)));
         } else if (!x.momentum) {
-            store_strip<P, EACH>(lds, s * EACH, h[s & 1], [&](int i, int j, const uint4& v) {
+            store_strip<P, EACH>(lds, s * EACH, h, [&](int i, int j, const uint4& v) {
                 const int row = tm0 + i, col = tn0 + j;
                 if (row >= x.m || col >= x.n) return;
                 uint16_t* to = static_cast<uint16_t*>(x.dst) + (long)row * x.n + col;
@@ -429,24 +476,22 @@ template <class P> __device__ __forceinline__ void update_done(P& g, uint8_t* ld
     }
 }
 
-template <class PW, class PT> __global__ __launch_bounds__(512) void update(List l, Update u, int now, bool last, float a) {
+template <class PW, class PT, Stage ST> __global__ __launch_bounds__(512) void update(List l, Span s, Update u, int now, float a) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[PW::LDS > PT::LDS ? PW::LDS : PT::LDS];
-    if (last && skipped(u)) return;
-    const int at = place_of(l), k = which(l, at);
-    const Matrix& x = l.x[k];
-    const int pp = x.pp(), id = at - l.first[k];
-    const int tm = tiles_of(x.mp, PW::BM), tn = tiles_of(x.np, PW::BN), G = min(tm, TOGETHER / PW::BM);
-    const int per = G * tn, f = id / per * G, size = min(tm - f, G), r = id - id / per * per, j = r / size, i = f + (r - j * size);
-    const Operand B{x.square(), pp, pp, pp};
-    auto go = [&](auto tag, const Operand& X, const Operand& Y) {
-        using P = decltype(tag);
-        P g;
-        g.template go<false>(lds, X, Y, Place{i * P::BM, j * P::BN, 0, pp / BK}, OneTile{},
-                             [&](const Place& t) { update_done<P>(g, lds, x, now, last, a, t.m0, t.n0); });
-    };
-    // (B is symmetric: its rows serve as columns)
-    if (x.tall()) go(PT{}, Operand{x.hi(now), x.np, x.mp, x.np}, B);
-    else go(PW{}, B, Operand{x.hi(now), x.np, x.np, x.mp});
+    if (ST == LAST && skipped(u)) return;
+    each_tile<PW::BM, false>(l, s, [&](const Matrix& x, const Tile& at, auto more) {
+        const int pp = x.pp();
+        const Operand B{x.square(), pp, pp, pp};
+        auto go = [&](auto tag, const Operand& X, const Operand& Y) {
+            using P = decltype(tag);
+            P g;
+            g.template go<false>(lds, X, Y, Place{at.m0, at.n0, 0, pp / BK}, more(pp / BK, P::NST),
+                                 [&](const Place& t) { update_done<P, ST>(g, lds, x, now, a, t.m0, t.n0); });
+        };
+        // (B is symmetric: its rows serve as columns)
+        if (x.tall()) go(PT{}, Operand{x.hi(now), x.np, x.mp, x.np}, B);
+        else go(PW{}, B, Operand{x.hi(now), x.np, x.np, x.mp});
+    });
 }
 
 // ------------------------------------------------------------------------------ host
@@ -466,6 +511,7 @@ struct Cost {
     int side, per_cu;
     double step, fixed;
 };
+constexpr double LAUNCH = 4;  // us of one more launch
 constexpr Cost COSTS[] = {{256, 1, 1.6, 8}, {128, 2, 1.05, 5}, {64, 2, .5, 3}};
 
 static int device_cus() {
@@ -483,7 +529,7 @@ static Matrix matrix(int m, int n) {
     x.m = m, x.n = n, x.mp = (int)up(m, BK), x.np = (int)up(n, BK);
     const int p = m < n ? m : n;
     x.s = 1.f;
-    while (4.f * x.s * x.s <= (float)(p < 16384 ? p : 16384)) x.s *= 2.f;
+    while (x.s < 32.f && 4.f * x.s * x.s <= (float)p) x.s *= 2.f;  // (a s^2 stays far below 65504)
     x.pieces = (int)ceil_div((long)m * ceil_div(n, 8), PIECE / 8);
     x.ld = n;
     return x;
@@ -518,28 +564,39 @@ template <class Get> static size_t workspace(int count, Get get) {
     return most;
 }
 
-// tiles of matrix x in a product: 0 gram or square, 1 update
-static long tiles(const Matrix& x, int kind, int side) {
+// tiles of matrix x in a product: the lower triangle of the Gram matrix or its square, or all of X
+static long tiles(const Matrix& x, bool lower, int side) {
     const long p = ceil_div(x.pp(), side);
-    return kind == 0 ? p * (p + 1) / 2 : ceil_div(x.mp, side) * ceil_div(x.np, side);
+    return lower ? p * (p + 1) / 2 : ceil_div(x.mp, side) * ceil_div(x.np, side);
 }
-// The shape that a product of the whole list is quickest in: tiles of 256 where they fill the CUs, smaller
-// ones (twice the operands' traffic for each halving) where there are few.
-static int shape(const List& l, int kind, bool gram, int cus) {
-    int best = 0;
+// How a product of the whole list is made: tiles of 256 where they fill the CUs, smaller ones (twice the
+// operands' traffic for each halving) where there are few; a last round that would fill few CUs in
+// quarters of its tiles.
+struct Way {
+    int shape;
+    bool quarters;  // the tiles behind the last full round
+};
+static Way way(const List& l, bool lower, bool gram, int cus) {
+    Way best{0, false};
     double least = 0;
     for (int i = 0; i < 3; i++) {
         const Cost& c = COSTS[i];
-        double work = 0, longest = 0, n = 0;
+        double work = 0, longest = 0, n = 0, quarter = 0;
         for (int k = 0; k < l.count; k++) {
             const Matrix& x = l.x[k];
-            const double steps = (gram ? (x.tall() ? x.mp : x.np) : x.pp()) / BK, t = c.fixed + steps * c.step, w = (double)tiles(x, kind, c.side);
+            const double steps = (gram ? (x.tall() ? x.mp : x.np) : x.pp()) / BK, t = c.fixed + steps * c.step, w = (double)tiles(x, lower, c.side);
+            const double q = i < 2 ? COSTS[i + 1].fixed + steps * COSTS[i + 1].step : 0;
             work += t * w, n += w;
-            longest = longest > t ? longest : t;
+            longest = longest > t ? longest : t, quarter = quarter > q ? quarter : q;
         }
-        double us = work / n * ceil(n / (cus * c.per_cu));
+        const double slots = cus * c.per_cu, full = floor(n / slots), left = n - full * slots, mean = work / n;
+        double us = mean * ceil(n / slots);
         us = us > longest ? us : longest;
-        if (i == 0 || us < least) least = us, best = i;
+        if (i == 0 || us < least) least = us, best = Way{i, false};
+        if (i == 0 && full >= 1 && left > 0) {
+            us = mean * full + quarter * ceil(4 * left / (cus * COSTS[1].per_cu)) + LAUNCH;
+            if (us < least) least = us, best = Way{i, true};
+        }
     }
     return best;
 }
@@ -565,28 +622,37 @@ static void run(List& l, const Update& u, const theseus_newton_schulz* ns, uint8
     momentum_norm<<<prefix(l, [](const Matrix& x) { return (long)x.pieces; }), 256, 0, st>>>(l, u, sums);
     const unsigned scale = prefix(l, [](const Matrix& x) { return ceil_div((long)x.mp * x.np, PIECE); });
     scale_split<<<scale, 256, 0, st>>>(l, u, sums);
-    const int sg = shape(l, 0, true, cus), ss = shape(l, 0, false, cus), su = shape(l, 1, false, cus);
-    auto with = [](int which, auto go) {
-        if (which == 0) go(Large{});
-        else if (which == 1) go(Middle{});
-        else go(Small{});
+    const Way wg = way(l, true, true, cus), ws2 = way(l, true, false, cus), wu = way(l, false, false, cus);
+    // one product: go(shape, workgroups, span)
+    auto with = [&](const Way& w, bool lower, auto go) {
+        const Cost& c = COSTS[w.shape];
+        const int total = (int)prefix(l, [&](const Matrix& x) { return tiles(x, lower, c.side); });
+        auto part = [&](int shape, const Span& s) {
+            const int slots = cus * COSTS[shape].per_cu / 8 * 8;
+            const unsigned n = s.count < slots || slots == 0 ? s.count : slots;
+            if (shape == 0) go(Large{}, n, s);
+            else if (shape == 1) go(Middle{}, n, s);
+            else go(Small{}, n, s);
+        };
+        const int slots = cus * c.per_cu, full = w.quarters ? total / slots * slots : total;
+        part(w.shape, Span{0, full, false});
+        if (full < total) part(w.shape + 1, Span{full, 4 * (total - full), true});
     };
     for (int i = 0; i < ns->steps; i++) {
         const int now = i & 1;
-        with(sg, [&](auto s) {
-            using S = decltype(s);
-            const unsigned n = prefix(l, [&](const Matrix& x) { return tiles(x, 0, COSTS[sg].side); });
-            gram<typename S::KK, typename S::NN><<<n, 512, 0, st>>>(l, now);
+        with(wg, true, [&](auto shape, unsigned n, const Span& s) {
+            using S = decltype(shape);
+            gram<typename S::KK, typename S::NN><<<n, 512, 0, st>>>(l, s, now);
         });
-        with(ss, [&](auto s) {
-            using S = decltype(s);
-            const unsigned n = prefix(l, [&](const Matrix& x) { return tiles(x, 0, COSTS[ss].side); });
-            square<typename S::KK><<<n, 512, 0, st>>>(l, ns->b, ns->c);
+        with(ws2, true, [&](auto shape, unsigned n, const Span& s) {
+            using S = decltype(shape);
+            square<typename S::KK><<<n, 512, 0, st>>>(l, s, ns->a, ns->b, ns->c);
         });
-        with(su, [&](auto s) {
-            using S = decltype(s);
-            const unsigned n = prefix(l, [&](const Matrix& x) { return tiles(x, 1, COSTS[su].side); });
-            update<typename S::KN, typename S::KK><<<n, 512, 0, st>>>(l, u, now, i + 1 == ns->steps, ns->a);
+        with(wu, false, [&](auto shape, unsigned n, const Span& s) {
+            using S = decltype(shape);
+            if (i + 1 == ns->steps) update<typename S::KN, typename S::KK, LAST><<<n, 512, 0, st>>>(l, s, u, now, ns->a);
+            else if (i + 2 == ns->steps) update<typename S::KN, typename S::KK, FIRST><<<n, 512, 0, st>>>(l, s, u, now, ns->a);
+            else update<typename S::KN, typename S::KK, BOTH><<<n, 512, 0, st>>>(l, s, u, now, ns->a);
         });
     }
 }
