@@ -367,8 +367,10 @@ template <class P> __global__ __launch_bounds__(512) void square(List l, Span s,
                     const float2 x0 = floats_of(v[tn][tm].x), x1 = floats_of(v[tn][tm].y);
                     const f32x4_t& z = g.acc[tn][tm];
                     float y[4] = {b * x0.x + cs * z[0], b * x0.y + cs * z[1], b * x1.x + cs * z[2], b * x1.y + cs * z[3]};
+                    if (t.m0 == t.n0) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] += m + 16 * tm == n + 16 * tn + e ? as : 0.f;
+                        for (int e = 0; e < 4; e++) y[e] += m + 16 * tm == n + 16 * tn + e ? as : 0.f;
+                    }
                     v[tn][tm] = make_uint2(half2_of(y[0], y[1]), half2_of(y[2], y[3]));
                 }
             store_both<P>(lds, v, x.square(), pp, t.m0, t.n0);
@@ -505,14 +507,20 @@ template <int BM, int WM, int WN, int NST> struct Shape {
 };
 using Large = Shape<256, 4, 2, 2>;
 using Middle = Shape<128, 4, 2, 2>;
+using Deep = Shape<128, 4, 2, 4>;
 using Small = Shape<64, 2, 4, 4>;
-// side, workgroups on a CU, us of a step of 64 along the contraction and of the rest
+// Side, workgroups on a CU; us of a step of 64 along the contraction where few workgroups run and where all do
+// (they share the caches and the power), of the rest of a tile, and what a square's or an update's epilogue adds.
+// From squares of 256 .. 4096, 192, 352 and 512 x 5120 and 4096, each made in all four: Gram matrices of
+// 768 x 768 take 23, 12, 11 and 7 us, of 2048 x 2048 44, 24, 19 and 24, of 192 x 5120 89, 48, 35 and 22, of four of
+// 5120 x 5120 522 in tiles of 256 with the last round in quarters; updates of 2048 x 2048 52, 31, 27 and 53.
 struct Cost {
     int side, per_cu;
-    double step, fixed;
+    double few, full, rest, epilogue;
 };
 constexpr double LAUNCH = 4;  // us of one more launch
-constexpr Cost COSTS[] = {{256, 1, 1.6, 8}, {128, 2, 1.05, 5}, {64, 2, .5, 3}};
+constexpr Cost COSTS[] = {{256, 1, 1.1, 1.75, 7, 8}, {128, 2, .56, 1.15, 5, 2}, {128, 1, .36, .6, 5, 2}, {64, 2, .2, .68, 4.5, 1}};
+constexpr int SHAPES = sizeof COSTS / sizeof *COSTS;
 
 static int device_cus() {
     int dev = 0, n = 0;
@@ -574,28 +582,34 @@ static long tiles(const Matrix& x, bool lower, int side) {
 // quarters of its tiles.
 struct Way {
     int shape;
-    bool quarters;  // the tiles behind the last full round
+    bool quarters;  // the tiles behind the last full round, in the next shape
 };
 static Way way(const List& l, bool lower, bool gram, int cus) {
-    Way best{0, false};
-    double least = 0;
-    for (int i = 0; i < 3; i++) {
-        const Cost& c = COSTS[i];
-        double work = 0, longest = 0, n = 0, quarter = 0;
+    // us of `count` of the list's tiles in a shape, as many as there are slots at once
+    auto round = [&](const Cost& c, double count) {
+        const double load = count / (cus * c.per_cu), step = c.few + (c.full - c.few) * (load < 1 ? load : 1);
+        double sum = 0, n = 0, longest = 0;
         for (int k = 0; k < l.count; k++) {
             const Matrix& x = l.x[k];
-            const double steps = (gram ? (x.tall() ? x.mp : x.np) : x.pp()) / BK, t = c.fixed + steps * c.step, w = (double)tiles(x, lower, c.side);
-            const double q = i < 2 ? COSTS[i + 1].fixed + steps * COSTS[i + 1].step : 0;
-            work += t * w, n += w;
-            longest = longest > t ? longest : t, quarter = quarter > q ? quarter : q;
+            const double w = (double)tiles(x, lower, c.side), t = c.rest + (gram ? 0 : c.epilogue) + step * (gram ? (x.tall() ? x.mp : x.np) : x.pp()) / BK;
+            sum += w * t, n += w;
+            longest = longest > t ? longest : t;
         }
-        const double slots = cus * c.per_cu, full = floor(n / slots), left = n - full * slots, mean = work / n;
-        double us = mean * ceil(n / slots);
-        us = us > longest ? us : longest;
+        return load < 1 ? longest : sum / n;
+    };
+    Way best{0, false};
+    double least = 0;
+    for (int i = 0; i < SHAPES; i++) {
+        const Cost& c = COSTS[i];
+        double n = 0;
+        for (int k = 0; k < l.count; k++) n += (double)tiles(l.x[k], lower, c.side);
+        const double slots = cus * c.per_cu, full = floor(n / slots), left = n - full * slots, rounds = full ? full * round(c, slots) : 0;
+        const double us = rounds + (left ? round(c, left) : 0);
         if (i == 0 || us < least) least = us, best = Way{i, false};
-        if (i == 0 && full >= 1 && left > 0) {
-            us = mean * full + quarter * ceil(4 * left / (cus * COSTS[1].per_cu)) + LAUNCH;
-            if (us < least) least = us, best = Way{i, true};
+        if (i == 0 && full && left) {
+            const double q = cus * COSTS[1].per_cu, many = floor(4 * left / q), few = 4 * left - many * q;
+            const double in4 = rounds + LAUNCH + (many ? many * round(COSTS[1], q) : 0) + (few ? round(COSTS[1], few) : 0);
+            if (in4 < least) least = in4, best = Way{i, true};
         }
     }
     return best;
@@ -632,6 +646,7 @@ static void run(List& l, const Update& u, const theseus_newton_schulz* ns, uint8
             const unsigned n = s.count < slots || slots == 0 ? s.count : slots;
             if (shape == 0) go(Large{}, n, s);
             else if (shape == 1) go(Middle{}, n, s);
+            else if (shape == 2) go(Deep{}, n, s);
             else go(Small{}, n, s);
         };
         const int slots = cus * c.per_cu, full = w.quarters ? total / slots * slots : total;
