@@ -39,9 +39,9 @@ typedef struct theseus_newton_schulz {
 } theseus_newton_schulz;
 
 typedef struct theseus_orthogonalize_matrix {
-    const void* x;          /* [rows][cols], row_stride >= cols elements from row to row       */
+    const void* x;          /* [rows][cols], row_stride elements from row to row               */
     void* out;              /* bfloat16 [rows][cols], contiguous                               */
-    long long row_stride;
+    long long row_stride;   /* cols .. 2^21 (of one row: not used)                             */
     int rows, cols;         /* 0 .. 2^17 (0: skipped)                                          */
     int dtype;              /* theseus_muon_dtype of x                                         */
 } theseus_orthogonalize_matrix;

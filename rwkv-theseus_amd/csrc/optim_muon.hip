@@ -25,6 +25,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "optim_norm.h"
 #include "vocab_gemm.h"
 
@@ -82,11 +84,11 @@ __device__ __forceinline__ float2 floats_of(uint32_t u) {
     const h2 h = __builtin_bit_cast(h2, u);
     return make_float2((float)h[0], (float)h[1]);
 }
-// x, y -> hi; what that rounds away, times LO -> lo
-__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+// x, y -> hi; what that rounds away, times BY -> lo
+template <int BY = (int)LO> __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
     hi = half2_of(x, y);
     const float2 h = floats_of(hi);
-    lo = half2_of((x - h.x) * LO, (y - h.y) * LO);
+    lo = half2_of((x - h.x) * BY, (y - h.y) * BY);
 }
 
 // ------------------------------------------------------------------------------ u, its norm, X_0
@@ -496,6 +498,338 @@ template <class PW, class PT, Stage ST> __global__ __launch_bounds__(512) void u
     });
 }
 
+// ------------------------------------------------------------------------------ short sides up to 128
+// A list without longer ones takes one launch a step.  X^T lies in the workspace as [q][P] in its two halves, P = 64
+// or 128.  A workgroup has a run of 16-row strips of it and a part of A from each of the run's
+// workgroups before: it adds the parts, forms B in LDS, and its waves take two strips each,
+//
+//   Y = B X           B's rows from LDS, X's columns (the strips' rows) as they lie in memory
+//
+// whose halves go to memory and the first one to LDS as well, from where the waves make a part of the next A, each a
+// row of tiles of its lower triangle, reading Y^T along its columns (LDS transpose reads).  Operands are
+// float16 as above, here with X's second half in the product too; X and B are scaled apart, so that this half
+// is no subnormal (X by 64, A by 64^2, B by 1024).  More workgroups shorten the strips' time and lengthen the
+// parts'.
+constexpr int SHORT = 128;
+constexpr int ALONE = 16;  // strips that one workgroup takes, all steps but the first in one launch
+constexpr float SX = 64.f, SB = 1024.f;
+
+template <int P> struct Few {
+    static constexpr int T = P / 16, TILES = T * (T + 1) / 2;
+    static constexpr int LD = P + 8;         // 16 bytes more: rows on other banks
+    static constexpr int HALVES = 8 / T;     // P = 64: two waves for a row of tiles, half of the strips each
+    static constexpr int Y = P * LD * 2;     // behind B: Y^T of 16 strips,
+    static constexpr int TURN = Y + 256 * LD * 2;        // the second halves of a strip for each wave
+    static constexpr int LDS = TURN + 8 * 16 * LD * 2;
+};
+// tile (i, j) of a lower triangle, row after row
+__device__ __forceinline__ constexpr int lower(int i, int j) { return i * (i + 1) / 2 + j; }
+
+struct FewArgs {
+    float a, b, c;
+    int steps;
+    int from, to;  // the steps of this launch: 0 makes X_0 and its A, 1 .. steps the products
+    const double* sums;
+};
+
+// A strip's elements in a matrix, for Y's accumulators d[t][e] (row 16 t + 4 q + e, column r16 of the strip).  Four
+// consecutive ones at once where they are (a tall matrix of whole tiles); else by byte offsets from the strip's first
+// element, behind the buffer for those that there are not.  (2^30 bytes: 128 rows of up to 2^21 elements.)
+template <int T> struct Strip {
+    static constexpr uint32_t BYTES = 1u << 30;
+    uint8_t* base;
+    uint32_t si, sj, first;
+    int rows, size;  // rows: from this lane's first
+    bool column, fours;
+    __device__ __forceinline__ Strip(const void* m, bool tall, int p, int len, int j0, long ld, int size, int r16, int q) : size(size) {
+        base = static_cast<uint8_t*>(const_cast<void*>(m)) + (tall ? j0 * ld : j0) * size;
+        si = (tall ? 1 : (int)ld) * size, sj = (tall ? (int)ld : 1) * size;
+        rows = p - 4 * q, column = j0 + r16 < len, fours = tall && p % 16 == 0;
+        first = 4 * q * si + r16 * sj;
+    }
+    __device__ __forceinline__ uint32_t at(int i, int j) const { return column && 16 * i + j < rows ? first + (16 * i + j) * si : 2 * BYTES; }
+    __device__ __forceinline__ void all(f32x4_t (&d)[T], bool fp32) const {
+        const auto of = wkv7::make_rsrc(base, BYTES);
+        if (fours) {
+            const uint8_t* from = base + (column ? first : 0);  // (what is not there: the strip's first ones, and left out)
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                const uint8_t* v = from + (16 * t < rows ? 16 * t * si : 0);
+                if (fp32) {
+                    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+                    const f4 y = *reinterpret_cast<const f4*>(v);
+                    d[t] = f32x4_t{y[0], y[1], y[2], y[3]};
+                } else {
+                    typedef uint16_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+                    const u4 y = *reinterpret_cast<const u4*>(v);
+                    d[t] = f32x4_t{bf16_to_f32(y[0]), bf16_to_f32(y[1]), bf16_to_f32(y[2]), bf16_to_f32(y[3])};
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < T; t++)
+                if (!column || 16 * t >= rows) d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        } else {
+#pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    d[t][e] = fp32 ? __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(of, at(t, e), 0, 0))
+                                   : bf16_to_f32(__builtin_amdgcn_raw_buffer_load_b16(of, at(t, e), 0, 0));
+        }
+    }
+    __device__ __forceinline__ void put(const f32x4_t (&d)[T], bool fp32) const {
+        const auto of = wkv7::make_rsrc(base, BYTES);
+        if (fours) {
+            if (!column) return;
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                if (16 * t >= rows) break;
+                uint8_t* v = base + first + 16 * t * si;
+                if (fp32) {
+                    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+                    *reinterpret_cast<f4*>(v) = f4{d[t][0], d[t][1], d[t][2], d[t][3]};
+                } else {
+                    typedef uint32_t u2 __attribute__((ext_vector_type(2), aligned(2)));
+                    *reinterpret_cast<u2*>(v) = u2{f32x2_to_bf16x2(d[t][0], d[t][1]), f32x2_to_bf16x2(d[t][2], d[t][3])};
+                }
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (fp32) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(d[t][e]), of, at(t, e), 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b16(wkv7::f32_to_bf16(d[t][e]), of, at(t, e), 0, 0);
+        }
+    }
+};
+
+// START: step 0, X_0 and its A from the call's matrix; else steps from .. to.
+template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, Update u, FewArgs f) {
+    using F = Few<P>;
+    constexpr int T = F::T, LD = F::LD;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[F::LDS];
+    __shared__ double red[8];
+    if (skipped(u)) return;
+    uint16_t *mat = reinterpret_cast<uint16_t*>(lds), *yt = reinterpret_cast<uint16_t*>(lds + F::Y);  // A, then B; Y^T
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int k = which(l, blockIdx.x), groups = l.first[k + 1] - l.first[k], group = blockIdx.x - l.first[k];
+    const Matrix& x = l.x[k];
+    const bool tall = x.tall();
+    const int p = tall ? x.n : x.m, len = tall ? x.m : x.n, strips = (len + 15) / 16, per = (strips + groups - 1) / groups;
+    const int first = group * per, last = min(first + per, strips);
+    uint16_t *xhi = x.ws, *xlo = xhi + (long)strips * 16 * P;                     // [q][P]
+    float* parts = reinterpret_cast<float*>(xlo + (long)strips * 16 * P);         // [2][groups][HALVES][TILES][64][4]
+    constexpr int PART = F::TILES * 256;
+    const float factor = u.result ? u.result[1] : u.factor;
+
+    for (int step = f.from; step <= f.to; step++) {
+        float by = 1.f / SB;
+        if constexpr (START) {  // the norm
+            double sum = 0;
+            for (int j = threadIdx.x; j < x.pieces; j += 512) sum += f.sums[x.piece0 + j];
+            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            if ((threadIdx.x & 63) == 0) red[wave] = sum;
+            __syncthreads();
+            sum = 0;
+            for (int w = 0; w < 8; w++) sum += red[w];
+            const double norm = sqrt(sum);
+            by = (float)(SX / (norm < u.eps ? (double)u.eps : norm));
+        } else {  // A's parts in order, A, B
+            const int count = groups * F::HALVES;
+            const float* from = parts + (long)((step - 1) & 1) * count * PART + 4 * threadIdx.x;
+            constexpr int MINE = (F::TILES * 64 + 511) / 512, BATCH = 40 / MINE < 8 ? 40 / MINE : 8;
+            f32x4_t s[MINE];
+#pragma unroll
+            for (int r = 0; r < MINE; r++) s[r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int g0 = 0; g0 < count; g0 += BATCH) {  // (a batch in flight, added one after the other)
+                f32x4_t v[BATCH][MINE];
+#pragma unroll
+                for (int g = 0; g < BATCH; g++)
+#pragma unroll
+                    for (int r = 0; r < MINE; r++)
+                        v[g][r] = *reinterpret_cast<const f32x4_t*>(from + (long)min(g0 + g, count - 1) * PART + (threadIdx.x + 512 * r < F::TILES * 64 ? 2048 * r : 0));
+#pragma unroll
+                for (int g = 0; g < BATCH; g++)
+#pragma unroll
+                    for (int r = 0; r < MINE; r++) s[r] = g0 + g < count ? s[r] + v[g][r] : s[r];
+            }
+#pragma unroll
+            for (int r = 0; r < MINE; r++) {
+                const int v = threadIdx.x + 512 * r;
+                if (v >= F::TILES * 64) break;
+                const int tile = v >> 6, rr = v & 15, qq = (v >> 4) & 3;
+                int i = 0;
+#pragma unroll
+                for (int n = 1; n < T; n++) i += tile >= lower(n, 0);
+                const int j = tile - lower(i, 0), row = 16 * i + 4 * qq, col = 16 * j + rr;
+                const uint2 h = make_uint2(half2_of(s[r][0], s[r][1]), half2_of(s[r][2], s[r][3]));
+                *reinterpret_cast<uint2*>(mat + col * LD + row) = h;
+                if (i != j) {
+                    mat[row * LD + col] = (uint16_t)h.x, mat[(row + 1) * LD + col] = (uint16_t)(h.x >> 16);
+                    mat[(row + 2) * LD + col] = (uint16_t)h.y, mat[(row + 3) * LD + col] = (uint16_t)(h.y >> 16);
+                }
+            }
+            __syncthreads();
+            // wave w: rows 16 (w % T) .., of P = 64 half of the columns each
+            const int lane = thread_here() & 63, r16 = lane & 15, q = lane >> 4;
+            constexpr int N = T / F::HALVES;
+            const int ti = wave % T, tj0 = wave / T * N;
+            f32x4_t acc[N];
+#pragma unroll
+            for (int n = 0; n < N; n++) acc[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < P / 32; ks++) {
+                const uint4 av = *reinterpret_cast<const uint4*>(mat + (16 * ti + r16) * LD + 32 * ks + 8 * q);
+#pragma unroll
+                for (int n = 0; n < N; n++)
+                    acc[n] = wkv7::mma32h(acc[n], av, *reinterpret_cast<const uint4*>(mat + (16 * (tj0 + n) + r16) * LD + 32 * ks + 8 * q));
+            }
+            const float fa = f.a * SB, fb = f.b * (SB / (SX * SX)), fc = f.c * (SB / (SX * SX * SX * SX));
+            uint2 b[N];
+#pragma unroll
+            for (int n = 0; n < N; n++) {  // (row 16 ti + 4 q + e, column 16 (tj0 + n) + r16; A from the mirrored place)
+                const int row = 16 * ti + 4 * q, col = 16 * (tj0 + n) + r16;
+                const uint2 av = *reinterpret_cast<const uint2*>(mat + col * LD + row);
+                const float2 a0 = floats_of(av.x), a1 = floats_of(av.y);
+                const float y[4] = {fb * a0.x + fc * acc[n][0], fb * a0.y + fc * acc[n][1], fb * a1.x + fc * acc[n][2], fb * a1.y + fc * acc[n][3]};
+                b[n] = make_uint2(half2_of(y[0] + (row == col ? fa : 0.f), y[1] + (row + 1 == col ? fa : 0.f)),
+                                  half2_of(y[2] + (row + 2 == col ? fa : 0.f), y[3] + (row + 3 == col ? fa : 0.f)));
+            }
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < N; n++) *reinterpret_cast<uint2*>(mat + (16 * (tj0 + n) + r16) * LD + 16 * ti + 4 * q) = b[n];
+            __syncthreads();
+        }
+        // 16 strips at a time
+        const int row = wave % T, half = wave / T;  // of the next A's tiles
+        f32x4_t gram[T];
+#pragma unroll
+        for (int t = 0; t < T; t++) gram[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int s0 = first; s0 < last; s0 += 16) {
+            const int lane = thread_here() & 63, r16 = lane & 15, q = lane >> 4;
+            const int strip = s0 + 2 * wave, have = min(last - strip, 2);
+            // (a wave without a second strip makes the first one again, and leaves it out)
+            auto strip_of = [&](int s) { return min(strip + s, last - 1); };
+            auto make = [&] {
+            f32x4_t d[2][T];
+            if constexpr (START) {
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const int j0 = 16 * strip_of(s);
+                    const Strip<T> src(x.src, tall, p, len, j0, x.ld, x.fp32 ? 4 : 2, r16, q);
+                    src.all(d[s], x.fp32);
+                    if (x.momentum) {
+                        const Strip<T> mom(x.momentum, tall, p, len, j0, x.n, 4, r16, q);
+                        f32x4_t m[T];
+                        mom.all(m, true);
+#pragma unroll
+                        for (int t = 0; t < T; t++) d[s][t] = u.nesterov ? u.mu * m[t] + (1.f - u.mu) * (d[s][t] * factor) : m[t];
+                    }
+                }
+            } else {
+                uint4 xh[2][P / 32], xl[2][P / 32];
+#pragma unroll
+                for (int s = 0; s < 2; s++)
+#pragma unroll
+                    for (int ks = 0; ks < P / 32; ks++) {
+                        const int at = (16 * strip_of(s) + r16) * P + 32 * ks + 8 * q;
+                        xh[s][ks] = *reinterpret_cast<const uint4*>(xhi + at);
+                        xl[s][ks] = *reinterpret_cast<const uint4*>(xlo + at);
+                    }
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    d[0][t] = d[1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int ks = 0; ks < P / 32; ks++) {
+                        const uint4 b = *reinterpret_cast<const uint4*>(mat + (16 * t + r16) * LD + 32 * ks + 8 * q);
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            d[s][t] = wkv7::mma32h(d[s][t], b, xh[s][ks]);
+                            d[s][t] = wkv7::mma32h(d[s][t], b, xl[s][ks]);
+                        }
+                    }
+                }
+                if (step == f.steps) {
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        if (s >= have) break;
+                        const Strip<T> dst(x.dst, tall, p, len, 16 * (strip + s), x.n, x.momentum ? 4 : 2, r16, q);
+                        const float to = by / SX, step_by = x.step * to;
+                        if (x.momentum) {
+                            f32x4_t w[T];
+                            dst.all(w, true);
+#pragma unroll
+                            for (int t = 0; t < T; t++) d[s][t] = w[t] * x.keep - step_by * d[s][t];
+                        } else {
+#pragma unroll
+                            for (int t = 0; t < T; t++) d[s][t] *= to;
+                        }
+                        dst.put(d[s], x.momentum);
+                    }
+                    return;
+                }
+            }
+            // whole rows of X^T to memory through LDS, the first halves staying there
+            uint16_t* turn = reinterpret_cast<uint16_t*>(lds + F::TURN) + wave * 16 * LD;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                uint16_t* mine = yt + (32 * wave + 16 * s) * LD;
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    uint2 h, o;
+                    split<1>(d[s][t][0] * by, d[s][t][1] * by, h.x, o.x);
+                    split<1>(d[s][t][2] * by, d[s][t][3] * by, h.y, o.y);
+                    if (s >= have) h = make_uint2(0, 0);
+                    *reinterpret_cast<uint2*>(mine + r16 * LD + 16 * t + 4 * q) = h;
+                    *reinterpret_cast<uint2*>(turn + r16 * LD + 16 * t + 4 * q) = o;
+                }
+                wkv7::wave_lds_fence();
+                constexpr int CH = P / 8;
+#pragma unroll
+                for (int v = 0; v < 16 * CH / 64; v++) {
+                    const int j = (64 * v + lane) / CH, col = 8 * ((64 * v + lane) % CH), at = (16 * (strip + s) + j) * P + col;
+                    const uint4 h = *reinterpret_cast<const uint4*>(mine + j * LD + col), o = *reinterpret_cast<const uint4*>(turn + j * LD + col);
+                    if (s < have) {
+                        *reinterpret_cast<uint4*>(xhi + at) = h;
+                        *reinterpret_cast<uint4*>(xlo + at) = o;
+                    }
+                }
+                wkv7::wave_lds_fence();
+            }
+            };
+            if (s0 > first) __syncthreads();  // (the strips before are still read)
+            if (have > 0) make();
+            if (!START && step == f.steps) continue;
+            __syncthreads();
+            // (lane: rows 4 q + (r16 >> 2) and 16 behind of 32 of Y^T, four columns, turned by the read)
+            const uint16_t* at = yt + (4 * q + (r16 >> 2)) * LD + 4 * (r16 & 3);
+            const int pairs = (min(last - s0, 16) + 1) / 2;  // (of strips: rows beyond the last one's are zero)
+            auto frag = [&](int ks, int t) {
+                const uint2 lo = wkv7::tr_at(at + 32 * ks * LD + 16 * t), hi = wkv7::tr_at(at + (32 * ks + 16) * LD + 16 * t);
+                return make_uint4(lo.x, lo.y, hi.x, hi.y);
+            };
+#pragma unroll 4
+            for (int ks = half; ks < pairs; ks += F::HALVES) {
+                const uint4 a = frag(ks, row);
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    if (t > row) break;
+                    gram[t] = wkv7::mma32h(gram[t], a, frag(ks, t));
+                }
+            }
+        }
+        if (!START && step == f.steps) return;
+        f32x4_t* to = reinterpret_cast<f32x4_t*>(parts + (((long)(step & 1) * groups + group) * F::HALVES + half) * PART) + (thread_here() & 63);
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            if (t > row) break;
+            to[lower(row, t) * 64] = gram[t];
+        }
+        __syncthreads();  // (a workgroup alone goes on with the next step: its parts and X are read by other waves)
+    }
+}
+
 // ------------------------------------------------------------------------------ host
 static long up(long x, long to) { return (x + to - 1) / to * to; }
 static long ceil_div(long x, long y) { return (x + y - 1) / y; }
@@ -530,6 +864,22 @@ static int device_cus() {
 
 constexpr size_t MOST = 4ull << 30;  // bytes of the matrices of a launch together, if it has more than one
 
+// A matrix of a list of short sides: strips, and workgroups where `matrices` share the card: two
+// strips for each wave, more where the parts of so many workgroups take longer.
+static bool is_short(int m, int n) { return (m < n ? m : n) <= SHORT; }
+static long strips_of(const Matrix& x) { return ceil_div(x.m < x.n ? x.n : x.m, 16); }
+static long groups_of(const Matrix& x, int matrices) {
+    const long strips = strips_of(x), share = 256 / matrices > 1 ? 256 / matrices : 1;
+    if (strips <= ALONE) return 1;
+    long n = 1;
+    while (n * n < 2 * strips) n++;
+    const long pairs = ceil_div(strips, 16);
+    n = n < pairs ? n : pairs, n = n < share ? n : share;
+    return ceil_div(strips, ceil_div(strips, n));  // (none without strips)
+}
+static size_t short_bytes(const Matrix& x) {  // (beside any others)
+    return up(strips_of(x) * 16 * SHORT * 4 + 2 * groups_of(x, 1) * Few<SHORT>::TILES * 1024, 256);  // (P = 64: two parts of 10 KB each, less)
+}
 static size_t bytes_of(const Matrix& x) { return 2 * (4 * (size_t)x.mp * x.np + 2 * (size_t)x.pp() * x.pp()); }
 
 static Matrix matrix(int m, int n) {
@@ -543,14 +893,22 @@ static Matrix matrix(int m, int n) {
     return x;
 }
 
+// Whether a call has short sides alone (beside longer ones they take part in the products' launches).
+template <class Get> static bool only_short(int count, Get get) {
+    for (int i = 0; i < count; i++) {
+        const Matrix x = get(i);
+        if (x.m && x.n && !is_short(x.m, x.n)) return false;
+    }
+    return true;
+}
 // The list's matrices from `next` on that one set of launches takes.
-template <class Get> static bool take(int count, int& next, Get get, List& l, size_t& bytes, long& pieces) {
+template <class Get> static bool take(int count, int& next, Get get, bool all_short, List& l, size_t& bytes, long& pieces) {
     l.count = 0;
     bytes = 0, pieces = 0;
     while (next < count && l.count < MAX) {
         Matrix x = get(next);
         if (x.m && x.n) {
-            const size_t size = bytes_of(x);
+            const size_t size = all_short ? short_bytes(x) : bytes_of(x);
             if (l.count && bytes + size > MOST) break;
             x.piece0 = (int)pieces;
             pieces += x.pieces;
@@ -568,7 +926,8 @@ template <class Get> static size_t workspace(int count, Get get) {
     long pieces;
     int next = 0;
     List l;
-    while (take(count, next, get, l, bytes, pieces)) most = most > bytes + sums_bytes(pieces) ? most : bytes + sums_bytes(pieces);
+    const bool all_short = only_short(count, get);
+    while (take(count, next, get, all_short, l, bytes, pieces)) most = most > bytes + sums_bytes(pieces) ? most : bytes + sums_bytes(pieces);
     return most;
 }
 
@@ -625,15 +984,32 @@ template <class Set> static unsigned prefix(List& l, Set groups) {
     return (unsigned)at;
 }
 
-static void run(List& l, const Update& u, const theseus_newton_schulz* ns, uint8_t* ws, long pieces, hipStream_t st) {
+static void run(List& l, const Update& u, const theseus_newton_schulz* ns, bool all_short, uint8_t* ws, long pieces, hipStream_t st) {
     double* sums = reinterpret_cast<double*>(ws);
     uint8_t* at = ws + sums_bytes(pieces);
     for (int k = 0; k < l.count; k++) {
         l.x[k].ws = reinterpret_cast<uint16_t*>(at);
-        at += bytes_of(l.x[k]);
+        at += all_short ? short_bytes(l.x[k]) : bytes_of(l.x[k]);
     }
     const int cus = device_cus();
     momentum_norm<<<prefix(l, [](const Matrix& x) { return (long)x.pieces; }), 256, 0, st>>>(l, u, sums);
+    if (all_short) {
+        int longest = 0;
+        for (int k = 0; k < l.count; k++) {
+            const int p = l.x[k].m < l.x[k].n ? l.x[k].m : l.x[k].n;
+            longest = longest > p ? longest : p;
+        }
+        const unsigned n = prefix(l, [&](const Matrix& x) { return groups_of(x, l.count); });
+        const int each = (int)n == l.count ? ns->steps : 1;  // (a workgroup a matrix: all steps at once)
+        auto go = [&](auto P) {
+            few<decltype(P)::value, true><<<n, 512, 0, st>>>(l, u, FewArgs{ns->a, ns->b, ns->c, ns->steps, 0, 0, sums});
+            for (int i = 1; i <= ns->steps; i += each)
+                few<decltype(P)::value, false><<<n, 512, 0, st>>>(l, u, FewArgs{ns->a, ns->b, ns->c, ns->steps, i, i + each - 1, sums});
+        };
+        if (longest <= 64) go(std::integral_constant<int, 64>{});
+        else go(std::integral_constant<int, SHORT>{});
+        return;
+    }
     const unsigned scale = prefix(l, [](const Matrix& x) { return ceil_div((long)x.mp * x.np, PIECE); });
     scale_split<<<scale, 256, 0, st>>>(l, u, sums);
     const Way wg = way(l, true, true, cus), ws2 = way(l, true, false, cus), wu = way(l, false, false, cus);
@@ -678,11 +1054,12 @@ static int check(const theseus_newton_schulz* ns) {
         return THESEUS_WKV7_ERR_SHAPE;
     return THESEUS_WKV7_OK;
 }
+constexpr long long MAX_STRIDE = 1ll << 21;  // elements from row to row, in 32-bit byte offsets within a strip
 static bool fits(long long m, long long n) { return m >= 0 && n >= 0 && m <= 1 << 17 && n <= 1 << 17; }
 
 static Matrix get_orth(const theseus_orthogonalize_matrix& s) {
     Matrix x = matrix(s.rows, s.cols);
-    x.src = s.x, x.ld = s.row_stride, x.dst = s.out, x.fp32 = s.dtype == THESEUS_MUON_FP32;
+    x.src = s.x, x.ld = s.rows > 1 ? s.row_stride : s.cols, x.dst = s.out, x.fp32 = s.dtype == THESEUS_MUON_FP32;
     return x;
 }
 static Matrix get_muon(const theseus_muon_matrix& s) {
@@ -695,7 +1072,7 @@ static int check(const theseus_orthogonalize_matrix* ms, int count) {
     if (count && !ms) return THESEUS_WKV7_ERR_NULL;
     for (int i = 0; i < count; i++) {
         const theseus_orthogonalize_matrix& s = ms[i];
-        if (!fits(s.rows, s.cols) || (s.rows > 1 && s.row_stride < s.cols)) return THESEUS_WKV7_ERR_SHAPE;
+        if (!fits(s.rows, s.cols) || (s.rows > 1 && (s.row_stride < s.cols || s.row_stride > MAX_STRIDE))) return THESEUS_WKV7_ERR_SHAPE;
         if (s.dtype != THESEUS_MUON_BF16 && s.dtype != THESEUS_MUON_FP32) return THESEUS_WKV7_ERR_DTYPE;
         if (s.rows && s.cols && (!s.x || !s.out)) return THESEUS_WKV7_ERR_NULL;
     }
@@ -749,7 +1126,8 @@ int theseus_orthogonalize(const theseus_orthogonalize_matrix* ms, int count, con
     size_t bytes;
     long pieces;
     int next = 0;
-    while (muon::take(count, next, get, l, bytes, pieces)) muon::run(l, u, ns, static_cast<uint8_t*>(workspace), pieces, stream);
+    const bool all_short = muon::only_short(count, get);
+    while (muon::take(count, next, get, all_short, l, bytes, pieces)) muon::run(l, u, ns, all_short, static_cast<uint8_t*>(workspace), pieces, stream);
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }
 
@@ -778,7 +1156,8 @@ int theseus_muon_step(const theseus_muon_matrix* ms, int count, const theseus_ne
     size_t bytes;
     long pieces;
     int next = 0;
-    while (muon::take(count, next, get, l, bytes, pieces)) muon::run(l, u, ns, static_cast<uint8_t*>(workspace), pieces, stream);
+    const bool all_short = muon::only_short(count, get);
+    while (muon::take(count, next, get, all_short, l, bytes, pieces)) muon::run(l, u, ns, all_short, static_cast<uint8_t*>(workspace), pieces, stream);
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }
 

@@ -188,7 +188,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
 # ------------------------------------------------------------------------------ orthogonalised updates
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # of the usual five steps: singular values to 0.68 .. 1.21 in few of them
-_MAX_SIDE = 1 << 17
+_MAX_SIDE, _MAX_STRIDE = 1 << 17, 1 << 21  # include/theseus_muon.h
 
 
 def _schulz(steps, coefficients, eps):
@@ -243,7 +243,7 @@ def orthogonalize(x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
             continue
         m, n = t.shape[-2:]
         t = t.detach().reshape(-1, m, n)
-        if t.stride(2) != 1 and n > 1 or t.stride(1) < n and m > 1:
+        if t.stride(2) != 1 and n > 1 or m > 1 and not n <= t.stride(1) <= _MAX_STRIDE:
             t = t.contiguous()
         held.append(t)  # (until the call has been made)
         apart, size, at, to = t.stride(0) * t.element_size(), 2 * m * n, t.data_ptr(), out.data_ptr()
