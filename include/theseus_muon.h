@@ -65,7 +65,7 @@ int theseus_orthogonalize(const theseus_orthogonalize_matrix* matrices, int coun
  * not finite (may be NULL where max_norm < 0).  With skip_nonfinite such a norm leaves every param
  * and momentum unchanged. */
 size_t theseus_muon_workspace_size(const theseus_muon_matrix* matrices, int count);
-int theseus_muon_step(const theseus_muon_matrix* matrices, int count, const theseus_newton_schulz* ns, float momentum,
+int theseus_muon_step(const theseus_muon_matrix* matrices, int count, const theseus_newton_schulz* ns, double momentum,
                       int nesterov, float grad_scale, float max_norm, int skip_nonfinite, float* result, void* workspace,
                       size_t workspace_bytes, hipStream_t stream);
 

@@ -93,7 +93,7 @@ template <int BY = (int)LO> __device__ __forceinline__ void split(float x, float
 
 // ------------------------------------------------------------------------------ u, its norm, X_0
 struct Update {
-    float mu;
+    float mu, nu;  // momentum, and 1 - momentum
     int nesterov;
     float factor;         // of the gradients, where result is null
     const float* result;  // of the norm pass: the factor, and whether nothing may change
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void momentum_norm(List l, Update u, double* _
             load8(m, x.momentum, at, count, true);
             for (int e = 0; e < 8; e++) {
                 g[e] *= f;
-                m[e] = u.mu * m[e] + (1.f - u.mu) * g[e];
+                m[e] = u.mu * m[e] + u.nu * g[e];
             }
             if (count >= 8) {
                 Eight<float>::type v;
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256) void momentum_norm(List l, Update u, double* _
             } else {
                 for (int e = 0; e < count; e++) x.momentum[at + e] = m[e];
             }
-            for (int e = 0; e < 8; e++) g[e] = u.nesterov ? u.mu * m[e] + (1.f - u.mu) * g[e] : m[e];
+            for (int e = 0; e < 8; e++) g[e] = u.nesterov ? u.mu * m[e] + u.nu * g[e] : m[e];
         }
         for (int e = 0; e < 8; e++) sum += (double)g[e] * g[e];
     }
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void scale_split(List l, Update u, const doubl
         if (x.momentum) {
             float m[8];
             load8(m, x.momentum, row * x.n + col, count, true);
-            for (int e = 0; e < 8; e++) g[e] = u.nesterov ? u.mu * m[e] + (1.f - u.mu) * (g[e] * f) : m[e];
+            for (int e = 0; e < 8; e++) g[e] = u.nesterov ? u.mu * m[e] + u.nu * (g[e] * f) : m[e];
         }
         uint4 hi, lo;
         split(g[0] * by, g[1] * by, hi.x, lo.x);
@@ -724,7 +724,7 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
                         f32x4_t m[T];
                         mom.all(m, true);
 #pragma unroll
-                        for (int t = 0; t < T; t++) d[s][t] = u.nesterov ? u.mu * m[t] + (1.f - u.mu) * (d[s][t] * factor) : m[t];
+                        for (int t = 0; t < T; t++) d[s][t] = u.nesterov ? u.mu * m[t] + u.nu * (d[s][t] * factor) : m[t];
                     }
                 }
             } else {
@@ -1120,8 +1120,9 @@ int theseus_orthogonalize(const theseus_orthogonalize_matrix* ms, int count, con
     if (int e = muon::check(ms, count)) return e;
     auto get = [&](int i) { return muon::get_orth(ms[i]); };
     const size_t need = muon::workspace(count, get);
-    if (need && (!workspace || workspace_bytes < need)) return THESEUS_WKV7_ERR_WORKSPACE;
-    const muon::Update u{0.f, 0, 1.f, nullptr, 0, ns->eps};
+    if (!need) return THESEUS_WKV7_OK;
+    if (!workspace || workspace_bytes < need) return THESEUS_WKV7_ERR_WORKSPACE;
+    const muon::Update u{0.f, 1.f, 0, 1.f, nullptr, 0, ns->eps};
     muon::List l;
     size_t bytes;
     long pieces;
@@ -1137,7 +1138,7 @@ size_t theseus_muon_workspace_size(const theseus_muon_matrix* ms, int count) {
     return norm > step ? norm : step;
 }
 
-int theseus_muon_step(const theseus_muon_matrix* ms, int count, const theseus_newton_schulz* ns, float momentum, int nesterov,
+int theseus_muon_step(const theseus_muon_matrix* ms, int count, const theseus_newton_schulz* ns, double momentum, int nesterov,
                       float grad_scale, float max_norm, int skip_nonfinite, float* result, void* workspace, size_t workspace_bytes,
                       hipStream_t stream) {
     if (int e = muon::check(ns)) return e;
@@ -1145,12 +1146,13 @@ int theseus_muon_step(const theseus_muon_matrix* ms, int count, const theseus_ne
     const bool norm = max_norm >= 0.f;
     if (norm && !result) return THESEUS_WKV7_ERR_NULL;
     const size_t need = theseus_muon_workspace_size(ms, count);
+    if (!need && !norm) return THESEUS_WKV7_OK;
     if (need && (!workspace || workspace_bytes < need)) return THESEUS_WKV7_ERR_WORKSPACE;
     if (norm) {
         double* partial = static_cast<double*>(workspace);
         optim::launch_norm(partial, muon::norm_pass(ms, count, partial, stream), grad_scale, max_norm, result, stream);
     }
-    const muon::Update u{momentum, nesterov, grad_scale, norm ? result : nullptr, skip_nonfinite, ns->eps};
+    const muon::Update u{(float)momentum, (float)(1.0 - momentum), nesterov, grad_scale, norm ? result : nullptr, skip_nonfinite, ns->eps};
     auto get = [&](int i) { return muon::get_muon(ms[i]); };
     muon::List l;
     size_t bytes;

@@ -74,7 +74,7 @@ def _lib():
         lib.theseus_orthogonalize.restype = i32
         lib.theseus_muon_workspace_size.argtypes = [ctypes.POINTER(_Matrix), i32]
         lib.theseus_muon_workspace_size.restype = sz
-        lib.theseus_muon_step.argtypes = [ctypes.POINTER(_Matrix), i32, ctypes.POINTER(_Schulz), f32, i32, f32, f32, i32, vp, vp, sz, vp]
+        lib.theseus_muon_step.argtypes = [ctypes.POINTER(_Matrix), i32, ctypes.POINTER(_Schulz), ctypes.c_double, i32, f32, f32, i32, vp, vp, sz, vp]
         lib.theseus_muon_step.restype = i32
         _bound = True
     return lib
