@@ -318,6 +318,83 @@ template <class P> __device__ __forceinline__ void store_both(uint8_t* lds, cons
     }
 }
 
+// 64 x 64 tiles, for products of few tiles, whose steps are as long as their waits: four waves of 32 x 32 on each
+// half of a step, their sums added at the end, and a step's fragments are read a whole step ahead, so that
+// a step has one wait in which the reads, the matrix instructions and the barrier run together (353 x 1021:
+// 0.25 us a step with eight waves on the tile, half steps one after the other).  Interface and layouts of Product;
+// one tile a call.
+template <int NST_, Lay LX_, Lay LY_> struct Slim {
+    static constexpr int BM = 64, BN = 64, WM = 2, WN = 2, NST = NST_, TM = 2, TN = 2;
+    static constexpr Lay LX = LX_, LY = LY_;
+    static constexpr bool PERM = LX == RowN || LY == RowN;
+    static constexpr int STAGE = (BM + BN) * BK * 2, EPILOGUE = 8 * TN * 512, SUMS = 4 * TM * TN * 1024;
+    static constexpr int LDS = NST * STAGE, THREADS = 512, PIECES = 2;
+    static_assert(SUMS + EPILOGUE <= LDS && NST >= 3, "stages");
+    f32x4_t acc[TN][TM];
+
+    __device__ static __forceinline__ uint8_t* epilogue(uint8_t* lds) { return lds + SUMS; }
+
+    template <bool, class Next, class Done>
+    __device__ __forceinline__ void go(uint8_t* lds, const Operand& X, const Operand& Y, Place at, Next, Done done) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2;
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+        Loader<LX, BM, PERM> lx(X, at.m0, at.step0 * BK, wave, lane);
+        Loader<LY, BN, PERM> ly(Y, at.n0, at.step0 * BK, wave, lane);
+        const Reader<LX, BM, PERM> rx((wave >> 1 & 1) * 32, lane);
+        const Reader<LY, BN, PERM> ry((wave & 1) * 32, lane);
+        auto load = [&](int stage, bool more) {
+            lx.issue(lds0 + stage * STAGE, 0, wave);
+            ly.issue(lds0 + stage * STAGE + BM * BK * 2, 0, wave);
+            lx.advance(more), ly.advance(more);
+        };
+#pragma unroll
+        for (int s = 0; s < NST; s++) load(s, s + 1 < at.steps);
+#pragma unroll
+        for (int tn = 0; tn < TN; tn++)
+#pragma unroll
+            for (int tm = 0; tm < TM; tm++) acc[tn][tm] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        struct Fragments {
+            uint4 x[TM], y[TN];
+        } a, b;
+        auto read = [&](Fragments& f, int stage) {
+#pragma unroll
+            for (int i = 0; i < TM; i++) f.x[i] = rx.get(lds, stage * STAGE, i, half);
+#pragma unroll
+            for (int i = 0; i < TN; i++) f.y[i] = ry.get(lds, stage * STAGE + BM * BK * 2, i, half);
+        };
+        int cur = 0;
+        auto step = [&](const Fragments& now, Fragments& then, int s) {
+            // the next stage has landed, and every wave has this one's fragments
+            wait_barrier<(NST - 2) * PIECES>();
+            const int next = cur + 1 == NST ? 0 : cur + 1;
+            load(cur, s + NST + 1 < at.steps);
+            read(then, next);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int tn = 0; tn < TN; tn++)
+#pragma unroll
+                for (int tm = 0; tm < TM; tm++) acc[tn][tm] = wkv7::mma32h(acc[tn][tm], now.y[tn], now.x[tm]);
+            cur = next;
+        };
+        wait_barrier<(NST - 1) * PIECES>();
+        read(a, 0);
+        int s = 0;
+        for (; s + 1 < at.steps; s += 2) step(a, b, s), step(b, a, s + 1);
+        if (s < at.steps) step(a, b, s);
+        wkv7::vm_wait_n<0>();
+        __syncthreads();
+        f32x4_t* sums = reinterpret_cast<f32x4_t*>(lds) + (wave & 3) * (TM * TN * 64) + lane;
+        if (half)
+#pragma unroll
+            for (int t = 0; t < TM * TN; t++) sums[64 * t] = acc[t / TM][t % TM];
+        __syncthreads();
+        if (half) return;
+#pragma unroll
+        for (int t = 0; t < TM * TN; t++) acc[t / TM][t % TM] += sums[64 * t];
+        done(at);
+    }
+};
+
 template <class P> __device__ __forceinline__ uint2 halves(const P& g, int tn, int tm) {
     const f32x4_t& a = g.acc[tn][tm];
     return make_uint2(half2_of(a[0], a[1]), half2_of(a[2], a[3]));
@@ -842,7 +919,11 @@ template <int BM, int WM, int WN, int NST> struct Shape {
 using Large = Shape<256, 4, 2, 2>;
 using Middle = Shape<128, 4, 2, 2>;
 using Deep = Shape<128, 4, 2, 4>;
-using Small = Shape<64, 2, 4, 4>;
+struct Small {
+    using KK = Slim<4, RowK, RowK>;
+    using NN = Slim<4, RowN, RowN>;
+    using KN = Slim<4, RowK, RowN>;
+};
 // Side, workgroups on a CU; us of a step of 64 along the contraction where few workgroups run and where all do
 // (they share the caches and the power), of the rest of a tile, and what a square's or an update's epilogue adds.
 // From squares of 256 .. 4096, 192, 352 and 512 x 5120 and 4096, each made in all four: Gram matrices of
