@@ -39,10 +39,11 @@ using wkv7::f32x2_to_bf16x2;
 constexpr int MAX = 32;         // matrices of a launch
 constexpr int TOGETHER = 1024;  // rows of a product whose tiles run together
 constexpr int PIECE = 8192;     // elements of a workgroup of the norm's pass
+constexpr int SPLITS = 8;       // of A's contraction at most
 constexpr float LO = 2048.f;    // of X's second half, so that it is no subnormal
 
 // One matrix.  Its part of the workspace: X hi, X lo, the next X hi and lo ([mp][np] each, zero
-// beyond m and n), A and B ([pp][pp], pp the padded short side).
+// beyond m and n), A and B ([pp][pp], pp the padded short side), and where A has few tiles SPLITS parts of it.
 struct Matrix {
     const void* src;  // the gradient, or X
     long ld;          // of src
@@ -61,6 +62,7 @@ struct Matrix {
     __device__ uint16_t* lo(int which) const { return hi(which) + size(); }
     __device__ uint16_t* gram() const { return ws + 4 * size(); }
     __device__ uint16_t* square() const { return gram() + (long)pp() * pp(); }
+    __device__ float* parts() const { return reinterpret_cast<float*>(square() + (long)pp() * pp()); }  // of A, where it is split
 };
 struct List {
     int count;
@@ -207,7 +209,8 @@ __global__ __launch_bounds__(256) void scale_split(List l, Update u, const doubl
 // both operands.
 struct Span {
     int from, count;
-    bool quarters;  // of tiles of twice the side
+    bool quarters;   // of tiles of twice the side
+    int splits = 1;  // parts of each tile's contraction, one after the other
 };
 __device__ __forceinline__ int number_of(const Span& s, int t) {
     const int each = s.count >> 3;
@@ -241,15 +244,18 @@ __device__ __forceinline__ void any_tile(int TM, int TN, int G, int k, int& i, i
 __device__ __forceinline__ int tiles_of(int x, int by) { return (x + by - 1) / by; }
 
 struct Tile {
-    int matrix, m0, n0;
+    int matrix, m0, n0, part, number;  // number: in its matrix
     bool none;  // a quarter beyond the matrix, or above the diagonal
 };
 template <int SIDE, bool LOWER> __device__ __forceinline__ Tile tile_at(const List& l, const Span& s, int t) {
     int id = number_of(s, t), part = 0;
-    if (s.quarters) part = id & 3, id >>= 2;
-    id += s.from;
     Tile r;
+    r.part = 0;
+    if (s.quarters) part = id & 3, id >>= 2;
+    else if (s.splits > 1) r.part = id % s.splits, id /= s.splits;
+    id += s.from;
     r.matrix = which(l, id);
+    r.number = id - l.first[r.matrix];
     const Matrix& x = l.x[r.matrix];
     const int side = s.quarters ? 2 * SIDE : SIDE, M = LOWER ? x.pp() : x.mp, N = LOWER ? M : x.np;
     int i, j;
@@ -271,7 +277,7 @@ template <int SIDE, bool LOWER, class Make> __device__ __forceinline__ void each
                 const int then = t + gridDim.x;
                 if (steps <= NST || then >= s.count) return false;
                 const Tile to = tile_at<SIDE, LOWER>(l, s, then);
-                if (to.matrix != at.matrix || to.none) return false;
+                if (to.matrix != at.matrix || to.none || s.splits > 1) return false;
                 t = then;
                 p = Place{to.m0, to.n0, 0, steps};
                 return true;
@@ -407,7 +413,18 @@ template <class PW, class PT> __global__ __launch_bounds__(512) void gram(List l
         auto go = [&](auto tag, const Operand& o, int inner) {
             using P = decltype(tag);
             P g;
-            g.template go<false>(lds, o, o, Place{at.m0, at.n0, 0, inner / BK}, more(inner / BK, P::NST), [&](const Place& t) {
+            const int all = inner / BK, each = (all + s.splits - 1) / s.splits, first = at.part * each;
+            // (a part without steps makes one of zeros: from the last step, times nothing)
+            g.template go<false>(lds, o, o, Place{at.m0, at.n0, min(first, all - 1), max(min(each, all - first), 0)}, more(each, P::NST), [&](const Place& t) {
+                if (s.splits > 1) {
+                    const int thread = thread_here();
+                    f32x4_t* to = reinterpret_cast<f32x4_t*>(x.parts()) + ((long)at.number * s.splits + at.part) * (P::BM * P::BN / 4) + (thread >> 6) * (P::TM * P::TN * 64) + (thread & 63);
+#pragma unroll
+                    for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+                        for (int tm = 0; tm < P::TM; tm++) to[(tn * P::TM + tm) * 64] = g.acc[tn][tm];
+                    return;
+                }
                 uint2 v[P::TN][P::TM];
 #pragma unroll
                 for (int tn = 0; tn < P::TN; tn++)
@@ -419,6 +436,35 @@ template <class PW, class PT> __global__ __launch_bounds__(512) void gram(List l
         if (x.tall()) go(PT{}, Operand{x.hi(now), x.np, x.np, x.mp}, x.mp);
         else go(PW{}, Operand{x.hi(now), x.np, x.mp, x.np}, x.np);
     });
+}
+
+// A's parts added in order: a workgroup a tile, whose accumulators lie as gram's waves left them
+template <class P> __global__ __launch_bounds__(256) void sum_gram(List l, Span s) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS];
+    const int splits = s.splits;
+    s.splits = 1;
+    const Tile at = tile_at<P::BM, true>(l, s, blockIdx.x);
+    const Matrix& x = l.x[at.matrix];
+    const f32x4_t* from = reinterpret_cast<const f32x4_t*>(x.parts()) + (long)at.number * splits * (P::BM * P::BN / 4) + (threadIdx.x >> 6) * (P::TM * P::TN * 64) + (threadIdx.x & 63);
+    f32x4_t v[SPLITS][P::TM * P::TN];
+#pragma unroll
+    for (int k = 0; k < SPLITS; k++)
+#pragma unroll
+        for (int t = 0; t < P::TM * P::TN; t++) v[k][t] = from[(long)min(k, splits - 1) * (P::BM * P::BN / 4) + t * 64];
+    P g;
+#pragma unroll
+    for (int t = 0; t < P::TM * P::TN; t++) {
+        f32x4_t sum = v[0][t];
+#pragma unroll
+        for (int k = 1; k < SPLITS; k++) sum = k < splits ? sum + v[k][t] : sum;
+        g.acc[t / P::TM][t % P::TM] = sum;
+    }
+    uint2 h[P::TN][P::TM];
+#pragma unroll
+    for (int tn = 0; tn < P::TN; tn++)
+#pragma unroll
+        for (int tm = 0; tm < P::TM; tm++) h[tn][tm] = halves(g, tn, tm);
+    store_both<P>(lds, h, x.gram(), x.pp(), at.m0, at.n0);
 }
 
 // s^2 (a I + b A + c A^2) of A, with s^2 A in memory
@@ -927,14 +973,14 @@ struct Small {
 // Side, workgroups on a CU; us of a step of 64 along the contraction where few workgroups run and where all do
 // (they share the caches and the power), of the rest of a tile, and what a square's or an update's epilogue adds.
 // From squares of 256 .. 4096, 192, 352 and 512 x 5120 and 4096, each made in all four: Gram matrices of
-// 768 x 768 take 23, 12, 11 and 7 us, of 2048 x 2048 44, 24, 19 and 24, of 192 x 5120 89, 48, 35 and 22, of four of
-// 5120 x 5120 522 in tiles of 256 with the last round in quarters; updates of 2048 x 2048 52, 31, 27 and 53.
+// 768 x 768 take 23, 12, 11 and 7 us, of 2048 x 2048 44, 24, 19 and 23, of 192 x 5120 89, 48, 33 and 18, of four of
+// 5120 x 5120 522 in tiles of 256 with the last round in quarters; updates of 2048 x 2048 52, 31, 27 and 43.
 struct Cost {
     int side, per_cu;
     double few, full, rest, epilogue;
 };
 constexpr double LAUNCH = 4;  // us of one more launch
-constexpr Cost COSTS[] = {{256, 1, 1.1, 1.75, 7, 8}, {128, 2, .56, 1.15, 5, 2}, {128, 1, .36, .6, 5, 2}, {64, 2, .2, .68, 4.5, 1}};
+constexpr Cost COSTS[] = {{256, 1, 1.1, 1.75, 7, 8}, {128, 2, .56, 1.15, 5, 2}, {128, 1, .36, .6, 5, 2}, {64, 2, .17, .52, 4.2, 1}};
 constexpr int SHAPES = sizeof COSTS / sizeof *COSTS;
 
 static int device_cus() {
@@ -961,7 +1007,16 @@ static long groups_of(const Matrix& x, int matrices) {
 static size_t short_bytes(const Matrix& x) {  // (beside any others)
     return up(strips_of(x) * 16 * SHORT * 4 + 2 * groups_of(x, 1) * Few<SHORT>::TILES * 1024, 256);  // (P = 64: two parts of 10 KB each, less)
 }
-static size_t bytes_of(const Matrix& x) { return 2 * (4 * (size_t)x.mp * x.np + 2 * (size_t)x.pp() * x.pp()); }
+// A's contraction is split where its tiles of 64 leave CUs idle: up to this many tiles
+constexpr long SPLIT_TILES = 128;
+static bool splits(const Matrix& x) {
+    const long p = x.pp() / 64;
+    return p * (p + 1) / 2 <= SPLIT_TILES;
+}
+static size_t bytes_of(const Matrix& x) {
+    const size_t p = x.pp() / 64;
+    return 2 * (4 * (size_t)x.mp * x.np + 2 * (size_t)x.pp() * x.pp()) + (splits(x) ? p * (p + 1) / 2 * SPLITS * 64 * 64 * 4 : 0);
+}
 
 static Matrix matrix(int m, int n) {
     Matrix x{};
@@ -1022,16 +1077,17 @@ static long tiles(const Matrix& x, bool lower, int side) {
 // quarters of its tiles.
 struct Way {
     int shape;
-    bool quarters;  // the tiles behind the last full round, in the next shape
+    bool quarters;   // the tiles behind the last full round, in the next shape
+    int splits = 1;  // of every tile's contraction, added by a launch of its own
 };
 static Way way(const List& l, bool lower, bool gram, int cus) {
     // us of `count` of the list's tiles in a shape, as many as there are slots at once
-    auto round = [&](const Cost& c, double count) {
+    auto round = [&](const Cost& c, double count, int splits = 1) {
         const double load = count / (cus * c.per_cu), step = c.few + (c.full - c.few) * (load < 1 ? load : 1);
         double sum = 0, n = 0, longest = 0;
         for (int k = 0; k < l.count; k++) {
             const Matrix& x = l.x[k];
-            const double w = (double)tiles(x, lower, c.side), t = c.rest + (gram ? 0 : c.epilogue) + step * (gram ? (x.tall() ? x.mp : x.np) : x.pp()) / BK;
+            const double w = (double)tiles(x, lower, c.side), t = c.rest + (gram ? 0 : c.epilogue) + step * ceil((gram ? (x.tall() ? x.mp : x.np) : x.pp()) / BK / (double)splits);
             sum += w * t, n += w;
             longest = longest > t ? longest : t;
         }
@@ -1050,6 +1106,14 @@ static Way way(const List& l, bool lower, bool gram, int cus) {
             const double q = cus * COSTS[1].per_cu, many = floor(4 * left / q), few = 4 * left - many * q;
             const double in4 = rounds + LAUNCH + (many ? many * round(COSTS[1], q) : 0) + (few ? round(COSTS[1], few) : 0);
             if (in4 < least) least = in4, best = Way{i, true};
+        }
+        if (i == SHAPES - 1 && gram) {
+            bool all = true;
+            for (int k = 0; k < l.count; k++) all &= splits(l.x[k]);
+            for (int k = 2; all && k <= SPLITS && n * k <= slots; k++) {
+                const double in = round(c, n * k, k) + LAUNCH + 2;
+                if (in < least) least = in, best = Way{i, false, k};
+            }
         }
     }
     return best;
@@ -1107,7 +1171,7 @@ static void run(List& l, const Update& u, const theseus_newton_schulz* ns, bool 
             else go(Small{}, n, s);
         };
         const int slots = cus * c.per_cu, full = w.quarters ? total / slots * slots : total;
-        part(w.shape, Span{0, full, false});
+        part(w.shape, Span{0, full * w.splits, false, w.splits});
         if (full < total) part(w.shape + 1, Span{full, 4 * (total - full), true});
     };
     for (int i = 0; i < ns->steps; i++) {
@@ -1115,6 +1179,8 @@ static void run(List& l, const Update& u, const theseus_newton_schulz* ns, bool 
         with(wg, true, [&](auto shape, unsigned n, const Span& s) {
             using S = decltype(shape);
             gram<typename S::KK, typename S::NN><<<n, 512, 0, st>>>(l, s, now);
+            if constexpr (std::is_same_v<S, Small>)
+                if (s.splits > 1) sum_gram<typename S::KK><<<(unsigned)(s.count / s.splits), 256, 0, st>>>(l, Span{0, s.count / s.splits, false, s.splits});
         });
         with(ws2, true, [&](auto shape, unsigned n, const Span& s) {
             using S = decltype(shape);
