@@ -71,10 +71,12 @@ struct List {
 };
 static_assert(sizeof(List) < 4000, "kernel arguments");
 
+// (all of them at once, a lane each: one wait instead of one a matrix)
 __device__ __forceinline__ int which(const List& l, int b) {
-    int i = 0;
-    while (i + 1 < l.count && l.first[i + 1] <= b) i++;
-    return i;
+    static_assert(MAX < 64, "lanes");
+    const int lane = threadIdx.x & 63, n = l.count;
+    if (n == 1) return 0;
+    return __builtin_popcountll(__ballot(lane < n && l.first[min(lane, MAX)] <= b)) - 1;
 }
 
 __device__ __forceinline__ uint32_t half2_of(float x, float y) {
