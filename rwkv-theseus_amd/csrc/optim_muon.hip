@@ -79,6 +79,7 @@ __device__ __forceinline__ int which(const List& l, int b) {
     return __builtin_popcountll(__ballot(lane < n && l.first[min(lane, MAX)] <= b)) - 1;
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint32_t half2_of(float x, float y) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, h2{(_Float16)x, (_Float16)y});
@@ -545,7 +546,12 @@ template <class P, Stage ST> __device__ __forceinline__ void update_done(P& g, u
     if constexpr (ST != LAST) fetch(0);
     auto put = [&](uint16_t* to) {
         return [&x, to, tm0, tn0](int i, int j, const uint4& v) {
-            if (tm0 + i < x.mp && tn0 + j < x.np) *reinterpret_cast<uint4*>(to + (long)(tm0 + i) * x.np + tn0 + j) = v;
+            if (tm0 + i >= x.mp || tn0 + j >= x.np) return;
+            u32x4* at = reinterpret_cast<u32x4*>(to + (long)(tm0 + i) * x.np + tn0 + j);
+            // (a large X does not stay cached until the next step: streamed, four of 5120 x 5120 1026 -> 1002 us;
+            // smaller ones are slower so, 768 x 768 23.9 -> 25.0)
+            if constexpr (P::BM == 256) __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, at);
+            else *at = u32x4{v.x, v.y, v.z, v.w};
         };
     };
 #pragma unroll
