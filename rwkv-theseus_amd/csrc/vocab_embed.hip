@@ -36,19 +36,18 @@ template <int N, typename T> struct Vec {
 template <typename T> struct Vec<1, T> {
     typedef T type;
 };
-template <int N> __device__ __forceinline__ void load(float (&x)[N], const uint16_t* p) {
-    const auto v = *reinterpret_cast<const typename Vec<N, uint16_t>::type*>(p);
-    if constexpr (N == 1) x[0] = bf16_to_f32(v);
+// ONCE: values that nobody reads again, past the caches
+template <int N, bool ONCE = false, typename T> __device__ __forceinline__ void load(float (&x)[N], const T* p) {
+    const auto* at = reinterpret_cast<const typename Vec<N, T>::type*>(p);
+    const auto v = ONCE ? __builtin_nontemporal_load(at) : *at;
+    auto value = [](auto y) {
+        if constexpr (sizeof(T) == 2) return bf16_to_f32(y);
+        else return y;
+    };
+    if constexpr (N == 1) x[0] = value(v);
     else
 #pragma unroll
-        for (int e = 0; e < N; e++) x[e] = bf16_to_f32(v[e]);
-}
-template <int N> __device__ __forceinline__ void load(float (&x)[N], const float* p) {
-    const auto v = *reinterpret_cast<const typename Vec<N, float>::type*>(p);
-    if constexpr (N == 1) x[0] = v;
-    else
-#pragma unroll
-        for (int e = 0; e < N; e++) x[e] = v[e];
+        for (int e = 0; e < N; e++) x[e] = value(v[e]);
 }
 template <int N> __device__ __forceinline__ void store(uint16_t* p, const float (&x)[N]) {
     if constexpr (N == 1) *p = f32_to_bf16(x[0]);
@@ -366,8 +365,9 @@ __global__ __launch_bounds__(256) void sum_runs(Runs s, const uint32_t* __restri
         for (int j = 0; j < BATCH; j++) {
             const long i = min(i0 + j, r.to - 1);
             key[j] = keys[i];
-            // (a token that adds nothing is not loaded: the run's first one is instead)
-            load<N>(x[j], grad + (long)(key[j] < s.V ? places[i] : places[r.from]) * s.ldg + col);
+            // (a token that adds nothing is not loaded: the run's first one is instead; streamed, 168 MB of
+            // them and the rest 239 -> 224 us)
+            load<N, true>(x[j], grad + (long)(key[j] < s.V ? places[i] : places[r.from]) * s.ldg + col);
         }
         key[BATCH] = keys[min(i0 + BATCH, s.M - 1)];
 #pragma unroll
@@ -529,7 +529,9 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
     auto at = [&](size_t off) { return reinterpret_cast<uint32_t*>(ws + off); };
     const Digits dg = digits(V);
     const Fill f{dweight, V * D * (weight_dtype == THESEUS_EMBED_BF16 ? 2l : 4l)};
-    const long want = ceil_div(f.bytes, THREADS * 16 * 4), fills = want < 1024 ? want : 1024;
+    // four stores a thread: enough workgroups that some are always starting (671 MB behind a sort of 16384 tokens, the whole
+    // gradient with its lookup: 281 us with 1024 of them, 242 with 8192, 239 so)
+    const long want = ceil_div(f.bytes, THREADS * 16 * 4), fills = want < 1 << 21 ? want : 1 << 21;
     const uint32_t *keys = at(p.keys), *places = at(p.places);
     if (M <= ONE) {
         auto sort = [&](auto rounds) {
