@@ -4,10 +4,11 @@ A frozen teacher and a student (embedding, one TimeMix layer, head) read the sam
 teacher's logits only each token's largest k and the row's log-sum-exp are kept (``top_logits``);
 the student learns from them (``linear_top_distillation``) and from the next tokens
 (``linear_cross_entropy``) without forming its own logits, its float32 parameters stepped by
-``FusedAdamW``.  Afterwards it is sampled from one token at a time, ``top_logits`` again on the
+``FusedAdamW`` (with --muon the layer's matrices by ``FusedMuon``), its tokens taken in by
+``embedding``.  Afterwards it is sampled from one token at a time, ``top_logits`` again on the
 logits of a step.
 
-    python examples/distill_student.py [--steps 30] [--vocab 8192] [--width 256]
+    python examples/distill_student.py [--steps 30] [--vocab 8192] [--width 256] [--muon]
 """
 import argparse
 import sys
@@ -18,9 +19,9 @@ from torch import nn
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "rwkv-theseus_amd"))
 
-from theseus.optim import FusedAdamW  # noqa: E402
+from theseus.optim import FusedAdamW, FusedMuon  # noqa: E402
 from theseus.timemix import TimeMix  # noqa: E402
-from theseus.vocab import linear_cross_entropy, linear_top_distillation, top_logits  # noqa: E402
+from theseus.vocab import embedding, linear_cross_entropy, linear_top_distillation, top_logits  # noqa: E402
 
 
 class Model(nn.Module):
@@ -33,18 +34,31 @@ class Model(nn.Module):
 
     def forward(self, ids, state=None):
         """Hidden states for the head [B,T,C] (bfloat16 under autocast) and the carried state."""
-        x = self.embed(ids).to(torch.bfloat16)
+        x = embedding(ids, self.embed.weight, dtype=torch.bfloat16)
         out, state = self.mix(x, state)
         return self.norm((x + out).float()).to(torch.bfloat16), state
 
 
-def distill(steps=30, vocab=8192, width=256, batch=4, tokens=128, k=32, temperature=2.0, share=.5, seed=0, device="cuda"):
+    def matrices(self):
+        """The layer's matrices: what an orthogonalised update is for."""
+        return [p for p in self.mix.parameters() if p.dim() == 2 and p is not self.mix.r_k]
+
+
+def optimizers(student, muon):
+    if not muon:
+        return [FusedAdamW(student.parameters(), lr=3e-3)]
+    matrices = student.matrices()
+    rest = [p for p in student.parameters() if all(p is not m for m in matrices)]
+    return [FusedMuon(matrices, lr=3e-3, scale="rms"), FusedAdamW(rest, lr=3e-3)]
+
+
+def distill(steps=30, vocab=8192, width=256, batch=4, tokens=128, k=32, temperature=2.0, share=.5, seed=0, device="cuda", muon=False):
     """Returns the student, and the first and last steps' (distillation, cross entropy) losses."""
     torch.manual_seed(seed)
     teacher = Model(vocab, width).to(device).requires_grad_(False)
     teacher.head.weight.mul_(8)  # (an untrained head's logits hardly differ: give the teacher opinions)
     student = Model(vocab, width).to(device)
-    opt = FusedAdamW(student.parameters(), lr=3e-3)
+    opts = optimizers(student, muon)
     ids = torch.randint(vocab, (batch, tokens + 1), device=device)
     losses = []
     for _ in range(steps):
@@ -56,8 +70,9 @@ def distill(steps=30, vocab=8192, width=256, batch=4, tokens=128, k=32, temperat
             kd = linear_top_distillation(h, student.head.weight, values, indices, temperature=temperature, teacher_lse=lse)
             ce = linear_cross_entropy(h, student.head.weight, ids[:, 1:])
         (share * kd + (1 - share) * ce).backward()
-        opt.step_after_backward(max_norm=1.0)
-        opt.zero_grad(set_to_none=True)
+        for opt in opts:
+            opt.step_after_backward(max_norm=1.0)
+            opt.zero_grad(set_to_none=True)
         losses.append((kd.detach(), ce.detach()))
     return student, [tuple(float(x) for x in losses[i]) for i in (0, -1)]
 
@@ -81,7 +96,8 @@ if __name__ == "__main__":
     ap.add_argument("--steps", type=int, default=30)
     ap.add_argument("--vocab", type=int, default=8192)
     ap.add_argument("--width", type=int, default=256)
+    ap.add_argument("--muon", action="store_true")
     a = ap.parse_args()
-    student, ((kd0, ce0), (kd1, ce1)) = distill(a.steps, a.vocab, a.width)
+    student, ((kd0, ce0), (kd1, ce1)) = distill(a.steps, a.vocab, a.width, muon=a.muon)
     print(f"distillation {kd0:.3f} -> {kd1:.3f}, cross entropy {ce0:.3f} -> {ce1:.3f} in {a.steps} steps")
     print("sampled:", sample(student, torch.zeros(1, dtype=torch.int64, device="cuda"), 16)[0].tolist())

@@ -1,6 +1,8 @@
 """A student's training step on the framework's own operators from its tokens to its updated weights: embedding,
 TimeMix layer, vocabulary loss, their gradients, FusedMuon for the layer's matrices and FusedAdamW for the rest."""
+import importlib.util
 import math
+from pathlib import Path
 
 import pytest
 import torch
@@ -103,3 +105,17 @@ def test_a_step_from_tokens_to_weights(vocab, width, batch, tokens):
     student.zero_grad(set_to_none=True)
     student.loss(ids, _own).backward()
     assert all(torch.isfinite(p.grad).all() for p in student.parameters())
+
+
+def test_the_example_runs_with_both_optimizers():
+    path = Path(__file__).resolve().parents[1] / "examples" / "distill_student.py"
+    spec = importlib.util.spec_from_file_location("distill_student", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    for muon in (False, True):
+        print(f"  example muon={muon}", flush=True)
+        student, losses = m.distill(steps=3, vocab=1000, width=128, batch=2, tokens=40, muon=muon)
+        assert all(math.isfinite(x) for pair in losses for x in pair)
+        assert all(torch.isfinite(p).all() for p in student.parameters())
+    ids = m.sample(student, torch.tensor([3, 5], device="cuda"), 3)
+    assert ids.shape == (2, 3) and int(ids.min()) >= 0 and int(ids.max()) < 1000
