@@ -13,13 +13,18 @@
 //
 // Numerics.  Operands are float16: bfloat16 has 8 times their rounding, and the polynomial magnifies
 // it (a Gaussian 768 x 768: 1.0e-2 from the exact result instead of 1.3e-3, where rounding the result
-// to bfloat16 costs 1.7e-3).  s, a power of two near sqrt(p), keeps their values (X near 1 / sqrt(q),
-// A near 1 after the first steps and s^2 / p before) inside float16's range.  Where u has few strong directions, rounding X itself
-// would add to it a matrix outside of its row and column spaces, which the polynomials raise by a
-// each step, 485 in five, while the strong directions stay at 1 (rank 64: 2.3e-2 off, rank 1:
-// 0.15).  Products with a rounded factor have their errors inside these spaces, which grow as X does; so
-// X is held in two halves, hi + lo / 2048, hi alone goes into the products, and both into a X: at most 1.7e-3 on all
-// spectra that were tried.
+// to bfloat16 costs 1.7e-3).  s, a power of two up to 32 near sqrt(p), keeps their values (X near 1 / sqrt(q), A near 1
+// after the first steps and s^2 / p before, B up to a s^2) inside float16's range.  Where u has few strong
+// directions, rounding X would add to it a matrix outside of its row and column spaces, which the polynomials
+// raise by a each step, 485 in five, while the strong directions stay at 1 (rank 64 of 768: 2.3e-2 off, rank 1:
+// 0.15).  The other roundings' errors lie inside one of these spaces and grow as X does.  So X is held in two
+// halves, hi + lo / 2048: hi goes into the products, a lo is added to the next X; only the last step's X, whose
+// rounding is raised 3.4 times at most, is hi alone.  At most 2.6e-3 on all spectra that were tried.
+//
+// What bounds it (the ten matrices of a layer of width 5120, a step in 10.84 ms).  The products' cores run at
+// 1.3 PFLOP/s, the card's power limit; a tile's end, in which all CUs write at once, is 9 % of a Gram matrix' time
+// (440 us of 522 in tiles of 256, without their ends 403), the last round the rest.  Small matrices are
+// bound by their launches, 4 to 5 us each with nothing to do, three a step.
 #include "../../include/theseus_muon.h"
 #include "../../include/theseus_wkv7.h"
 
@@ -38,7 +43,7 @@ using wkv7::f32x2_to_bf16x2;
 
 constexpr int MAX = 32;         // matrices of a launch
 constexpr int TOGETHER = 1024;  // rows of a product whose tiles run together
-constexpr int PIECE = 8192;     // elements of a workgroup of the norm's pass
+constexpr int PIECE = 2048;     // elements of a workgroup of the passes ahead of the products, `each` times
 constexpr int SPLITS = 8;       // of A's contraction at most
 constexpr float LO = 2048.f;    // of X's second half, so that it is no subnormal
 
@@ -51,7 +56,7 @@ struct Matrix {
     void* dst;        // float32 param, or bfloat16 out
     uint16_t* ws;
     int m, n, mp, np;  // and padded to steps of the products
-    int piece0, pieces;  // of the norm's partial sums
+    int piece0, pieces, each;  // of the norm's partial sums; PIECEs of a workgroup
     float s;
     float keep, step;
     int fp32;  // src
@@ -142,8 +147,8 @@ __global__ __launch_bounds__(256) void momentum_norm(List l, Update u, double* _
     const int per = (x.n + 7) / 8;
     const long all = (long)x.m * per;
     double sum = 0;
-    for (int j = 0; j < PIECE / 2048; j++) {
-        const long c = (long)k * (PIECE / 8) + j * 256 + threadIdx.x;
+    for (int j = 0; j < x.each; j++) {
+        const long c = ((long)k * x.each + j) * 256 + threadIdx.x;
         if (c >= all) break;
         const long row = c / per;
         const int col = (int)(c - row * per) * 8, count = x.n - col;
@@ -184,8 +189,8 @@ __global__ __launch_bounds__(256) void scale_split(List l, Update u, const doubl
     const float f = u.result ? u.result[1] : u.factor;
     const int per = x.np / 8;
     const long all = (long)x.mp * per;
-    for (int j = 0; j < PIECE / 2048; j++) {
-        const long c = (long)k * (PIECE / 8) + j * 256 + threadIdx.x;
+    for (int j = 0; j < x.each; j++) {
+        const long c = ((long)k * x.each + j) * 256 + threadIdx.x;
         if (c >= all) break;
         const long row = c / per;
         const int col = (int)(c - row * per) * 8, count = row < x.m ? x.n - col : 0;
@@ -769,22 +774,27 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
         } else {  // A's parts in order, A, B
             const int count = groups * F::HALVES;
             const float* from = parts + (long)((step - 1) & 1) * count * PART + 4 * threadIdx.x;
-            constexpr int MINE = (F::TILES * 64 + 511) / 512, BATCH = 40 / MINE < 8 ? 40 / MINE : 8;
+            constexpr int MINE = (F::TILES * 64 + 511) / 512;
             f32x4_t s[MINE];
 #pragma unroll
             for (int r = 0; r < MINE; r++) s[r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            for (int g0 = 0; g0 < count; g0 += BATCH) {  // (a batch in flight, added one after the other)
-                f32x4_t v[BATCH][MINE];
+            auto add = [&](auto batch) {  // (a batch in flight, added one after the other)
+                constexpr int BATCH = decltype(batch)::value;
+                for (int g0 = 0; g0 < count; g0 += BATCH) {
+                    f32x4_t v[BATCH][MINE];
 #pragma unroll
-                for (int g = 0; g < BATCH; g++)
+                    for (int g = 0; g < BATCH; g++)
 #pragma unroll
-                    for (int r = 0; r < MINE; r++)
-                        v[g][r] = *reinterpret_cast<const f32x4_t*>(from + (long)min(g0 + g, count - 1) * PART + (threadIdx.x + 512 * r < F::TILES * 64 ? 2048 * r : 0));
+                        for (int r = 0; r < MINE; r++)
+                            v[g][r] = *reinterpret_cast<const f32x4_t*>(from + (long)min(g0 + g, count - 1) * PART + (threadIdx.x + 512 * r < F::TILES * 64 ? 2048 * r : 0));
 #pragma unroll
-                for (int g = 0; g < BATCH; g++)
+                    for (int g = 0; g < BATCH; g++)
 #pragma unroll
-                    for (int r = 0; r < MINE; r++) s[r] = g0 + g < count ? s[r] + v[g][r] : s[r];
-            }
+                        for (int r = 0; r < MINE; r++) s[r] = g0 + g < count ? s[r] + v[g][r] : s[r];
+                }
+            };
+            if (groups == 1) add(std::integral_constant<int, F::HALVES>{});
+            else add(std::integral_constant<int, 10>{});
 #pragma unroll
             for (int r = 0; r < MINE; r++) {
                 const int v = threadIdx.x + 512 * r;
@@ -1032,7 +1042,8 @@ static Matrix matrix(int m, int n) {
     const int p = m < n ? m : n;
     x.s = 1.f;
     while (x.s < 32.f && 4.f * x.s * x.s <= (float)p) x.s *= 2.f;  // (a s^2 stays far below 65504)
-    x.pieces = (int)ceil_div((long)m * ceil_div(n, 8), PIECE / 8);
+    x.each = (long)m * n > 1 << 20 ? 4 : 1;  // (few elements: every load at once rather than few workgroups)
+    x.pieces = (int)ceil_div((long)m * ceil_div(n, 8), PIECE / 8 * x.each);
     x.ld = n;
     return x;
 }
@@ -1163,7 +1174,7 @@ static void run(List& l, const Update& u, const theseus_newton_schulz* ns, bool 
         else go(std::integral_constant<int, SHORT>{});
         return;
     }
-    const unsigned scale = prefix(l, [](const Matrix& x) { return ceil_div((long)x.mp * x.np, PIECE); });
+    const unsigned scale = prefix(l, [](const Matrix& x) { return ceil_div((long)x.mp * x.np, PIECE * x.each); });
     scale_split<<<scale, 256, 0, st>>>(l, u, sums);
     const Way wg = way(l, true, true, cus), ws2 = way(l, true, false, cus), wu = way(l, false, false, cus);
     // one product: go(shape, workgroups, span)
