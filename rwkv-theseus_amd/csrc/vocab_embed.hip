@@ -13,6 +13,7 @@
 //   sum_runs     a run of tokens x 256 threads of eight columns, eight tokens' rows in flight.
 //   add_parts    where a stretch begins that crosses runs: its parts in order.
 // More tokens are sorted by many workgroups: digit counts, their prefix sums, places, per digit.
+// Few tokens (up to 1024 of narrow rows, 256 of wide ones) take one launch, few_tokens.
 #include "../../include/theseus_embed.h"
 #include "../../include/theseus_wkv7.h"
 
@@ -426,9 +427,135 @@ __global__ __launch_bounds__(256) void add_parts(Runs s, const uint32_t* __restr
     store<N>(dweight + (long)key * s.D + col, sum);
 }
 
+// ------------------------------------------------------------------------------ few tokens
+// One launch, no workspace: a workgroup has `rows` of the table's rows, looks through all tokens for theirs, sorts
+// those few by counting, and writes each of its rows once, zeros or a sum.  `lanes` threads cover a row's columns (a
+// slab of 256 N of them), and the 256 / lanes groups of threads take the rows in turn; a row of more than ALONE
+// tokens is shared by the groups, their sums added in order: at most ALONE batches of BATCH tokens each.
+constexpr int MOST = 1024;  // tokens
+constexpr int ROWS = 256;   // of a workgroup
+constexpr int ALONE = 16, BATCH = 16;
+
+struct FewTokens {
+    int M;
+    long V, skip;
+    int D, rows, slabs, lanes;
+    long ldg;
+    float scale;
+};
+template <int N, typename G, typename W>
+__global__ __launch_bounds__(256) void few_tokens(FewTokens s, const int64_t* __restrict__ ids, const G* __restrict__ grad, W* __restrict__ dweight) {
+    __shared__ uint16_t place[MOST], row[MOST], sorted[MOST];
+    __shared__ int count[ROWS], start[ROWS];
+    __shared__ int found[MOST / 64];
+    __shared__ float parts[256 * N];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const long v0 = (long)(blockIdx.x / s.slabs) * s.rows;
+    const int rows = (int)min((long)s.rows, s.V - v0), slab = blockIdx.x % s.slabs;
+    // this workgroup's tokens, in their order
+    int mine[MOST / 256];
+    uint64_t votes[MOST / 256];
+#pragma unroll
+    for (int j = 0; j < MOST / 256; j++) {
+        const int i = 256 * j + t;
+        const int64_t id = i < s.M ? ids[i] : -1;
+        mine[j] = id >= v0 && id < v0 + rows && id != s.skip ? (int)(id - v0) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < MOST / 256; j++) {
+        votes[j] = __ballot(mine[j] >= 0);
+        if (lane == 0) found[4 * j + wave] = __popcll(votes[j]);
+    }
+    count[t] = 0;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < MOST / 64; k++) {
+        if ((k & 3) == wave && mine[k >> 2] >= 0) {
+            const int to = n + __popcll(votes[k >> 2] & ((1ull << lane) - 1));
+            place[to] = 256 * (k >> 2) + t, row[to] = mine[k >> 2];
+            atomicAdd(&count[mine[k >> 2]], 1);  // (counts: their order changes nothing)
+        }
+        n += found[k];
+    }
+    __syncthreads();
+    if (n) {
+        for (int r = t; r < rows; r += 256) {
+            int before = 0;
+            for (int k = 0; k < r; k++) before += count[k];
+            start[r] = before;
+        }
+        __syncthreads();
+        for (int i = t; i < n; i += 256) {
+            int before = start[row[i]];
+            for (int k = 0; k < i; k++) before += row[k] == row[i];
+            sorted[before] = place[i];
+        }
+        __syncthreads();
+    }
+    const int groups = 256 / s.lanes, group = t / s.lanes, at = t - group * s.lanes, chunk = slab * 256 + at;
+    const bool there = chunk * N < s.D;
+    const int col = column<N>(there ? chunk : 0, s.D);
+    auto sum_of = [&](float (&sum)[N], int from, int to) {
+#pragma unroll
+        for (int e = 0; e < N; e++) sum[e] = 0.f;
+        for (int i0 = from; i0 < to; i0 += BATCH) {
+            float x[BATCH][N];
+#pragma unroll
+            for (int j = 0; j < BATCH; j++) load<N, true>(x[j], grad + (long)sorted[min(i0 + j, to - 1)] * s.ldg + col);
+#pragma unroll
+            for (int j = 0; j < BATCH; j++)
+                if (i0 + j < to)
+#pragma unroll
+                    for (int e = 0; e < N; e++) sum[e] += x[j][e];
+        }
+    };
+    auto put = [&](int r, float (&sum)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; e++) sum[e] *= s.scale;
+        store<N>(dweight + (v0 + r) * s.D + col, sum);
+    };
+    if (there)
+        for (int r = group; r < rows; r += groups) {
+            float sum[N] = {};
+            if (count[r] == 0) store<N>(dweight + (v0 + r) * s.D + col, sum);
+            else if (count[r] <= ALONE) {
+                sum_of(sum, start[r], start[r] + count[r]);
+                put(r, sum);
+            }
+        }
+    if (n <= ALONE) return;
+    for (int r = 0; r < rows; r++) {
+        const int c = count[r];
+        if (c <= ALONE) continue;
+        const int each = (c + groups - 1) / groups, from = start[r] + min(group * each, c), to = start[r] + min(group * each + each, c);
+        float sum[N];
+        sum_of(sum, from, to);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < N; e++) parts[N * t + e] = sum[e];
+        __syncthreads();
+        if (group == 0 && there) {
+            for (int g = 1; g < groups; g++)
+#pragma unroll
+                for (int e = 0; e < N; e++) sum[e] += parts[N * (g * s.lanes + at) + e];
+            put(r, sum);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------ host
 static int check(long M, long V, int D) {
     return M < 0 || M > (1l << 30) || V < 1 || V > (1l << 22) || D < 1 || D > (1 << 17) ? THESEUS_WKV7_ERR_SHAPE : THESEUS_WKV7_OK;
+}
+template <class Go> static void with_types(int from, int to, Go go) {
+    if (from == THESEUS_EMBED_BF16) {
+        if (to == THESEUS_EMBED_BF16) go(uint16_t{}, uint16_t{});
+        else go(uint16_t{}, float{});
+    } else {
+        if (to == THESEUS_EMBED_BF16) go(float{}, uint16_t{});
+        else go(float{}, float{});
+    }
 }
 static bool known(int dtype) { return dtype == THESEUS_EMBED_BF16 || dtype == THESEUS_EMBED_FP32; }
 
@@ -458,6 +585,23 @@ static Plan plan(long M, long V, int D) {
     p.parts = take((size_t)p.runs * 2 * D * 4);
     p.bytes = at;
     return p;
+}
+
+// threads for a row's columns; whether few_tokens takes this many tokens
+static int lanes_of(int D) {
+    const long chunks = D >= 8 ? ceil_div(D, 8) : D;
+    int lanes = 1;
+    while (lanes < 256 && lanes < chunks) lanes *= 2;
+    return lanes;
+}
+static bool is_few(long M, int D) { return M <= MOST && M <= ALONE * BATCH * (256 / lanes_of(D)); }
+
+template <int N, typename G, typename W>
+static void launch_few(FewTokens s, const int64_t* ids, const void* grad, void* dweight, hipStream_t st) {
+    s.lanes = lanes_of(s.D), s.slabs = (int)ceil_div(ceil_div(s.D, N), 256);
+    const long share = ceil_div(s.V * s.slabs, 1024);  // (rows for about four workgroups on a CU)
+    s.rows = (int)(share < 1 ? 1 : share > ROWS ? ROWS : share);
+    few_tokens<N, G, W><<<(unsigned)(ceil_div(s.V, s.rows) * s.slabs), 256, 0, st>>>(s, ids, static_cast<const G*>(grad), static_cast<W*>(dweight));
 }
 
 template <int N, typename W, typename O>
@@ -501,18 +645,12 @@ int theseus_embed_lookup(long long M, long long V, int D, int weight_dtype, int 
         if (D >= 8) embed::launch_lookup<8, W, O>(M, V, D, ids, weight, weight_stride, scale, out, stream);
         else embed::launch_lookup<1, W, O>(M, V, D, ids, weight, weight_stride, scale, out, stream);
     };
-    if (weight_dtype == THESEUS_EMBED_BF16) {
-        if (out_dtype == THESEUS_EMBED_BF16) go(uint16_t{}, uint16_t{});
-        else go(uint16_t{}, float{});
-    } else {
-        if (out_dtype == THESEUS_EMBED_BF16) go(float{}, uint16_t{});
-        else go(float{}, float{});
-    }
+    embed::with_types(weight_dtype, out_dtype, go);
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }
 
 size_t theseus_embed_grad_workspace_size(long long M, long long V, int D) {
-    return embed::check(M, V, D) ? 0 : embed::plan(M, V, D).bytes;
+    return embed::check(M, V, D) || embed::is_few(M, D) ? 0 : embed::plan(M, V, D).bytes;
 }
 
 int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weight_dtype, const int64_t* ids, long long skip,
@@ -523,8 +661,18 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
     if (M > 1 && grad_stride != 0 && grad_stride < D) return THESEUS_WKV7_ERR_SHAPE;
     if (!known(grad_dtype) || !known(weight_dtype)) return THESEUS_WKV7_ERR_DTYPE;
     if (!dweight || (M && (!ids || !grad))) return THESEUS_WKV7_ERR_NULL;
+    if (is_few(M, D)) {
+        const FewTokens s{(int)M, V, skip, D, 0, 0, 0, grad_stride, scale};
+        with_types(grad_dtype, weight_dtype, [&](auto g, auto w) {
+            using G = decltype(g);
+            using W = decltype(w);
+            if (D >= 8) launch_few<8, G, W>(s, ids, grad, dweight, stream);
+            else launch_few<1, G, W>(s, ids, grad, dweight, stream);
+        });
+        return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
+    }
     const Plan p = plan(M, V, D);
-    if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return THESEUS_WKV7_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < p.bytes) return THESEUS_WKV7_ERR_WORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     auto at = [&](size_t off) { return reinterpret_cast<uint32_t*>(ws + off); };
     const Digits dg = digits(V);
@@ -553,7 +701,7 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
             q.keys_out = at(second ? p.keys2 : p.keys), q.places_out = at(second ? p.places2 : p.places);
         }
     }
-    if (M) {
+    {
         const Runs s{M, V, D, p.each, 0, grad_stride, scale};
         float* parts = reinterpret_cast<float*>(ws + p.parts);
         auto go = [&](auto g, auto w) {
@@ -562,13 +710,7 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
             if (D >= 8) launch_sums<8, G, W>(s, p.runs, keys, places, grad, parts, dweight, stream);
             else launch_sums<1, G, W>(s, p.runs, keys, places, grad, parts, dweight, stream);
         };
-        if (grad_dtype == THESEUS_EMBED_BF16) {
-            if (weight_dtype == THESEUS_EMBED_BF16) go(uint16_t{}, uint16_t{});
-            else go(uint16_t{}, float{});
-        } else {
-            if (weight_dtype == THESEUS_EMBED_BF16) go(float{}, uint16_t{});
-            else go(float{}, float{});
-        }
+        with_types(grad_dtype, weight_dtype, go);
     }
     return hipGetLastError() == hipSuccess ? THESEUS_WKV7_OK : THESEUS_WKV7_ERR_LAUNCH;
 }

@@ -55,7 +55,8 @@ def _grad_close(got, ids, up, V, scale, skip=None):
 
 # M, D, V: one token, no vector of eight, around a vector, around the sorts' sizes and the runs' ends
 SIZES = [(1, 1, 1), (1, 8, 5), (5, 7, 3), (17, 9, 40), (64, 64, 7), (33, 1001, 50), (2047, 12, 300), (2049, 20, 1000),
-         (16384, 8, 70), (16385, 16, 5000), (40001, 9, 130000), (300, 2050, 20), (70, 4104, 33)]
+         (16384, 8, 70), (16385, 16, 5000), (40001, 9, 130000), (300, 2050, 20), (70, 4104, 33),
+         (256, 3000, 12), (257, 3000, 12), (1023, 256, 2000), (1024, 64, 40), (1025, 64, 40), (512, 512, 700), (513, 512, 700), (900, 3, 70000)]
 
 
 @gpu
@@ -77,7 +78,7 @@ def test_rows_and_gradient_match_float64(M, D, V, wt, ot):
 
 @gpu
 @pytest.mark.parametrize("tokens", ["same", "falling", "1", "15", "16", "17", "31", "32", "48", "100"])
-@pytest.mark.parametrize("M", [15, 16, 17, 32, 33, 500, 5000, 40000])
+@pytest.mark.parametrize("M", [15, 16, 17, 32, 33, 500, 1024, 1025, 5000, 40000])
 def test_stretches_of_one_token_inside_and_across_runs(M, tokens):
     print(f"  stretches M={M} {tokens}", flush=True)
     V, D = 997, 10
@@ -321,10 +322,11 @@ def test_refusals_of_the_c_abi_before_launching():
         assert look(wt=a) == look(ot=a) == grad(gt=a) == grad(wt=a) == 2
     assert look(ids=None) == look(w=None) == look(out=None) == 3
     assert grad(ids=None) == grad(g=None) == grad(dw=None) == 3
-    need = lib.theseus_embed_grad_workspace_size(4, 9, 8)
-    assert need > 0 and grad(n=need - 1) == 4 and grad(ws=None) == 4
+    need = lib.theseus_embed_grad_workspace_size(4000, 9, 8)
+    assert need > 0 and grad(M=4000, n=need - 1) == 4 and grad(M=4000, ws=None) == 4
     assert look(M=0, ids=None, w=None, out=None) == 0
     assert lib.theseus_embed_grad_workspace_size(-1, 9, 8) == 0
+    assert lib.theseus_embed_grad_workspace_size(256, 65536, 5120) == 0  # (few tokens: one launch)
     sizes = [lib.theseus_embed_grad_workspace_size(M, 65536, 64) for M in (1, 100, 16384, 16385, 1 << 20)]
     assert sizes == sorted(sizes)
 
