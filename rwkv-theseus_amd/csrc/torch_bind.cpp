@@ -16,6 +16,8 @@
 #include <cstring>
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include "../../include/theseus_embed.h"
 #include "../../include/theseus_gdn_ex.h"
@@ -380,51 +382,57 @@ std::tuple<Tensor, Tensor, Tensor> vocab_top(const Tensor& x, int64_t k, double 
     return {values, indices, lse};
 }
 
-// theseus.vocab.embedding for a table w [V][D] with rows apart and ids [M], checked there.
-struct Embedding : torch::autograd::Function<Embedding> {
-    static int type(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 ? THESEUS_EMBED_BF16 : THESEUS_EMBED_FP32; }
-    static Tensor lookup(const Tensor& w, const Tensor& ids, double scale, bool fp32) {
-        c10::OptionalDeviceGuard guard(w.device());
-        const int64_t M = ids.size(0), V = w.size(0), D = w.size(1);
-        const Tensor out = at::empty({M, D}, w.options().dtype(fp32 ? torch::kFloat32 : torch::kBFloat16));
-        raise_status(theseus_embed_lookup(M, V, (int)D, type(w), type(out), ids.data_ptr<int64_t>(), w.data_ptr(), std::max(w.stride(0), D),
-                                          (float)scale, out.data_ptr(), stream_of(w)),
-                     "theseus_vocab");
-        return out;
-    }
-    static Tensor forward(AutogradContext* ctx, const Tensor& w, const Tensor& ids, double scale, int64_t skip, bool fp32) {
-        ctx->save_for_backward({ids});
-        ctx->saved_data["V"] = w.size(0), ctx->saved_data["D"] = w.size(1), ctx->saved_data["fp32"] = w.scalar_type() == torch::kFloat32;
-        ctx->saved_data["scale"] = scale, ctx->saved_data["skip"] = skip;
-        return lookup(w, ids, scale, fp32);
-    }
-    static variable_list backward(AutogradContext* ctx, variable_list g) {
-        auto& d = ctx->saved_data;
-        const Tensor ids = ctx->get_saved_variables()[0];
-        const int64_t M = ids.size(0), V = d["V"].toInt(), D = d["D"].toInt();
+// theseus.vocab.embedding for a table w [V][D] with rows apart and ids [M], checked there.  A node of its own: a short
+// call's host time is mostly the engine's, and torch::autograd::Function adds its dictionary to it.
+int embed_type(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 ? THESEUS_EMBED_BF16 : THESEUS_EMBED_FP32; }
+struct EmbeddingGrad : torch::autograd::Node {
+    torch::autograd::SavedVariable ids;
+    int64_t V, D, skip;
+    float scale;
+    bool fp32;
+    std::string name() const override { return "EmbeddingBackward"; }
+    void release_variables() override { ids.reset_data(); }
+    variable_list apply(variable_list&& g) override {
+        if (!g[0].defined()) return {Tensor()};
+        const Tensor at = ids.unpack();
         Tensor grad = g[0].scalar_type() == torch::kBFloat16 ? g[0] : g[0].to(torch::kFloat32);
         if (grad.stride(1) != 1 || (grad.stride(0) < D && grad.stride(0) != 0)) grad = grad.contiguous();
-        c10::OptionalDeviceGuard guard(grad.device());
-        Tensor dw = at::empty({V, D}, grad.options().dtype(d["fp32"].toBool() ? torch::kFloat32 : torch::kBFloat16));
-        const size_t need = theseus_embed_grad_workspace_size(M, V, (int)D);
-        const Tensor ws = scratch(need, grad);
-        raise_status(theseus_embed_grad(M, V, (int)D, type(grad), type(dw), ids.data_ptr<int64_t>(), d["skip"].toInt(), grad.data_ptr(),
-                                        grad.stride(0), (float)d["scale"].toDouble(), dw.data_ptr(), ptr(ws), need, stream_of(grad)),
-                     "theseus_vocab");
+        Tensor dw;
+        {
+            at::NoGradGuard no_grad;
+            c10::OptionalDeviceGuard guard(grad.device());
+            dw = at::empty({V, D}, grad.options().dtype(fp32 ? torch::kFloat32 : torch::kBFloat16));
+            const size_t need = theseus_embed_grad_workspace_size(at.size(0), V, (int)D);
+            const Tensor ws = scratch(need, grad);
+            raise_status(theseus_embed_grad(at.size(0), V, (int)D, embed_type(grad), embed_type(dw), at.data_ptr<int64_t>(), skip, grad.data_ptr(),
+                                            grad.stride(0), scale, dw.data_ptr(), ptr(ws), need, stream_of(grad)),
+                         "theseus_vocab");
+        }
         variable_list o{dw};
         if (at::GradMode::is_enabled()) {  // (create_graph: a later derivative through this raises)
             o[0].requires_grad_();
             o = (*std::make_shared<torch::autograd::DelayedError>("theseus_vocab: embedding is differentiable once", 1))(std::move(o));
         }
-        o.resize(5);
         return o;
     }
 };
 
 Tensor embedding(const Tensor& w, const Tensor& ids, double scale, int64_t skip, bool fp32) {
     py::gil_scoped_release free;
-    if (at::GradMode::is_enabled() && w.requires_grad()) return Embedding::apply(w, ids, scale, skip, fp32);
-    return Embedding::lookup(w, ids, scale, fp32);
+    c10::OptionalDeviceGuard guard(w.device());
+    const int64_t M = ids.size(0), V = w.size(0), D = w.size(1);
+    const Tensor out = at::empty({M, D}, w.options().dtype(fp32 ? torch::kFloat32 : torch::kBFloat16));
+    raise_status(theseus_embed_lookup(M, V, (int)D, embed_type(w), embed_type(out), ids.data_ptr<int64_t>(), w.data_ptr(), std::max(w.stride(0), D),
+                                      (float)scale, out.data_ptr(), stream_of(w)),
+                 "theseus_vocab");
+    if (at::GradMode::is_enabled() && w.requires_grad()) {
+        const std::shared_ptr<EmbeddingGrad> node(new EmbeddingGrad(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(w));
+        node->ids = torch::autograd::SavedVariable(ids, false);
+        node->V = V, node->D = D, node->skip = skip, node->scale = (float)scale, node->fp32 = embed_type(w) == THESEUS_EMBED_FP32;
+        torch::autograd::set_history(out, node);
+    }
+    return out;
 }
 
 }  // namespace
