@@ -15,9 +15,11 @@
  *
  * All pointers are device memory on the current device; the lists and ns are read during the call only (host
  * memory).  Nothing is allocated or synchronised, so the calls may be captured into a graph.  Results
- * are deterministic.  The products take float16 operands (scaled into its range) and add in float32;
- * X itself is held in two float16 halves, 22 bits.  Finite inputs whose X_i stay below 1.3 in every singular value
- * (the usual coefficients) cannot overflow.  Status codes are those of theseus_wkv7.h.
+ * are deterministic: the same list gives the same bits (in another list a matrix' sums may be cut otherwise).  The
+ * products take float16 operands (scaled into its range) and add in float32; X itself is held in two float16 halves, 22
+ * bits, the last step's operand in one.  Coefficients that keep the singular values of X_0 .. X_{steps-1} below 3 and
+ * |a + b s^2 + c s^4| below 32 for them cannot overflow; others may, and give values that are not finite.
+ * Status codes are those of theseus_wkv7.h.
  */
 #ifndef THESEUS_MUON_H
 #define THESEUS_MUON_H
@@ -35,7 +37,7 @@ enum theseus_muon_dtype { THESEUS_MUON_BF16 = 0, THESEUS_MUON_FP32 = 1 };
 typedef struct theseus_newton_schulz {
     int steps;      /* 1 .. 100                */
     float a, b, c;  /* finite                  */
-    float eps;      /* >= 0                    */
+    float eps;      /* >= 0, less than 1e-30 as 1e-30 */
 } theseus_newton_schulz;
 
 typedef struct theseus_orthogonalize_matrix {

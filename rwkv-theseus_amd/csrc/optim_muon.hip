@@ -1042,7 +1042,9 @@ static Matrix matrix(int m, int n) {
     const int p = m < n ? m : n;
     x.s = 1.f;
     while (x.s < 32.f && 4.f * x.s * x.s <= (float)p) x.s *= 2.f;  // (a s^2 stays far below 65504)
-    x.each = (long)m * n > 1 << 20 ? 4 : 1;  // (few elements: every load at once rather than few workgroups)
+    // (few elements: every load at once rather than few workgroups; many: at most 4096 sums, which every workgroup of X_0 adds)
+    const long many = ceil_div((long)m * n, 4096l * PIECE);
+    x.each = (long)m * n <= 1 << 20 ? 1 : many < 4 ? 4 : (int)many;
     x.pieces = (int)ceil_div((long)m * ceil_div(n, 8), PIECE / 8 * x.each);
     x.ld = n;
     return x;
@@ -1220,6 +1222,7 @@ static int check(const theseus_newton_schulz* ns) {
         return THESEUS_WKV7_ERR_SHAPE;
     return THESEUS_WKV7_OK;
 }
+static float eps_of(const theseus_newton_schulz* ns) { return ns->eps > 1e-30f ? ns->eps : 1e-30f; }  // (64 over it is finite)
 constexpr long long MAX_STRIDE = 1ll << 21;  // elements from row to row, in 32-bit byte offsets within a strip
 static bool fits(long long m, long long n) { return m >= 0 && n >= 0 && m <= 1 << 17 && n <= 1 << 17; }
 
@@ -1288,7 +1291,7 @@ int theseus_orthogonalize(const theseus_orthogonalize_matrix* ms, int count, con
     const size_t need = muon::workspace(count, get);
     if (!need) return THESEUS_WKV7_OK;
     if (!workspace || workspace_bytes < need) return THESEUS_WKV7_ERR_WORKSPACE;
-    const muon::Update u{0.f, 1.f, 0, 1.f, nullptr, 0, ns->eps};
+    const muon::Update u{0.f, 1.f, 0, 1.f, nullptr, 0, muon::eps_of(ns)};
     muon::List l;
     size_t bytes;
     long pieces;
@@ -1318,7 +1321,7 @@ int theseus_muon_step(const theseus_muon_matrix* ms, int count, const theseus_ne
         double* partial = static_cast<double*>(workspace);
         optim::launch_norm(partial, muon::norm_pass(ms, count, partial, stream), grad_scale, max_norm, result, stream);
     }
-    const muon::Update u{(float)momentum, (float)(1.0 - momentum), nesterov, grad_scale, norm ? result : nullptr, skip_nonfinite, ns->eps};
+    const muon::Update u{(float)momentum, (float)(1.0 - momentum), nesterov, grad_scale, norm ? result : nullptr, skip_nonfinite, muon::eps_of(ns)};
     auto get = [&](int i) { return muon::get_muon(ms[i]); };
     muon::List l;
     size_t bytes;

@@ -26,6 +26,7 @@ include/theseus_muon.h).  The reference trains with AdamW only.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -191,13 +192,32 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # of the usual five steps: singular va
 _MAX_SIDE, _MAX_STRIDE = 1 << 17, 1 << 21  # include/theseus_muon.h
 
 
+@functools.lru_cache(maxsize=64)
+def _in_range(steps, a, b, c):
+    """Whether singular values from 0 .. 1 stay in what float16 products hold: the largest in 1/4 .. 3 until the last step,
+    |a + b s^2 + c s^4| up to 32 (a grid of 512, so 1 % of room)."""
+    largest = 1.0
+    for _ in range(steps):
+        if not .25 <= largest <= 2.97:
+            return False
+        grid = [largest * i / 512 for i in range(513)]
+        factors = [abs(a + (b + c * s * s) * s * s) for s in grid]
+        if max(factors) > 31.7:
+            return False
+        largest = max(s * f for s, f in zip(grid, factors))
+    return True
+
+
 def _schulz(steps, coefficients, eps):
     if not 1 <= steps <= 100:
         raise ValueError(f"theseus_muon: steps must be in 1 .. 100, got {steps}")
     if len(coefficients) != 3 or not all(math.isfinite(c) and abs(c) < 1e6 for c in coefficients):
         raise ValueError(f"theseus_muon: expected three finite coefficients, got {coefficients}")
-    if not 0 <= eps < float("inf"):
-        raise ValueError(f"theseus_muon: eps must not be negative, got {eps}")
+    if not 0 <= eps <= 3.4028234663852886e38:
+        raise ValueError(f"theseus_muon: eps must not be negative, and finite in float32, got {eps}")
+    if not _in_range(int(steps), *(float(c) for c in coefficients)):
+        raise ValueError(f"theseus_muon: {steps} steps with coefficients {coefficients} leave float16's range (largest singular values "
+                         "out of 1/4 .. 3, or factors above 32)")
     return _Schulz(int(steps), *(float(c) for c in coefficients), float(eps))
 
 
@@ -219,10 +239,11 @@ def orthogonalize(x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     (on the short side; the norm per matrix).  x: a tensor [..., m, n] (leading dimensions: that many
     matrices) or a list of them, bfloat16 or float32, sides up to 2^17; rows may lie apart.  Returns
     bfloat16 tensors of the same shapes (a list for a list): with the usual coefficients the singular
-    values themselves end anywhere in 0.68 .. 1.21.  All matrices share the launches.  The products take float16 operands
-    and add in float32, X is held in 22 bits: off by 2e-3 of the exact polynomial's norm, most of
-    it the result's rounding.  A matrix with a value that is not finite comes back NaN.  Not
-    differentiable."""
+    values themselves end anywhere in 0.68 .. 1.21; others are taken that keep the largest ones in 1/4 .. 3 and
+    |a + b s^2 + c s^4| below 32.  Norms below 1e-30 count as 1e-30 where eps is less.  All matrices share the launches.
+    The products take float16 operands and add in float32, X is held in 22 bits: off by 2e-3 to 3e-3 of the exact
+    polynomial's norm, 1.7e-3 of it the result's rounding.  The same list gives the same bits on every run (in another list a
+    matrix' sums may be cut otherwise).  A matrix with a value that is not finite comes back NaN.  Not differentiable."""
     ns = _schulz(steps, coefficients, eps)
     xs = [x] if isinstance(x, torch.Tensor) else list(x)
     if not xs:

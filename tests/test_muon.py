@@ -115,6 +115,17 @@ def test_scale_invariance_zeros_and_eps(m, n):
 
 
 @gpu
+@pytest.mark.parametrize("m,n", [(40, 50), (129, 140)])
+def test_tiny_norms_without_eps(m, n):
+    """Norms below 1e-30 count as 1e-30: no factor beyond float32, and zeros stay zeros."""
+    x = _gradient(m, n).cuda()
+    assert (orthogonalize(torch.zeros_like(x), eps=0.0) == 0).all()
+    for norm in (1e-28, 1e-33):
+        tiny = x * (norm / float(x.norm()))
+        _close(orthogonalize(tiny, eps=0.0), _exact(tiny, eps=1e-30))
+
+
+@gpu
 @pytest.mark.parametrize("m,n", [(40, 50), (300, 200)])
 def test_values_that_are_not_finite_make_their_matrix_nan(m, n):
     xs = [_gradient(m, n, i).cuda() for i in range(3)]
@@ -205,15 +216,19 @@ def test_same_bits_every_time_other_streams_and_graphs():
 
 
 @gpu
-def test_offsets_past_32_bits():
+@pytest.mark.parametrize("wide", [False, True])
+def test_offsets_past_32_bits(wide):
     """131072 x 17000 (4.5 GB): row i has its one in column i mod 17000, so the columns are orthogonal and
-    each is scaled by itself."""
+    each is scaled by itself.  And its transposed matrix."""
     m, n = 131072, 17000
     print(f"  orth {m}x{n}", flush=True)
     x = torch.zeros(m, n, dtype=BF, device="cuda")
     rows = torch.arange(m, device="cuda")
     x[rows, rows % n] = 1.0
+    if wide:
+        x = x.t().contiguous()
     out = orthogonalize(x)
+    out = out.t() if wide else out
     got = out[rows, rows % n].double()
     ones = torch.bincount(rows % n).double()
     s = ones.sqrt() / math.sqrt(m)
@@ -413,6 +428,21 @@ def test_muon_abi_rejects_bad_arguments_before_launching():
     assert step() == 4 and step(m=0) == 0
     sizes = [lib.theseus_muon_workspace_size((optim._Matrix * 1)(optim._Matrix(p, p, p, m, m, 1.0, .1)), 1) for m in (1, 64, 129, 512, 5120)]
     assert sizes == sorted(sizes) and sizes[0] > 0
+
+
+@pytest.mark.parametrize("steps,coefficients,fine", [
+    (100, optim.COEFFICIENTS, True), (100, (2.0, -1.5, .5), True), (100, (1.5, -.5, 0.0), True), (5, (1.0, 0.0, 0.0), True),
+    (1, (30.0, 0.0, 0.0), True), (2, (30.0, 0.0, 0.0), False), (1, (40.0, 0.0, 0.0), False), (2, (2.9, 0.0, 0.0), True), (3, (2.0, 0.0, 0.0), False),
+    (2, (.3, 0.0, 0.0), True), (3, (.3, 0.0, 0.0), False), (5, (8.28721, -23.5959, 17.3004), False), (5, (-3.4445, 4.7750, -2.0315), True)])
+def test_coefficients_that_leave_the_range_are_refused(steps, coefficients, fine):
+    """a s alone multiplies the largest singular value by a; the others' growth was followed on a fine grid."""
+    for call in (lambda: orthogonalize([], steps=steps, coefficients=coefficients),
+                 lambda: FusedMuon([torch.nn.Parameter(torch.zeros(3, 3))], steps=steps, coefficients=coefficients)):
+        if fine:
+            call()
+        else:
+            with pytest.raises(ValueError, match="float16's range"):
+                call()
 
 
 def test_constructor_validates():
