@@ -14,6 +14,7 @@
 
 #include <cstdlib>
 #include <cstring>
+#include <limits>
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -382,8 +383,8 @@ std::tuple<Tensor, Tensor, Tensor> vocab_top(const Tensor& x, int64_t k, double 
     return {values, indices, lse};
 }
 
-// theseus.vocab.embedding for a table w [V][D] with rows apart and ids [M], checked there.  A node of its own: a short
-// call's host time is mostly the engine's, and torch::autograd::Function adds its dictionary to it.
+// theseus.vocab.embedding.  A node of its own: a short call's host time is mostly the engine's, and
+// torch::autograd::Function adds its dictionary to it.
 int embed_type(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 ? THESEUS_EMBED_BF16 : THESEUS_EMBED_FP32; }
 struct EmbeddingGrad : torch::autograd::Node {
     torch::autograd::SavedVariable ids;
@@ -395,16 +396,18 @@ struct EmbeddingGrad : torch::autograd::Node {
     variable_list apply(variable_list&& g) override {
         if (!g[0].defined()) return {Tensor()};
         const Tensor at = ids.unpack();
-        Tensor grad = g[0].scalar_type() == torch::kBFloat16 ? g[0] : g[0].to(torch::kFloat32);
-        if (grad.stride(1) != 1 || (grad.stride(0) < D && grad.stride(0) != 0)) grad = grad.contiguous();
+        const int64_t M = at.numel();
         Tensor dw;
         {
             at::NoGradGuard no_grad;
+            Tensor grad = g[0].dim() == 2 ? g[0] : g[0].reshape({M, D});
+            if (grad.scalar_type() != torch::kBFloat16) grad = grad.to(torch::kFloat32);
+            if (grad.stride(1) != 1 || (grad.stride(0) < D && grad.stride(0) != 0)) grad = grad.contiguous();
             c10::OptionalDeviceGuard guard(grad.device());
             dw = at::empty({V, D}, grad.options().dtype(fp32 ? torch::kFloat32 : torch::kBFloat16));
-            const size_t need = theseus_embed_grad_workspace_size(at.size(0), V, (int)D);
+            const size_t need = theseus_embed_grad_workspace_size(M, V, (int)D);
             const Tensor ws = scratch(need, grad);
-            raise_status(theseus_embed_grad(at.size(0), V, (int)D, embed_type(grad), embed_type(dw), at.data_ptr<int64_t>(), skip, grad.data_ptr(),
+            raise_status(theseus_embed_grad(M, V, (int)D, embed_type(grad), embed_type(dw), at.data_ptr<int64_t>(), skip, grad.data_ptr(),
                                             grad.stride(0), scale, dw.data_ptr(), ptr(ws), need, stream_of(grad)),
                          "theseus_vocab");
         }
@@ -417,11 +420,22 @@ struct EmbeddingGrad : torch::autograd::Node {
     }
 };
 
-Tensor embedding(const Tensor& w, const Tensor& ids, double scale, int64_t skip, bool fp32) {
+// Nothing where an argument is not as the kernels take it: theseus/vocab.py then lays it out or says what is wrong.
+std::optional<Tensor> embedding(const Tensor& ids, const Tensor& w, double scale, std::optional<int64_t> padding_idx, std::optional<at::ScalarType> dtype) {
+    auto known = [](at::ScalarType t) { return t == torch::kBFloat16 || t == torch::kFloat32; };
+    if (!w.is_cuda() || w.layout() != at::kStrided || w.dim() != 2 || !known(w.scalar_type()) || !ids.is_cuda() || ids.layout() != at::kStrided ||
+        ids.scalar_type() != torch::kInt64 || ids.device() != w.device() || !ids.is_contiguous() || !known(dtype.value_or(w.scalar_type())))
+        return {};
+    const int64_t M = ids.numel(), V = w.size(0), D = w.size(1);
+    const int64_t skip = !padding_idx ? -1 : *padding_idx < 0 ? *padding_idx + V : *padding_idx;
+    if (V < 1 || D < 1 || V > 1 << 22 || D > 1 << 17 || M > 1 << 30 || w.stride(1) != 1 || (V > 1 && w.stride(0) < D) ||
+        (padding_idx && (skip < 0 || skip >= V)) || !(std::abs(scale) <= std::numeric_limits<float>::max()))
+        return {};
     py::gil_scoped_release free;
     c10::OptionalDeviceGuard guard(w.device());
-    const int64_t M = ids.size(0), V = w.size(0), D = w.size(1);
-    const Tensor out = at::empty({M, D}, w.options().dtype(fp32 ? torch::kFloat32 : torch::kBFloat16));
+    at::DimVector sizes(ids.sizes());
+    sizes.push_back(D);
+    const Tensor out = at::empty(sizes, w.options().dtype(dtype.value_or(w.scalar_type())));
     raise_status(theseus_embed_lookup(M, V, (int)D, embed_type(w), embed_type(out), ids.data_ptr<int64_t>(), w.data_ptr(), std::max(w.stride(0), D),
                                       (float)scale, out.data_ptr(), stream_of(w)),
                  "theseus_vocab");

@@ -431,7 +431,7 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
     """``scale * weight[ids]`` in ``dtype`` (the weight's own if None), and the weight's gradient.
 
     ids [...] int64, weight [V, D] bfloat16 or float32 (rows may lie apart), dtype one of the same
-    two: a float32 table gives bfloat16 rows in one pass, product and rounding once.  An index
+    two: a float32 table gives bfloat16 rows in one pass, the float32 product rounded once.  An index
     outside the vocabulary makes its row NaN and has no part in the gradient (the device is not
     asked before the call returns).  ``padding_idx`` (negative: from the end): tokens of this index
     get the table's row like the others, but add nothing to its gradient.  Returns [..., D].
@@ -439,6 +439,11 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
     The gradient has the weight's type and is written whole, rows without tokens as 0.  Each row is
     the float32 sum over its tokens in their order, times ``scale``, rounded once: the same bits on
     every run.  Differentiable once; raises if the ids were changed in place before the backward."""
+    native = _native(weight, ids)
+    if native is not None:
+        out = native.embedding(ids, weight, scale, padding_idx, dtype)
+        if out is not None:
+            return out
     w, flat = _table(weight, ids)
     scale = float(scale)
     if not math.isfinite(scale) or abs(scale) > 3.4028234663852886e38:
@@ -451,9 +456,8 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
     dtype = weight.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise TypeError(f"theseus_vocab: dtype must be bfloat16 or float32, got {dtype}")
-    native = _native(w, flat)
     if native is not None:
-        out = native.embedding(w, flat, scale, skip, dtype == torch.float32)
+        out = native.embedding(flat, w, scale, padding_idx, dtype)
     elif _direct(w):
         out = _lookup(w, flat, scale, dtype)
     else:
