@@ -21,10 +21,10 @@
 // halves, hi + lo / 2048: hi goes into the products, a lo is added to the next X; only the last step's X, whose
 // rounding is raised 3.4 times at most, is hi alone.  At most 2.6e-3 on all spectra that were tried.
 //
-// What bounds it (the ten matrices of a layer of width 5120, a step in 10.84 ms).  The products' cores run at
-// 1.3 PFLOP/s, the card's power limit; a tile's end, in which all CUs write at once, is 9 % of a Gram matrix' time
-// (440 us of 522 in tiles of 256, without their ends 403), the last round the rest.  Small matrices are
-// bound by their launches, 4 to 5 us each with nothing to do, three a step.
+// What bounds it (the ten matrices of a layer of width 5120, a step in 10.8 ms: Gram matrices 5 x 513 us, squares 5 x 536,
+// updates 5 x 1003, momentum and X_0 497).  The products' cores run at 1.3 PFLOP/s, the card's power limit; a tile's end, in
+// which all CUs write at once, is 9 % of a Gram matrix' time (of 433 us in tiles of 256), the last round, in
+// quarters, 80 us of it.  Small matrices are bound by their launches, 4 to 8 us each, three a step.
 #include "../../include/theseus_muon.h"
 #include "../../include/theseus_wkv7.h"
 
@@ -992,7 +992,7 @@ struct Small {
 // (they share the caches and the power), of the rest of a tile, and what a square's or an update's epilogue adds.
 // From squares of 256 .. 4096, 192, 352 and 512 x 5120 and 4096, each made in all four: Gram matrices of
 // 768 x 768 take 23, 12, 11 and 7 us, of 2048 x 2048 44, 24, 19 and 23, of 192 x 5120 89, 48, 33 and 18, of four of
-// 5120 x 5120 522 in tiles of 256 with the last round in quarters; updates of 2048 x 2048 52, 31, 27 and 43.
+// 5120 x 5120 513 in tiles of 256 with the last round in quarters; updates of 2048 x 2048 52, 31, 27 and 43.
 struct Cost {
     int side, per_cu;
     double few, full, rest, epilogue;
