@@ -647,7 +647,7 @@ template <class PW, class PT, Stage ST> __global__ __launch_bounds__(512) void u
 // is no subnormal (X by 64, A by 64^2, B by 1024).  More workgroups shorten the strips' time and lengthen the
 // parts'.
 constexpr int SHORT = 128;
-constexpr int ALONE = 16;  // strips that one workgroup takes, all steps but the first in one launch
+constexpr int ALONE = 16;  // strips that one workgroup takes: a list of such matrices takes one launch in all
 constexpr float SX = 64.f, SB = 1024.f;
 
 template <int P> struct Few {
@@ -664,7 +664,7 @@ __device__ __forceinline__ constexpr int lower(int i, int j) { return i * (i + 1
 struct FewArgs {
     float a, b, c;
     int steps;
-    int from, to;  // the steps of this launch: 0 makes X_0 and its A, 1 .. steps the products
+    int step;  // of this launch: 0 makes X_0 and its A, 1 .. steps the products
     const double* sums;
 };
 
@@ -740,8 +740,18 @@ template <int T> struct Strip {
     }
 };
 
-// START: step 0, X_0 and its A from the call's matrix; else steps from .. to.
-template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, Update u, FewArgs f) {
+// (a workgroup's LDS alone: what goes to memory need not have arrived)
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// START: step 0, X_0 and its A from the call's matrix.  STEP: one of the others.  WHOLE: a workgroup a matrix, the momentum and
+// its norm, then all steps, A's parts staying in LDS.
+enum Part { START, STEP, WHOLE };
+template <int P, Part KIND> __global__ __launch_bounds__(512) void few(List l, Update u, FewArgs f) {
     using F = Few<P>;
     constexpr int T = F::T, LD = F::LD;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[F::LDS];
@@ -757,13 +767,61 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
     uint16_t *xhi = x.ws, *xlo = xhi + (long)strips * 16 * P;                     // [q][P]
     float* parts = reinterpret_cast<float*>(xlo + (long)strips * 16 * P);         // [2][groups][HALVES][TILES][64][4]
     constexpr int PART = F::TILES * 256;
+    float* near = reinterpret_cast<float*>(lds + F::Y);  // WHOLE: [HALVES][TILES][64][4]
+    static_assert(F::HALVES * PART * 4 <= F::TURN - F::Y, "LDS");
     const float factor = u.result ? u.result[1] : u.factor;
+    uint4 xh[2][P / 32], xl[2][P / 32];  // X's columns of this wave's two strips of those from s0 on, on their way while A is made
+    auto load_x = [&](int s0) {
+        const int lane = thread_here() & 63;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int ks = 0; ks < P / 32; ks++) {  // (a wave without a second strip makes the last one again, and leaves it out)
+                const int at = (16 * min(s0 + 2 * wave + s, last - 1) + (lane & 15)) * P + 32 * ks + 8 * (lane >> 4);
+                xh[s][ks] = *reinterpret_cast<const uint4*>(xhi + at);
+                xl[s][ks] = *reinterpret_cast<const uint4*>(xlo + at);
+            }
+    };
 
-    for (int step = f.from; step <= f.to; step++) {
+    auto make_step = [&](auto first_one, const int step) {
+        constexpr bool start = decltype(first_one)::value;
         float by = 1.f / SB;
-        if constexpr (START) {  // the norm
+        f32x4_t d[2][T];
+        // u in strips s0 + 2 wave and the next one; WHOLE: with the momentum's step and the sum of squares
+        auto load_u = [&](int s0) {
+            const int lane = thread_here() & 63, r16 = lane & 15, q = lane >> 4;
             double sum = 0;
-            for (int j = threadIdx.x; j < x.pieces; j += 512) sum += f.sums[x.piece0 + j];
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const int j0 = 16 * min(s0 + 2 * wave + s, last - 1);
+                const bool mine = s0 + 2 * wave + s < last;
+                const Strip<T> src(x.src, tall, p, len, j0, x.ld, x.fp32 ? 4 : 2, r16, q);
+                src.all(d[s], x.fp32);
+                if (x.momentum) {
+                    const Strip<T> mom(x.momentum, tall, p, len, j0, x.n, 4, r16, q);
+                    f32x4_t m[T];
+                    mom.all(m, true);
+                    if constexpr (KIND == WHOLE) {
+#pragma unroll
+                        for (int t = 0; t < T; t++) m[t] = u.mu * m[t] + u.nu * (d[s][t] * factor);
+                        if (mine) mom.put(m, true);
+                    }
+#pragma unroll
+                    for (int t = 0; t < T; t++) d[s][t] = u.nesterov ? u.mu * m[t] + u.nu * (d[s][t] * factor) : m[t];
+                }
+                if (KIND == WHOLE && mine)
+#pragma unroll
+                    for (int t = 0; t < T; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sum += (double)d[s][t][e] * d[s][t][e];
+            }
+            return sum;
+        };
+        if constexpr (start) {  // the norm
+            double sum = 0;
+            if constexpr (KIND == WHOLE) sum = load_u(first);
+            else
+                for (int j = threadIdx.x; j < x.pieces; j += 512) sum += f.sums[x.piece0 + j];
             for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
             if ((threadIdx.x & 63) == 0) red[wave] = sum;
             __syncthreads();
@@ -773,13 +831,21 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
             by = (float)(SX / (norm < u.eps ? (double)u.eps : norm));
         } else {  // A's parts in order, A, B
             const int count = groups * F::HALVES;
-            const float* from = parts + (long)((step - 1) & 1) * count * PART + 4 * threadIdx.x;
             constexpr int MINE = (F::TILES * 64 + 511) / 512;
             f32x4_t s[MINE];
 #pragma unroll
             for (int r = 0; r < MINE; r++) s[r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            auto add = [&](auto batch) {  // (a batch in flight, added one after the other)
-                constexpr int BATCH = decltype(batch)::value;
+            if constexpr (KIND == WHOLE) {
+                wkv7::vm_wait_n<0>();  // (this wave's X is written)
+                load_x(first);
+#pragma unroll
+                for (int h = 0; h < F::HALVES; h++)
+#pragma unroll
+                    for (int r = 0; r < MINE; r++)
+                        s[r] += *reinterpret_cast<const f32x4_t*>(near + h * PART + 4 * threadIdx.x + (threadIdx.x + 512 * r < F::TILES * 64 ? 2048 * r : 0));
+            } else {  // (a batch in flight, added one after the other)
+                constexpr int BATCH = 10;
+                const float* from = parts + (long)((step - 1) & 1) * count * PART + 4 * threadIdx.x;
                 for (int g0 = 0; g0 < count; g0 += BATCH) {
                     f32x4_t v[BATCH][MINE];
 #pragma unroll
@@ -790,16 +856,18 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
 #pragma unroll
                     for (int g = 0; g < BATCH; g++)
 #pragma unroll
-                        for (int r = 0; r < MINE; r++) s[r] = g0 + g < count ? s[r] + v[g][r] : s[r];
+                        for (int r = 0; r < MINE; r++) {
+                            if (g0 + g >= count) break;
+                            asm volatile("");  // (a branch: selects would cost as much as the sums)
+                            s[r] += v[g][r];
+                        }
                 }
-            };
-            if (groups == 1) add(std::integral_constant<int, F::HALVES>{});
-            else add(std::integral_constant<int, 10>{});
+                load_x(first);
+            }
 #pragma unroll
             for (int r = 0; r < MINE; r++) {
-                const int v = threadIdx.x + 512 * r;
-                if (v >= F::TILES * 64) break;
-                const int tile = v >> 6, rr = v & 15, qq = (v >> 4) & 3;
+                const int tile = wave + 8 * r, rr = threadIdx.x & 15, qq = threadIdx.x >> 4 & 3;
+                if (tile >= F::TILES) break;
                 int i = 0;
 #pragma unroll
                 for (int n = 1; n < T; n++) i += tile >= lower(n, 0);
@@ -811,7 +879,7 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
                     mat[(row + 2) * LD + col] = (uint16_t)h.y, mat[(row + 3) * LD + col] = (uint16_t)(h.y >> 16);
                 }
             }
-            __syncthreads();
+            lds_barrier();
             // wave w: rows 16 (w % T) .., of P = 64 half of the columns each
             const int lane = thread_here() & 63, r16 = lane & 15, q = lane >> 4;
             constexpr int N = T / F::HALVES;
@@ -837,10 +905,10 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
                 b[n] = make_uint2(half2_of(y[0] + (row == col ? fa : 0.f), y[1] + (row + 1 == col ? fa : 0.f)),
                                   half2_of(y[2] + (row + 2 == col ? fa : 0.f), y[3] + (row + 3 == col ? fa : 0.f)));
             }
-            __syncthreads();
+            lds_barrier();
 #pragma unroll
             for (int n = 0; n < N; n++) *reinterpret_cast<uint2*>(mat + (16 * (tj0 + n) + r16) * LD + 16 * ti + 4 * q) = b[n];
-            __syncthreads();
+            lds_barrier();
         }
         // 16 strips at a time
         const int row = wave % T, half = wave / T;  // of the next A's tiles
@@ -850,34 +918,10 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
         for (int s0 = first; s0 < last; s0 += 16) {
             const int lane = thread_here() & 63, r16 = lane & 15, q = lane >> 4;
             const int strip = s0 + 2 * wave, have = min(last - strip, 2);
-            // (a wave without a second strip makes the first one again, and leaves it out)
-            auto strip_of = [&](int s) { return min(strip + s, last - 1); };
             auto make = [&] {
-            f32x4_t d[2][T];
-            if constexpr (START) {
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const int j0 = 16 * strip_of(s);
-                    const Strip<T> src(x.src, tall, p, len, j0, x.ld, x.fp32 ? 4 : 2, r16, q);
-                    src.all(d[s], x.fp32);
-                    if (x.momentum) {
-                        const Strip<T> mom(x.momentum, tall, p, len, j0, x.n, 4, r16, q);
-                        f32x4_t m[T];
-                        mom.all(m, true);
-#pragma unroll
-                        for (int t = 0; t < T; t++) d[s][t] = u.nesterov ? u.mu * m[t] + u.nu * (d[s][t] * factor) : m[t];
-                    }
-                }
+            if constexpr (start) {
+                if constexpr (KIND == START) load_u(s0);
             } else {
-                uint4 xh[2][P / 32], xl[2][P / 32];
-#pragma unroll
-                for (int s = 0; s < 2; s++)
-#pragma unroll
-                    for (int ks = 0; ks < P / 32; ks++) {
-                        const int at = (16 * strip_of(s) + r16) * P + 32 * ks + 8 * q;
-                        xh[s][ks] = *reinterpret_cast<const uint4*>(xhi + at);
-                        xl[s][ks] = *reinterpret_cast<const uint4*>(xlo + at);
-                    }
 #pragma unroll
                 for (int t = 0; t < T; t++) {
                     d[0][t] = d[1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -939,10 +983,11 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
                 wkv7::wave_lds_fence();
             }
             };
-            if (s0 > first) __syncthreads();  // (the strips before are still read)
+            if (s0 > first) lds_barrier();  // (the strips before are still read)
             if (have > 0) make();
-            if (!START && step == f.steps) continue;
-            __syncthreads();
+            if (!start && s0 + 16 < last) load_x(s0 + 16);
+            if (!start && step == f.steps) continue;
+            lds_barrier();
             // (lane: rows 4 q + (r16 >> 2) and 16 behind of 32 of Y^T, four columns, turned by the read)
             const uint16_t* at = yt + (4 * q + (r16 >> 2)) * LD + 4 * (r16 & 3);
             const int pairs = (min(last - s0, 16) + 1) / 2;  // (of strips: rows beyond the last one's are zero)
@@ -950,7 +995,6 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
                 const uint2 lo = wkv7::tr_at(at + 32 * ks * LD + 16 * t), hi = wkv7::tr_at(at + (32 * ks + 16) * LD + 16 * t);
                 return make_uint4(lo.x, lo.y, hi.x, hi.y);
             };
-#pragma unroll 4
             for (int ks = half; ks < pairs; ks += F::HALVES) {
                 const uint4 a = frag(ks, row);
 #pragma unroll
@@ -960,15 +1004,25 @@ template <int P, bool START> __global__ __launch_bounds__(512) void few(List l, 
                 }
             }
         }
-        if (!START && step == f.steps) return;
-        f32x4_t* to = reinterpret_cast<f32x4_t*>(parts + (((long)(step & 1) * groups + group) * F::HALVES + half) * PART) + (thread_here() & 63);
+        if (!start && step == f.steps) return;
+        f32x4_t* to;
+        if constexpr (KIND == WHOLE) {
+            lds_barrier();  // (Y^T, in whose place the parts go, is still read)
+            to = reinterpret_cast<f32x4_t*>(near + half * PART) + (thread_here() & 63);
+        } else {
+            to = reinterpret_cast<f32x4_t*>(parts + (((long)(step & 1) * groups + group) * F::HALVES + half) * PART) + (thread_here() & 63);
+        }
 #pragma unroll
         for (int t = 0; t < T; t++) {
             if (t > row) break;
             to[lower(row, t) * 64] = gram[t];
         }
-        __syncthreads();  // (a workgroup alone goes on with the next step: its parts and X are read by other waves)
-    }
+        if constexpr (KIND == WHOLE) lds_barrier();
+    };
+    if constexpr (KIND != STEP) make_step(std::true_type{}, 0);
+    if constexpr (KIND == STEP) make_step(std::false_type{}, f.step);
+    if constexpr (KIND == WHOLE)
+        for (int step = 1; step <= f.steps; step++) make_step(std::false_type{}, step);
 }
 
 // ------------------------------------------------------------------------------ host
@@ -1158,19 +1212,25 @@ static void run(List& l, const Update& u, const theseus_newton_schulz* ns, bool 
         at += all_short ? short_bytes(l.x[k]) : bytes_of(l.x[k]);
     }
     const int cus = device_cus();
-    momentum_norm<<<prefix(l, [](const Matrix& x) { return (long)x.pieces; }), 256, 0, st>>>(l, u, sums);
+    int longest = 0;
+    bool whole = all_short;
+    for (int k = 0; k < l.count; k++) {
+        const int p = l.x[k].m < l.x[k].n ? l.x[k].m : l.x[k].n;
+        longest = longest > p ? longest : p;
+        whole &= strips_of(l.x[k]) <= ALONE;
+    }
+    if (!whole) momentum_norm<<<prefix(l, [](const Matrix& x) { return (long)x.pieces; }), 256, 0, st>>>(l, u, sums);
     if (all_short) {
-        int longest = 0;
-        for (int k = 0; k < l.count; k++) {
-            const int p = l.x[k].m < l.x[k].n ? l.x[k].m : l.x[k].n;
-            longest = longest > p ? longest : p;
-        }
         const unsigned n = prefix(l, [&](const Matrix& x) { return groups_of(x, l.count); });
-        const int each = (int)n == l.count ? ns->steps : 1;  // (a workgroup a matrix: all steps at once)
         auto go = [&](auto P) {
-            few<decltype(P)::value, true><<<n, 512, 0, st>>>(l, u, FewArgs{ns->a, ns->b, ns->c, ns->steps, 0, 0, sums});
-            for (int i = 1; i <= ns->steps; i += each)
-                few<decltype(P)::value, false><<<n, 512, 0, st>>>(l, u, FewArgs{ns->a, ns->b, ns->c, ns->steps, i, i + each - 1, sums});
+            constexpr int side = decltype(P)::value;
+            FewArgs f{ns->a, ns->b, ns->c, ns->steps, 0, sums};
+            if (whole) {
+                few<side, WHOLE><<<n, 512, 0, st>>>(l, u, f);
+                return;
+            }
+            few<side, START><<<n, 512, 0, st>>>(l, u, f);
+            for (f.step = 1; f.step <= ns->steps; f.step++) few<side, STEP><<<n, 512, 0, st>>>(l, u, f);
         };
         if (longest <= 64) go(std::integral_constant<int, 64>{});
         else go(std::integral_constant<int, SHORT>{});
