@@ -1030,10 +1030,7 @@ template <int P, Part KIND> __global__ __launch_bounds__(512) void few(List l, U
                 for (int ks = half; ks < pairs; ks += F::HALVES) {
                     const uint4 a = frag(ks, row);
 #pragma unroll
-                    for (int t = 0; t < T; t++) {
-                        if (t > row) break;
-                        gram[t] = wkv7::mma32h(gram[t], a, frag(ks, t));
-                    }
+                    for (int t = 0; t < T; t++) gram[t] = wkv7::mma32h(gram[t], a, frag(ks, t));  // (all reads at once; those above the diagonal are left out)
                 }
             }
         }
