@@ -267,7 +267,8 @@ MATRICES = [(96, 96), (40, 256), (256, 40), (1, 33), (33, 1), (300, 257)]
 @gpu
 @pytest.mark.parametrize("nesterov", [True, False])
 @pytest.mark.parametrize("scale", ["shape", "rms"])
-@pytest.mark.parametrize("shapes", [MATRICES, [(64, 64), (20, 100), (128, 50)]], ids=["any", "short"])
+@pytest.mark.parametrize("shapes", [MATRICES, [(64, 64), (20, 100), (128, 50)], [(64, 700), (901, 128), (33, 20), (300, 61)]],
+                         ids=["any", "short", "long and short"])
 def test_three_steps_match_float64(shapes, scale, nesterov):
     lr, wd, mu = .02, .1, .9
     g = torch.Generator().manual_seed(1)
@@ -293,7 +294,7 @@ def test_three_steps_match_float64(shapes, scale, nesterov):
 
 
 @gpu
-@pytest.mark.parametrize("shapes", [MATRICES, [(64, 64), (20, 100)]], ids=["any", "short"])
+@pytest.mark.parametrize("shapes", [MATRICES, [(64, 64), (20, 100)], [(64, 700), (901, 128)]], ids=["any", "short", "long and short"])
 def test_step_after_backward_scales_clips_and_raises(shapes):
     def fresh(seed=0):
         g = torch.Generator().manual_seed(seed)
