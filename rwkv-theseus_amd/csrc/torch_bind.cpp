@@ -420,6 +420,19 @@ struct EmbeddingGrad : torch::autograd::Node {
     }
 };
 
+// A backward captured into a graph while a graph of the same leaf from another stream lives would draw that stream into
+// the capture, and end the process: the leaf's accumulator keeps the stream that it was made on.
+void check_capture(const Tensor& w) {
+    const auto held = w.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(w) : nullptr;
+    if (!held) return;
+    hipStreamCaptureStatus now = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream_of(w), &now) != hipSuccess || now == hipStreamCaptureStatusNone) return;
+    const auto made_on = held->stream();
+    TORCH_CHECK(!made_on || *made_on == c10::impl::VirtualGuardImpl(w.device().type()).getStream(w.device()),
+                "theseus_vocab: embedding is captured into a graph while an autograd graph of its weight from another stream lives: free "
+                "that one (its outputs and losses) first");
+}
+
 // Nothing where an argument is not as the kernels take it: theseus/vocab.py then lays it out or says what is wrong.
 std::optional<Tensor> embedding(const Tensor& ids, const Tensor& w, double scale, std::optional<int64_t> padding_idx, std::optional<at::ScalarType> dtype) {
     auto known = [](at::ScalarType t) { return t == torch::kBFloat16 || t == torch::kFloat32; };
@@ -433,13 +446,15 @@ std::optional<Tensor> embedding(const Tensor& ids, const Tensor& w, double scale
         return {};
     py::gil_scoped_release free;
     c10::OptionalDeviceGuard guard(w.device());
+    const bool differentiable = at::GradMode::is_enabled() && w.requires_grad();
+    if (differentiable) check_capture(w);
     at::DimVector sizes(ids.sizes());
     sizes.push_back(D);
     const Tensor out = at::empty(sizes, w.options().dtype(dtype.value_or(w.scalar_type())));
     raise_status(theseus_embed_lookup(M, V, (int)D, embed_type(w), embed_type(out), ids.data_ptr<int64_t>(), w.data_ptr(), std::max(w.stride(0), D),
                                       (float)scale, out.data_ptr(), stream_of(w)),
                  "theseus_vocab");
-    if (at::GradMode::is_enabled() && w.requires_grad()) {
+    if (differentiable) {
         const std::shared_ptr<EmbeddingGrad> node(new EmbeddingGrad(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(w));
         node->ids = torch::autograd::SavedVariable(ids, false);

@@ -438,7 +438,8 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
 
     The gradient has the weight's type and is written whole, rows without tokens as 0.  Each row is
     the float32 sum over its tokens in their order, times ``scale``, rounded once: the same bits on
-    every run.  Differentiable once; raises if the ids were changed in place before the backward."""
+    every run.  Differentiable once; raises if the ids were changed in place before the backward, and
+    if the call is captured into a graph while an eager one of the same weight lives."""
     native = _native(weight, ids)
     if native is not None:
         out = native.embedding(ids, weight, scale, padding_idx, dtype)

@@ -291,6 +291,34 @@ def test_on_another_stream_and_in_a_graph():
 
 
 @gpu
+def test_a_capture_beside_a_living_graph_of_the_weight_is_refused():
+    """Whose backward would draw the other graph's stream into the capture; once that graph is gone, the same capture works."""
+    ids = torch.randint(500, (2000,), generator=torch.Generator().manual_seed(0)).cuda()
+    w, up = torch.randn(500, 40, device="cuda", requires_grad=True), torch.randn(2000, 40, device="cuda")
+    eager = vocab.embedding(ids, w)
+    want = eager.detach(), torch.autograd.grad(eager, (w,), up, retain_graph=True)[0]
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="from another stream lives"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            vocab.embedding(ids, w)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with torch.no_grad():  # (nothing to go back through)
+            vocab.embedding(ids, w)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = vocab.embedding(ids, w)
+        dw, = torch.autograd.grad(out, (w,), up)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.detach(), want[0]) and torch.equal(dw, want[1])
+        again = vocab.embedding(ids, w.detach())
+        assert torch.equal(again, want[0])
+    del out, dw, graph
+
+
+@gpu
 def test_offsets_past_32_bits():
     """A table of 4.6 GB (450001 x 5120): rows around 2^32 bytes, and rows behind."""
     V, D = 450001, 5120
