@@ -428,10 +428,12 @@ __global__ __launch_bounds__(256) void add_parts(Runs s, const uint32_t* __restr
 }
 
 // ------------------------------------------------------------------------------ few tokens
-// One launch, no workspace: a workgroup has `rows` of the table's rows, looks through all tokens for theirs, sorts
-// those few by counting, and writes each of its rows once, zeros or a sum.  `lanes` threads cover a row's columns (a
-// slab of 256 N of them), and the 256 / lanes groups of threads take the rows in turn; a row of more than ALONE
+// One launch, no workspace: a workgroup has `rows` of the table's rows, writes their zeros, looks through all tokens for
+// theirs, sorts those few by counting, and writes the rows that have some again.  `lanes` threads cover a row's columns (256 N
+// of them at a time), and the 256 / lanes groups of threads take the rows in turn; a row of more than ALONE
 // tokens is shared by the groups, their sums added in order: at most ALONE batches of BATCH tokens each.
+// Bound by the zeros (200 tokens, 32768 x 2560 float32 with its lookup: 68 us, the zeros alone 49; rows written one by one,
+// zeros or sums, in slabs of 256 chunks: 101) or, of small tables, by latency (512 tokens, 8192 x 256: 7.4 us).
 constexpr int MOST = 1024;  // tokens
 constexpr int ROWS = 256;   // of a workgroup
 constexpr int ALONE = 16, BATCH = 16;
@@ -439,7 +441,7 @@ constexpr int ALONE = 16, BATCH = 16;
 struct FewTokens {
     int M;
     long V, skip;
-    int D, rows, slabs, lanes;
+    int D, rows, lanes;
     long ldg;
     float scale;
 };
@@ -448,10 +450,13 @@ __global__ __launch_bounds__(256) void few_tokens(FewTokens s, const int64_t* __
     __shared__ uint16_t place[MOST], row[MOST], sorted[MOST];
     __shared__ int count[ROWS], start[ROWS];
     __shared__ int found[MOST / 64];
+    __shared__ uint16_t present[ROWS];  // the rows that have tokens
+    __shared__ int waves[4];
     __shared__ float parts[256 * N];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const long v0 = (long)(blockIdx.x / s.slabs) * s.rows;
-    const int rows = (int)min((long)s.rows, s.V - v0), slab = blockIdx.x % s.slabs;
+    const long v0 = (long)blockIdx.x * s.rows;
+    const int rows = (int)min((long)s.rows, s.V - v0);
+    fill(dweight + v0 * s.D, (long)rows * s.D * sizeof(W), 0, 1);
     // this workgroup's tokens, in their order
     int mine[MOST / 256];
     uint64_t votes[MOST / 256];
@@ -479,67 +484,74 @@ __global__ __launch_bounds__(256) void few_tokens(FewTokens s, const int64_t* __
         n += found[k];
     }
     __syncthreads();
-    if (n) {
-        for (int r = t; r < rows; r += 256) {
-            int before = 0;
-            for (int k = 0; k < r; k++) before += count[k];
-            start[r] = before;
-        }
-        __syncthreads();
-        for (int i = t; i < n; i += 256) {
-            int before = start[row[i]];
-            for (int k = 0; k < i; k++) before += row[k] == row[i];
-            sorted[before] = place[i];
-        }
-        __syncthreads();
+    if (n == 0) return;
+    const uint64_t some = __ballot(count[t] > 0);
+    if (lane == 0) waves[wave] = __popcll(some);
+    if (count[t] > 0) {
+        int before = 0;
+        for (int k = 0; k < t; k++) before += count[k];
+        start[t] = before;
     }
-    const int groups = 256 / s.lanes, group = t / s.lanes, at = t - group * s.lanes, chunk = slab * 256 + at;
-    const bool there = chunk * N < s.D;
-    const int col = column<N>(there ? chunk : 0, s.D);
-    auto sum_of = [&](float (&sum)[N], int from, int to) {
+    __syncthreads();
+    int all = 0, at_row = 0;
 #pragma unroll
-        for (int e = 0; e < N; e++) sum[e] = 0.f;
-        for (int i0 = from; i0 < to; i0 += BATCH) {
-            float x[BATCH][N];
+    for (int w = 0; w < 4; w++) at_row += w < wave ? waves[w] : 0, all += waves[w];
+    if (count[t] > 0) present[at_row + __popcll(some & ((1ull << lane) - 1))] = t;
+    for (int i = t; i < n; i += 256) {
+        int before = start[row[i]];
+        for (int k = 0; k < i; k++) before += row[k] == row[i];
+        sorted[before] = place[i];
+    }
+    __syncthreads();
+    const int groups = 256 / s.lanes, group = t / s.lanes, at = t - group * s.lanes;
+    for (int c0 = 0; c0 * N < s.D; c0 += 256) {
+        const int chunk = c0 + at;
+        const bool there = chunk * N < s.D;
+        const int col = column<N>(there ? chunk : 0, s.D);
+        auto sum_of = [&](float (&sum)[N], int from, int to) {
 #pragma unroll
-            for (int j = 0; j < BATCH; j++) load<N, true>(x[j], grad + (long)sorted[min(i0 + j, to - 1)] * s.ldg + col);
+            for (int e = 0; e < N; e++) sum[e] = 0.f;
+            for (int i0 = from; i0 < to; i0 += BATCH) {
+                float x[BATCH][N];
 #pragma unroll
-            for (int j = 0; j < BATCH; j++)
-                if (i0 + j < to)
+                for (int j = 0; j < BATCH; j++) load<N, true>(x[j], grad + (long)sorted[min(i0 + j, to - 1)] * s.ldg + col);
 #pragma unroll
-                    for (int e = 0; e < N; e++) sum[e] += x[j][e];
-        }
-    };
-    auto put = [&](int r, float (&sum)[N]) {
+                for (int j = 0; j < BATCH; j++)
+                    if (i0 + j < to)
 #pragma unroll
-        for (int e = 0; e < N; e++) sum[e] *= s.scale;
-        store<N>(dweight + (v0 + r) * s.D + col, sum);
-    };
-    if (there)
-        for (int r = group; r < rows; r += groups) {
-            float sum[N] = {};
-            if (count[r] == 0) store<N>(dweight + (v0 + r) * s.D + col, sum);
-            else if (count[r] <= ALONE) {
+                        for (int e = 0; e < N; e++) sum[e] += x[j][e];
+            }
+        };
+        auto put = [&](int r, float (&sum)[N]) {
+#pragma unroll
+            for (int e = 0; e < N; e++) sum[e] *= s.scale;
+            store<N>(dweight + (v0 + r) * s.D + col, sum);
+        };
+        if (there)
+            for (int k = group; k < all; k += groups) {
+                const int r = present[k];
+                if (count[r] > ALONE) continue;
+                float sum[N];
                 sum_of(sum, start[r], start[r] + count[r]);
                 put(r, sum);
             }
-        }
-    if (n <= ALONE) return;
-    for (int r = 0; r < rows; r++) {
-        const int c = count[r];
-        if (c <= ALONE) continue;
-        const int each = (c + groups - 1) / groups, from = start[r] + min(group * each, c), to = start[r] + min(group * each + each, c);
-        float sum[N];
-        sum_of(sum, from, to);
-        __syncthreads();
+        if (n <= ALONE) continue;
+        for (int k = 0; k < all; k++) {
+            const int r = present[k], c = count[r];
+            if (c <= ALONE) continue;
+            const int each = (c + groups - 1) / groups, from = start[r] + min(group * each, c), to = start[r] + min(group * each + each, c);
+            float sum[N];
+            sum_of(sum, from, to);
+            __syncthreads();
 #pragma unroll
-        for (int e = 0; e < N; e++) parts[N * t + e] = sum[e];
-        __syncthreads();
-        if (group == 0 && there) {
-            for (int g = 1; g < groups; g++)
+            for (int e = 0; e < N; e++) parts[N * t + e] = sum[e];
+            __syncthreads();
+            if (group == 0 && there) {
+                for (int g = 1; g < groups; g++)
 #pragma unroll
-                for (int e = 0; e < N; e++) sum[e] += parts[N * (g * s.lanes + at) + e];
-            put(r, sum);
+                    for (int e = 0; e < N; e++) sum[e] += parts[N * (g * s.lanes + at) + e];
+                put(r, sum);
+            }
         }
     }
 }
@@ -598,10 +610,11 @@ static bool is_few(long M, int D) { return M <= MOST && M <= ALONE * BATCH * (25
 
 template <int N, typename G, typename W>
 static void launch_few(FewTokens s, const int64_t* ids, const void* grad, void* dweight, hipStream_t st) {
-    s.lanes = lanes_of(s.D), s.slabs = (int)ceil_div(ceil_div(s.D, N), 256);
-    const long share = ceil_div(s.V * s.slabs, 1024);  // (rows for about four workgroups on a CU)
-    s.rows = (int)(share < 1 ? 1 : share > ROWS ? ROWS : share);
-    few_tokens<N, G, W><<<(unsigned)(ceil_div(s.V, s.rows) * s.slabs), 256, 0, st>>>(s, ids, static_cast<const G*>(grad), static_cast<W*>(dweight));
+    s.lanes = lanes_of(s.D);
+    // rows for about four workgroups on a CU, of at most 64 KB
+    const long share = ceil_div(s.V, 1024), most = 65536 / (s.D * (long)sizeof(W)), least = share < most ? share : most;
+    s.rows = (int)(least < 1 ? 1 : least > ROWS ? ROWS : least);
+    few_tokens<N, G, W><<<(unsigned)ceil_div(s.V, s.rows), 256, 0, st>>>(s, ids, static_cast<const G*>(grad), static_cast<W*>(dweight));
 }
 
 template <int N, typename W, typename O>
@@ -662,7 +675,7 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
     if (!known(grad_dtype) || !known(weight_dtype)) return THESEUS_WKV7_ERR_DTYPE;
     if (!dweight || (M && (!ids || !grad))) return THESEUS_WKV7_ERR_NULL;
     if (is_few(M, D)) {
-        const FewTokens s{(int)M, V, skip, D, 0, 0, 0, grad_stride, scale};
+        const FewTokens s{(int)M, V, skip, D, 0, 0, grad_stride, scale};
         with_types(grad_dtype, weight_dtype, [&](auto g, auto w) {
             using G = decltype(g);
             using W = decltype(w);
