@@ -89,6 +89,19 @@ def test_stretches_of_one_token_inside_and_across_runs(M, tokens):
 
 
 @gpu
+@pytest.mark.parametrize("tokens", ["same", "16", "17", "48"])
+@pytest.mark.parametrize("M,D", [(256, 2500), (200, 2051), (512, 1000), (1024, 260), (100, 4)])
+def test_stretches_of_few_tokens_in_rows_of_all_widths(M, D, tokens):
+    """The one launch's rows that one group of threads adds, and those that all groups share."""
+    print(f"  few tokens M={M} D={D} {tokens}", flush=True)
+    V = 61
+    w, up, ids = _inputs(M, D, V, M, BF, FP, tokens)
+    wc = w.cuda().requires_grad_()
+    dw, = torch.autograd.grad(vocab.embedding(ids.cuda(), wc, dtype=FP), (wc,), up.cuda())
+    _grad_close(dw, ids, up, V, 1.0)
+
+
+@gpu
 def test_sorted_tokens_keep_their_order():
     """A sum whose value depends on the order: 2^24, ones that it swallows one by one, -2^24.  In the
     tokens' order nothing is left; sums of another order leave some ones."""
