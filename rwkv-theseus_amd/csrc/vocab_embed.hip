@@ -699,6 +699,7 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
             sort_fill<decltype(rounds)::value><<<(unsigned)(1 + fills), THREADS, 0, stream>>>((int)M, V, skip, dg, ids, at(p.keys), at(p.places), f);
         };
         if (M <= 2 * THREADS) sort(std::integral_constant<int, 2>{});
+        else if (M <= 4 * THREADS) sort(std::integral_constant<int, 4>{});
         else if (M <= 6 * THREADS) sort(std::integral_constant<int, 6>{});
         else sort(std::integral_constant<int, ONE / THREADS>{});
     } else {

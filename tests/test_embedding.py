@@ -56,7 +56,8 @@ def _grad_close(got, ids, up, V, scale, skip=None):
 # M, D, V: one token, no vector of eight, around a vector, around the sorts' sizes and the runs' ends
 SIZES = [(1, 1, 1), (1, 8, 5), (5, 7, 3), (17, 9, 40), (64, 64, 7), (33, 1001, 50), (2047, 12, 300), (2049, 20, 1000),
          (16384, 8, 70), (16385, 16, 5000), (40001, 9, 130000), (300, 2050, 20), (70, 4104, 33),
-         (256, 3000, 12), (257, 3000, 12), (1023, 256, 2000), (1024, 64, 40), (1025, 64, 40), (512, 512, 700), (513, 512, 700), (900, 3, 70000)]
+         (256, 3000, 12), (257, 3000, 12), (1023, 256, 2000), (1024, 64, 40), (1025, 64, 40), (512, 512, 700), (513, 512, 700), (900, 3, 70000), (4096, 24, 900), (4097, 24, 900),
+         (6144, 8, 900), (6145, 8, 900)]
 
 
 @gpu
