@@ -441,7 +441,7 @@ std::optional<Tensor> embedding(const Tensor& ids, const Tensor& w, double scale
         return {};
     const int64_t M = ids.numel(), V = w.size(0), D = w.size(1);
     const int64_t skip = !padding_idx ? -1 : *padding_idx < 0 ? *padding_idx + V : *padding_idx;
-    if (V < 1 || D < 1 || V > 1 << 22 || D > 1 << 17 || M > 1 << 30 || w.stride(1) != 1 || (V > 1 && w.stride(0) < D) ||
+    if (V < 1 || D < 1 || V > 1 << 22 || D > 1 << 17 || M > 1 << 30 || (D > 1 && w.stride(1) != 1) || (V > 1 && w.stride(0) < D) ||
         (padding_idx && (skip < 0 || skip >= V)) || !(std::abs(scale) <= std::numeric_limits<float>::max()))
         return {};
     py::gil_scoped_release free;

@@ -457,10 +457,7 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
     dtype = weight.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise TypeError(f"theseus_vocab: dtype must be bfloat16 or float32, got {dtype}")
-    if native is not None:
-        out = native.embedding(flat, w, scale, padding_idx, dtype)
-    elif _direct(w):
-        out = _lookup(w, flat, scale, dtype)
-    else:
-        out = _Embedding.apply(w, flat, scale, skip, dtype)
+    out = None if native is None else native.embedding(flat, w, scale, padding_idx, dtype)
+    if out is None:
+        out = _lookup(w, flat, scale, dtype) if _direct(w) else _Embedding.apply(w, flat, scale, skip, dtype)
     return out if ids.dim() == 1 else out.reshape(*ids.shape, w.shape[1])

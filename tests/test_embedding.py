@@ -201,6 +201,31 @@ def test_strides_and_alignment():
 
 
 @gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("table", ["transposed row", "column of a transposed table", "every third of it", "one number", "one number of all"])
+def test_tables_of_one_column_of_any_stride(table, native, monkeypatch):
+    """Of a dimension of one element torch keeps any stride, and calls the tensor contiguous all the same."""
+    if not native:
+        monkeypatch.setattr(vocab, "_native", lambda *a: None)
+    g = torch.Generator().manual_seed(0)
+    big = torch.randn(7, 60, generator=g).cuda()
+    w = {"transposed row": torch.randn(1, 33, generator=g).cuda().t(), "column of a transposed table": big.t()[:, :1],
+         "every third of it": big.t()[::3, 2:3], "one number": big.t()[5:6, 1:2], "one number of all": big.t()[5:6, 1:2].expand(9, 1)}[table]
+    assert w.shape[1] == 1 and w.stride(1) != 1
+    V = w.shape[0]
+    for shape in ((40,), (3000,), (6, 5), (), (0,)):
+        ids = torch.randint(V, shape, generator=g)
+        for dtype in (FP, BF):
+            v = w.detach().requires_grad_()
+            out = vocab.embedding(ids.cuda(), v, scale=2.0, dtype=dtype)
+            assert torch.equal(out.detach(), (2.0 * w[ids.cuda()]).to(dtype))
+            up = torch.randn(*shape, 1, generator=g).to(dtype)
+            dw, = torch.autograd.grad(out, (v,), up.cuda())
+            assert dw.shape == w.shape
+            _grad_close(dw, ids.reshape(-1), up.reshape(-1, 1), V, 2.0)
+
+
+@gpu
 def test_gradient_matches_differences():
     """The float32 gradient of a smooth function of the rows against central differences of it in float64."""
     g = torch.Generator().manual_seed(2)
