@@ -62,10 +62,10 @@ int theseus_orthogonalize(const theseus_orthogonalize_matrix* matrices, int coun
                           void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* factor = grad_scale min(1, max_norm / (norm + 1e-6)) with the L2 norm of grad_scale grad over all matrices,
- * formed in device memory ahead of the step; max_norm < 0: grad_scale alone, no norm.  result: 3
+ * formed in device memory ahead of the step; max_norm < 0 or NaN: grad_scale alone, no norm.  result: 3
  * floats of device memory as theseus_adamw_step writes them, norm, factor and 1 where the norm is
- * not finite (may be NULL where max_norm < 0).  With skip_nonfinite such a norm leaves every param
- * and momentum unchanged. */
+ * not finite (without a norm NaN, grad_scale and 0 if there is anything to step; may then be NULL).  With
+ * skip_nonfinite a norm that is not finite leaves every param and momentum unchanged. */
 size_t theseus_muon_workspace_size(const theseus_muon_matrix* matrices, int count);
 int theseus_muon_step(const theseus_muon_matrix* matrices, int count, const theseus_newton_schulz* ns, double momentum,
                       int nesterov, float grad_scale, float max_norm, int skip_nonfinite, float* result, void* workspace,

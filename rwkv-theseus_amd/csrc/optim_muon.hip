@@ -1415,9 +1415,9 @@ int theseus_muon_step(const theseus_muon_matrix* ms, int count, const theseus_ne
     const size_t need = theseus_muon_workspace_size(ms, count);
     if (!need && !norm) return THESEUS_WKV7_OK;
     if (need && (!workspace || workspace_bytes < need)) return THESEUS_WKV7_ERR_WORKSPACE;
-    if (norm) {
-        double* partial = static_cast<double*>(workspace);
-        optim::launch_norm(partial, muon::norm_pass(ms, count, partial, stream), grad_scale, max_norm, result, stream);
+    if (result) {  // (written without a norm too: a caller may read it)
+        double* partial = norm ? static_cast<double*>(workspace) : nullptr;
+        optim::launch_norm(partial, norm ? muon::norm_pass(ms, count, partial, stream) : 0, grad_scale, max_norm, result, stream);
     }
     const muon::Update u{(float)momentum, (float)(1.0 - momentum), nesterov, grad_scale, norm ? result : nullptr, skip_nonfinite, muon::eps_of(ns)};
     auto get = [&](int i) { return muon::get_muon(ms[i]); };

@@ -332,6 +332,28 @@ def test_step_after_backward_scales_clips_and_raises(shapes):
 
 
 @gpu
+@pytest.mark.parametrize("limit", [-1.0, -math.inf, math.nan])
+@pytest.mark.parametrize("shapes", [[(64, 64), (20, 100)], [(64, 700), (901, 128)], [(300, 257)]], ids=["whole", "short", "long"])
+def test_limits_that_are_none(shapes, limit):
+    """A negative max_norm or NaN: no norm and no clipping, as FusedAdamW, with NaN for the norm and no error."""
+    def fresh(cls):
+        ps = [_gradient(*s, seed=9).cuda().requires_grad_() for s in shapes]
+        for i, p in enumerate(ps):
+            p.grad = _gradient(*p.shape, seed=i).cuda()
+        return ps, cls(ps, lr=.02)
+    want, opt = fresh(FusedMuon)
+    opt.step_after_backward(grad_scale=.5)
+    for old in (0.0, 1.0):  # (what the memory of the result may hold)
+        for cls in (FusedMuon, optim.FusedAdamW):
+            ps, opt = fresh(cls)
+            held = [torch.full((3,), old, device="cuda") for _ in range(8)]
+            del held
+            norm = opt.step_after_backward(grad_scale=.5, max_norm=limit)
+            assert math.isnan(norm)
+            assert cls is not FusedMuon or all(torch.equal(p, q) for p, q in zip(ps, want))
+
+
+@gpu
 def test_state_dict_and_scheduler():
     g = torch.Generator().manual_seed(0)
     make = lambda: [torch.randn(s, generator=torch.Generator().manual_seed(5)).cuda().requires_grad_() for s in ((50, 60), (200, 140))]  # noqa: E731
