@@ -348,15 +348,18 @@ class FusedMuon(torch.optim.Optimizer):
 
     def _run(self, grad_scale, max_norm, error_if_nonfinite):
         hyper, entries, device = self._entries()
-        if not entries:
+        norm, limit = max_norm is not None, -1.0 if max_norm is None else float(max_norm)
+        if device is None or not (entries or norm):
             return None
+        if not entries and not limit >= 0:  # (nothing to step, and no norm)
+            return torch.full((), math.nan, device=device)
         momentum, nesterov, coefficients, eps, steps = hyper
-        ns, lib, count, norm = _schulz(steps, coefficients, eps), _lib(), len(entries), max_norm is not None
+        ns, lib, count = _schulz(steps, coefficients, eps), _lib(), len(entries)
         arr = (_Matrix * count)(*entries)
         result = torch.empty(3, dtype=torch.float32, device=device) if norm else None
         _run_muon(device, int(lib.theseus_muon_workspace_size(arr, count)),
                   lambda ws, nbytes, stream: lib.theseus_muon_step(
-                      arr, count, ctypes.byref(ns), momentum, int(nesterov), float(grad_scale), float(max_norm) if norm else -1.0,
+                      arr, count, ctypes.byref(ns), momentum, int(nesterov), float(grad_scale), limit,
                       int(error_if_nonfinite), result.data_ptr() if norm else None, ws, nbytes, stream))
         if norm and error_if_nonfinite and bool(result[2].item()):
             raise RuntimeError(NONFINITE_MSG)  # (the kernels left every parameter unchanged)

@@ -354,6 +354,19 @@ def test_limits_that_are_none(shapes, limit):
 
 
 @gpu
+def test_parameters_without_elements_have_a_norm():
+    """FusedAdamW's result for them: 0."""
+    for cls in (FusedMuon, optim.FusedAdamW):
+        ps = [torch.nn.Parameter(torch.zeros(s, device="cuda")) for s in ((0, 5), (4, 0))]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        opt = cls(ps, lr=.02)
+        assert float(opt.step_after_backward(max_norm=1.0)) == 0.0
+        assert opt.step_after_backward() is None
+        assert math.isnan(opt.step_after_backward(max_norm=-1.0))
+
+
+@gpu
 def test_state_dict_and_scheduler():
     g = torch.Generator().manual_seed(0)
     make = lambda: [torch.randn(s, generator=torch.Generator().manual_seed(5)).cuda().requires_grad_() for s in ((50, 60), (200, 140))]  # noqa: E731
