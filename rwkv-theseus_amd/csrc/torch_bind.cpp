@@ -457,7 +457,8 @@ std::optional<Tensor> embedding(const Tensor& ids, const Tensor& w, double scale
     if (differentiable) {
         const std::shared_ptr<EmbeddingGrad> node(new EmbeddingGrad(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(w));
-        node->ids = torch::autograd::SavedVariable(ids, false);
+        // (tokens of inference mode have no version: a copy)
+        node->ids = torch::autograd::SavedVariable(ids.is_inference() ? ids.clone() : ids, false);
         node->V = V, node->D = D, node->skip = skip, node->scale = (float)scale, node->fp32 = embed_type(w) == THESEUS_EMBED_FP32;
         torch::autograd::set_history(out, node);
     }

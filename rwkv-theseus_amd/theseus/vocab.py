@@ -372,7 +372,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, skip, dtype):
         w, ids = _table(weight, ids)
-        ctx.save_for_backward(ids)
+        ctx.save_for_backward(ids.clone() if ids.is_inference() else ids)
         ctx.table, ctx.constants = (w.shape[0], w.shape[1], w.dtype), (scale, skip)
         return _lookup(w, ids, scale, dtype)
 

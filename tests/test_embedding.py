@@ -287,6 +287,24 @@ def test_autograd_contract(native, monkeypatch):
 
 
 @gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_tokens_made_in_inference_mode(native, monkeypatch):
+    """Sampled tokens, say: a copy is kept for the gradient, as of the losses' labels."""
+    if not native:
+        monkeypatch.setattr(vocab, "_native", lambda *a: None)
+    with torch.inference_mode():
+        ids = torch.randint(20, (6, 4), device="cuda")
+    w = torch.randn(20, 8, device="cuda", requires_grad=True)
+    kept = ids.clone()
+    out = vocab.embedding(ids, w)
+    assert torch.equal(out.detach(), w.detach()[kept])
+    with torch.inference_mode():
+        ids.zero_()
+    dw, = torch.autograd.grad(out.sum(), (w,))
+    _grad_close(dw, kept.reshape(-1).cpu(), torch.ones(24, 8), 20, 1.0)
+
+
+@gpu
 def test_a_trace_runs_again_and_forward_mode_is_refused():
     w = torch.randn(20, 8, device="cuda")
     f = lambda i, t: vocab.embedding(i, t, scale=2.0)  # noqa: E731
