@@ -15,6 +15,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <limits>
+#include <unordered_set>
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -420,17 +421,27 @@ struct EmbeddingGrad : torch::autograd::Node {
     }
 };
 
-// A backward captured into a graph while a graph of the same leaf from another stream lives would draw that stream into
-// the capture, and end the process: the leaf's accumulator keeps the stream that it was made on.
+// A captured backward runs each node on the stream that the node was made on: one that was made outside of the capture
+// would draw its stream into it, and end the process.  Such are the nodes of a weight that was computed there, and of each
+// leaf below the accumulator of an eager graph that lives.
 void check_capture(const Tensor& w) {
-    const auto held = w.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(w) : nullptr;
+    const auto held = w.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(w) : w.grad_fn();
     if (!held) return;
     hipStreamCaptureStatus now = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream_of(w), &now) != hipSuccess || now == hipStreamCaptureStatusNone) return;
-    const auto made_on = held->stream();
-    TORCH_CHECK(!made_on || *made_on == c10::impl::VirtualGuardImpl(w.device().type()).getStream(w.device()),
-                "theseus_vocab: embedding is captured into a graph while an autograd graph of its weight from another stream lives: free "
-                "that one (its outputs and losses) first");
+    const auto here = c10::impl::VirtualGuardImpl(w.device().type()).getStream(w.device());
+    std::vector<torch::autograd::Node*> nodes{held.get()};
+    std::unordered_set<torch::autograd::Node*> seen{held.get()};
+    while (!nodes.empty()) {
+        torch::autograd::Node* const node = nodes.back();
+        nodes.pop_back();
+        const auto made_on = node->stream();
+        TORCH_CHECK(!made_on || *made_on == here,
+                    "theseus_vocab: embedding is captured into a graph while an autograd graph of its weight from another stream lives: free "
+                    "that one (its outputs and losses) first");
+        for (const auto& edge : node->next_edges())
+            if (edge.function && seen.insert(edge.function.get()).second) nodes.push_back(edge.function.get());
+    }
 }
 
 // Nothing where an argument is not as the kernels take it: theseus/vocab.py then lays it out or says what is wrong.

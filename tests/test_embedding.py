@@ -376,6 +376,32 @@ def test_a_capture_beside_a_living_graph_of_the_weight_is_refused():
 
 
 @gpu
+def test_a_capture_of_a_computed_weight_beside_a_living_graph_is_refused():
+    """A weight that is rounded inside the capture from a leaf of that graph, and one that was rounded before it."""
+    ids = torch.randint(500, (2000,), generator=torch.Generator().manual_seed(0)).cuda()
+    table, up = torch.randn(500, 40, device="cuda", requires_grad=True), torch.randn(2000, 40, device="cuda").bfloat16()
+    eager = vocab.embedding(ids, table.to(BF))
+    want = eager.detach(), torch.autograd.grad(eager, (table,), up, retain_graph=True)[0]
+    early = table.detach().requires_grad_().to(BF)
+    torch.cuda.synchronize()
+    for weight in (lambda: table.to(BF), lambda: early):
+        with pytest.raises(RuntimeError, match="from another stream lives"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                vocab.embedding(ids, weight())
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = vocab.embedding(ids, table.to(BF))
+        dw, = torch.autograd.grad(out, (table,), up)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.detach(), want[0]) and torch.equal(dw, want[1])
+        assert torch.equal(vocab.embedding(ids, table.detach().to(BF)), want[0])
+    del out, dw, graph
+
+
+@gpu
 def test_offsets_past_32_bits():
     """A table of 4.6 GB (450001 x 5120): rows around 2^32 bytes, and rows behind."""
     V, D = 450001, 5120
