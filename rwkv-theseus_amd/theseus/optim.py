@@ -31,6 +31,7 @@ import math
 
 import torch
 
+from .fused import _direct
 from .wkv7 import extension
 
 
@@ -248,6 +249,8 @@ def orthogonalize(x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     xs = [x] if isinstance(x, torch.Tensor) else list(x)
     if not xs:
         return []
+    if not _direct(*xs):
+        raise RuntimeError("theseus_muon: orthogonalize has no forward-mode derivative, and no trace or functorch transform takes it in")
     outs, entries, held, device = [], [], [], xs[0].device
     for t in xs:
         if not t.is_cuda:

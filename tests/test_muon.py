@@ -393,6 +393,21 @@ def test_state_dict_and_scheduler():
 
 
 @gpu
+def test_traces_and_forward_mode_are_refused():
+    """Where the bare kernels would leave nothing behind, or drop the tangent."""
+    x = _gradient(30, 40).cuda()
+    call = lambda t: orthogonalize(t)  # noqa: E731
+    with pytest.raises(RuntimeError, match="theseus_muon: orthogonalize has no"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    with pytest.raises(RuntimeError, match="theseus_muon: orthogonalize has no"):
+        torch.func.vmap(call)(x[None])
+    with pytest.raises(RuntimeError, match="theseus_muon: orthogonalize has no"):
+        with torch.autograd.forward_ad.dual_level():
+            orthogonalize([torch.autograd.forward_ad.make_dual(x, x)])
+    assert orthogonalize(x.clone().requires_grad_()).requires_grad is False
+
+
+@gpu
 def test_refusals_on_the_gpu():
     w = torch.zeros(4, 4, device="cuda")
     for x, error, match in [(w.half(), TypeError, "bfloat16 or float32"), (w[0], ValueError, "m, n"), ([w, w.cpu()], ValueError, "CUDA"),
