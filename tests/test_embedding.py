@@ -119,6 +119,28 @@ def test_sorted_tokens_keep_their_order():
 
 
 @gpu
+@pytest.mark.parametrize("digits", [1, 2, 3])
+@pytest.mark.parametrize("M", [250, 1000, 1500, 2048, 4000, 6000, 16000, 40000, 70000])
+def test_every_sort_keeps_the_tokens_order(M, digits):
+    """Sixteen tokens a row, dealt over all waves and blocks: 2^25, fourteen ones that it swallows (its neighbours are 4 apart),
+    -2^25.  In the tokens' order nothing is left of any row; a last token ahead of another or a first one behind three leaves
+    some.  A run has a multiple of 16 tokens, so that no row is added in parts."""
+    print(f"  order M={M} digits={digits}", flush=True)
+    rows = M // 16
+    V = {1: rows, 2: 1 << 17, 3: (1 << 20) + 1}[digits]
+    at = torch.arange(rows) * (V // rows)
+    g = torch.Generator().manual_seed(M)
+    ids = torch.cat([at.repeat(16), torch.full((M - 16 * rows,), -1)])[torch.randperm(M, generator=g)]
+    order = ids.argsort(stable=True)
+    order = order[ids[order] >= 0].reshape(rows, 16)
+    up = torch.ones(M, 8)
+    up[order[:, 0]], up[order[:, 15]] = 2.0 ** 25, -2.0 ** 25
+    w = torch.zeros(V, 8, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(vocab.embedding(ids.cuda(), w), (w,), up.cuda())
+    assert not dw.any()
+
+
+@gpu
 @pytest.mark.parametrize("M,D,V", [(4300001, 1, 3), (4300001, 1, 1 << 22), (200000, 8, 1 << 20)])
 def test_many_tokens(M, D, V):
     """More blocks than one pass over their counts takes; one, two and three digits."""

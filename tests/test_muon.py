@@ -367,6 +367,38 @@ def test_parameters_without_elements_have_a_norm():
 
 
 @gpu
+@pytest.mark.parametrize("shapes", [[(8 + 3 * i, 1 + 37 * i % 700) for i in range(40)], [(20 + 9 * i, 30 + 53 * i % 300) for i in range(40)]],
+                         ids=["short", "long and short"])
+def test_a_step_of_more_matrices_than_a_launch_takes(shapes):
+    """One norm and clip factor over two sets of launches, which share the workspace; one that is not finite behind the first set."""
+    assert len(shapes) > 32
+    g = torch.Generator().manual_seed(0)
+    ps = [torch.randn(s, generator=g).cuda().requires_grad_() for s in shapes]
+    for i, p in enumerate(ps):
+        p.grad = _gradient(*p.shape, seed=i).cuda()
+    opt = FusedMuon(ps, lr=.02, weight_decay=.1, momentum=.9)
+    for i, p in enumerate(ps):
+        opt.state[p]["momentum_buffer"] = _gradient(*p.shape, seed=50 + i).cuda()
+    held = lambda: [t.detach().clone() for p in ps for t in (p, opt.state[p]["momentum_buffer"])]  # noqa: E731
+    old = [(p.detach().double(), opt.state[p]["momentum_buffer"].double()) for p in ps]
+    want = math.sqrt(sum(float(p.grad.double().square().sum()) for p in ps))
+    clip = .3 * want
+    norm = opt.step_after_backward(max_norm=clip)
+    assert abs(float(norm) - want) <= 1e-6 * want
+    for i, (p, (w, b)) in enumerate(zip(ps, old)):
+        new, buf, step = _step64(w, p.grad, b, .02, .1, .9, True, "shape", clip / (want + 1e-6))
+        _params_close(p, new, step, f"param {i}")
+        assert float((opt.state[p]["momentum_buffer"].double() - buf).norm()) <= 1e-6 * float(buf.norm())
+    ps[35].grad[3, 0] = math.nan
+    before = held()
+    with pytest.raises(RuntimeError, match="non-finite"):
+        opt.step_after_backward(max_norm=clip)
+    assert all(torch.equal(a, b) for a, b in zip(before, held()))
+    opt.step_after_backward(max_norm=clip, error_if_nonfinite=False)
+    assert all(torch.isnan(p).all() for p in ps)
+
+
+@gpu
 def test_state_dict_and_scheduler():
     g = torch.Generator().manual_seed(0)
     make = lambda: [torch.randn(s, generator=torch.Generator().manual_seed(5)).cuda().requires_grad_() for s in ((50, 60), (200, 140))]  # noqa: E731
