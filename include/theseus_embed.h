@@ -7,7 +7,7 @@
  *
  * Pointers are device memory on the current device, tables and rows bfloat16 or float32 (any mix),
  * aligned to their elements.  Products and sums are float32, rounded once to the result's type.
- * The sums run in the tokens' order, in parts whose bounds follow from M and the indices alone:
+ * The sums run in the tokens' order, in parts whose bounds follow from M, D and the indices alone:
  * results are deterministic.  Nothing is allocated or synchronised, so the calls may be captured
  * into a graph.  Status codes are those of theseus_wkv7.h: sizes out of range
  * THESEUS_WKV7_ERR_SHAPE, an unknown type _ERR_DTYPE.

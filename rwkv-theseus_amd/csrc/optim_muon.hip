@@ -646,7 +646,7 @@ template <class PW, class PT, Stage ST> __global__ __launch_bounds__(512) void u
 // float16 as above, here with X's second half in the product too; X and B are scaled apart, so that this half
 // is no subnormal (X by 64, A by 64^2, B by 1024).  More workgroups shorten the strips' time and lengthen the
 // parts'.  Four 2560 x 128 take 17 us a step: the launch 4, the parts 5.5, B 2, Y 1.5, its halves 2.7, the next A 1.
-// 64 x 64 takes 21 us in all, 3.4 a step, each phase as long as its loads and LDS reads.
+// 64 x 64 takes 21 us in all, 3.4 a step: each phase as long as its loads and LDS reads, X's halves to memory and back among them.
 constexpr int SHORT = 128;
 constexpr int ALONE = 16;  // strips that one workgroup takes: a list of such matrices takes one launch in all
 constexpr float SX = 64.f, SB = 1024.f;

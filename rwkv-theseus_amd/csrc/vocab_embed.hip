@@ -10,7 +10,7 @@
 // space, a padding) costs no more than the others.  Three launches up to ONE tokens:
 //   sort_fill    workgroup 0 sorts in LDS, least significant digit first; the others meanwhile
 //                write the table's zeros, most of the bytes: rows with tokens are written again.
-//   sum_runs     a run of tokens x 256 threads of eight columns, eight tokens' rows in flight.
+//   sum_runs     a run of tokens x 256 threads of eight columns, 16 tokens' rows in flight (8 of float32).
 //   add_parts    where a stretch begins that crosses runs: its parts in order.
 // More tokens are sorted by many workgroups: digit counts, their prefix sums, places, per digit.
 // Few tokens (up to 1024 of narrow rows, 256 of wide ones) take one launch, few_tokens.
@@ -599,7 +599,10 @@ static Plan plan(long M, long V, int D) {
     return p;
 }
 
-// threads for a row's columns; whether few_tokens takes this many tokens
+// threads for a row's columns; whether few_tokens takes this many tokens: as many as its LDS and its batches for one row hold.
+// Against the sort and sums (float32 tables, us): 8192 x 256 with 16 tokens 6.1 and 14.3, 512 8.4 and 17.9, 1024 10.1 and 18.3;
+// 65536 x 256 with 1024 17.5 and 21.7; 8192 x 2560 with 256 23.1 and 24.2, 8192 x 5120 with 256 37.2 and 34.7; tables whose zeros
+// take longer the same either way.
 static int lanes_of(int D) {
     const long chunks = D >= 8 ? ceil_div(D, 8) : D;
     int lanes = 1;
@@ -698,6 +701,7 @@ int theseus_embed_grad(long long M, long long V, int D, int grad_dtype, int weig
         auto sort = [&](auto rounds) {
             sort_fill<decltype(rounds)::value><<<(unsigned)(1 + fills), THREADS, 0, stream>>>((int)M, V, skip, dg, ids, at(p.keys), at(p.places), f);
         };
+        // (rounds for all of ONE whatever M: 2048 tokens, 8192 x 256, 39 us for 19, 4096 40 for 22, 6144 41 for 26)
         if (M <= 2 * THREADS) sort(std::integral_constant<int, 2>{});
         else if (M <= 4 * THREADS) sort(std::integral_constant<int, 4>{});
         else if (M <= 6 * THREADS) sort(std::integral_constant<int, 6>{});

@@ -30,10 +30,6 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ f32x4_t mma32h(f32x4_t acc, uint4 a, uint4 b) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), acc, 0, 0, 0);
 }
-typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ f32x4_t mma16h(f32x4_t acc, uint2 a, uint2 b) {
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a), __builtin_bit_cast(f16x4_t, b), acc, 0, 0, 0);
-}
 __device__ __forceinline__ f32x4_t mma32(f32x4_t acc, uint4 a, uint4 b) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                    __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);

@@ -438,8 +438,10 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None, dtype=None):
 
     The gradient has the weight's type and is written whole, rows without tokens as 0.  Each row is
     the float32 sum over its tokens in their order, times ``scale``, rounded once: the same bits on
-    every run.  Differentiable once; raises if the ids were changed in place before the backward, and
-    if the call is captured into a graph while an eager one of the same weight lives."""
+    every run.  (That order is sorted for: of narrow tables with some thousand tokens, 4096 of 8192 x 256
+    say, an ``index_add_`` in no order is faster.)  Differentiable once; raises if the ids were changed in place
+    before the backward, and, with the native functions built, if the call is captured into a graph while an eager
+    one of the same weight, or of what it was computed from, lives."""
     native = _native(weight, ids)
     if native is not None:
         out = native.embedding(ids, weight, scale, padding_idx, dtype)
