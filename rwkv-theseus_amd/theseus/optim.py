@@ -385,5 +385,5 @@ class FusedMuon(torch.optim.Optimizer):
         """``step`` on the gradients times ``grad_scale``, clipped to ``max_norm`` over this optimizer's
         parameters: FusedAdamW.step_after_backward's arguments, result and errors.  (Scaling all of a run's
         gradients alike changes nothing but eps' part; clipping weighs this step's against the momentum.  A step that
-        is left out for its norm takes as long as any other.)"""
+        is left out for its norm may take as long as any other.)"""
         return self._run(grad_scale, max_norm, error_if_nonfinite)

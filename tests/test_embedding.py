@@ -440,6 +440,24 @@ def test_offsets_past_32_bits():
     assert not dw.any()
 
 
+@gpu
+def test_rows_past_32_bits():
+    """Rows of 4.6 GB (450001 tokens of 5120): each against the table, and the gradient of small whole numbers, whose sums are exact."""
+    M, V, D = 450001, 300, 5120
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randn(V, D, generator=g, device="cuda").bfloat16().requires_grad_()
+    ids = torch.randint(V, (M,), generator=g, device="cuda")
+    out = vocab.embedding(ids, w, dtype=BF)
+    for at in range(0, M, 50000):
+        assert torch.equal(out.detach()[at:at + 50000], w.detach()[ids[at:at + 50000]])
+    up = torch.randint(-1, 2, (M, D), generator=g, device="cuda", dtype=torch.int8).bfloat16()
+    dw, = torch.autograd.grad(out, (w,), up)
+    ref = torch.zeros(V, D, device="cuda")
+    for at in range(0, M, 50000):
+        ref.index_add_(0, ids[at:at + 50000], up[at:at + 50000].float())
+    assert torch.equal(dw, ref.bfloat16())
+
+
 # ------------------------------------------------------------------------------ refusals
 def test_refusals_of_the_c_abi_before_launching():
     lib = vocab._lib()

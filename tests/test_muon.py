@@ -399,6 +399,41 @@ def test_a_step_of_more_matrices_than_a_launch_takes(shapes):
 
 
 @gpu
+@pytest.mark.parametrize("clip", [False, True])
+@pytest.mark.parametrize("shapes", [[(64, 64), (20, 100)], [(64, 700), (901, 128)], [(300, 257), (40, 60)]], ids=["whole", "short", "long"])
+def test_a_captured_step_runs_again(shapes, clip):
+    """Every replay steps parameters and momentum on, from the gradients that are then in place: the eager steps' bits."""
+    def fresh():
+        ps = [_gradient(*s, seed=9).cuda().requires_grad_() for s in shapes]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        return ps, FusedMuon(ps, lr=.02, momentum=.9)
+
+    def step(opt):
+        if clip:
+            return opt.step_after_backward(grad_scale=.5, max_norm=1e-3, error_if_nonfinite=False)
+        opt.step()
+
+    (ps, opt), (qs, other) = fresh(), fresh()
+    for o in (opt, other):  # (the momentum's memory, outside of the capture)
+        step(o)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = step(opt)
+    for n in range(4):
+        for i, (p, q) in enumerate(zip(ps, qs)):
+            p.grad.copy_(_gradient(*p.shape, seed=10 * n + i))
+            q.grad.copy_(p.grad)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(other)
+        assert not clip or torch.equal(norm, want)
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q) and torch.equal(opt.state[p]["momentum_buffer"], other.state[q]["momentum_buffer"])
+    del graph, norm
+
+
+@gpu
 def test_state_dict_and_scheduler():
     g = torch.Generator().manual_seed(0)
     make = lambda: [torch.randn(s, generator=torch.Generator().manual_seed(5)).cuda().requires_grad_() for s in ((50, 60), (200, 140))]  # noqa: E731
